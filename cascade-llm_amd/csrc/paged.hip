@@ -1,0 +1,594 @@
+// The operators of a KV cache kept in pages (gfx950): rotary positions with
+// the write of K and V rows into pages, attention of one new token a
+// sequence over its pages, and copies of pages.
+//
+// A page holds page_size consecutive positions of a sequence for every KV
+// head, head-major: rows of one head are contiguous, so that a wave's loads
+// cover whole runs of page_size x head_dim x 2 bytes.  Page p of a layer's K
+// (or V) pool starts p * page_stride elements behind the pool's start, head
+// g of it g * head_stride further.  A page table row lists the pages of one
+// sequence in order.  page_size is a power of two of at least 8: the eight
+// consecutive rows that a lane group handles then share a page, and a page
+// lookup is a shift.
+//
+// Device-held indices (rows, positions, lengths, page numbers) are checked
+// in the kernels before they form an address: what they reject is left out
+// and CASCADE_PAGED_ERANGE is or-ed into the caller's error word.
+#include <cfloat>
+
+#include "cascade_device.h"
+#include "cascade_internal.h"
+
+namespace cascade {
+
+__device__ __forceinline__ void flag_range(int32_t *error) {
+  if (error != nullptr)
+    __hip_atomic_fetch_or(error, CASCADE_PAGED_ERANGE, __ATOMIC_RELAXED,
+                          __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---------------------------------------------------------------- append
+struct AppendArgs {
+  const uint16_t *q, *k, *v;  // token t, head h at t * token + h * head
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  const int32_t *positions;
+  const int32_t *rows;  // nullable: token t belongs to table row t
+  const int32_t *table;
+  int64_t table_stride;
+  int64_t sequences;
+  int32_t max_pages;
+  const uint16_t *cos, *sin;  // [rope_positions, rope_dim / 2], nullable
+  int64_t rope_positions;
+  int32_t rope_dim;
+  int32_t interleaved;
+  uint16_t *q_out;
+  int64_t qo_token, qo_head;
+  uint16_t *k_pages, *v_pages;
+  int64_t page_stride, head_stride;
+  int32_t num_pages;
+  int32_t page_shift;
+  int32_t q_heads, kv_heads, dim;
+  int32_t *error;
+};
+
+constexpr int kAppendThreads = 256;
+
+// One workgroup a token.  A thread's unit is 16 dims of one head as two
+// 16-byte vectors: for rotated dims the two vectors whose elements form
+// pairs (half layout: 8 dims and the 8 dims rope_dim / 2 behind them;
+// interleaved: 16 neighbouring dims), so that both read one vector of cos
+// and one of sin; other dims are copied.  Products and sums in fp32 and one
+// rounding.
+__global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a) {
+  const int64_t t = blockIdx.x;
+  const int64_t pos = a.positions[t];
+  const int64_t row = a.rows != nullptr ? a.rows[t] : t;
+  if (pos < 0 || row < 0) return;  // a padding token
+  const int64_t slot_page = pos >> a.page_shift;
+  bool ok = row < a.sequences && slot_page < a.max_pages &&
+            (a.rope_dim == 0 || pos < a.rope_positions);
+  const int64_t page = ok ? a.table[row * a.table_stride + slot_page] : -1;
+  ok = page >= 0 && page < a.num_pages;
+  if (!ok) {
+    if (threadIdx.x == 0) flag_range(a.error);
+    return;
+  }
+  const int64_t slot = pos & ((int64_t{1} << a.page_shift) - 1);
+  const int64_t base = page * a.page_stride + slot * a.dim;
+  const int per_head = a.dim / 16;
+  const int rotated = a.rope_dim / 16;
+  const int half = a.rope_dim / 2;
+  const int units = (a.q_heads + 2 * a.kv_heads) * per_head;
+  for (int u = threadIdx.x; u < units; u += kAppendThreads) {
+    int head = u / per_head;
+    const int part = u % per_head;
+    const uint16_t *src;
+    uint16_t *dst;
+    bool turn = part < rotated;
+    if (head < a.q_heads) {
+      src = a.q + t * a.q_token + head * a.q_head;
+      dst = a.q_out + t * a.qo_token + head * a.qo_head;
+    } else if ((head -= a.q_heads) < a.kv_heads) {
+      src = a.k + t * a.k_token + head * a.k_head;
+      dst = a.k_pages + base + head * a.head_stride;
+    } else {
+      head -= a.kv_heads;
+      src = a.v + t * a.v_token + head * a.v_head;
+      dst = a.v_pages + base + head * a.head_stride;
+      turn = false;
+    }
+    const bool split = turn && !a.interleaved;
+    const int d0 = split ? 8 * part : 16 * part;
+    const int d1 = split ? half + 8 * part : 16 * part + 8;
+    u32x4 x = *reinterpret_cast<const u32x4 *>(src + d0);
+    u32x4 y = *reinterpret_cast<const u32x4 *>(src + d1);
+    if (turn) {
+      const u32x4 c = *reinterpret_cast<const u32x4 *>(a.cos + pos * half + 8 * part);
+      const u32x4 s = *reinterpret_cast<const u32x4 *>(a.sin + pos * half + 8 * part);
+      if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t xi = x[i], yi = y[i], ci = c[i >> 1], si = s[i >> 1];
+          const uint32_t cj = c[2 + (i >> 1)], sj = s[2 + (i >> 1)];
+          const float cx = i & 1 ? hi_bf16(ci) : lo_bf16(ci);
+          const float sx = i & 1 ? hi_bf16(si) : lo_bf16(si);
+          const float cy = i & 1 ? hi_bf16(cj) : lo_bf16(cj);
+          const float sy = i & 1 ? hi_bf16(sj) : lo_bf16(sj);
+          x[i] = pack_bf16x2(lo_bf16(xi) * cx - hi_bf16(xi) * sx,
+                             hi_bf16(xi) * cx + lo_bf16(xi) * sx);
+          y[i] = pack_bf16x2(lo_bf16(yi) * cy - hi_bf16(yi) * sy,
+                             hi_bf16(yi) * cy + lo_bf16(yi) * sy);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t xi = x[i], yi = y[i], ci = c[i], si = s[i];
+          x[i] = pack_bf16x2(lo_bf16(xi) * lo_bf16(ci) - lo_bf16(yi) * lo_bf16(si),
+                             hi_bf16(xi) * hi_bf16(ci) - hi_bf16(yi) * hi_bf16(si));
+          y[i] = pack_bf16x2(lo_bf16(yi) * lo_bf16(ci) + lo_bf16(xi) * lo_bf16(si),
+                             hi_bf16(yi) * hi_bf16(ci) + hi_bf16(xi) * hi_bf16(si));
+        }
+      }
+    }
+    *reinterpret_cast<u32x4 *>(dst + d0) = x;
+    *reinterpret_cast<u32x4 *>(dst + d1) = y;
+  }
+}
+
+// ------------------------------------------------------------- attention
+struct PagedAttnArgs {
+  const uint16_t *q;  // batch row b, head h at b * q_token + h * q_head
+  int64_t q_token, q_head;
+  const uint16_t *k_pages, *v_pages;
+  int64_t page_stride, head_stride;
+  int32_t num_pages;
+  int32_t page_shift;
+  const int32_t *table;
+  int64_t table_stride;
+  int64_t sequences;
+  const int32_t *lengths;
+  const int32_t *rows;  // nullable: batch row b reads table row b
+  int32_t max_length;
+  int32_t group;  // query heads a KV head, at most 16
+  float scale_log2;
+  uint16_t *out;  // [batch, q_heads, dim]
+  int64_t out_token, out_head;
+  int32_t *error;
+};
+
+constexpr int kPagedWaves = 4;
+constexpr int kPagedBlock = 32;  // positions a wave step
+constexpr int kPagedGroup = 16;  // MFMA columns
+
+__device__ __forceinline__ float paged_exp2(float x) {
+  return __builtin_amdgcn_exp2f(x);
+}
+
+// One workgroup per (batch row, KV head); each wave runs an online softmax
+// over every fourth block of 32 positions and the waves merge in LDS.  The
+// products are v_mfma_f32_16x16x32_bf16 with the query heads of the KV head
+// as columns (zeros past group):
+//   S = K_blk q^T    two 16-row tiles x D / 32 chunks
+//   O += V_blk^T P   D / 16 tiles, K = the 32 positions
+// Lane (c, g4) = (l % 16, l / 16) owns the scores of head c at rows
+// 8 g4 .. 8 g4 + 7 (the row order inside a K tile is chosen for that), which
+// is its piece of the P operand.  V rows are loaded whole (16 lanes a row,
+// dims DV c .. DV c + DV - 1 with DV = D / 16) and transposed in registers.
+// Scores carry scale * log2(e).  The running maximum starts at -FLT_MAX, so
+// a block whose rows are all left out keeps it and adds nothing; a sequence
+// with no row at all ends with a zero sum and writes zeros.
+template <int D>
+__global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
+    PagedAttnArgs a) {
+  constexpr int DV = D / 16;  // dims a lane holds of a V row
+  constexpr int KC = D / 32;  // 32-dim chunks
+  __shared__ float s_ml[kPagedWaves][kPagedGroup][2];
+  __shared__ float s_acc[kPagedWaves][kPagedGroup][D];
+  const int b = blockIdx.x;
+  const int g = blockIdx.y;
+  const int G = a.group;
+  const int tid = threadIdx.x;
+  const int lane = tid & (kWave - 1);
+  const int wave = tid / kWave;
+  const int c16 = lane & 15;
+  const int g4 = lane >> 4;
+  const int64_t row = a.rows != nullptr ? a.rows[b] : b;
+  if (row < 0) return;  // a padding row
+  if (row >= a.sequences) {
+    if (tid == 0) flag_range(a.error);
+    return;
+  }
+  int len = a.lengths[row];
+  if (len < 0 || len > a.max_length) {
+    if (tid == 0) flag_range(a.error);
+    len = min(max(len, 0), a.max_length);
+  }
+  const int last = len - 1;
+  const int32_t *table = a.table + row * a.table_stride;
+  const uint16_t *kb = a.k_pages + g * a.head_stride;
+  const uint16_t *vb = a.v_pages + g * a.head_stride;
+  const int page_mask = (1 << a.page_shift) - 1;
+
+  u32x4 qop[KC];
+#pragma unroll
+  for (int c = 0; c < KC; ++c)
+    qop[c] = c16 < G ? *reinterpret_cast<const u32x4 *>(
+                           a.q + b * a.q_token + (g * G + c16) * a.q_head +
+                           32 * c + 8 * g4)
+                     : u32x4{0u, 0u, 0u, 0u};
+  const uint32_t head_mask = c16 < G ? 0xffffffffu : 0u;
+
+  float m = -FLT_MAX, l = 0.0f;
+  f32x4 o[DV];
+#pragma unroll
+  for (int e = 0; e < DV; ++e) o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  for (int r0 = wave * kPagedBlock; r0 < len; r0 += kPagedWaves * kPagedBlock) {
+    // K tile rows 8 (i / 4) + i % 4 + 4 hf: group i / 4 of eight; rows past
+    // the end repeat the last row
+    const int kg = min(r0 + 8 * (c16 >> 2), last);
+    const int vg = min(r0 + 8 * g4, last);
+    int kpage = table[kg >> a.page_shift];
+    int vpage = table[vg >> a.page_shift];
+    const bool vbad = vpage < 0 || vpage >= a.num_pages;
+    if (kpage < 0 || kpage >= a.num_pages) kpage = 0;
+    if (vbad) {
+      vpage = 0;
+      flag_range(a.error);
+    }
+    const uint16_t *kp = kb + kpage * a.page_stride;
+    const uint16_t *vp = vb + vpage * a.page_stride;
+    u32x4 kt[2][KC];
+    uint32_t vt[8][DV / 2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int r = min(r0 + 8 * (c16 >> 2) + (c16 & 3) + 4 * hf, last) & page_mask;
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+        kt[hf][c] = __builtin_nontemporal_load(
+            reinterpret_cast<const u32x4 *>(kp + r * D + 32 * c + 8 * g4));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = min(r0 + 8 * g4 + j, last) & page_mask;
+      const uint32_t *src = reinterpret_cast<const uint32_t *>(vp + r * D + DV * c16);
+      if constexpr (DV == 8) {
+        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vt[j][i] = x[i];
+      } else {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(src));
+        vt[j][0] = x[0];
+        vt[j][1] = x[1];
+      }
+    }
+    if (vbad) {  // what another sequence's page holds takes no part, NaN neither
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < DV / 2; ++i) vt[j][i] = 0u;
+    }
+    f32x4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      s0 = mfma_16x16x32_bf16(kt[0][c], qop[c], s0);
+      s1 = mfma_16x16x32_bf16(kt[1][c], qop[c], s1);
+    }
+    float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
+    float bmax = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      s[j] = r0 + 8 * g4 + j < len && !vbad ? s[j] * a.scale_log2 : -INFINITY;
+      bmax = fmaxf(bmax, s[j]);
+    }
+    bmax = xor32_max(xor16_max(bmax));
+    const float mnew = fmaxf(m, bmax);
+    const float alpha = paged_exp2(m - mnew);
+    m = mnew;
+    float p[8], psum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = paged_exp2(s[j] - mnew);
+      psum += p[j];
+    }
+    l = fmaf(l, alpha, psum);
+    u32x4 pop;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      pop[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]) & head_mask;
+    if (alpha != 1.0f) {
+#pragma unroll
+      for (int e = 0; e < DV; ++e) o[e] *= alpha;
+    }
+#pragma unroll
+    for (int e = 0; e < DV; ++e) {
+      const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
+      u32x4 vop;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        vop[i] = __builtin_amdgcn_perm(vt[2 * i + 1][e >> 1], vt[2 * i][e >> 1], sel);
+      o[e] = mfma_16x16x32_bf16(vop, pop, o[e]);
+    }
+  }
+
+  l = xor32_sum(xor16_sum(l));
+  if (c16 < G) {
+    // o[e][r] = O[dim DV (4 g4 + r) + e][head c16]
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < DV; ++e) s_acc[wave][c16][DV * (4 * g4 + r) + e] = o[e][r];
+    if (g4 == 0) {
+      s_ml[wave][c16][0] = m;
+      s_ml[wave][c16][1] = l;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < G * D; i += kPagedWaves * kWave) {
+    const int h = i / D;
+    const int d = i % D;
+    float mm = -FLT_MAX;
+#pragma unroll
+    for (int w = 0; w < kPagedWaves; ++w) mm = fmaxf(mm, s_ml[w][h][0]);
+    float den = 0.0f, r = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kPagedWaves; ++w) {
+      const float wt = paged_exp2(s_ml[w][h][0] - mm);
+      den = fmaf(wt, s_ml[w][h][1], den);
+      r = fmaf(wt, s_acc[w][h][d], r);
+    }
+    a.out[b * a.out_token + (g * G + h) * a.out_head + d] =
+        f32_to_bf16(den == 0.0f ? 0.0f : r / den);
+  }
+}
+
+// ----------------------------------------------------------------- copies
+struct CopyPagesArgs {
+  unsigned char *base;  // page p of plane i at i * plane_bytes + p * page_bytes
+  int64_t plane_bytes;
+  int64_t page_bytes;
+  int32_t num_pages;
+  int32_t planes;
+  const int32_t *pairs;  // [count][2]: source, destination
+  int64_t pieces;        // pieces a page
+  int64_t total;         // count * planes * pieces
+  int32_t *error;
+};
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyVecs = 4;  // 16-byte vectors a thread and piece
+constexpr int64_t kCopyPiece = int64_t{kCopyThreads} * kCopyVecs * 16;
+
+// One workgroup copies a piece of 16 KiB of one page of one plane.
+__global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyPagesArgs a) {
+  for (int64_t w = blockIdx.x; w < a.total; w += gridDim.x) {
+    const int64_t piece = w % a.pieces;
+    const int64_t rest = w / a.pieces;
+    const int64_t plane = rest % a.planes;
+    const int64_t pair = rest / a.planes;
+    const int32_t src = a.pairs[2 * pair];
+    const int32_t dst = a.pairs[2 * pair + 1];
+    if (src < 0 || dst < 0) continue;  // a padding pair
+    if (src >= a.num_pages || dst >= a.num_pages) {
+      if (threadIdx.x == 0) flag_range(a.error);
+      continue;
+    }
+    unsigned char *plane_base = a.base + plane * a.plane_bytes;
+    const unsigned char *from = plane_base + src * a.page_bytes;
+    unsigned char *to = plane_base + dst * a.page_bytes;
+    u32x4 x[kCopyVecs];
+#pragma unroll
+    for (int i = 0; i < kCopyVecs; ++i) {
+      const int64_t at = piece * kCopyPiece + (int64_t{i} * kCopyThreads + threadIdx.x) * 16;
+      if (at < a.page_bytes) x[i] = *reinterpret_cast<const u32x4 *>(from + at);
+    }
+#pragma unroll
+    for (int i = 0; i < kCopyVecs; ++i) {
+      const int64_t at = piece * kCopyPiece + (int64_t{i} * kCopyThreads + threadIdx.x) * 16;
+      if (at < a.page_bytes) *reinterpret_cast<u32x4 *>(to + at) = x[i];
+    }
+  }
+}
+
+static bool page_shift_of(int64_t page_size, int32_t *shift) {
+  if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1))) return false;
+  *shift = __builtin_ctzll(static_cast<unsigned long long>(page_size));
+  return true;
+}
+
+static bool stride_ok(int64_t stride) { return stride >= 0 && (stride & 7) == 0; }
+
+}  // namespace cascade
+
+using namespace cascade;
+
+extern "C" int cascade_paged_append_bf16(
+    const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
+    int64_t k_token_stride, int64_t k_head_stride, const void *v,
+    int64_t v_token_stride, int64_t v_head_stride, int64_t tokens,
+    int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+    const int32_t *positions, const int32_t *rows, const int32_t *page_table,
+    int64_t table_stride, int64_t sequences, int64_t max_pages,
+    const void *rope_cos, const void *rope_sin, int64_t rope_positions,
+    int64_t rope_dim, int interleaved, void *q_out, int64_t q_out_token_stride,
+    int64_t q_out_head_stride, void *k_pages, void *v_pages, int64_t page_stride,
+    int64_t page_head_stride, int64_t num_pages, int64_t page_size,
+    int32_t *error_flag, void *stream) {
+  if (k == nullptr || v == nullptr || positions == nullptr || page_table == nullptr ||
+      k_pages == nullptr || v_pages == nullptr)
+    return CASCADE_EINVAL;
+  if (n_q_heads < 0 || (n_q_heads > 0 && (q == nullptr || q_out == nullptr)))
+    return CASCADE_EINVAL;
+  if (tokens <= 0 || tokens > 0x7fffffff || n_kv_heads <= 0 || sequences <= 0 ||
+      max_pages <= 0 || table_stride < max_pages || num_pages <= 0 ||
+      num_pages > 0x7fffffff)
+    return CASCADE_EINVAL;
+  AppendArgs a{};
+  if (head_dim < 16 || head_dim > 1024 || (head_dim & 15) || n_q_heads > 1024 ||
+      n_kv_heads > 1024 || !page_shift_of(page_size, &a.page_shift) ||
+      max_pages * page_size > 0x7fffffff)
+    return CASCADE_ESHAPE;
+  if (rope_dim < 0 || rope_dim > head_dim || (rope_dim & 15)) return CASCADE_ESHAPE;
+  if (rope_dim > 0 &&
+      (rope_cos == nullptr || rope_sin == nullptr || rope_positions <= 0))
+    return CASCADE_EINVAL;
+  if (page_head_stride < page_size * head_dim ||
+      page_stride < (n_kv_heads - 1) * page_head_stride + page_size * head_dim)
+    return CASCADE_EINVAL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(rope_cos) ||
+      !aligned16(rope_sin) || !aligned16(q_out) || !aligned16(k_pages) ||
+      !aligned16(v_pages) || (reinterpret_cast<uintptr_t>(positions) & 3) ||
+      (reinterpret_cast<uintptr_t>(rows) & 3) ||
+      (reinterpret_cast<uintptr_t>(page_table) & 3) ||
+      (reinterpret_cast<uintptr_t>(error_flag) & 3))
+    return CASCADE_EALIGN;
+  const int64_t strides[] = {q_token_stride, q_head_stride, k_token_stride,
+                             k_head_stride,  v_token_stride, v_head_stride,
+                             q_out_token_stride, q_out_head_stride, page_stride,
+                             page_head_stride};
+  for (int64_t s : strides)
+    if (!stride_ok(s)) return CASCADE_EALIGN;
+  a.q = static_cast<const uint16_t *>(q);
+  a.k = static_cast<const uint16_t *>(k);
+  a.v = static_cast<const uint16_t *>(v);
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.k_token = k_token_stride;
+  a.k_head = k_head_stride;
+  a.v_token = v_token_stride;
+  a.v_head = v_head_stride;
+  a.positions = positions;
+  a.rows = rows;
+  a.table = page_table;
+  a.table_stride = table_stride;
+  a.sequences = sequences;
+  a.max_pages = static_cast<int32_t>(max_pages);
+  a.cos = static_cast<const uint16_t *>(rope_cos);
+  a.sin = static_cast<const uint16_t *>(rope_sin);
+  a.rope_positions = rope_positions;
+  a.rope_dim = static_cast<int32_t>(rope_dim);
+  a.interleaved = interleaved;
+  a.q_out = static_cast<uint16_t *>(q_out);
+  a.qo_token = q_out_token_stride;
+  a.qo_head = q_out_head_stride;
+  a.k_pages = static_cast<uint16_t *>(k_pages);
+  a.v_pages = static_cast<uint16_t *>(v_pages);
+  a.page_stride = page_stride;
+  a.head_stride = page_head_stride;
+  a.num_pages = static_cast<int32_t>(num_pages);
+  a.q_heads = static_cast<int32_t>(n_q_heads);
+  a.kv_heads = static_cast<int32_t>(n_kv_heads);
+  a.dim = static_cast<int32_t>(head_dim);
+  a.error = error_flag;
+  return launch_kernel(paged_append_kernel, dim3(static_cast<unsigned>(tokens)),
+                       dim3(kAppendThreads), 0, static_cast<hipStream_t>(stream), a);
+}
+
+extern "C" size_t cascade_paged_attention_workspace_bytes(int64_t batch,
+                                                          int64_t n_q_heads,
+                                                          int64_t n_kv_heads,
+                                                          int64_t head_dim,
+                                                          int64_t max_length) {
+  if (batch <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads ||
+      n_q_heads / n_kv_heads > kPagedGroup || (head_dim != 64 && head_dim != 128) ||
+      max_length <= 0 || max_length > 0x7fffffff - 64)
+    return 0;
+  return 256;
+}
+
+extern "C" int cascade_paged_decode_attention_bf16(
+    const void *q, int64_t q_token_stride, int64_t q_head_stride,
+    const void *k_pages, const void *v_pages, int64_t page_stride,
+    int64_t page_head_stride, int64_t num_pages, int64_t page_size,
+    const int32_t *page_table, int64_t table_stride, int64_t sequences,
+    const int32_t *lengths, const int32_t *rows, int64_t batch, int64_t max_length,
+    int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim, float scale,
+    void *out, int64_t out_token_stride, int64_t out_head_stride, void *workspace,
+    size_t workspace_bytes, int32_t *error_flag, void *stream) {
+  if (q == nullptr || k_pages == nullptr || v_pages == nullptr ||
+      page_table == nullptr || lengths == nullptr || out == nullptr ||
+      workspace == nullptr)
+    return CASCADE_EINVAL;
+  if (batch <= 0 || batch > 0xffff || n_kv_heads <= 0 || sequences <= 0 ||
+      num_pages <= 0 || num_pages > 0x7fffffff || max_length <= 0)
+    return CASCADE_EINVAL;
+  PagedAttnArgs a{};
+  if ((head_dim != 64 && head_dim != 128) || n_q_heads <= 0 || n_q_heads % n_kv_heads ||
+      n_q_heads / n_kv_heads > kPagedGroup || n_kv_heads > 0xffff ||
+      !page_shift_of(page_size, &a.page_shift) || max_length > 0x7fffffff - 64)
+    return CASCADE_ESHAPE;
+  if (table_stride < (max_length + page_size - 1) / page_size ||
+      page_head_stride < page_size * head_dim ||
+      page_stride < (n_kv_heads - 1) * page_head_stride + page_size * head_dim)
+    return CASCADE_EINVAL;
+  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
+      !aligned16(workspace) || (reinterpret_cast<uintptr_t>(page_table) & 3) ||
+      (reinterpret_cast<uintptr_t>(lengths) & 3) ||
+      (reinterpret_cast<uintptr_t>(rows) & 3) ||
+      (reinterpret_cast<uintptr_t>(error_flag) & 3))
+    return CASCADE_EALIGN;
+  const int64_t strides[] = {q_token_stride, q_head_stride, page_stride,
+                             page_head_stride, out_token_stride, out_head_stride};
+  for (int64_t s : strides)
+    if (!stride_ok(s)) return CASCADE_EALIGN;
+  if (workspace_bytes < cascade_paged_attention_workspace_bytes(
+                            batch, n_q_heads, n_kv_heads, head_dim, max_length))
+    return CASCADE_EWORKSPACE;
+  a.q = static_cast<const uint16_t *>(q);
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.k_pages = static_cast<const uint16_t *>(k_pages);
+  a.v_pages = static_cast<const uint16_t *>(v_pages);
+  a.page_stride = page_stride;
+  a.head_stride = page_head_stride;
+  a.num_pages = static_cast<int32_t>(num_pages);
+  a.table = page_table;
+  a.table_stride = table_stride;
+  a.sequences = sequences;
+  a.lengths = lengths;
+  a.rows = rows;
+  a.max_length = static_cast<int32_t>(max_length);
+  a.group = static_cast<int32_t>(n_q_heads / n_kv_heads);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = static_cast<uint16_t *>(out);
+  a.out_token = out_token_stride;
+  a.out_head = out_head_stride;
+  a.error = error_flag;
+  const dim3 grid(static_cast<unsigned>(batch), static_cast<unsigned>(n_kv_heads));
+  const dim3 block(kPagedWaves * kWave);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (head_dim == 128)
+    return launch_kernel(paged_attention_kernel<128>, grid, block, 0, s, a);
+  return launch_kernel(paged_attention_kernel<64>, grid, block, 0, s, a);
+}
+
+extern "C" int cascade_copy_pages(void *pages, int64_t planes, int64_t plane_bytes,
+                                  int64_t num_pages, int64_t page_bytes,
+                                  const int32_t *pairs, int64_t count,
+                                  int32_t *error_flag, void *stream) {
+  if (pages == nullptr || pairs == nullptr) return CASCADE_EINVAL;
+  if (planes <= 0 || planes > 0x7fffffff || num_pages <= 0 || num_pages > 0x7fffffff ||
+      page_bytes <= 0 || count <= 0 || count > 0x7fffffff ||
+      page_bytes > (int64_t{1} << 40) || plane_bytes < 0 ||
+      (planes > 1 && plane_bytes / num_pages < page_bytes))
+    return CASCADE_EINVAL;
+  if ((page_bytes & 15) || (plane_bytes & 15) || !aligned16(pages) ||
+      (reinterpret_cast<uintptr_t>(pairs) & 3) ||
+      (reinterpret_cast<uintptr_t>(error_flag) & 3))
+    return CASCADE_EALIGN;
+  CopyPagesArgs a{};
+  a.base = static_cast<unsigned char *>(pages);
+  a.plane_bytes = plane_bytes;
+  a.page_bytes = page_bytes;
+  a.num_pages = static_cast<int32_t>(num_pages);
+  a.planes = static_cast<int32_t>(planes);
+  a.pairs = pairs;
+  a.pieces = (page_bytes + kCopyPiece - 1) / kCopyPiece;
+  if (a.pieces > INT64_MAX / planes / count) return CASCADE_EINVAL;
+  a.total = a.pieces * planes * count;
+  a.error = error_flag;
+  const int64_t blocks = a.total < (1 << 24) ? a.total : (1 << 24);
+  return launch_kernel(copy_pages_kernel, dim3(static_cast<unsigned>(blocks)),
+                       dim3(kCopyThreads), 0, static_cast<hipStream_t>(stream), a);
+}

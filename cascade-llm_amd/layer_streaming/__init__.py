@@ -6,6 +6,14 @@ libcascade_hip.so (see ``layer_streaming._hip``), which must be built --
 nothing here falls back to other device code.
 """
 
+from ._hip import (
+    copy_pages,
+    paged_append,
+    paged_attention_workspace_bytes,
+    paged_decode_attention,
+    sample,
+    sample_workspace_bytes,
+)
 from .graph import DecodeGraph
 from .llama31 import (
     LLAMA31_8B_MODEL_ID,
@@ -13,6 +21,7 @@ from .llama31 import (
     Llama31DecodeExecutor,
     SimpleKVCache,
 )
+from .paged import PagedKVCache
 from .plan import (
     Granularity,
     HostPlacement,
@@ -41,6 +50,7 @@ __all__ = [
     "Llama31Config",
     "Llama31DecodeExecutor",
     "ModelPlan",
+    "PagedKVCache",
     "PinnedStagingWeightStore",
     "ResidentDeviceArena",
     "ResidentTransformerRuntime",
@@ -51,6 +61,12 @@ __all__ = [
     "VocabStreamingRuntime",
     "WeightStoreMode",
     "build_llama31_8b_plan",
+    "copy_pages",
     "create_weight_store",
     "merge_topk",
+    "paged_append",
+    "paged_attention_workspace_bytes",
+    "paged_decode_attention",
+    "sample",
+    "sample_workspace_bytes",
 ]

@@ -34,6 +34,7 @@ LIBRARY_NAME = "libcascade_hip.so"
 _I64 = ctypes.c_int64
 _P = ctypes.c_void_p
 _F = ctypes.c_float
+_D = ctypes.c_double
 _INT = ctypes.c_int
 _SZ = ctypes.c_size_t
 _U64 = ctypes.c_uint64
@@ -105,6 +106,27 @@ _SIGNATURES = {
     "cascade_gemm_ws_bf16": (_INT, [_P, _P, _P, _I64, _I64, _I64, _P, _SZ, _P]),
     "cascade_gemm_residual_ws_bf16": (
         _INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _SZ, _P]),
+    "cascade_paged_append_bf16": (
+        _INT,
+        [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64,
+         _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _INT, _P, _I64, _I64,
+         _P, _P, _I64, _I64, _I64, _I64, _P, _P],
+    ),
+    "cascade_paged_attention_workspace_bytes": (
+        _SZ, [_I64, _I64, _I64, _I64, _I64]),
+    "cascade_paged_decode_attention_bf16": (
+        _INT,
+        [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P,
+         _I64, _I64, _I64, _I64, _I64, _F, _P, _I64, _I64, _P, _SZ, _P, _P],
+    ),
+    "cascade_copy_pages": (
+        _INT, [_P, _I64, _I64, _I64, _I64, _P, _I64, _P, _P]),
+    "cascade_sample_workspace_bytes": (_SZ, [_I64, _I64]),
+    "cascade_sample_f32": (
+        _INT,
+        [_P, _I64, _I64, _I64, _P, _P, _D, _P, _I64, _P, _D, _P, _D, _P, _P, _P,
+         _SZ, _P],
+    ),
     "cascade_embedding_gather_bf16": (
         _INT, [_P, _I64, _I64, _P, _I64, _P, _P, _P]),
     "cascade_decode_step_begin_bf16": (
@@ -129,13 +151,15 @@ _SIGNATURES = {
     "cascade_time_next_launch": (_INT, [_U64, _U64]),
 }
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 ESHAPE = 1003  # CASCADE_ESHAPE
 # fused decode attention: sync buffer size and the bits it ors into the
 # caller's error word (include/cascade_hip.h)
 ATTENTION_SYNC_BYTES = 1024
 ATTN_EPLACEMENT = 2
 ATTN_ETIMEOUT = 4
+# or-ed into a paged operator's error word by an index out of range
+PAGED_ERANGE = 8
 # the fused form needs one KV head per XCD and at least 8 splits of 32 rows
 FUSED_ATTENTION_KV_HEADS = 8
 FUSED_ATTENTION_MIN_LEN = 225
@@ -871,6 +895,363 @@ def device_copy(dst, src, stream=None):
     require_device(dst, "dst", src.dtype, src.numel())
     call("cascade_device_copy", dst.data_ptr(), src.data_ptr(),
          src.numel() * src.element_size(), stream_handle(stream))
+
+
+# ------------------------------------------- paged KV cache and sampling
+# These operators take strided views, and launch on the current stream of the
+# tensors' own device (or on ``stream``).
+
+
+def _placed(device, name, tensor, dtype, dim=None):
+    """A tensor of this device, dtype and number of dimensions."""
+
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError("{} must be a torch.Tensor".format(name))
+    if tensor.device != device:
+        raise ValueError("{} must live on {}, got {}".format(
+            name, device, tensor.device))
+    if tensor.dtype != dtype:
+        raise TypeError("{} must be {}, got {}".format(name, dtype, tensor.dtype))
+    if dim is not None and tensor.dim() != dim:
+        raise ValueError("{} must have {} dimensions".format(name, dim))
+    return tensor
+
+
+def _gpu_of(name, tensor):
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError("{} must be a torch.Tensor".format(name))
+    if tensor.device.type != "cuda":
+        raise ValueError("{} must live on the GPU, got {}".format(
+            name, tensor.device))
+    return tensor.device
+
+
+def _int32_vector(device, name, tensor, count=None):
+    _placed(device, name, tensor, torch.int32, 1)
+    if count is not None and tensor.shape[0] != count:
+        raise ValueError("{} holds {} entries, expected {}".format(
+            name, tensor.shape[0], count))
+    if tensor.shape[0] > 1 and tensor.stride(0) != 1:
+        raise ValueError("{} must be contiguous".format(name))
+    return tensor.data_ptr()
+
+
+def _strides(name, tensor):
+    """(outer, inner) strides of a [.., .., dim] view with contiguous dims."""
+
+    outer, inner, last = tensor.stride()
+    n_outer, n_inner, dim = tensor.shape
+    if dim > 1 and last != 1:
+        raise ValueError("{}: the last dimension must be contiguous".format(name))
+    # the stride of a dimension of one says nothing
+    return outer if n_outer > 1 else 0, inner if n_inner > 1 else 0
+
+
+def _apart(name, tensor):
+    """Refuse an output whose rows share memory (an expanded view)."""
+
+    dim = tensor.shape[-1]
+    spans = sorted((stride, size) for stride, size in zip(
+        tensor.stride()[:-1], tensor.shape[:-1]) if size > 1)
+    for stride, size in spans:
+        if stride < dim:
+            raise ValueError("{}: rows overlap".format(name))
+        dim = stride * (size - 1) + dim
+
+
+def _error_word(device, error_flag):
+    if error_flag is None:
+        return 0
+    _placed(device, "error_flag", error_flag, torch.int32)
+    if error_flag.numel() < 1:
+        raise ValueError("error_flag is empty")
+    return error_flag.data_ptr()
+
+
+def _page_pools(device, k_pages, v_pages):
+    """Check two [pages, kv_heads, page_size, head_dim] pools of one layout
+    and return (page stride, head stride)."""
+
+    _placed(device, "k_pages", k_pages, torch.bfloat16, 4)
+    _placed(device, "v_pages", v_pages, torch.bfloat16, 4)
+    page_stride, head_stride, row, last = k_pages.stride()
+    if k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+        raise ValueError("k_pages and v_pages differ in shape or layout")
+    pages, heads, page_size, dim = k_pages.shape
+    if (dim > 1 and last != 1) or (page_size > 1 and row != dim):
+        raise ValueError("the rows of a page's head must be contiguous")
+    if heads == 1:
+        head_stride = page_size * dim
+    if pages == 1:
+        page_stride = heads * head_stride
+    return page_stride, head_stride
+
+
+def _page_table(device, page_table):
+    _placed(device, "page_table", page_table, torch.int32, 2)
+    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+        raise ValueError("the rows of page_table must be contiguous")
+    sequences, width = page_table.shape
+    stride = width if sequences == 1 else page_table.stride(0)
+    if stride < width:
+        raise ValueError("the rows of page_table overlap")
+    return page_table.data_ptr(), stride
+
+
+def _call_on(device, stream, name, *args):
+    """Call an entry point whose last argument is the stream, with the
+    tensors' device current."""
+
+    if stream is None:
+        handle = torch.cuda.current_stream(device).cuda_stream
+    else:
+        handle = stream.cuda_stream
+    if device.index is None or device.index == torch.cuda.current_device():
+        code = getattr(load(), name)(*args, handle)
+    else:
+        with torch.cuda.device(device):
+            code = getattr(load(), name)(*args, handle)
+    if code != 0:
+        _check(name, code)
+
+
+def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
+                 rope=None, interleaved=False, q_out=None, error_flag=None,
+                 stream=None):
+    """Rotate projected rows by their positions and write K and V into pages.
+
+    ``q`` [tokens, heads, dim] (or None), ``k`` and ``v`` [tokens, kv_heads,
+    dim]: bf16 views with contiguous dims.  Token t sits at ``positions[t]``
+    of page table row ``rows[t]`` (row t without ``rows``); a negative position
+    or row marks padding, of which nothing is written.  ``rope``: (cos, sin)
+    tables, bf16 [positions, r / 2]; the first r dims of a head turn, in pairs
+    (i, i + r / 2) or, ``interleaved``, (2 i, 2 i + 1).  None copies the rows
+    as they are.  ``q_out`` (q itself by default) receives the rotated q rows
+    and is returned.  Pools are [pages, kv_heads, page_size, dim] views,
+    ``page_table`` int32 [sequences, pages of one].  An index out of range
+    leaves its token out and ors PAGED_ERANGE into ``error_flag``."""
+
+    device = _gpu_of("k", k)
+    _placed(device, "k", k, torch.bfloat16, 3)
+    _placed(device, "v", v, torch.bfloat16, 3)
+    tokens, kv_heads, dim = k.shape
+    if v.shape != k.shape:
+        raise ValueError("k and v differ in shape")
+    page_stride, head_stride = _page_pools(device, k_pages, v_pages)
+    pages, pool_heads, page_size, pool_dim = k_pages.shape
+    if (pool_heads, pool_dim) != (kv_heads, dim):
+        raise ValueError("the pools hold {} heads of {}, the rows {} of {}".format(
+            pool_heads, pool_dim, kv_heads, dim))
+    q_heads = 0
+    q_args, out_args = (0, 0, 0), (0, 0, 0)
+    if q is not None:
+        _placed(device, "q", q, torch.bfloat16, 3)
+        q_heads = q.shape[1]
+        if q.shape != (tokens, q_heads, dim):
+            raise ValueError("q and k differ in tokens or head size")
+        q_args = (q.data_ptr(),) + _strides("q", q)
+        if q_out is None:
+            q_out = q
+        if q_out is not q:
+            _placed(device, "q_out", q_out, torch.bfloat16, 3)
+            if q_out.shape != q.shape:
+                raise ValueError("q_out and q differ in shape")
+        _apart("q_out", q_out)
+        out_args = (q_out.data_ptr(),) + _strides("q_out", q_out)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    table, table_stride = _page_table(device, page_table)
+    sequences, max_pages = page_table.shape
+    pos = _int32_vector(device, "positions", positions, tokens)
+    row = 0 if rows is None else _int32_vector(device, "rows", rows, tokens)
+    if rows is None and tokens > sequences:
+        raise ValueError("more tokens than page table rows (give rows)")
+    cos = sin = rope_positions = rope_dim = 0
+    if rope is not None:
+        cos_t, sin_t = rope
+        _placed(device, "rope cos", cos_t, torch.bfloat16, 2)
+        _placed(device, "rope sin", sin_t, torch.bfloat16, 2)
+        if cos_t.shape != sin_t.shape:
+            raise ValueError("rope cos and sin differ in shape")
+        if not (cos_t.is_contiguous() and sin_t.is_contiguous()):
+            raise ValueError("the rope tables must be contiguous")
+        rope_positions, rope_dim = cos_t.shape[0], 2 * cos_t.shape[1]
+        cos, sin = cos_t.data_ptr(), sin_t.data_ptr()
+    error = _error_word(device, error_flag)
+    if tokens == 0:
+        return q_out
+    _call_on(device, stream, "cascade_paged_append_bf16", *q_args, k.data_ptr(),
+             *_strides("k", k), v.data_ptr(), *_strides("v", v), tokens, q_heads,
+             kv_heads, dim, pos, row, table, table_stride, sequences, max_pages,
+             cos, sin, rope_positions, rope_dim, 1 if interleaved else 0, *out_args,
+             k_pages.data_ptr(), v_pages.data_ptr(), page_stride, head_stride,
+             pages, page_size, error)
+    return q_out
+
+
+def paged_attention_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim,
+                                    max_length):
+    """Workspace bytes of paged_decode_attention for up to ``batch`` rows of
+    up to ``max_length`` positions."""
+
+    size = load().cascade_paged_attention_workspace_bytes(
+        int(batch), int(n_q_heads), int(n_kv_heads), int(head_dim),
+        int(max_length))
+    if size == 0:
+        raise ValueError("unsupported paged attention shape")
+    return int(size)
+
+
+def paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out,
+                           workspace, scale, rows=None, max_length=None,
+                           error_flag=None, stream=None):
+    """One-token GQA attention of every batch row over its sequence's pages.
+
+    ``q`` and ``out`` [batch, heads, dim]; batch row b reads positions
+    [0, lengths[r]) of page table row r = ``rows[b]`` (b without ``rows``); a
+    negative row is padding, whose output stays as it is.  ``lengths``: int32,
+    one a table row, at most ``max_length`` (default: what a table row
+    holds).  An empty sequence gives zeros.  Positions on a page outside the
+    pool are left out and flagged, as are longer lengths and larger rows
+    (PAGED_ERANGE in ``error_flag``).  ``workspace``:
+    paged_attention_workspace_bytes(...) uint8, one for calls that may
+    overlap."""
+
+    device = _gpu_of("q", q)
+    _placed(device, "q", q, torch.bfloat16, 3)
+    batch, q_heads, dim = q.shape
+    page_stride, head_stride = _page_pools(device, k_pages, v_pages)
+    pages, kv_heads, page_size, pool_dim = k_pages.shape
+    if pool_dim != dim:
+        raise ValueError("the pools hold heads of {}, q of {}".format(pool_dim, dim))
+    _placed(device, "out", out, torch.bfloat16, 3)
+    if out.shape != q.shape:
+        raise ValueError("out and q differ in shape")
+    _apart("out", out)
+    table, table_stride = _page_table(device, page_table)
+    sequences, max_pages = page_table.shape
+    lens = _int32_vector(device, "lengths", lengths, sequences)
+    row = 0 if rows is None else _int32_vector(device, "rows", rows, batch)
+    if rows is None and batch > sequences:
+        raise ValueError("more rows than page table rows (give rows)")
+    if max_length is None:
+        max_length = max_pages * page_size
+    elif not 0 < max_length <= max_pages * page_size:
+        raise ValueError("max_length {} is outside the page table's {}".format(
+            max_length, max_pages * page_size))
+    _placed(device, "workspace", workspace, torch.uint8, 1)
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    error = _error_word(device, error_flag)
+    if batch == 0:
+        return out
+    _call_on(device, stream, "cascade_paged_decode_attention_bf16", q.data_ptr(),
+             *_strides("q", q), k_pages.data_ptr(), v_pages.data_ptr(), page_stride,
+             head_stride, pages, page_size, table, table_stride, sequences, lens, row,
+             batch, int(max_length), q_heads, kv_heads, dim, float(scale),
+             out.data_ptr(), *_strides("out", out), workspace.data_ptr(),
+             workspace.numel(), error)
+    return out
+
+
+def copy_pages(pages, pairs, error_flag=None, stream=None):
+    """Copy page pairs[i, 0] over page pairs[i, 1] in every plane of ``pages``.
+
+    ``pages``: a contiguous pool [layers, 2, pages, ...] (or [planes, pages,
+    ...] with ``pages.dim()`` 4 or less); ``pairs``: int32 [n, 2].  The pairs
+    are copied in no order: no destination may occur twice or be another
+    pair's source.  A negative page marks padding; one outside the pool
+    leaves its pair out and flags PAGED_ERANGE.  Returns ``pages``."""
+
+    device = _gpu_of("pages", pages)
+    if not pages.is_contiguous():
+        raise ValueError("pages must be contiguous")
+    if pages.dim() < 3:
+        raise ValueError("pages must be [layers, 2, pages, ...] or [planes, pages, ...]")
+    lead = 2 if pages.dim() >= 5 else 1
+    count = pages.shape[lead]
+    planes = 1
+    for size in pages.shape[:lead]:
+        planes *= size
+    _placed(device, "pairs", pairs, torch.int32, 2)
+    if pairs.shape[1] != 2 or not pairs.is_contiguous():
+        raise ValueError("pairs must be contiguous [n, 2]")
+    error = _error_word(device, error_flag)
+    if pairs.shape[0] == 0 or pages.numel() == 0:
+        return pages
+    plane_bytes = pages.numel() * pages.element_size() // planes
+    _call_on(device, stream, "cascade_copy_pages", pages.data_ptr(), planes,
+             plane_bytes, count, plane_bytes // count, pairs.data_ptr(),
+             pairs.shape[0], error)
+    return pages
+
+
+def sample_workspace_bytes(rows, vocab):
+    """Workspace bytes of sample for up to ``rows`` rows of ``vocab`` logits."""
+
+    size = load().cascade_sample_workspace_bytes(int(rows), int(vocab))
+    if size == 0:
+        raise ValueError("unsupported sampling shape (rows={}, vocab={})".format(
+            rows, vocab))
+    return int(size)
+
+
+def _setting(device, name, value, dtype, rows):
+    """(pointer, value) of a per-row tensor or one number for all rows."""
+
+    if not isinstance(value, torch.Tensor):
+        return 0, value
+    _placed(device, name, value, dtype, 1)
+    if value.shape[0] != rows or (rows > 1 and value.stride(0) != 1):
+        raise ValueError("{} must be contiguous with one value a row".format(name))
+    return value.data_ptr(), 0
+
+
+def sample(logits, uniform, ids, workspace, temperature=1.0, top_k=0, top_p=1.0,
+           min_p=0.0, logprobs=None, stream=None):
+    """Draw one token a row of fp32 ``logits`` [rows, vocab] into ``ids``
+    (int64 [rows], returned).
+
+    ``uniform``: fp32 [rows], a number in [0, 1) a row.  The settings apply in
+    the order temperature, top-k, top-p, min-p; each is a number, or a tensor
+    with one value a row (fp32; top_k int32).  temperature 0 takes the largest
+    logit; top_k 0, top_p 1 and min_p 0 are off.  ``logprobs`` (fp32 [rows])
+    receives the log-probability the token was drawn with.  A row with a NaN,
+    or with every token at -inf, yields -1 (and NaN).  ``workspace``:
+    sample_workspace_bytes(rows, vocab) uint8, one for calls that may
+    overlap."""
+
+    device = _gpu_of("logits", logits)
+    _placed(device, "logits", logits, torch.float32, 2)
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("the rows of logits must be contiguous")
+    row_stride = vocab if rows == 1 else logits.stride(0)
+    if row_stride < vocab:
+        raise ValueError("the rows of logits overlap")
+    for name, tensor, dtype in (("uniform", uniform, torch.float32),
+                                ("ids", ids, torch.int64),
+                                ("logprobs", logprobs, torch.float32)):
+        if tensor is None and name == "logprobs":
+            continue
+        _placed(device, name, tensor, dtype, 1)
+        if tensor.shape[0] != rows or (rows > 1 and tensor.stride(0) != 1):
+            raise ValueError("{} must be contiguous with one value a row".format(name))
+    t_ptr, t = _setting(device, "temperature", temperature, torch.float32, rows)
+    k_ptr, k = _setting(device, "top_k", top_k, torch.int32, rows)
+    p_ptr, p = _setting(device, "top_p", top_p, torch.float32, rows)
+    m_ptr, m = _setting(device, "min_p", min_p, torch.float32, rows)
+    _placed(device, "workspace", workspace, torch.uint8, 1)
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    if rows == 0:
+        return ids
+    _call_on(device, stream, "cascade_sample_f32", logits.data_ptr(),
+             row_stride, rows, vocab, uniform.data_ptr(), t_ptr,
+             float(t), k_ptr, int(k), p_ptr, float(p), m_ptr, float(m),
+             ids.data_ptr(), 0 if logprobs is None else logprobs.data_ptr(),
+             workspace.data_ptr(), workspace.numel())
+    return ids
 
 
 # ------------------------------------------------------------ copy pipeline

@@ -36,8 +36,11 @@ extern "C" {
    exports are gone.  3: cascade_decode_attention_fused_bf16 /
    _fused_at_bf16 added.  4: cascade_topk_f32 added.  5: the split-K
    workspace forms cascade_gemm_ws_bf16 / cascade_gemm_residual_ws_bf16 and
-   cascade_gemm_workspace_bytes added. */
-#define CASCADE_ABI_VERSION 5
+   cascade_gemm_workspace_bytes added.  6: the paged KV cache
+   (cascade_paged_append_bf16, cascade_paged_decode_attention_bf16,
+   cascade_paged_attention_workspace_bytes, cascade_copy_pages) and sampling
+   (cascade_sample_f32, cascade_sample_workspace_bytes) added. */
+#define CASCADE_ABI_VERSION 6
 
 /* Argument errors (no work enqueued). */
 #define CASCADE_EINVAL 1001     /* null pointer, bad size or count */
@@ -311,6 +314,85 @@ int cascade_prefill_attention_bf16(const void *q, const void *k_cache,
                                    int64_t head_dim, float scale, void *out,
                                    void *stream);
 
+/* ------------------------------------------------------- paged KV cache
+ * The KV cache of several sequences in pages of page_size consecutive
+ * positions (a power of two, 8..1024), so that sequences with a common
+ * beginning share its pages.  Page p of a layer's K (V) pool starts at
+ * k_pages (v_pages) + p * page_stride elements; KV head g of it g *
+ * page_head_stride further; its rows (head_dim elements each) are
+ * contiguous.  Row s of page_table (table_stride entries apart) lists the
+ * pages of sequence s in order.  Entries, positions, lengths and row numbers
+ * are device int32: what is out of range forms no address, is left out as
+ * described below, and ors CASCADE_PAGED_ERANGE into *error_flag (a device
+ * int32, nullable).  Strides are in elements, multiples of 8.  No
+ * counterpart in the reference, whose cache holds one request
+ * (layer_streaming/llama31.py:34-54).                                      */
+#define CASCADE_PAGED_ERANGE 8
+/* Rotary positions and the cache write of `tokens` projected rows.  Token t
+ * sits at position positions[t] of table row rows[t] (rows null: row t).
+ * q (head h of token t at q + t * q_token_stride + h * q_head_stride; n_q_heads
+ * may be 0) is rotated into q_out, which may be q itself; k is rotated and v
+ * copied into the token's page row.  The first rope_dim dims of a head (a
+ * multiple of 16; 0: no rotation, null tables) are rotated by row
+ * positions[t] of rope_cos / rope_sin (bf16 [rope_positions, rope_dim / 2]):
+ * dims (i, i + rope_dim / 2) pair up, or with `interleaved` dims (2 i,
+ * 2 i + 1); fp32 arithmetic, one rounding.  head_dim: a multiple of 16, at
+ * most 1024.  A negative position or row is a padding token: nothing of it
+ * is written, and no error.  A token whose position is outside the table
+ * row, the rope tables or whose page is outside [0, num_pages) is left out
+ * whole and flagged.  Two tokens at one position of one row leave either's
+ * values there.  Does for pages what cascade_qkv_rope_bf16 does for the
+ * contiguous cache (llama31.py:44-50, :206-212).                           */
+int cascade_paged_append_bf16(
+    const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
+    int64_t k_token_stride, int64_t k_head_stride, const void *v,
+    int64_t v_token_stride, int64_t v_head_stride, int64_t tokens,
+    int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+    const int32_t *positions, const int32_t *rows, const int32_t *page_table,
+    int64_t table_stride, int64_t sequences, int64_t max_pages,
+    const void *rope_cos, const void *rope_sin, int64_t rope_positions,
+    int64_t rope_dim, int interleaved, void *q_out, int64_t q_out_token_stride,
+    int64_t q_out_head_stride, void *k_pages, void *v_pages, int64_t page_stride,
+    int64_t page_head_stride, int64_t num_pages, int64_t page_size,
+    int32_t *error_flag, void *stream);
+/* GQA attention of one query token a sequence: batch row b reads positions
+ * [0, lengths[r]) of table row r = rows[b] (rows null: r = b):
+ *   out[b, h] = bf16(softmax(q[b, h] . K_g^T * scale) . V_g), g = h / G,
+ * G = n_q_heads / n_kv_heads <= 16, head_dim 64 or 128.  A length of 0
+ * gives zeros.  max_length bounds the lengths (a longer one is flagged and
+ * cut to it); the table rows hold at least ceil(max_length / page_size)
+ * entries.  A negative rows[b] is a padding row: out[b] stays as it is.  A row
+ * number >= sequences is flagged and leaves out[b] too.  Positions on a
+ * page outside [0, num_pages) are left out as if masked, and flagged.
+ * The workspace needs no zero-fill and holds nothing between calls; calls
+ * that may overlap need one each.
+ * Does for pages what cascade_decode_attention_at_bf16 does for the
+ * contiguous cache (llama31.py:213-234).                                   */
+size_t cascade_paged_attention_workspace_bytes(int64_t batch, int64_t n_q_heads,
+                                               int64_t n_kv_heads,
+                                               int64_t head_dim,
+                                               int64_t max_length);
+int cascade_paged_decode_attention_bf16(
+    const void *q, int64_t q_token_stride, int64_t q_head_stride,
+    const void *k_pages, const void *v_pages, int64_t page_stride,
+    int64_t page_head_stride, int64_t num_pages, int64_t page_size,
+    const int32_t *page_table, int64_t table_stride, int64_t sequences,
+    const int32_t *lengths, const int32_t *rows, int64_t batch, int64_t max_length,
+    int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim, float scale,
+    void *out, int64_t out_token_stride, int64_t out_head_stride, void *workspace,
+    size_t workspace_bytes, int32_t *error_flag, void *stream);
+/* Copies page pairs[2 i] over page pairs[2 i + 1] (device int32) in each of
+ * `planes` planes (the K and V pools of every layer: page p of plane j at
+ * pages + j * plane_bytes + p * page_bytes; both multiples of 16 bytes).  A
+ * pair with a negative page is padding; a page >= num_pages is flagged and
+ * its pair left out.  The pairs are copied in no order: no destination may
+ * occur twice or be another pair's source (a fork's and a compaction's
+ * copies never do).                                                        */
+int cascade_copy_pages(void *pages, int64_t planes, int64_t plane_bytes,
+                       int64_t num_pages, int64_t page_bytes,
+                       const int32_t *pairs, int64_t count, int32_t *error_flag,
+                       void *stream);
+
 /* ------------------------------------------------------ LM head + top-k
  * One vocabulary chunk: logits[r] = W[r] . h (fp32, not rounded to bf16) for
  * rows r < rows, then an exact running top-k over everything seen since the
@@ -342,6 +424,35 @@ int cascade_lm_head_topk_bf16(const void *w, int64_t rows, int64_t k,
 int cascade_topk_f32(const float *logits, int64_t rows, int64_t top_k,
                      void *workspace, size_t workspace_bytes,
                      float *out_values, int64_t *out_indices, void *stream);
+
+/* ------------------------------------------------------------- sampling
+ * One token a row of fp32 logits (row r at logits + r * row_stride, vocab <=
+ * 2^19 of them), drawn by inversion with uniform[r] in [0, 1) (values
+ * outside are taken as the nearest inside, NaN as 0):
+ *   w_i = exp((x_i - max x) / T);  K = the top_k largest x (of equal ones
+ *   the lowest indices);  P = the shortest run of K, largest first, whose mass
+ *   reaches top_p * mass(K);  S = the i of P with w_i >= min_p (the likeliest
+ *   always stays);  ids[r] = the first i of S, by index, at which the mass
+ *   of S exceeds uniform * mass(S);  logprobs[r] (nullable) = log(w_i / mass(S)).
+ * Each setting is a device array with a value per row or, where that is
+ * null, the value given for all.  T <= 0 takes the largest logit (lowest
+ * index, log-probability 0); top_k <= 0, top_p >= 1 and min_p <= 0 are off.
+ * Weights are fp64 rounded to multiples of 2^-44 of the largest and summed
+ * exactly.  -inf is never drawn; a row with a NaN, or of nothing but -inf,
+ * yields id -1 and a NaN log-probability.  The workspace
+ * (cascade_sample_workspace_bytes, 0 for an unsupported shape) needs no
+ * zero-fill and holds nothing between calls.  Stands beside the greedy
+ * torch.topk(...)[..., 0] of the reference's token loop
+ * (tools/run_llama31.py:105-121), which has no sampling.                   */
+size_t cascade_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int cascade_sample_f32(const float *logits, int64_t row_stride, int64_t rows,
+                       int64_t vocab, const float *uniform,
+                       const float *temperature, double temperature_value,
+                       const int32_t *top_k, int64_t top_k_value,
+                       const float *top_p, double top_p_value,
+                       const float *min_p, double min_p_value, int64_t *ids,
+                       float *logprobs, void *workspace, size_t workspace_bytes,
+                       void *stream);
 
 /* ----------------------------------------------------------- embedding
  * out[i, :] = table[ids[i], :] for i < n_ids (ids are int64 on the device).

@@ -1,0 +1,154 @@
+"""Sampling against its plain 64-bit form: the same token for every setting,
+and its log-probability; ties, masks, infinities, NaN, settings per row, and
+row lengths around the kernel's tiles."""
+
+import math
+
+import pytest
+import torch
+
+from layer_streaming import _hip
+from paged_cases import sample as plain
+
+pytestmark = pytest.mark.gpu
+
+
+def draw(logits, uniform, device, **settings):
+    rows, vocab = logits.shape
+    ids = torch.full((rows,), -9, dtype=torch.int64, device=device)
+    logprobs = torch.full((rows,), 9.0, device=device)
+    ws = torch.full((_hip.sample_workspace_bytes(rows, vocab),), 0xFF, dtype=torch.uint8,
+                    device=device)
+    placed = {k: v.to(device) if isinstance(v, torch.Tensor) else v
+              for k, v in settings.items()}
+    got = _hip.sample(logits.to(device), uniform.to(device), ids, ws, logprobs=logprobs,
+                      **placed)
+    assert got is ids
+    torch.cuda.synchronize(device)
+    return ids.cpu(), logprobs.cpu()
+
+
+def check(logits, uniform, device, **settings):
+    ids, logprobs = draw(logits, uniform, device, **settings)
+    for r in range(logits.shape[0]):
+        mine = {k: v[r].item() if isinstance(v, torch.Tensor) else v
+                for k, v in settings.items()}
+        token, logprob, weight = plain(logits[r], uniform[r], **mine)
+        assert int(ids[r]) == token, (r, mine, int(ids[r]), token)
+        got = float(logprobs[r])
+        if math.isnan(logprob):
+            assert math.isnan(got)
+            continue
+        # one rounding to fp32; weights are multiples of 2^-44 of the largest
+        # (half a step of the token's own, and of each of the sum's)
+        tol = 2.0 ** -24 * abs(logprob) + 2.0 ** -45 / weight + logits.shape[1] * 2.0 ** -45
+        assert abs(got - logprob) <= tol, (r, mine, got, logprob)
+
+
+SETTINGS = [dict(), dict(temperature=0.0), dict(top_k=1), dict(top_k=5), dict(top_k=100000),
+            dict(top_p=0.0), dict(top_p=0.4), dict(top_p=0.999), dict(min_p=0.05),
+            dict(min_p=1.0), dict(min_p=7.0), dict(temperature=0.3, top_k=40, top_p=0.9),
+            dict(temperature=1.7, top_k=200, top_p=0.7, min_p=0.02),
+            dict(temperature=0.01), dict(temperature=100.0, top_p=0.5),
+            dict(temperature=2.0, top_k=700, top_p=0.99)]
+
+
+@pytest.mark.parametrize("settings", SETTINGS, ids=str)
+@pytest.mark.parametrize("vocab", [1, 2, 63, 1000, 1025, 8193])
+def test_settings(gpu_device, vocab, settings):
+    print("sample", vocab, settings, flush=True)
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randn(4, vocab, generator=g) * 3
+    uniform = torch.tensor([0.0, 0.3, 0.77, 1.0 - 2.0 ** -24])
+    check(logits, uniform, gpu_device, **settings)
+
+
+@pytest.mark.parametrize("settings", SETTINGS[2:], ids=str)
+def test_ties(gpu_device, settings):
+    # few distinct values, both zeros, runs of one value over many tiles
+    g = torch.Generator().manual_seed(7)
+    logits = (torch.randn(5, 5000, generator=g) * 2).round() / 2
+    logits[0, logits[0] == 0] = -0.0
+    logits[1] = 0.25
+    logits[2, 10:] = -3.0
+    logits[3, ::2] = -math.inf
+    check(logits, torch.rand(5, generator=g), gpu_device, **settings)
+
+
+def test_masks_infinities_and_nan(gpu_device):
+    g = torch.Generator().manual_seed(8)
+    logits = torch.randn(9, 3000, generator=g) * 4
+    low = torch.finfo(torch.float32).min
+    logits[0] = -math.inf                      # nothing left
+    logits[1, :] = -math.inf
+    logits[1, 1234] = -50.0                    # one token left
+    logits[2] = low                            # all at the type's lowest value
+    logits[3, 1:] = low
+    logits[4, 77] = math.nan
+    logits[5, [5, 900]] = math.inf             # two certain tokens
+    logits[6, :2999] = -math.inf
+    logits[7, 100:] = -math.inf
+    logits[8] *= 1e30
+    uniform = torch.tensor([0.1, 0.9, 0.5, 0.999, 0.2, 0.7, 0.0, 0.6, 0.4])
+    for settings in (dict(), dict(top_k=3), dict(top_p=0.5), dict(min_p=0.5),
+                     dict(temperature=0.0), dict(temperature=0.5, top_k=50, top_p=0.9)):
+        check(logits, uniform, gpu_device, **settings)
+    ids, logprobs = draw(logits, uniform, gpu_device)
+    assert ids[0] == -1 and ids[4] == -1
+    assert math.isnan(float(logprobs[0])) and math.isnan(float(logprobs[4]))
+
+
+def test_uniform_outside_is_taken_as_the_nearest_inside(gpu_device):
+    logits = torch.randn(5, 400, generator=torch.Generator().manual_seed(9))
+    uniform = torch.tensor([-1.0, 1.0, 5.0, math.inf, math.nan])
+    ids, _ = draw(logits, uniform, gpu_device)
+    assert ids.tolist() == [0, 399, 399, 399, 0]
+
+
+def test_settings_per_row(gpu_device):
+    g = torch.Generator().manual_seed(10)
+    rows, vocab = 23, 4097
+    logits = torch.randn(rows, vocab, generator=g) * 2.5
+    settings = dict(
+        temperature=torch.where(torch.rand(rows, generator=g) < 0.2, 0.0,
+                                0.2 + torch.rand(rows, generator=g)),
+        top_k=torch.randint(-1, 60, (rows,), generator=g, dtype=torch.int32),
+        top_p=0.2 + torch.rand(rows, generator=g), min_p=torch.rand(rows, generator=g) * 0.1)
+    check(logits, torch.rand(rows, generator=g), gpu_device, **settings)
+    # and mixed with one number for all
+    settings["temperature"] = 0.9
+    settings["top_k"] = 0
+    check(logits, torch.rand(rows, generator=g), gpu_device, **settings)
+
+
+@pytest.mark.parametrize("vocab", [32000, 128256])
+def test_whole_vocabularies(gpu_device, vocab):
+    print("sample", vocab, flush=True)
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randn(3, vocab, generator=g) * 2.2
+    logits[1] = logits[1].to(torch.bfloat16).float()  # many ties
+    wide = torch.full((3, vocab + 5), math.nan)
+    wide[:, :vocab] = logits
+    uniform = torch.rand(3, generator=g)
+    for settings in (dict(temperature=0.8, top_k=40, top_p=0.95), dict(), dict(top_p=0.99),
+                     dict(temperature=1.5, top_k=20000, top_p=0.9, min_p=0.001)):
+        check(logits, uniform, gpu_device, **settings)
+        a, _ = draw(logits, uniform, gpu_device, **settings)
+        ids = torch.empty(3, dtype=torch.int64, device=gpu_device)
+        ws = torch.empty(_hip.sample_workspace_bytes(3, vocab), dtype=torch.uint8,
+                         device=gpu_device)
+        _hip.sample(wide.to(gpu_device)[:, :vocab], uniform.to(gpu_device), ids, ws,
+                    **settings)
+        assert torch.equal(a, ids.cpu())
+
+
+def test_frequencies(gpu_device):
+    # evenly spaced uniforms: each token's count is its probability, to one
+    # draw either way
+    n = 4096
+    logits = torch.tensor([0.5, -1.0, 2.0, -math.inf, 1.0, 0.0, -2.0])
+    uniform = (torch.arange(n) + 0.5) / n
+    ids, _ = draw(logits.repeat(n, 1), uniform, gpu_device, temperature=1.3)
+    p = torch.softmax(logits.double() / 1.3, 0)
+    counts = torch.bincount(ids, minlength=7)
+    assert bool(((counts - p * n).abs() <= 1.0).all())
