@@ -148,26 +148,124 @@ struct PagedAttnArgs {
   int64_t sequences;
   const int32_t *lengths;
   const int32_t *rows;  // nullable: batch row b reads table row b
+  int32_t batch;
   int32_t max_length;
+  int32_t kv_heads;
   int32_t group;  // query heads a KV head, at most 16
   float scale_log2;
   uint16_t *out;  // [batch, q_heads, dim]
   int64_t out_token, out_head;
   int32_t *error;
+  // split runs (SPLIT kernels): see "Runs"
+  int32_t target;   // runs wanted
+  int32_t *plan;    // [batch][2]: first run of a batch row, and how many
+  float *part_ml;   // [run][q_heads][2]: maximum (log2 units), sum
+  float *part_acc;  // [run][q_heads][D]
 };
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kPagedWaves = 4;
 constexpr int kPagedBlock = 32;  // positions a wave step
 constexpr int kPagedGroup = 16;  // MFMA columns
+constexpr int kPagedMinRun = 4;  // blocks
+constexpr int kPagedMaxBatch = 1024;  // of a split launch
+constexpr int kPagedTarget = 1024;    // workgroups wanted of one
+constexpr size_t kPagedAlign = 256;
 
 __device__ __forceinline__ float paged_exp2(float x) {
   return __builtin_amdgcn_exp2f(x);
 }
 
-// One workgroup per (batch row, KV head); each wave runs an online softmax
-// over every fourth block of 32 positions and the waves merge in LDS.  The
-// products are v_mfma_f32_16x16x32_bf16 with the query heads of the KV head
-// as columns (zeros past group):
+// Table row and length of batch row b.  row < 0: nothing to do.
+struct PagedRow {
+  int64_t row;
+  int32_t len;
+};
+
+__device__ __forceinline__ PagedRow paged_row(const PagedAttnArgs &a, int b, bool flag) {
+  PagedRow r{-1, 0};
+  if (b >= a.batch) return r;
+  r.row = a.rows != nullptr ? a.rows[b] : b;
+  if (r.row >= a.sequences) {
+    if (flag) flag_range(a.error);
+    r.row = -1;
+  }
+  if (r.row < 0) return r;
+  r.len = a.lengths[r.row];
+  if (r.len < 0 || r.len > a.max_length) {
+    if (flag) flag_range(a.error);
+    r.len = min(max(r.len, 0), a.max_length);
+  }
+  return r;
+}
+
+// Runs.  The lengths are on the device, so the launch is sized for any of
+// them and each workgroup finds its own piece of work: the blocks of 32
+// positions of all batch rows are cut into runs of `size` blocks,
+//   size = max(kPagedMinRun, ceil(blocks of all rows / target)),
+// a multiple of the workgroup's waves, and row b gets max(1, ceil(blocks_b /
+// size)) runs, numbered through the batch.  There are at most target + batch
+// runs whatever the lengths, all but a row's last of one size, so a ragged
+// batch and a single long sequence both fill the device.  Every wave works
+// this out for itself from the lengths (64 rows at a time), with no barrier.
+struct PagedRun {
+  int b;      // batch row; -1: no such run
+  int64_t row;
+  int len;
+  int first;  // blocks [first, end) of the row
+  int end;
+  int index;  // number of the row's first run
+  int count;  // runs of the row
+};
+
+__device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, int lane,
+                                             bool flag) {
+  uint64_t blocks = 0;
+  for (int base = 0; base < a.batch; base += kWave)
+    blocks += static_cast<uint32_t>((paged_row(a, base + lane, flag).len + kPagedBlock - 1) /
+                                    kPagedBlock);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) blocks += __shfl_xor(blocks, d);
+  uint64_t want = (blocks + a.target - 1) / a.target;
+  want = (want + kPagedWaves - 1) / kPagedWaves * kPagedWaves;
+  // (no row has more than 2^26 blocks)
+  const int size = static_cast<int>(
+      min(max(want, static_cast<uint64_t>(kPagedMinRun)), uint64_t{1} << 26));
+  int before = 0;
+  for (int base = 0; base < a.batch; base += kWave) {
+    const PagedRow r = paged_row(a, base + lane, false);
+    const int nb = (r.len + kPagedBlock - 1) / kPagedBlock;
+    const int mine = r.row < 0 ? 0 : max(1, (nb + size - 1) / size);
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
+    }
+    upto += before;
+    const uint64_t past = __ballot(upto > run);
+    if (past != 0) {
+      const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      PagedRun out;
+      out.b = base + at;
+      out.row = __shfl(r.row, at);
+      out.len = __shfl(r.len, at);
+      out.count = __shfl(mine, at);
+      out.index = __shfl(upto, at) - out.count;
+      out.first = (run - out.index) * size;
+      out.end = min(out.first + size, (out.len + kPagedBlock - 1) / kPagedBlock);
+      return out;
+    }
+    before = __shfl(upto, kWave - 1);
+  }
+  return PagedRun{-1, -1, 0, 0, 0, 0, 0};
+}
+
+// Workgroup (run, KV head), or (batch row, KV head) without SPLIT; each wave
+// runs an online softmax over every fourth block of 32 positions and the
+// waves merge in LDS.  The products are v_mfma_f32_16x16x32_bf16 with the
+// query heads of the KV head as columns (zeros past group):
 //   S = K_blk q^T    two 16-row tiles x D / 32 chunks
 //   O += V_blk^T P   D / 16 tiles, K = the 32 positions
 // Lane (c, g4) = (l % 16, l / 16) owns the scores of head c at rows
@@ -177,31 +275,44 @@ __device__ __forceinline__ float paged_exp2(float x) {
 // Scores carry scale * log2(e).  The running maximum starts at -FLT_MAX, so
 // a block whose rows are all left out keeps it and adds nothing; a sequence
 // with no row at all ends with a zero sum and writes zeros.
-template <int D>
+template <int D, bool SPLIT>
 __global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
     PagedAttnArgs a) {
   constexpr int DV = D / 16;  // dims a lane holds of a V row
   constexpr int KC = D / 32;  // 32-dim chunks
   __shared__ float s_ml[kPagedWaves][kPagedGroup][2];
   __shared__ float s_acc[kPagedWaves][kPagedGroup][D];
-  const int b = blockIdx.x;
-  const int g = blockIdx.y;
+  const int g = static_cast<int>(blockIdx.x) % a.kv_heads;
+  const int run = static_cast<int>(blockIdx.x) / a.kv_heads;
   const int G = a.group;
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
   const int wave = tid / kWave;
   const int c16 = lane & 15;
   const int g4 = lane >> 4;
-  const int64_t row = a.rows != nullptr ? a.rows[b] : b;
-  if (row < 0) return;  // a padding row
-  if (row >= a.sequences) {
-    if (tid == 0) flag_range(a.error);
-    return;
-  }
-  int len = a.lengths[row];
-  if (len < 0 || len > a.max_length) {
-    if (tid == 0) flag_range(a.error);
-    len = min(max(len, 0), a.max_length);
+  int b, len, first, end, count = 1;
+  int64_t row;
+  if constexpr (SPLIT) {
+    const PagedRun r = find_run(a, run, lane, blockIdx.x == 0 && wave == 0);
+    if (r.b < 0) return;
+    b = r.b;
+    row = r.row;
+    len = r.len;
+    first = r.first;
+    end = r.end;
+    count = r.count;
+    if (run == r.index && g == 0 && tid == 0) {
+      a.plan[2 * b] = run;
+      a.plan[2 * b + 1] = count;
+    }
+  } else {
+    b = run;
+    const PagedRow r = paged_row(a, b, g == 0 && tid == 0);
+    if (r.row < 0) return;
+    row = r.row;
+    len = r.len;
+    first = 0;
+    end = (len + kPagedBlock - 1) / kPagedBlock;
   }
   const int last = len - 1;
   const int32_t *table = a.table + row * a.table_stride;
@@ -223,52 +334,49 @@ __global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
 #pragma unroll
   for (int e = 0; e < DV; ++e) o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  for (int r0 = wave * kPagedBlock; r0 < len; r0 += kPagedWaves * kPagedBlock) {
-    // K tile rows 8 (i / 4) + i % 4 + 4 hf: group i / 4 of eight; rows past
-    // the end repeat the last row
-    const int kg = min(r0 + 8 * (c16 >> 2), last);
-    const int vg = min(r0 + 8 * g4, last);
-    int kpage = table[kg >> a.page_shift];
-    int vpage = table[vg >> a.page_shift];
+  // A lane reads K rows of group c16 / 4 of eight of a block and V rows of
+  // group g4; a group lies in one page.  Groups past the end take the last
+  // row's page: its rows are memory of the pool whatever they hold.
+  auto pages_of = [&](int blk, int &kpage, int &vpage) {
+    kpage = table[min(blk * kPagedBlock + 8 * (c16 >> 2), last) >> a.page_shift];
+    vpage = table[min(blk * kPagedBlock + 8 * g4, last) >> a.page_shift];
+  };
+  int kpage = 0, vpage = 0;
+  if (first + wave < end) pages_of(first + wave, kpage, vpage);
+  for (int blk = first + wave; blk < end; blk += kPagedWaves) {
+    const int r0 = blk * kPagedBlock;
     const bool vbad = vpage < 0 || vpage >= a.num_pages;
     if (kpage < 0 || kpage >= a.num_pages) kpage = 0;
     if (vbad) {
       vpage = 0;
       flag_range(a.error);
     }
-    const uint16_t *kp = kb + kpage * a.page_stride;
-    const uint16_t *vp = vb + vpage * a.page_stride;
+    // K tile row i is block row 8 (i / 4) + i % 4 + 4 hf
+    const uint16_t *kp = kb + kpage * a.page_stride +
+                         (((r0 + 8 * (c16 >> 2)) & page_mask) + (c16 & 3)) * D + 8 * g4;
+    const uint16_t *vp = vb + vpage * a.page_stride + ((r0 + 8 * g4) & page_mask) * D + DV * c16;
     u32x4 kt[2][KC];
     uint32_t vt[8][DV / 2];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int r = min(r0 + 8 * (c16 >> 2) + (c16 & 3) + 4 * hf, last) & page_mask;
+    for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
       for (int c = 0; c < KC; ++c)
         kt[hf][c] = __builtin_nontemporal_load(
-            reinterpret_cast<const u32x4 *>(kp + r * D + 32 * c + 8 * g4));
-    }
+            reinterpret_cast<const u32x4 *>(kp + 4 * hf * D + 32 * c));
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int r = min(r0 + 8 * g4 + j, last) & page_mask;
-      const uint32_t *src = reinterpret_cast<const uint32_t *>(vp + r * D + DV * c16);
       if constexpr (DV == 8) {
-        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src));
+        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vp + j * D));
 #pragma unroll
         for (int i = 0; i < 4; ++i) vt[j][i] = x[i];
       } else {
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(src));
+        const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(vp + j * D));
         vt[j][0] = x[0];
         vt[j][1] = x[1];
       }
     }
-    if (vbad) {  // what another sequence's page holds takes no part, NaN neither
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < DV / 2; ++i) vt[j][i] = 0u;
-    }
+    // the next block's pages, while this one's rows are on their way
+    if (blk + kPagedWaves < end) pages_of(blk + kPagedWaves, kpage, vpage);
     f32x4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
@@ -300,6 +408,16 @@ __global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
     if (alpha != 1.0f) {
 #pragma unroll
       for (int e = 0; e < DV; ++e) o[e] *= alpha;
+    }
+    if (r0 + kPagedBlock > len || __any(vbad)) {
+      // rows past the end, or of another sequence's page, take no part
+      // whatever they hold: 0 times a NaN would be one
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool out = vbad || r0 + 8 * g4 + j >= len;
+#pragma unroll
+        for (int i = 0; i < DV / 2; ++i) vt[j][i] = out ? 0u : vt[j][i];
+      }
     }
 #pragma unroll
     for (int e = 0; e < DV; ++e) {
@@ -338,9 +456,99 @@ __global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
       den = fmaf(wt, s_ml[w][h][1], den);
       r = fmaf(wt, s_acc[w][h][d], r);
     }
-    a.out[b * a.out_token + (g * G + h) * a.out_head + d] =
-        f32_to_bf16(den == 0.0f ? 0.0f : r / den);
+    if (!SPLIT || count == 1) {
+      a.out[b * a.out_token + (g * G + h) * a.out_head + d] =
+          f32_to_bf16(den == 0.0f ? 0.0f : r / den);
+    } else {
+      const int64_t slot = static_cast<int64_t>(run) * (a.kv_heads * G) + g * G + h;
+      a.part_acc[slot * D + d] = r;
+      if (d == 0) {
+        a.part_ml[2 * slot] = mm;
+        a.part_ml[2 * slot + 1] = den;
+      }
+    }
   }
+}
+
+// Joins the runs of one (batch row, query head):
+//   out = sum_r 2^(m_r - M) acc_r / sum_r 2^(m_r - M) l_r,  M = max_r m_r.
+// Wave-sized slices of the workgroup take every kMergeSlices-th run each, in
+// order, and add up in LDS.  Rows of one run were written already.
+constexpr int kPagedMergeThreads = 512;
+
+template <int D>
+__global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(PagedAttnArgs a) {
+  constexpr int kSlices = kPagedMergeThreads / D;
+  __shared__ float s_max[kPagedMergeThreads / kWave];
+  __shared__ float s_acc[kSlices][D];
+  __shared__ float s_den[kSlices];
+  const int heads = a.kv_heads * a.group;
+  const int b = static_cast<int>(blockIdx.x) / heads;
+  const int h = static_cast<int>(blockIdx.x) % heads;
+  const int tid = threadIdx.x;
+  if (paged_row(a, b, false).row < 0) return;
+  const int index = a.plan[2 * b], count = a.plan[2 * b + 1];
+  if (count <= 1) return;
+  const int64_t base = static_cast<int64_t>(index) * heads + h;
+  float mm = -FLT_MAX;
+  for (int r = tid; r < count; r += kPagedMergeThreads)
+    mm = fmaxf(mm, a.part_ml[2 * (base + static_cast<int64_t>(r) * heads)]);
+  mm = wave_max(mm);
+  if ((tid & (kWave - 1)) == 0) s_max[tid / kWave] = mm;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPagedMergeThreads / kWave; ++w) mm = fmaxf(mm, s_max[w]);
+  const int slice = tid / D;
+  const int d = tid % D;
+  float den = 0.0f, acc = 0.0f;
+#pragma unroll 4
+  for (int r = slice; r < count; r += kSlices) {
+    const int64_t slot = base + static_cast<int64_t>(r) * heads;
+    const float w = paged_exp2(a.part_ml[2 * slot] - mm);
+    den = fmaf(w, a.part_ml[2 * slot + 1], den);
+    acc = fmaf(w, a.part_acc[slot * D + d], acc);
+  }
+  s_acc[slice][d] = acc;
+  if (d == 0) s_den[slice] = den;
+  __syncthreads();
+  if (slice == 0) {
+#pragma unroll
+    for (int k = 1; k < kSlices; ++k) {
+      acc += s_acc[k][d];
+      den += s_den[k];
+    }
+    a.out[b * a.out_token + h * a.out_head + d] =
+        f32_to_bf16(den == 0.0f ? 0.0f : acc / den);
+  }
+}
+
+// Whether a launch splits, and its sizes.  Rows of at most one shortest run
+// need none; past kPagedMaxBatch rows every wave's walk over the lengths would
+// cost more than the balance is worth, and the rows fill the device.
+struct PagedPlan {
+  bool split;
+  int64_t target;
+  int64_t runs;  // at most
+  size_t plan_bytes, ml_bytes, acc_bytes;
+};
+
+static PagedPlan paged_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                            int64_t max_length) {
+  PagedPlan p{};
+  const int64_t blocks = (max_length + kPagedBlock - 1) / kPagedBlock;
+  p.split = blocks > kPagedMinRun && batch <= kPagedMaxBatch;
+  if (!p.split) return p;
+  p.target = (kPagedTarget + kv_heads - 1) / kv_heads;
+  p.runs = p.target + batch;
+  const int64_t most = batch * ((blocks + kPagedMinRun - 1) / kPagedMinRun);
+  if (p.runs > most) p.runs = most;
+  auto rounded = [](int64_t bytes) {
+    return (static_cast<size_t>(bytes) + kPagedAlign - 1) / kPagedAlign * kPagedAlign;
+  };
+  p.plan_bytes = rounded(batch * 8);
+  p.ml_bytes = rounded(p.runs * q_heads * 8);
+  p.acc_bytes = rounded(p.runs * q_heads * dim * 4);
+  return p;
 }
 
 // ----------------------------------------------------------------- copies
@@ -494,7 +702,8 @@ extern "C" size_t cascade_paged_attention_workspace_bytes(int64_t batch,
       n_q_heads / n_kv_heads > kPagedGroup || (head_dim != 64 && head_dim != 128) ||
       max_length <= 0 || max_length > 0x7fffffff - 64)
     return 0;
-  return 256;
+  const PagedPlan p = paged_plan(batch, n_q_heads, n_kv_heads, head_dim, max_length);
+  return kPagedAlign + p.plan_bytes + p.ml_bytes + p.acc_bytes;
 }
 
 extern "C" int cascade_paged_decode_attention_bf16(
@@ -510,12 +719,12 @@ extern "C" int cascade_paged_decode_attention_bf16(
       page_table == nullptr || lengths == nullptr || out == nullptr ||
       workspace == nullptr)
     return CASCADE_EINVAL;
-  if (batch <= 0 || batch > 0xffff || n_kv_heads <= 0 || sequences <= 0 ||
+  if (batch <= 0 || batch > 0x7fffffff || n_kv_heads <= 0 || sequences <= 0 ||
       num_pages <= 0 || num_pages > 0x7fffffff || max_length <= 0)
     return CASCADE_EINVAL;
   PagedAttnArgs a{};
   if ((head_dim != 64 && head_dim != 128) || n_q_heads <= 0 || n_q_heads % n_kv_heads ||
-      n_q_heads / n_kv_heads > kPagedGroup || n_kv_heads > 0xffff ||
+      n_q_heads / n_kv_heads > kPagedGroup || n_kv_heads > 0xffff || batch * n_q_heads > 0x7fffffff ||
       !page_shift_of(page_size, &a.page_shift) || max_length > 0x7fffffff - 64)
     return CASCADE_ESHAPE;
   if (table_stride < (max_length + page_size - 1) / page_size ||
@@ -555,12 +764,34 @@ extern "C" int cascade_paged_decode_attention_bf16(
   a.out_token = out_token_stride;
   a.out_head = out_head_stride;
   a.error = error_flag;
-  const dim3 grid(static_cast<unsigned>(batch), static_cast<unsigned>(n_kv_heads));
+  a.batch = static_cast<int32_t>(batch);
+  a.kv_heads = static_cast<int32_t>(n_kv_heads);
+  const PagedPlan p = paged_plan(batch, n_q_heads, n_kv_heads, head_dim, max_length);
   const dim3 block(kPagedWaves * kWave);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (head_dim == 128)
-    return launch_kernel(paged_attention_kernel<128>, grid, block, 0, s, a);
-  return launch_kernel(paged_attention_kernel<64>, grid, block, 0, s, a);
+  if (!p.split) {
+    const dim3 grid(static_cast<unsigned>(batch * n_kv_heads));
+    return head_dim == 128
+               ? launch_kernel(paged_attention_kernel<128, false>, grid, block, 0, s, a)
+               : launch_kernel(paged_attention_kernel<64, false>, grid, block, 0, s, a);
+  }
+  unsigned char *ws = static_cast<unsigned char *>(workspace);
+  a.target = static_cast<int32_t>(p.target);
+  a.plan = reinterpret_cast<int32_t *>(ws);
+  a.part_ml = reinterpret_cast<float *>(ws + p.plan_bytes);
+  a.part_acc = reinterpret_cast<float *>(ws + p.plan_bytes + p.ml_bytes);
+  const dim3 grid(static_cast<unsigned>(p.runs * n_kv_heads));
+  const dim3 merge(static_cast<unsigned>(batch * n_q_heads));
+  const dim3 merge_block(kPagedMergeThreads);
+  if (head_dim == 128) {
+    const hipError_t e =
+        launch_kernel(paged_attention_kernel<128, true>, grid, block, 0, s, a);
+    if (e != hipSuccess) return e;
+    return launch_kernel(paged_merge_kernel<128>, merge, merge_block, 0, s, a);
+  }
+  const hipError_t e = launch_kernel(paged_attention_kernel<64, true>, grid, block, 0, s, a);
+  if (e != hipSuccess) return e;
+  return launch_kernel(paged_merge_kernel<64>, merge, merge_block, 0, s, a);
 }
 
 extern "C" int cascade_copy_pages(void *pages, int64_t planes, int64_t plane_bytes,
