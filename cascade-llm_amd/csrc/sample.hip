@@ -12,9 +12,21 @@
 // computed in fp64 and rounded once to a multiple of 2^-44 (a 64-bit integer;
 // the 2^19 logits a row may hold sum to less than 2^64), and integer sums do
 // not depend on their order, so neither does the token on how the row was
-// cut up.  A token below 2^-45 of the likeliest one is never drawn.  The
-// cuts K and P are found by counting: histograms of 11 bits of the ordered
-// logits, from the top down.
+// cut up.  A token below 2^-45 of the likeliest one is never drawn.
+//
+// Four launches cut a row into chunks, so that a few rows fill the device:
+//   1. sample_max_kernel     a chunk's largest logit
+//   2. sample_weigh_kernel   2048 bins of (x_i - max) / T, with the number
+//                            and the mass of their tokens (rows with a top-k
+//                            or top-p), or the chunk's mass (other rows)
+//   3. sample_collect_kernel the bins in which K and P end, from those sums;
+//                            their tokens go to a list, the mass of the
+//                            bins above is kept by chunk
+//   4. sample_draw_kernel    one workgroup a row: sorts the list, finds the
+//                            two ends in it, draws a chunk and then its token
+// A row whose list would be longer than kListMax (ends in runs of equal
+// logits) is instead cut by the last launch alone, which counts 11 bits of
+// the ordered logits at a time over the row.
 #include "cascade_device.h"
 #include "cascade_internal.h"
 
@@ -28,6 +40,14 @@ constexpr int kSampleBins = 2048;
 constexpr int kWeightBits = 44;
 constexpr u64 kWeightOne = u64{1} << kWeightBits;
 constexpr int64_t kSampleMaxVocab = int64_t{1} << 19;
+constexpr int kListMax = 4096;
+constexpr int kChunkThreads = 256;
+constexpr int kChunkStep = 4;  // logits a thread loads at once
+constexpr int kChunkMin = 2048;
+constexpr int kChunkMax = 16384;
+constexpr int kChunkWorkgroups = 512;  // wanted of a launch
+// bins per unit of log2 weight: 2048 bins hold the 45 units that count
+constexpr double kBinsPerLog2 = kSampleBins / 45.0;
 
 struct SampleArgs {
   const float *logits;
@@ -44,6 +64,29 @@ struct SampleArgs {
   double min_p_value;
   int64_t *ids;
   float *logprobs;  // nullable
+  // the row's cut into chunks, and the workspace (row r's part first)
+  int32_t chunk;
+  int32_t chunks;
+  u64 *chunk_max;   // [rows][chunks]: key of the largest logit
+  u64 *chunk_mass;  // [rows][chunks]
+  u64 *bin_mass;    // [rows][kSampleBins]
+  uint32_t *bin_count;
+  struct RowEnds *ends;  // [rows]
+  u64 *list;             // [rows][kListMax] keys
+  uint32_t *list_count;  // [rows]
+};
+
+// Where K and P end in the bins (bin 0 holds the largest logits).
+struct RowEnds {
+  u64 above_k;   // mass of the bins above K's last one
+  u64 above_p;   // and above P's first candidate
+  u64 total;     // mass of the row
+  uint32_t need_k;  // tokens that K takes of its last bin
+  uint32_t before;  // list entries in bins above K's last one
+  uint32_t entries; // list entries
+  int32_t first;    // bins first .. last_p, and last_k, are listed
+  int32_t last_p;   // -1: no top-p
+  int32_t last_k;   // -1: no top-k
 };
 
 struct RowSettings {
@@ -92,6 +135,13 @@ __device__ __forceinline__ u64 fixed_exp2(double y) {
   return static_cast<u64>(ldexp(p, static_cast<int>(n) + kWeightBits) + 0.5);
 }
 
+// Bin of logit x, which has a weight.
+__device__ __forceinline__ int weight_bin(float x, float mx, double scale) {
+  if (x == mx) return 0;
+  const double y = (static_cast<double>(x) - static_cast<double>(mx)) * scale;
+  return min(static_cast<int>(-y * kBinsPerLog2), kSampleBins - 1);
+}
+
 // Weight of logit x in a row whose largest logit is mx: 2^44 for the largest
 // itself (also where it is infinite), 0 for -inf.
 __device__ __forceinline__ u64 fixed_weight(float x, float mx, double scale) {
@@ -112,6 +162,7 @@ __device__ __forceinline__ u64 wave_prefix(u64 v, int lane) {
 
 // Inclusive prefix sum over the workgroup in thread order, and its total.
 // Two barriers; `lds` may be reused after the second.
+template <int WAVES = kSampleWaves>
 __device__ __forceinline__ u64 block_prefix(u64 v, u64 *lds, u64 *total) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = threadIdx.x / kWave;
@@ -120,7 +171,7 @@ __device__ __forceinline__ u64 block_prefix(u64 v, u64 *lds, u64 *total) {
   __syncthreads();
   u64 before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kSampleWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     const u64 s = lds[w];
     if (w < wave) before += s;
     all += s;
@@ -230,29 +281,347 @@ __device__ Cut find_cut(const float *x, int n, float mx, double scale, Cut in, u
   return cut;
 }
 
-// One workgroup a row.
-__global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a) {
-  __shared__ SampleShared sh;
-  const int row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const int n = a.vocab;
-  const float *x = a.logits + row * a.row_stride;
-  const RowSettings set = row_settings(a, row);
-
-  // the largest key (its logit, and the lowest index that has it); a NaN
-  // sorts above every number
+// Largest key of a row from its chunks'.  All threads return it.
+__device__ __forceinline__ u64 row_max(const SampleArgs &a, int row) {
   u64 best = 0;
-  for (int i = tid; i < n; i += kSampleThreads) {
-    const u64 key = topk_key(x[i], static_cast<uint32_t>(i));
+  for (int c = threadIdx.x & (kWave - 1); c < a.chunks; c += kWave) {
+    const u64 key = a.chunk_max[static_cast<int64_t>(row) * a.chunks + c];
     best = key > best ? key : best;
   }
+  return wave_max_u64(best);
+}
+
+// A row with a NaN or without any number yields no token.
+__device__ __forceinline__ bool no_token(float mx) { return mx != mx || mx == -INFINITY; }
+
+// Calls f(logit, index) for the chunk's logits, kChunkStep loads at once.
+template <typename F>
+__device__ __forceinline__ void for_chunk(const SampleArgs &a, int row, int chunk, F f) {
+  const float *x = a.logits + row * a.row_stride;
+  const int begin = chunk * a.chunk;
+  const int end = min(begin + a.chunk, a.vocab);
+  for (int base = begin + static_cast<int>(threadIdx.x); base < end;
+       base += kChunkThreads * kChunkStep) {
+    float v[kChunkStep];
+#pragma unroll
+    for (int j = 0; j < kChunkStep; ++j)
+      v[j] = x[min(base + j * kChunkThreads, end - 1)];
+#pragma unroll
+    for (int j = 0; j < kChunkStep; ++j)
+      if (base + j * kChunkThreads < end) f(v[j], base + j * kChunkThreads);
+  }
+}
+
+__global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a) {
+  __shared__ u64 s_key[kChunkThreads / kWave];
+  const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
+  const int row = static_cast<int>(blockIdx.x) / a.chunks;
+  const int tid = threadIdx.x;
+  // the bins and the list of the row start empty
+  u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins;
+  uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins;
+  for (int i = chunk * kChunkThreads + tid; i < kSampleBins; i += a.chunks * kChunkThreads) {
+    mass[i] = 0;
+    count[i] = 0;
+  }
+  if (chunk == 0 && tid == 0) a.list_count[row] = 0;
+  u64 best = 0;
+  for_chunk(a, row, chunk, [&](float v, int i) {
+    const u64 key = topk_key(v, static_cast<uint32_t>(i));
+    best = key > best ? key : best;
+  });
   best = wave_max_u64(best);
-  if ((tid & (kWave - 1)) == 0) sh.scan[tid / kWave] = best;
+  if ((tid & (kWave - 1)) == 0) s_key[tid / kWave] = best;
   __syncthreads();
-  for (int w = 0; w < kSampleWaves; ++w) best = sh.scan[w] > best ? sh.scan[w] : best;
+  if (tid == 0) {
+#pragma unroll
+    for (int w = 1; w < kChunkThreads / kWave; ++w) best = s_key[w] > best ? s_key[w] : best;
+    a.chunk_max[static_cast<int64_t>(row) * a.chunks + chunk] = best;
+  }
+}
+
+__global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs a) {
+  __shared__ u64 s_mass[kSampleBins];
+  __shared__ uint32_t s_count[kSampleBins];
+  const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
+  const int row = static_cast<int>(blockIdx.x) / a.chunks;
+  const int tid = threadIdx.x;
+  const RowSettings set = row_settings(a, row);
+  const float mx = key_value(row_max(a, row));
+  if (set.greedy || no_token(mx)) return;
+  if (set.top_k <= 0 && set.top_p >= 1.0) {
+    u64 sum = 0;
+    for_chunk(a, row, chunk, [&](float v, int) {
+      const u64 w = fixed_weight(v, mx, set.scale);
+      sum += w >= set.min_w ? w : 0;
+    });
+    u64 total;
+    block_prefix<kChunkThreads / kWave>(sum, s_mass, &total);
+    if (tid == 0) a.chunk_mass[static_cast<int64_t>(row) * a.chunks + chunk] = total;
+    return;
+  }
+  for (int i = tid; i < kSampleBins; i += kChunkThreads) {
+    s_mass[i] = 0;
+    s_count[i] = 0;
+  }
   __syncthreads();
+  for_chunk(a, row, chunk, [&](float v, int) {
+    const u64 w = fixed_weight(v, mx, set.scale);
+    if (w == 0) return;
+    const int b = weight_bin(v, mx, set.scale);
+    atomicAdd(&s_mass[b], w);
+    atomicAdd(&s_count[b], 1u);
+  });
+  __syncthreads();
+  u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins;
+  uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins;
+  for (int i = tid; i < kSampleBins; i += kChunkThreads)
+    if (s_count[i] != 0) {
+      atomicAdd(&mass[i], s_mass[i]);
+      atomicAdd(&count[i], s_count[i]);
+    }
+}
+
+// The smallest whole mass that reaches top_p of `mass`, in [1, mass].
+__device__ __forceinline__ u64 top_p_mass(double top_p, u64 mass) {
+  const double need = ceil(top_p * static_cast<double>(mass));
+  const u64 n = need >= 1.0 ? static_cast<u64>(need) : 1;
+  return n < mass ? n : mass;
+}
+
+// The ends of K and P in the row's bins (every thread of 256 has eight bins).
+// K's last bin is exact; P's is known up to what K takes of its last bin, so
+// every bin in which P could end is listed.
+__device__ RowEnds find_ends(const SampleArgs &a, int row, const RowSettings &set) {
+  constexpr int kPer = kSampleBins / kChunkThreads;
+  __shared__ u64 s_scan[kChunkThreads / kWave];
+  __shared__ RowEnds s_ends;
+  __shared__ uint32_t s_above[2];  // count above the first listed bin, above K's last
+  __shared__ uint32_t s_upto;      // count up to P's last candidate
+  const int tid = threadIdx.x;
+  const u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins + tid * kPer;
+  const uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins + tid * kPer;
+  u64 m[kPer], msum = 0;
+  uint32_t n[kPer];
+  u64 nsum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    m[i] = mass[i];
+    n[i] = count[i];
+    msum += m[i];
+    nsum += n[i];
+  }
+  u64 total, live;
+  u64 m_at = block_prefix<kChunkThreads / kWave>(msum, s_scan, &total) - msum;
+  u64 n_at = block_prefix<kChunkThreads / kWave>(nsum, s_scan, &live) - nsum;
+  if (tid == 0) {
+    s_ends = RowEnds{0, 0, total, 0, 0, 0, 0, -1, -1};
+    s_above[0] = s_above[1] = s_upto = 0;
+  }
+  __syncthreads();
+  const bool use_k = set.top_k > 0 && static_cast<u64>(set.top_k) < live;
+  const bool use_p = set.top_p < 1.0;
+  u64 k_least = total, k_most = total;  // bounds of K's mass
+  if (use_k) {
+    const u64 need = static_cast<u64>(set.top_k);
+    u64 ma = m_at, na = n_at;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (na < need && need <= na + n[i]) {
+        s_ends.above_k = ma;
+        s_ends.need_k = static_cast<uint32_t>(need - na);
+        s_ends.last_k = tid * kPer + i;
+        s_above[1] = static_cast<uint32_t>(na);
+        s_ends.total = ma + m[i];  // for now: the most K can hold
+        s_ends.entries = n[i];
+      }
+      ma += m[i];
+      na += n[i];
+    }
+    __syncthreads();
+    k_most = s_ends.total;
+    k_least = s_ends.above_k + 1;
+  }
+  if (use_p) {
+    const u64 least = top_p_mass(set.top_p, k_least), most = top_p_mass(set.top_p, k_most);
+    u64 ma = m_at, na = n_at;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (ma < least && least <= ma + m[i]) {
+        s_ends.first = tid * kPer + i;
+        s_ends.above_p = ma;
+        s_above[0] = static_cast<uint32_t>(na);
+      }
+      if (ma < most && most <= ma + m[i]) {
+        s_ends.last_p = tid * kPer + i;
+        s_upto = static_cast<uint32_t>(na + n[i]);
+      }
+      ma += m[i];
+      na += n[i];
+    }
+  }
+  __syncthreads();
+  RowEnds e = s_ends;
+  e.total = total;
+  if (use_p && use_k) {
+    if (e.last_p >= e.last_k) {  // one run of bins: first .. last_k
+      e.before = s_above[1] - s_above[0];
+      e.entries += e.before;
+      e.last_p = e.last_k;
+    } else {
+      e.before = s_upto - s_above[0];
+      e.entries += e.before;
+    }
+  } else if (use_p) {
+    e.entries = s_upto - s_above[0];
+    e.before = e.entries;
+  } else if (use_k) {
+    e.first = e.last_k;
+  }
+  return e;
+}
+
+__global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArgs a) {
+  __shared__ u64 s_keys[kListMax];
+  __shared__ uint32_t s_count, s_at;
+  __shared__ u64 s_scan[kChunkThreads / kWave];
+  const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
+  const int row = static_cast<int>(blockIdx.x) / a.chunks;
+  const int tid = threadIdx.x;
+  const RowSettings set = row_settings(a, row);
+  const float mx = key_value(row_max(a, row));
+  if (set.greedy || no_token(mx) || (set.top_k <= 0 && set.top_p >= 1.0)) return;
+  const RowEnds e = find_ends(a, row, set);
+  if (chunk == 0 && tid == 0) a.ends[row] = e;
+  if (e.entries > kListMax) return;
+  // without a cut inside the bins (top_k of all tokens) nothing is listed
+  const int first = e.last_p < 0 && e.last_k < 0 ? kSampleBins : e.first;
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  u64 sum = 0;
+  for_chunk(a, row, chunk, [&](float v, int i) {
+    const u64 w = fixed_weight(v, mx, set.scale);
+    if (w == 0) return;
+    const int b = weight_bin(v, mx, set.scale);
+    if (b < first) {
+      sum += w >= set.min_w ? w : 0;
+    } else if (b <= e.last_p || b == e.last_k) {
+      s_keys[atomicAdd(&s_count, 1u)] = topk_key(v, static_cast<uint32_t>(i));
+    }
+  });
+  u64 total;
+  block_prefix<kChunkThreads / kWave>(sum, s_scan, &total);
+  const uint32_t mine = s_count;  // the row's e.entries at most
+  if (mine != 0) {
+    // the list's order does not matter: the draw sorts it
+    if (tid == 0) s_at = atomicAdd(&a.list_count[row], mine);
+    __syncthreads();
+    u64 *list = a.list + static_cast<int64_t>(row) * kListMax + s_at;
+    for (uint32_t i = tid; i < mine; i += kChunkThreads) list[i] = s_keys[i];
+  }
+  if (tid == 0) a.chunk_mass[static_cast<int64_t>(row) * a.chunks + chunk] = total;
+}
+
+struct DrawShared {
+  union {
+    SampleShared row;         // the counted cut of a whole row
+    u64 keys[kListMax];       // the sorted list
+  };
+  u64 mass[kSampleThreads];   // of the chunks
+  u64 scan[kSampleWaves];
+  u64 found[2];
+};
+
+// Sorts keys[0..n) in descending order (n a power of two, at least 2).
+__device__ __forceinline__ void sort_keys(u64 *keys, int n) {
+  for (int run = 2; run <= n; run *= 2)
+    for (int gap = run / 2; gap >= 1; gap /= 2) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += kSampleThreads) {
+        const int lo = 2 * i - (i & (gap - 1));
+        const int hi = lo + gap;
+        const u64 x = keys[lo], y = keys[hi];
+        if ((x < y) == ((lo & run) == 0)) {
+          keys[lo] = y;
+          keys[hi] = x;
+        }
+      }
+    }
+  __syncthreads();
+}
+
+// The key of the last token of the row's P (or K) from its list; `keys` in
+// LDS.  Positions of the sorted list: K's last bin starts at e.before.
+__device__ u64 list_cut(const SampleArgs &a, int row, const RowEnds &e, const RowSettings &set,
+                        float mx, DrawShared &sh) {
+  constexpr int kPer = kListMax / kSampleThreads;
+  const int tid = threadIdx.x;
+  const u64 *list = a.list + static_cast<int64_t>(row) * kListMax;
+  const int n = static_cast<int>(e.entries);
+  int padded = 2;
+  while (padded < n) padded *= 2;
+  for (int i = tid; i < padded; i += kSampleThreads) sh.keys[i] = i < n ? list[i] : 0;
+  sort_keys(sh.keys, padded);
+  const int last_k = static_cast<int>(e.before + e.need_k) - 1;
+  if (e.last_p < 0) return sh.keys[last_k];
+  // prefix sums of the weights, kPer neighbours a thread
+  u64 w[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = kPer * tid + i;
+    w[i] = at < n ? fixed_weight(key_value(sh.keys[at]), mx, set.scale) : 0;
+    sum += w[i];
+  }
+  u64 total;
+  const u64 start = block_prefix(sum, sh.scan, &total) - sum;
+  u64 mass_k = e.total;
+  if (e.last_k >= 0) {
+    // mass of the list before K's last bin, and up to K's last token
+    u64 upto = start;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int at = kPer * tid + i;
+      if (at == static_cast<int>(e.before)) sh.found[0] = upto;
+      upto += w[i];
+      if (at == last_k) sh.found[1] = upto;
+    }
+    __syncthreads();
+    mass_k = e.above_k + (sh.found[1] - sh.found[0]);
+    __syncthreads();
+  }
+  const u64 need = top_p_mass(set.top_p, mass_k);
+  u64 upto = e.above_p + start;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (upto < need && need <= upto + w[i]) sh.found[0] = kPer * tid + i;
+    upto += w[i];
+  }
+  __syncthreads();
+  return sh.keys[sh.found[0]];
+}
+
+// The cut of a row found over the whole row, as a key.
+__device__ u64 counted_cut(const float *x, int n, float mx, const RowSettings &set,
+                           u64 mass_all, u64 live, SampleShared &sh) {
+  Cut cut{0u, 0xffffffffu};
+  if (set.top_k > 0 && static_cast<u64>(set.top_k) < live)
+    cut = find_cut<false>(x, n, mx, set.scale, cut, static_cast<u64>(set.top_k), sh, &mass_all);
+  if (set.top_p < 1.0)
+    cut = find_cut<true>(x, n, mx, set.scale, cut, top_p_mass(set.top_p, mass_all), sh,
+                         &mass_all);
+  return (static_cast<u64>(cut.value) << 32) | (0xffffffffu - cut.index);
+}
+
+// One workgroup a row.
+__global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs a) {
+  __shared__ DrawShared sh;
+  const int row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const float *x = a.logits + row * a.row_stride;
+  const RowSettings set = row_settings(a, row);
+  const u64 best = row_max(a, row);
   const float mx = key_value(best);
-  const bool empty = mx != mx || mx == -INFINITY;
+  const bool empty = no_token(mx);
   if (empty || set.greedy) {
     if (tid == 0) {
       a.ids[row] = empty ? -1 : key_index(best);
@@ -260,59 +629,122 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
     }
     return;
   }
-
-  // number and mass of the tokens that have a weight
-  u64 live = 0, mass = 0;
-  for (int i = tid; i < n; i += kSampleThreads) {
-    const u64 w = fixed_weight(x[i], mx, set.scale);
-    live += w != 0 ? 1 : 0;
-    mass += w;
-  }
-  u64 live_all, mass_all;
-  block_prefix(live, sh.scan, &live_all);
-  block_prefix(mass, sh.scan, &mass_all);
-  Cut cut{0u, 0xffffffffu};
-  if (set.top_k > 0 && static_cast<u64>(set.top_k) < live_all)
-    cut = find_cut<false>(x, n, mx, set.scale, cut, static_cast<u64>(set.top_k), sh, &mass_all);
-  if (set.top_p < 1.0) {
-    const double need = ceil(set.top_p * static_cast<double>(mass_all));
-    u64 need_int = need >= 1.0 ? static_cast<u64>(need) : 1;
-    need_int = need_int < mass_all ? need_int : mass_all;
-    cut = find_cut<true>(x, n, mx, set.scale, cut, need_int, sh, &mass_all);
-  }
-  if (set.min_w > 0) {
-    mass = 0;
-    for (int i = tid; i < n; i += kSampleThreads) {
-      const u64 w = fixed_weight(x[i], mx, set.scale);
-      if (w >= set.min_w && keeps(cut, ordered_bits(x[i]), i)) mass += w;
+  u64 cut = 0;
+  u64 mass = 0;
+  const u64 *chunk_mass = a.chunk_mass + static_cast<int64_t>(row) * a.chunks;
+  if (set.top_k <= 0 && set.top_p >= 1.0) {
+    if (tid < a.chunks) mass = chunk_mass[tid];
+  } else {
+    const RowEnds e = a.ends[row];
+    if (e.entries > kListMax) {
+      u64 live = 0, sum = 0;
+      for (int i = tid; i < a.vocab; i += kSampleThreads) {
+        const u64 w = fixed_weight(x[i], mx, set.scale);
+        live += w != 0 ? 1 : 0;
+        sum += w;
+      }
+      u64 live_all, mass_all;
+      block_prefix(live, sh.scan, &live_all);
+      block_prefix(sum, sh.scan, &mass_all);
+      cut = counted_cut(x, a.vocab, mx, set, mass_all, live_all, sh.row);
+      // the chunks' masses, a wave a chunk
+      for (int c = tid / kWave; c < a.chunks; c += kSampleWaves) {
+        const int end = min((c + 1) * a.chunk, a.vocab);
+        u64 part = 0;
+        for (int i = c * a.chunk + (tid & (kWave - 1)); i < end; i += kWave) {
+          const u64 w = fixed_weight(x[i], mx, set.scale);
+          if (w >= set.min_w && topk_key(x[i], static_cast<uint32_t>(i)) >= cut) part += w;
+        }
+        part = wave_prefix(part, tid & (kWave - 1));
+        if ((tid & (kWave - 1)) == kWave - 1) sh.mass[c] = part;
+      }
+      __syncthreads();
+      if (tid < a.chunks) mass = sh.mass[tid];
+    } else {
+      if (tid < a.chunks) sh.mass[tid] = chunk_mass[tid];
+      if (e.entries > 0) {
+        cut = list_cut(a, row, e, set, mx, sh);
+        // what the list adds to its chunks
+        for (int i = tid; i < static_cast<int>(e.entries); i += kSampleThreads) {
+          const u64 key = sh.keys[i];
+          const u64 w = fixed_weight(key_value(key), mx, set.scale);
+          if (key >= cut && w >= set.min_w)
+            atomicAdd(&sh.mass[key_index(key) / a.chunk], w);
+        }
+      }
+      __syncthreads();
+      if (tid < a.chunks) mass = sh.mass[tid];
     }
-    block_prefix(mass, sh.scan, &mass_all);
   }
-  // the draw
+  // the draw: a chunk, then a token in it
+  u64 total;
+  const u64 upto = block_prefix(mass, sh.scan, &total);
   double u = static_cast<double>(a.uniform[row]);
   u = u > 0.0 ? u : 0.0;  // NaN too
-  const double t = u * static_cast<double>(mass_all);
-  u64 target = t < static_cast<double>(mass_all) ? static_cast<u64>(t) : mass_all - 1;
-  target = target < mass_all ? target : mass_all - 1;
-  u64 seen = 0;
-  for (int base = 0; base < n; base += kSampleThreads) {
-    const int i = base + tid;
-    u64 w = 0;
-    if (i < n) {
-      w = fixed_weight(x[i], mx, set.scale);
-      if (w < set.min_w || !keeps(cut, ordered_bits(x[i]), i)) w = 0;
+  const double t = u * static_cast<double>(total);
+  u64 target = t < static_cast<double>(total) ? static_cast<u64>(t) : total - 1;
+  target = target < total ? target : total - 1;
+  if (upto - mass <= target && target < upto) {
+    sh.found[0] = static_cast<u64>(tid);
+    sh.found[1] = target - (upto - mass);
+  }
+  __syncthreads();
+  const int begin = static_cast<int>(sh.found[0]) * a.chunk;
+  const int end = min(begin + a.chunk, a.vocab);
+  target = sh.found[1];
+  // neighbouring tokens to a thread, so that one prefix sum orders them all
+  constexpr int kPer = kChunkMax / kSampleThreads;
+  const int per = a.chunk / kSampleThreads;
+  u64 w[kPer], sum = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = begin + tid * per + j;
+    w[j] = 0;
+    if (j < per && i < end) {
+      const float v = x[i];
+      w[j] = fixed_weight(v, mx, set.scale);
+      if (w[j] < set.min_w || topk_key(v, static_cast<uint32_t>(i)) < cut) w[j] = 0;
     }
-    u64 total;
-    const u64 end = seen + block_prefix(w, sh.scan, &total);
-    if (w != 0 && end > target && end - w <= target) {
-      a.ids[row] = i;
+    sum += w[j];
+  }
+  u64 all;
+  u64 at = block_prefix(sum, sh.scan, &all) - sum;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (w[j] != 0 && at <= target && target < at + w[j]) {
+      a.ids[row] = begin + tid * per + j;
       if (a.logprobs != nullptr)
         a.logprobs[row] = static_cast<float>(
-            log(static_cast<double>(w) / static_cast<double>(mass_all)));
+            log(static_cast<double>(w[j]) / static_cast<double>(total)));
     }
-    seen += total;
-    if (seen > target) break;  // uniform
+    at += w[j];
   }
+}
+
+// A row's chunks: enough of them to fill the device with few rows, as large
+// as possible otherwise (fewer sums to join).
+struct SamplePlan {
+  int64_t chunk, chunks;
+  size_t max_bytes, bin_mass_bytes, bin_count_bytes, ends_bytes, list_bytes, count_bytes;
+};
+
+static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
+  SamplePlan p{};
+  const int64_t want = (kChunkWorkgroups + rows - 1) / rows;
+  p.chunk = (vocab + want - 1) / want;
+  p.chunk = (p.chunk + kSampleThreads - 1) / kSampleThreads * kSampleThreads;
+  if (p.chunk < kChunkMin) p.chunk = kChunkMin;
+  if (p.chunk > kChunkMax) p.chunk = kChunkMax;
+  p.chunks = (vocab + p.chunk - 1) / p.chunk;
+  auto rounded = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+  const size_t r = static_cast<size_t>(rows);
+  p.max_bytes = rounded(r * p.chunks * sizeof(u64));
+  p.bin_mass_bytes = rounded(r * kSampleBins * sizeof(u64));
+  p.bin_count_bytes = rounded(r * kSampleBins * sizeof(uint32_t));
+  p.ends_bytes = rounded(r * sizeof(RowEnds));
+  p.list_bytes = rounded(r * kListMax * sizeof(u64));
+  p.count_bytes = rounded(r * sizeof(uint32_t));
+  return p;
 }
 
 }  // namespace cascade
@@ -321,7 +753,9 @@ using namespace cascade;
 
 extern "C" size_t cascade_sample_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows <= 0 || vocab <= 0 || vocab > kSampleMaxVocab || rows > 0xffff) return 0;
-  return 256;
+  const SamplePlan p = sample_plan(rows, vocab);
+  return 2 * p.max_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes +
+         p.list_bytes + p.count_bytes;
 }
 
 extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64_t rows,
@@ -345,9 +779,50 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
     if (reinterpret_cast<uintptr_t>(p) & 3) return CASCADE_EALIGN;
   if ((reinterpret_cast<uintptr_t>(ids) & 7) || !aligned16(workspace)) return CASCADE_EALIGN;
   if (workspace_bytes < cascade_sample_workspace_bytes(rows, vocab)) return CASCADE_EWORKSPACE;
-  const SampleArgs a{logits, row_stride, static_cast<int32_t>(vocab), uniform,
-                     temperature, temperature_value, top_k, top_k_value, top_p,
-                     top_p_value, min_p, min_p_value, ids, logprobs};
-  return launch_kernel(sample_row_kernel, dim3(static_cast<unsigned>(rows)),
-                       dim3(kSampleThreads), 0, static_cast<hipStream_t>(stream), a);
+  const SamplePlan p = sample_plan(rows, vocab);
+  SampleArgs a{};
+  a.logits = logits;
+  a.row_stride = row_stride;
+  a.vocab = static_cast<int32_t>(vocab);
+  a.uniform = uniform;
+  a.temperature = temperature;
+  a.temperature_value = temperature_value;
+  a.top_k = top_k;
+  a.top_k_value = top_k_value;
+  a.top_p = top_p;
+  a.top_p_value = top_p_value;
+  a.min_p = min_p;
+  a.min_p_value = min_p_value;
+  a.ids = ids;
+  a.logprobs = logprobs;
+  a.chunk = static_cast<int32_t>(p.chunk);
+  a.chunks = static_cast<int32_t>(p.chunks);
+  unsigned char *ws = static_cast<unsigned char *>(workspace);
+  auto take = [&ws](size_t bytes) {
+    unsigned char *part = ws;
+    ws += bytes;
+    return part;
+  };
+  a.chunk_max = reinterpret_cast<u64 *>(take(p.max_bytes));
+  a.chunk_mass = reinterpret_cast<u64 *>(take(p.max_bytes));
+  a.bin_mass = reinterpret_cast<u64 *>(take(p.bin_mass_bytes));
+  a.bin_count = reinterpret_cast<uint32_t *>(take(p.bin_count_bytes));
+  a.ends = reinterpret_cast<RowEnds *>(take(p.ends_bytes));
+  a.list = reinterpret_cast<u64 *>(take(p.list_bytes));
+  a.list_count = reinterpret_cast<uint32_t *>(take(p.count_bytes));
+  const dim3 grid(static_cast<unsigned>(rows * p.chunks));
+  const dim3 block(kChunkThreads);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  hipError_t e = launch_kernel(sample_max_kernel, grid, block, 0, s, a);
+  if (e != hipSuccess) return e;
+  e = launch_kernel(sample_weigh_kernel, grid, block, 0, s, a);
+  if (e != hipSuccess) return e;
+  // numbers for all rows that cut nothing need no lists
+  if (top_k != nullptr || top_k_value > 0 || top_p != nullptr || top_p_value < 1.0 ||
+      min_p != nullptr || min_p_value > 1.0) {
+    e = launch_kernel(sample_collect_kernel, grid, block, 0, s, a);
+    if (e != hipSuccess) return e;
+  }
+  return launch_kernel(sample_draw_kernel, dim3(static_cast<unsigned>(rows)),
+                       dim3(kSampleThreads), 0, s, a);
 }
