@@ -42,12 +42,18 @@ constexpr u64 kWeightOne = u64{1} << kWeightBits;
 constexpr int64_t kSampleMaxVocab = int64_t{1} << 19;
 constexpr int kListMax = 4096;
 constexpr int kChunkThreads = 256;
-constexpr int kChunkStep = 4;  // logits a thread loads at once
+constexpr int kChunkStep = 4;  // vectors of four logits a thread loads at once
 constexpr int kChunkMin = 2048;
-constexpr int kChunkMax = 16384;
-constexpr int kChunkWorkgroups = 512;  // wanted of a launch
-// bins per unit of log2 weight: 2048 bins hold the 45 units that count
-constexpr double kBinsPerLog2 = kSampleBins / 45.0;
+constexpr int kChunkMax = 8192;
+constexpr int kChunkWorkgroups = 1024;  // wanted of a launch
+// The bins hold the 45 units of log2 weight that count, and what the fp32
+// arithmetic of weight_bin may be off there (45 x 3 x 2^-24 units).
+constexpr float kBinRange = 45.01f;
+constexpr float kBinsPerLog2 = kSampleBins / kBinRange;
+
+// Four logits behind a pointer aligned to four bytes (rows of odd length);
+// one 16-byte load all the same.
+typedef float f32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 
 struct SampleArgs {
   const float *logits;
@@ -67,7 +73,7 @@ struct SampleArgs {
   // the row's cut into chunks, and the workspace (row r's part first)
   int32_t chunk;
   int32_t chunks;
-  u64 *chunk_max;   // [rows][chunks]: key of the largest logit
+  float *chunk_max;  // [rows][chunks]: the largest logit, NaN if there is one
   u64 *chunk_mass;  // [rows][chunks]
   u64 *bin_mass;    // [rows][kSampleBins]
   uint32_t *bin_count;
@@ -83,7 +89,6 @@ struct RowEnds {
   u64 total;     // mass of the row
   uint32_t need_k;  // tokens that K takes of its last bin
   uint32_t before;  // list entries in bins above K's last one
-  uint32_t entries; // list entries
   int32_t first;    // bins first .. last_p, and last_k, are listed
   int32_t last_p;   // -1: no top-p
   int32_t last_k;   // -1: no top-k
@@ -112,11 +117,12 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs &a, int row
   return r;
 }
 
-// 2^(44 + y) rounded to an integer, y <= 0; 0 below y = -45.  2^f for
+// 2^(44 + y) rounded to an integer, y <= 0 (0 from y = -45 on).  2^f for
 // |f| <= 1/2 is the Taylor polynomial of e^(f ln 2) to the 12th power, whose
-// remainder is below 2e-16.
+// remainder is below 2e-16; adding 2^52 rounds to an integer and leaves it in
+// the low bits.
 __device__ __forceinline__ u64 fixed_exp2(double y) {
-  if (!(y > -45.0)) return 0;
+  y = fmax(y, -60.0);
   const double n = rint(y);
   const double z = (y - n) * 0.6931471805599453;
   double p = 1.0 / 479001600.0;
@@ -132,22 +138,23 @@ __device__ __forceinline__ u64 fixed_exp2(double y) {
   p = fma(p, z, 0.5);
   p = fma(p, z, 1.0);
   p = fma(p, z, 1.0);
-  return static_cast<u64>(ldexp(p, static_cast<int>(n) + kWeightBits) + 0.5);
+  const double v = ldexp(p, static_cast<int>(n) + kWeightBits) + 4503599627370496.0;
+  return static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
 }
 
-// Bin of logit x, which has a weight.
-__device__ __forceinline__ int weight_bin(float x, float mx, double scale) {
-  if (x == mx) return 0;
-  const double y = (static_cast<double>(x) - static_cast<double>(mx)) * scale;
-  return min(static_cast<int>(-y * kBinsPerLog2), kSampleBins - 1);
+// Bin of logit x: bin 0 holds the largest, -1 is past the last weight.  Only
+// the order matters (a larger logit is in no later bin), so fp32 does; halves
+// keep the difference of two finite logits finite.  scale2: 2 log2(e) / T.
+__device__ __forceinline__ int weight_bin(float x, float mx, float scale2) {
+  const float down = x == mx ? 0.0f : (0.5f * mx - 0.5f * x) * scale2;
+  return down < kBinRange ? min(static_cast<int>(down * kBinsPerLog2), kSampleBins - 1) : -1;
 }
 
 // Weight of logit x in a row whose largest logit is mx: 2^44 for the largest
 // itself (also where it is infinite), 0 for -inf.
 __device__ __forceinline__ u64 fixed_weight(float x, float mx, double scale) {
-  if (x == mx) return kWeightOne;
-  if (x == -INFINITY) return 0;
-  return fixed_exp2((static_cast<double>(x) - static_cast<double>(mx)) * scale);
+  const u64 w = fixed_exp2((static_cast<double>(x) - static_cast<double>(mx)) * scale);
+  return x == mx ? kWeightOne : x == -INFINITY ? 0 : w;
 }
 
 // Inclusive prefix sum over the wave's lanes.
@@ -281,39 +288,56 @@ __device__ Cut find_cut(const float *x, int n, float mx, double scale, Cut in, u
   return cut;
 }
 
-// Largest key of a row from its chunks'.  All threads return it.
-__device__ __forceinline__ u64 row_max(const SampleArgs &a, int row) {
-  u64 best = 0;
-  for (int c = threadIdx.x & (kWave - 1); c < a.chunks; c += kWave) {
-    const u64 key = a.chunk_max[static_cast<int64_t>(row) * a.chunks + c];
-    best = key > best ? key : best;
-  }
-  return wave_max_u64(best);
+// Maximum that a NaN wins.
+__device__ __forceinline__ float nan_max(float a, float b) { return max_f32(a, b); }
+
+__device__ __forceinline__ float wave_nan_max(float v) {
+  v = nan_max(v, dpp_float<0xB1>(v));
+  v = nan_max(v, dpp_float<0x4E>(v));
+  v = nan_max(v, dpp_float<0x141>(v));
+  v = nan_max(v, dpp_float<0x140>(v));
+  return xor32_max(xor16_max(v));
+}
+
+// Largest logit of a row from its chunks'.  All threads return it.
+__device__ __forceinline__ float row_max(const SampleArgs &a, int row) {
+  float best = -INFINITY;
+  for (int c = threadIdx.x & (kWave - 1); c < a.chunks; c += kWave)
+    best = nan_max(best, a.chunk_max[static_cast<int64_t>(row) * a.chunks + c]);
+  return wave_nan_max(best);
 }
 
 // A row with a NaN or without any number yields no token.
 __device__ __forceinline__ bool no_token(float mx) { return mx != mx || mx == -INFINITY; }
 
-// Calls f(logit, index) for the chunk's logits, kChunkStep loads at once.
+// Calls f(logit, index) for the chunk's logits, four neighbours to a thread,
+// with kChunkStep loads on their way.
 template <typename F>
 __device__ __forceinline__ void for_chunk(const SampleArgs &a, int row, int chunk, F f) {
+  constexpr int kSpan = 4 * kChunkThreads;
   const float *x = a.logits + row * a.row_stride;
   const int begin = chunk * a.chunk;
   const int end = min(begin + a.chunk, a.vocab);
-  for (int base = begin + static_cast<int>(threadIdx.x); base < end;
-       base += kChunkThreads * kChunkStep) {
-    float v[kChunkStep];
+  const int whole = begin + (end - begin) / 4 * 4;
+  for (int base = begin + 4 * static_cast<int>(threadIdx.x); base < whole;
+       base += kSpan * kChunkStep) {
+    f32x4_at4 v[kChunkStep];
 #pragma unroll
     for (int j = 0; j < kChunkStep; ++j)
-      v[j] = x[min(base + j * kChunkThreads, end - 1)];
+      v[j] = *reinterpret_cast<const f32x4_at4 *>(x + min(base + j * kSpan, whole - 4));
 #pragma unroll
     for (int j = 0; j < kChunkStep; ++j)
-      if (base + j * kChunkThreads < end) f(v[j], base + j * kChunkThreads);
+      if (base + j * kSpan < whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f(v[j][i], base + j * kSpan + i);
+      }
   }
+  const int rest = whole + static_cast<int>(threadIdx.x);
+  if (rest < end) f(x[rest], rest);
 }
 
 __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a) {
-  __shared__ u64 s_key[kChunkThreads / kWave];
+  __shared__ float s_max[kChunkThreads / kWave];
   const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
@@ -325,17 +349,14 @@ __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a)
     count[i] = 0;
   }
   if (chunk == 0 && tid == 0) a.list_count[row] = 0;
-  u64 best = 0;
-  for_chunk(a, row, chunk, [&](float v, int i) {
-    const u64 key = topk_key(v, static_cast<uint32_t>(i));
-    best = key > best ? key : best;
-  });
-  best = wave_max_u64(best);
-  if ((tid & (kWave - 1)) == 0) s_key[tid / kWave] = best;
+  float best = -INFINITY;
+  for_chunk(a, row, chunk, [&](float v, int) { best = nan_max(best, v); });
+  best = wave_nan_max(best);
+  if ((tid & (kWave - 1)) == 0) s_max[tid / kWave] = best;
   __syncthreads();
   if (tid == 0) {
 #pragma unroll
-    for (int w = 1; w < kChunkThreads / kWave; ++w) best = s_key[w] > best ? s_key[w] : best;
+    for (int w = 1; w < kChunkThreads / kWave; ++w) best = nan_max(best, s_max[w]);
     a.chunk_max[static_cast<int64_t>(row) * a.chunks + chunk] = best;
   }
 }
@@ -347,7 +368,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
   const RowSettings set = row_settings(a, row);
-  const float mx = key_value(row_max(a, row));
+  const float mx = row_max(a, row);
   if (set.greedy || no_token(mx)) return;
   if (set.top_k <= 0 && set.top_p >= 1.0) {
     u64 sum = 0;
@@ -360,26 +381,27 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
     if (tid == 0) a.chunk_mass[static_cast<int64_t>(row) * a.chunks + chunk] = total;
     return;
   }
+  // top-k needs the numbers, top-p the masses
+  const float scale2 = static_cast<float>(2.0 * set.scale);
+  const bool use_k = set.top_k > 0, use_p = set.top_p < 1.0;
   for (int i = tid; i < kSampleBins; i += kChunkThreads) {
     s_mass[i] = 0;
     s_count[i] = 0;
   }
   __syncthreads();
   for_chunk(a, row, chunk, [&](float v, int) {
-    const u64 w = fixed_weight(v, mx, set.scale);
-    if (w == 0) return;
-    const int b = weight_bin(v, mx, set.scale);
-    atomicAdd(&s_mass[b], w);
-    atomicAdd(&s_count[b], 1u);
+    const int b = weight_bin(v, mx, scale2);
+    if (b < 0) return;
+    if (use_k) atomicAdd(&s_count[b], 1u);
+    if (use_p) atomicAdd(&s_mass[b], fixed_weight(v, mx, set.scale));
   });
   __syncthreads();
   u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins;
   uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins;
-  for (int i = tid; i < kSampleBins; i += kChunkThreads)
-    if (s_count[i] != 0) {
-      atomicAdd(&mass[i], s_mass[i]);
-      atomicAdd(&count[i], s_count[i]);
-    }
+  for (int i = tid; i < kSampleBins; i += kChunkThreads) {
+    if (s_count[i] != 0) atomicAdd(&count[i], s_count[i]);
+    if (s_mass[i] != 0) atomicAdd(&mass[i], s_mass[i]);
+  }
 }
 
 // The smallest whole mass that reaches top_p of `mass`, in [1, mass].
@@ -396,9 +418,11 @@ __device__ RowEnds find_ends(const SampleArgs &a, int row, const RowSettings &se
   constexpr int kPer = kSampleBins / kChunkThreads;
   __shared__ u64 s_scan[kChunkThreads / kWave];
   __shared__ RowEnds s_ends;
-  __shared__ uint32_t s_above[2];  // count above the first listed bin, above K's last
-  __shared__ uint32_t s_upto;      // count up to P's last candidate
+  __shared__ u64 s_most;           // the most that K can weigh
+  __shared__ uint32_t s_above[2];  // tokens above the first listed bin, above K's last
+  __shared__ uint32_t s_upto;      // tokens up to P's last candidate
   const int tid = threadIdx.x;
+  const bool use_p = set.top_p < 1.0;
   const u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins + tid * kPer;
   const uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins + tid * kPer;
   u64 m[kPer], msum = 0;
@@ -412,16 +436,15 @@ __device__ RowEnds find_ends(const SampleArgs &a, int row, const RowSettings &se
     nsum += n[i];
   }
   u64 total, live;
-  u64 m_at = block_prefix<kChunkThreads / kWave>(msum, s_scan, &total) - msum;
-  u64 n_at = block_prefix<kChunkThreads / kWave>(nsum, s_scan, &live) - nsum;
+  const u64 m_at = block_prefix<kChunkThreads / kWave>(msum, s_scan, &total) - msum;
+  const u64 n_at = block_prefix<kChunkThreads / kWave>(nsum, s_scan, &live) - nsum;
   if (tid == 0) {
-    s_ends = RowEnds{0, 0, total, 0, 0, 0, 0, -1, -1};
+    s_ends = RowEnds{0, 0, total, 0, 0, 0, -1, -1};
     s_above[0] = s_above[1] = s_upto = 0;
   }
   __syncthreads();
   const bool use_k = set.top_k > 0 && static_cast<u64>(set.top_k) < live;
-  const bool use_p = set.top_p < 1.0;
-  u64 k_least = total, k_most = total;  // bounds of K's mass
+  u64 k_least = total, k_most = total;
   if (use_k) {
     const u64 need = static_cast<u64>(set.top_k);
     u64 ma = m_at, na = n_at;
@@ -431,17 +454,19 @@ __device__ RowEnds find_ends(const SampleArgs &a, int row, const RowSettings &se
         s_ends.above_k = ma;
         s_ends.need_k = static_cast<uint32_t>(need - na);
         s_ends.last_k = tid * kPer + i;
+        s_ends.first = tid * kPer + i;
         s_above[1] = static_cast<uint32_t>(na);
-        s_ends.total = ma + m[i];  // for now: the most K can hold
-        s_ends.entries = n[i];
+        s_most = ma + m[i];
       }
       ma += m[i];
       na += n[i];
     }
     __syncthreads();
-    k_most = s_ends.total;
-    k_least = s_ends.above_k + 1;
+    k_most = s_most;
+    // a token at least, if it has a weight
+    k_least = min(s_ends.above_k + 1, k_most);
   }
+  __syncthreads();
   if (use_p) {
     const u64 least = top_p_mass(set.top_p, k_least), most = top_p_mass(set.top_p, k_most);
     u64 ma = m_at, na = n_at;
@@ -462,21 +487,13 @@ __device__ RowEnds find_ends(const SampleArgs &a, int row, const RowSettings &se
   }
   __syncthreads();
   RowEnds e = s_ends;
-  e.total = total;
   if (use_p && use_k) {
     if (e.last_p >= e.last_k) {  // one run of bins: first .. last_k
       e.before = s_above[1] - s_above[0];
-      e.entries += e.before;
       e.last_p = e.last_k;
     } else {
       e.before = s_upto - s_above[0];
-      e.entries += e.before;
     }
-  } else if (use_p) {
-    e.entries = s_upto - s_above[0];
-    e.before = e.entries;
-  } else if (use_k) {
-    e.first = e.last_k;
   }
   return e;
 }
@@ -489,35 +506,39 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
   const RowSettings set = row_settings(a, row);
-  const float mx = key_value(row_max(a, row));
+  const float mx = row_max(a, row);
   if (set.greedy || no_token(mx) || (set.top_k <= 0 && set.top_p >= 1.0)) return;
   const RowEnds e = find_ends(a, row, set);
   if (chunk == 0 && tid == 0) a.ends[row] = e;
-  if (e.entries > kListMax) return;
   // without a cut inside the bins (top_k of all tokens) nothing is listed
   const int first = e.last_p < 0 && e.last_k < 0 ? kSampleBins : e.first;
+  const float scale2 = static_cast<float>(2.0 * set.scale);
   if (tid == 0) s_count = 0;
   __syncthreads();
   u64 sum = 0;
   for_chunk(a, row, chunk, [&](float v, int i) {
-    const u64 w = fixed_weight(v, mx, set.scale);
-    if (w == 0) return;
-    const int b = weight_bin(v, mx, set.scale);
+    const int b = weight_bin(v, mx, scale2);
+    if (b < 0) return;
     if (b < first) {
+      const u64 w = fixed_weight(v, mx, set.scale);
       sum += w >= set.min_w ? w : 0;
     } else if (b <= e.last_p || b == e.last_k) {
-      s_keys[atomicAdd(&s_count, 1u)] = topk_key(v, static_cast<uint32_t>(i));
+      const uint32_t at = atomicAdd(&s_count, 1u);
+      if (at < kListMax) s_keys[at] = topk_key(v, static_cast<uint32_t>(i));
     }
   });
   u64 total;
   block_prefix<kChunkThreads / kWave>(sum, s_scan, &total);
-  const uint32_t mine = s_count;  // the row's e.entries at most
+  const uint32_t mine = s_count;
   if (mine != 0) {
-    // the list's order does not matter: the draw sorts it
+    // the list's order does not matter: the draw sorts it.  A row of more
+    // than kListMax entries (list_count tells) gets no whole list.
     if (tid == 0) s_at = atomicAdd(&a.list_count[row], mine);
     __syncthreads();
-    u64 *list = a.list + static_cast<int64_t>(row) * kListMax + s_at;
-    for (uint32_t i = tid; i < mine; i += kChunkThreads) list[i] = s_keys[i];
+    const uint32_t at = s_at;
+    u64 *list = a.list + static_cast<int64_t>(row) * kListMax;
+    if (mine <= kListMax && at <= kListMax - mine)
+      for (uint32_t i = tid; i < mine; i += kChunkThreads) list[at + i] = s_keys[i];
   }
   if (tid == 0) a.chunk_mass[static_cast<int64_t>(row) * a.chunks + chunk] = total;
 }
@@ -530,6 +551,7 @@ struct DrawShared {
   u64 mass[kSampleThreads];   // of the chunks
   u64 scan[kSampleWaves];
   u64 found[2];
+  int first[2];
 };
 
 // Sorts keys[0..n) in descending order (n a power of two, at least 2).
@@ -552,12 +574,11 @@ __device__ __forceinline__ void sort_keys(u64 *keys, int n) {
 
 // The key of the last token of the row's P (or K) from its list; `keys` in
 // LDS.  Positions of the sorted list: K's last bin starts at e.before.
-__device__ u64 list_cut(const SampleArgs &a, int row, const RowEnds &e, const RowSettings &set,
-                        float mx, DrawShared &sh) {
+__device__ u64 list_cut(const SampleArgs &a, int row, int n, const RowEnds &e,
+                        const RowSettings &set, float mx, DrawShared &sh) {
   constexpr int kPer = kListMax / kSampleThreads;
   const int tid = threadIdx.x;
   const u64 *list = a.list + static_cast<int64_t>(row) * kListMax;
-  const int n = static_cast<int>(e.entries);
   int padded = 2;
   while (padded < n) padded *= 2;
   for (int i = tid; i < padded; i += kSampleThreads) sh.keys[i] = i < n ? list[i] : 0;
@@ -618,25 +639,47 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   const int row = blockIdx.x;
   const int tid = threadIdx.x;
   const float *x = a.logits + row * a.row_stride;
+  // what the earlier launches left, loaded at once (a row without cuts has
+  // no ends and no list: those words are not used then)
+  const u64 *chunk_mass = a.chunk_mass + static_cast<int64_t>(row) * a.chunks;
+  u64 mass = tid < a.chunks ? chunk_mass[tid] : 0;
+  const RowEnds e = a.ends[row];
+  const uint32_t entries = a.list_count[row];
+  double u = static_cast<double>(a.uniform[row]);
   const RowSettings set = row_settings(a, row);
-  const u64 best = row_max(a, row);
-  const float mx = key_value(best);
-  const bool empty = no_token(mx);
-  if (empty || set.greedy) {
+  const float mx = row_max(a, row);
+  if (no_token(mx)) {
     if (tid == 0) {
-      a.ids[row] = empty ? -1 : key_index(best);
-      if (a.logprobs != nullptr) a.logprobs[row] = empty ? __builtin_nanf("") : 0.0f;
+      a.ids[row] = -1;
+      if (a.logprobs != nullptr) a.logprobs[row] = __builtin_nanf("");
+    }
+    return;
+  }
+  if (set.greedy) {
+    // the first chunk that has the largest logit, its first token that has it
+    const bool has = tid < a.chunks &&
+                     a.chunk_max[static_cast<int64_t>(row) * a.chunks + tid] == mx;
+    if (tid == 0) sh.first[0] = sh.first[1] = 0x7fffffff;
+    __syncthreads();
+    if (has) atomicMin(&sh.first[0], tid);
+    __syncthreads();
+    const int begin = sh.first[0] * a.chunk;
+    const int end = min(begin + a.chunk, a.vocab);
+    for (int i = begin + tid; i < end; i += kSampleThreads)
+      if (x[i] == mx) {
+        atomicMin(&sh.first[1], i);
+        break;
+      }
+    __syncthreads();
+    if (tid == 0) {
+      a.ids[row] = sh.first[1];
+      if (a.logprobs != nullptr) a.logprobs[row] = 0.0f;
     }
     return;
   }
   u64 cut = 0;
-  u64 mass = 0;
-  const u64 *chunk_mass = a.chunk_mass + static_cast<int64_t>(row) * a.chunks;
-  if (set.top_k <= 0 && set.top_p >= 1.0) {
-    if (tid < a.chunks) mass = chunk_mass[tid];
-  } else {
-    const RowEnds e = a.ends[row];
-    if (e.entries > kListMax) {
+  if (set.top_k > 0 || set.top_p < 1.0) {
+    if (entries > kListMax) {
       u64 live = 0, sum = 0;
       for (int i = tid; i < a.vocab; i += kSampleThreads) {
         const u64 w = fixed_weight(x[i], mx, set.scale);
@@ -660,17 +703,14 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
       }
       __syncthreads();
       if (tid < a.chunks) mass = sh.mass[tid];
-    } else {
-      if (tid < a.chunks) sh.mass[tid] = chunk_mass[tid];
-      if (e.entries > 0) {
-        cut = list_cut(a, row, e, set, mx, sh);
-        // what the list adds to its chunks
-        for (int i = tid; i < static_cast<int>(e.entries); i += kSampleThreads) {
-          const u64 key = sh.keys[i];
-          const u64 w = fixed_weight(key_value(key), mx, set.scale);
-          if (key >= cut && w >= set.min_w)
-            atomicAdd(&sh.mass[key_index(key) / a.chunk], w);
-        }
+    } else if (entries > 0) {
+      if (tid < a.chunks) sh.mass[tid] = mass;
+      cut = list_cut(a, row, static_cast<int>(entries), e, set, mx, sh);
+      // what the list adds to its chunks
+      for (int i = tid; i < static_cast<int>(entries); i += kSampleThreads) {
+        const u64 key = sh.keys[i];
+        const u64 w = fixed_weight(key_value(key), mx, set.scale);
+        if (key >= cut && w >= set.min_w) atomicAdd(&sh.mass[key_index(key) / a.chunk], w);
       }
       __syncthreads();
       if (tid < a.chunks) mass = sh.mass[tid];
@@ -679,7 +719,6 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   // the draw: a chunk, then a token in it
   u64 total;
   const u64 upto = block_prefix(mass, sh.scan, &total);
-  double u = static_cast<double>(a.uniform[row]);
   u = u > 0.0 ? u : 0.0;  // NaN too
   const double t = u * static_cast<double>(total);
   u64 target = t < static_cast<double>(total) ? static_cast<u64>(t) : total - 1;
@@ -695,15 +734,20 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   // neighbouring tokens to a thread, so that one prefix sum orders them all
   constexpr int kPer = kChunkMax / kSampleThreads;
   const int per = a.chunk / kSampleThreads;
-  u64 w[kPer], sum = 0;
+  float v[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int i = begin + tid * per + j;
+    v[j] = j < per && i < end ? x[i] : -INFINITY;
+  }
+  u64 w[kPer], sum = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
     w[j] = 0;
-    if (j < per && i < end) {
-      const float v = x[i];
-      w[j] = fixed_weight(v, mx, set.scale);
-      if (w[j] < set.min_w || topk_key(v, static_cast<uint32_t>(i)) < cut) w[j] = 0;
+    if (j < per) {
+      const uint32_t i = static_cast<uint32_t>(begin + tid * per + j);
+      w[j] = fixed_weight(v[j], mx, set.scale);
+      if (w[j] < set.min_w || topk_key(v[j], i) < cut) w[j] = 0;
     }
     sum += w[j];
   }
@@ -725,7 +769,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
 // as possible otherwise (fewer sums to join).
 struct SamplePlan {
   int64_t chunk, chunks;
-  size_t max_bytes, bin_mass_bytes, bin_count_bytes, ends_bytes, list_bytes, count_bytes;
+  size_t max_bytes, mass_bytes, bin_mass_bytes, bin_count_bytes, ends_bytes, list_bytes, count_bytes;
 };
 
 static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
@@ -738,7 +782,8 @@ static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
   p.chunks = (vocab + p.chunk - 1) / p.chunk;
   auto rounded = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
   const size_t r = static_cast<size_t>(rows);
-  p.max_bytes = rounded(r * p.chunks * sizeof(u64));
+  p.max_bytes = rounded(r * p.chunks * sizeof(float));
+  p.mass_bytes = rounded(r * p.chunks * sizeof(u64));
   p.bin_mass_bytes = rounded(r * kSampleBins * sizeof(u64));
   p.bin_count_bytes = rounded(r * kSampleBins * sizeof(uint32_t));
   p.ends_bytes = rounded(r * sizeof(RowEnds));
@@ -754,7 +799,7 @@ using namespace cascade;
 extern "C" size_t cascade_sample_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows <= 0 || vocab <= 0 || vocab > kSampleMaxVocab || rows > 0xffff) return 0;
   const SamplePlan p = sample_plan(rows, vocab);
-  return 2 * p.max_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes +
+  return p.max_bytes + p.mass_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes +
          p.list_bytes + p.count_bytes;
 }
 
@@ -803,8 +848,8 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
     ws += bytes;
     return part;
   };
-  a.chunk_max = reinterpret_cast<u64 *>(take(p.max_bytes));
-  a.chunk_mass = reinterpret_cast<u64 *>(take(p.max_bytes));
+  a.chunk_max = reinterpret_cast<float *>(take(p.max_bytes));
+  a.chunk_mass = reinterpret_cast<u64 *>(take(p.mass_bytes));
   a.bin_mass = reinterpret_cast<u64 *>(take(p.bin_mass_bytes));
   a.bin_count = reinterpret_cast<uint32_t *>(take(p.bin_count_bytes));
   a.ends = reinterpret_cast<RowEnds *>(take(p.ends_bytes));
