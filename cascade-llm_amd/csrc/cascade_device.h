@@ -291,4 +291,55 @@ __device__ __forceinline__ int64_t key_index(uint64_t key) {
   return static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(key));
 }
 
+// ---- sorted lists of 64 keys, one per lane, largest in lane 0
+
+// The 32-bit halves of a key in this lane and in lane ^ J, in either order.
+template <int J>
+__device__ __forceinline__ void both_of(uint32_t v, uint32_t &a, uint32_t &b) {
+  if constexpr (J == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    a = r[0]; b = r[1];
+  } else if constexpr (J == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    a = r[0]; b = r[1];
+  } else {
+    a = v;
+    if constexpr (J == 8) b = dpp_u32<0x128>(v);                      // row_ror:8
+    else if constexpr (J == 4) b = dpp_u32<0x1B>(dpp_u32<0x141>(v));  // (7 - i) ^ 3
+    else if constexpr (J == 2) b = dpp_u32<0x4E>(v);
+    else b = dpp_u32<0xB1>(v);
+  }
+}
+
+// One compare-exchange with lane ^ J: lanes with `up` keep the larger key.
+template <int J>
+__device__ __forceinline__ uint64_t exchange(uint64_t v, bool up) {
+  uint32_t al, ah, bl, bh;
+  both_of<J>(static_cast<uint32_t>(v), al, bl);
+  both_of<J>(static_cast<uint32_t>(v >> 32), ah, bh);
+  const uint64_t a = (static_cast<uint64_t>(ah) << 32) | al;
+  const uint64_t b = (static_cast<uint64_t>(bh) << 32) | bl;
+  return (a > b) == up ? a : b;
+}
+
+// Sorts a bitonic run of K lanes, descending where `down` is false.
+template <int K>
+__device__ __forceinline__ uint64_t merge_run(uint64_t v, int lane, bool down) {
+  if constexpr (K >= 2) {
+    v = exchange<K / 2>(v, ((lane & (K / 2)) == 0) != down);
+    v = merge_run<K / 2>(v, lane, down);
+  }
+  return v;
+}
+
+// Bitonic sort of a wave's 64 keys, descending (21 compare-exchanges, no LDS).
+__device__ __forceinline__ uint64_t sort64(uint64_t v, int lane) {
+  v = merge_run<2>(v, lane, lane & 2);
+  v = merge_run<4>(v, lane, lane & 4);
+  v = merge_run<8>(v, lane, lane & 8);
+  v = merge_run<16>(v, lane, lane & 16);
+  v = merge_run<32>(v, lane, lane & 32);
+  return merge_run<64>(v, lane, false);
+}
+
 }  // namespace cascade

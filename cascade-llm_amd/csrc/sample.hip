@@ -46,6 +46,7 @@ constexpr int kChunkStep = 4;  // vectors of four logits a thread loads at once
 constexpr int kChunkMin = 2048;
 constexpr int kChunkMax = 8192;
 constexpr int kChunkWorkgroups = 1024;  // wanted of a launch
+constexpr int64_t kSliceRows = 256;  // rows of a launch (the workspace holds these)
 // The bins hold the 45 units of log2 weight that count, and what the fp32
 // arithmetic of weight_bin may be off there (45 x 3 x 2^-24 units).
 constexpr float kBinRange = 45.01f;
@@ -75,6 +76,7 @@ struct SampleArgs {
   int32_t chunks;
   float *chunk_max;  // [rows][chunks]: the largest logit, NaN if there is one
   u64 *chunk_mass;  // [rows][chunks]
+  u64 *chunk_bins;  // [rows][chunks][kSampleBins]: rows with a top-p
   u64 *bin_mass;    // [rows][kSampleBins]
   uint32_t *bin_count;
   struct RowEnds *ends;  // [rows]
@@ -177,7 +179,7 @@ __device__ __forceinline__ u64 block_prefix(u64 v, u64 *lds, u64 *total) {
   if (lane == kWave - 1) lds[wave] = v;
   __syncthreads();
   u64 before = 0, all = 0;
-#pragma unroll
+#pragma unroll 4
   for (int w = 0; w < WAVES; ++w) {
     const u64 s = lds[w];
     if (w < wave) before += s;
@@ -226,6 +228,7 @@ __device__ Cut find_cut(const float *x, int n, float mx, double scale, Cut in, u
       sh.mass[b] = 0;
     }
     __syncthreads();
+#pragma unroll 1
     for (int i = tid; i < n; i += kSampleThreads) {
       const float v = x[i];
       const uint32_t o = ordered_bits(v);
@@ -272,6 +275,7 @@ __device__ Cut find_cut(const float *x, int n, float mx, double scale, Cut in, u
   if (take < equal) {
     // the index of the take-th of them
     u64 seen = 0;
+#pragma unroll 1
     for (int base = 0; base < n; base += kSampleThreads) {
       const int i = base + tid;
       const bool hit = i < n && ordered_bits(x[i]) == prefix;
@@ -398,9 +402,11 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
   __syncthreads();
   u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins;
   uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins;
+  u64 *bins = a.chunk_bins + (static_cast<int64_t>(row) * a.chunks + chunk) * kSampleBins;
   for (int i = tid; i < kSampleBins; i += kChunkThreads) {
     if (s_count[i] != 0) atomicAdd(&count[i], s_count[i]);
     if (s_mass[i] != 0) atomicAdd(&mass[i], s_mass[i]);
+    if (use_p) bins[i] = s_mass[i];
   }
 }
 
@@ -513,13 +519,21 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   // without a cut inside the bins (top_k of all tokens) nothing is listed
   const int first = e.last_p < 0 && e.last_k < 0 ? kSampleBins : e.first;
   const float scale2 = static_cast<float>(2.0 * set.scale);
+  // the mass of the bins above the listed ones: from the chunk's own bins
+  // where they hold it (and min-p drops none of it)
+  const bool summed = set.top_p < 1.0 && set.min_w == 0;
+  u64 sum = 0;
+  if (summed) {
+    const u64 *bins = a.chunk_bins + (static_cast<int64_t>(row) * a.chunks + chunk) * kSampleBins;
+    for (int i = tid; i < first; i += kChunkThreads) sum += bins[i];
+  }
   if (tid == 0) s_count = 0;
   __syncthreads();
-  u64 sum = 0;
   for_chunk(a, row, chunk, [&](float v, int i) {
     const int b = weight_bin(v, mx, scale2);
     if (b < 0) return;
     if (b < first) {
+      if (summed) return;
       const u64 w = fixed_weight(v, mx, set.scale);
       sum += w >= set.min_w ? w : 0;
     } else if (b <= e.last_p || b == e.last_k) {
@@ -572,24 +586,63 @@ __device__ __forceinline__ void sort_keys(u64 *keys, int n) {
   __syncthreads();
 }
 
-// The key of the last token of the row's P (or K) from its list; `keys` in
-// LDS.  Positions of the sorted list: K's last bin starts at e.before.
-__device__ u64 list_cut(const SampleArgs &a, int row, int n, const RowEnds &e,
-                        const RowSettings &set, float mx, DrawShared &sh) {
-  constexpr int kPer = kListMax / kSampleThreads;
+// The same for up to 1024 keys, one a thread (v; 0 past the list): runs of 64
+// are sorted and merged in a wave's registers, and only the steps over a
+// longer gap go through LDS.  The sorted keys end up in keys[0..1024).
+__device__ __forceinline__ u64 sort_block(u64 v, int n, u64 *keys) {
   const int tid = threadIdx.x;
-  const u64 *list = a.list + static_cast<int64_t>(row) * kListMax;
-  int padded = 2;
-  while (padded < n) padded *= 2;
-  for (int i = tid; i < padded; i += kSampleThreads) sh.keys[i] = i < n ? list[i] : 0;
-  sort_keys(sh.keys, padded);
+  const int lane = tid & (kWave - 1);
+  const int runs = (n + kWave - 1) / kWave;  // uniform
+  if (tid / kWave < runs) {
+    v = merge_run<2>(v, lane, lane & 2);
+    v = merge_run<4>(v, lane, lane & 4);
+    v = merge_run<8>(v, lane, lane & 8);
+    v = merge_run<16>(v, lane, lane & 16);
+    v = merge_run<32>(v, lane, lane & 32);
+    v = merge_run<64>(v, lane, tid & 64);
+  }
+  int side = 1;  // the half of `keys` that the next step writes
+  for (int run = 2 * kWave; run < 2 * kWave * runs; run *= 2) {
+    const bool down = (tid & run) != 0;
+    for (int gap = run / 2; gap >= kWave; gap /= 2) {
+      u64 *half = keys + side * kSampleThreads;
+      half[tid] = v;
+      __syncthreads();
+      const u64 other = half[tid ^ gap];
+      v = (v > other) == (((tid & gap) == 0) != down) ? v : other;
+      side ^= 1;
+    }
+    v = merge_run<64>(v, lane, down);
+  }
+  __syncthreads();
+  keys[tid] = v;
+  __syncthreads();
+  return v;
+}
+
+// The key of the last token of the row's P (or K) in its list of n keys, of
+// which this thread has keys tid, tid + 1024, ...  PER: keys a thread holds.
+// Positions of the sorted list (in sh.keys): K's last bin starts at e.before.
+template <int PER>
+__device__ u64 list_cut(const SampleArgs &a, int row, int n, u64 mine, const RowEnds &e,
+                        const RowSettings &set, float mx, DrawShared &sh) {
+  const int tid = threadIdx.x;
+  if constexpr (PER == 1) {
+    sort_block(mine, n, sh.keys);
+  } else {
+    const u64 *list = a.list + static_cast<int64_t>(row) * kListMax;
+    int padded = 2;
+    while (padded < n) padded *= 2;
+    for (int i = tid; i < padded; i += kSampleThreads) sh.keys[i] = i < n ? list[i] : 0;
+    sort_keys(sh.keys, padded);
+  }
   const int last_k = static_cast<int>(e.before + e.need_k) - 1;
   if (e.last_p < 0) return sh.keys[last_k];
-  // prefix sums of the weights, kPer neighbours a thread
-  u64 w[kPer], sum = 0;
+  // prefix sums of the weights, PER neighbours a thread
+  u64 w[PER], sum = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int at = kPer * tid + i;
+  for (int i = 0; i < PER; ++i) {
+    const int at = PER * tid + i;
     w[i] = at < n ? fixed_weight(key_value(sh.keys[at]), mx, set.scale) : 0;
     sum += w[i];
   }
@@ -600,8 +653,8 @@ __device__ u64 list_cut(const SampleArgs &a, int row, int n, const RowEnds &e,
     // mass of the list before K's last bin, and up to K's last token
     u64 upto = start;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int at = kPer * tid + i;
+    for (int i = 0; i < PER; ++i) {
+      const int at = PER * tid + i;
       if (at == static_cast<int>(e.before)) sh.found[0] = upto;
       upto += w[i];
       if (at == last_k) sh.found[1] = upto;
@@ -613,8 +666,8 @@ __device__ u64 list_cut(const SampleArgs &a, int row, int n, const RowEnds &e,
   const u64 need = top_p_mass(set.top_p, mass_k);
   u64 upto = e.above_p + start;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    if (upto < need && need <= upto + w[i]) sh.found[0] = kPer * tid + i;
+  for (int i = 0; i < PER; ++i) {
+    if (upto < need && need <= upto + w[i]) sh.found[0] = PER * tid + i;
     upto += w[i];
   }
   __syncthreads();
@@ -645,6 +698,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   u64 mass = tid < a.chunks ? chunk_mass[tid] : 0;
   const RowEnds e = a.ends[row];
   const uint32_t entries = a.list_count[row];
+  const u64 key = a.list[static_cast<int64_t>(row) * kListMax + tid];
   double u = static_cast<double>(a.uniform[row]);
   const RowSettings set = row_settings(a, row);
   const float mx = row_max(a, row);
@@ -681,6 +735,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   if (set.top_k > 0 || set.top_p < 1.0) {
     if (entries > kListMax) {
       u64 live = 0, sum = 0;
+#pragma unroll 1
       for (int i = tid; i < a.vocab; i += kSampleThreads) {
         const u64 w = fixed_weight(x[i], mx, set.scale);
         live += w != 0 ? 1 : 0;
@@ -691,9 +746,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
       block_prefix(sum, sh.scan, &mass_all);
       cut = counted_cut(x, a.vocab, mx, set, mass_all, live_all, sh.row);
       // the chunks' masses, a wave a chunk
+#pragma unroll 1
       for (int c = tid / kWave; c < a.chunks; c += kSampleWaves) {
         const int end = min((c + 1) * a.chunk, a.vocab);
         u64 part = 0;
+#pragma unroll 1
         for (int i = c * a.chunk + (tid & (kWave - 1)); i < end; i += kWave) {
           const u64 w = fixed_weight(x[i], mx, set.scale);
           if (w >= set.min_w && topk_key(x[i], static_cast<uint32_t>(i)) >= cut) part += w;
@@ -705,7 +762,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
       if (tid < a.chunks) mass = sh.mass[tid];
     } else if (entries > 0) {
       if (tid < a.chunks) sh.mass[tid] = mass;
-      cut = list_cut(a, row, static_cast<int>(entries), e, set, mx, sh);
+      const int n = static_cast<int>(entries);
+      cut = n <= kSampleThreads
+                ? list_cut<1>(a, row, n, tid < n ? key : 0, e, set, mx, sh)
+                : list_cut<kListMax / kSampleThreads>(a, row, n, 0, e, set, mx, sh);
       // what the list adds to its chunks
       for (int i = tid; i < static_cast<int>(entries); i += kSampleThreads) {
         const u64 key = sh.keys[i];
@@ -740,28 +800,30 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
     const int i = begin + tid * per + j;
     v[j] = j < per && i < end ? x[i] : -INFINITY;
   }
-  u64 w[kPer], sum = 0;
+  const int mine = begin + tid * per;
+  auto weight_of = [&](float logit, int i) {
+    const u64 w = fixed_weight(logit, mx, set.scale);
+    return w >= set.min_w && topk_key(logit, static_cast<uint32_t>(i)) >= cut ? w : u64{0};
+  };
+  u64 sum = 0;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    w[j] = 0;
-    if (j < per) {
-      const uint32_t i = static_cast<uint32_t>(begin + tid * per + j);
-      w[j] = fixed_weight(v[j], mx, set.scale);
-      if (w[j] < set.min_w || topk_key(v[j], i) < cut) w[j] = 0;
-    }
-    sum += w[j];
-  }
+  for (int j = 0; j < kPer; ++j)
+    if (j < per) sum += weight_of(v[j], mine + j);
   u64 all;
   u64 at = block_prefix(sum, sh.scan, &all) - sum;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    if (w[j] != 0 && at <= target && target < at + w[j]) {
-      a.ids[row] = begin + tid * per + j;
-      if (a.logprobs != nullptr)
-        a.logprobs[row] = static_cast<float>(
-            log(static_cast<double>(w[j]) / static_cast<double>(total)));
+  if (at <= target && target < at + sum) {
+    // this thread's: its tokens again, one by one
+    for (int i = mine;; ++i) {
+      const u64 w = weight_of(x[i], i);
+      if (target < at + w) {
+        a.ids[row] = i;
+        if (a.logprobs != nullptr)
+          a.logprobs[row] = static_cast<float>(
+              log(static_cast<double>(w) / static_cast<double>(total)));
+        break;
+      }
+      at += w;
     }
-    at += w[j];
   }
 }
 
@@ -769,11 +831,12 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
 // as possible otherwise (fewer sums to join).
 struct SamplePlan {
   int64_t chunk, chunks;
-  size_t max_bytes, mass_bytes, bin_mass_bytes, bin_count_bytes, ends_bytes, list_bytes, count_bytes;
+  size_t max_bytes, mass_bytes, chunk_bins_bytes, bin_mass_bytes, bin_count_bytes, ends_bytes, list_bytes, count_bytes;
 };
 
 static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
   SamplePlan p{};
+  if (rows > kSliceRows) rows = kSliceRows;  // more rows go slice by slice
   const int64_t want = (kChunkWorkgroups + rows - 1) / rows;
   p.chunk = (vocab + want - 1) / want;
   p.chunk = (p.chunk + kSampleThreads - 1) / kSampleThreads * kSampleThreads;
@@ -784,6 +847,7 @@ static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
   const size_t r = static_cast<size_t>(rows);
   p.max_bytes = rounded(r * p.chunks * sizeof(float));
   p.mass_bytes = rounded(r * p.chunks * sizeof(u64));
+  p.chunk_bins_bytes = r * p.chunks * kSampleBins * sizeof(u64);
   p.bin_mass_bytes = rounded(r * kSampleBins * sizeof(u64));
   p.bin_count_bytes = rounded(r * kSampleBins * sizeof(uint32_t));
   p.ends_bytes = rounded(r * sizeof(RowEnds));
@@ -797,9 +861,9 @@ static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
 using namespace cascade;
 
 extern "C" size_t cascade_sample_workspace_bytes(int64_t rows, int64_t vocab) {
-  if (rows <= 0 || vocab <= 0 || vocab > kSampleMaxVocab || rows > 0xffff) return 0;
+  if (rows <= 0 || vocab <= 0 || vocab > kSampleMaxVocab || rows > 0x7fffffff) return 0;
   const SamplePlan p = sample_plan(rows, vocab);
-  return p.max_bytes + p.mass_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes +
+  return p.max_bytes + p.mass_bytes + p.chunk_bins_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes +
          p.list_bytes + p.count_bytes;
 }
 
@@ -813,7 +877,7 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
                                   size_t workspace_bytes, void *stream) {
   if (logits == nullptr || uniform == nullptr || ids == nullptr || workspace == nullptr)
     return CASCADE_EINVAL;
-  if (rows <= 0 || rows > 0xffff || vocab <= 0 || row_stride < vocab) return CASCADE_EINVAL;
+  if (rows <= 0 || rows > 0x7fffffff || vocab <= 0 || row_stride < vocab) return CASCADE_EINVAL;
   if (vocab > kSampleMaxVocab) return CASCADE_ESHAPE;
   // NaN settings are refused too
   if ((top_p == nullptr && !(top_p_value >= 0.0)) || (min_p == nullptr && !(min_p_value >= 0.0)) ||
@@ -826,20 +890,12 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
   if (workspace_bytes < cascade_sample_workspace_bytes(rows, vocab)) return CASCADE_EWORKSPACE;
   const SamplePlan p = sample_plan(rows, vocab);
   SampleArgs a{};
-  a.logits = logits;
   a.row_stride = row_stride;
   a.vocab = static_cast<int32_t>(vocab);
-  a.uniform = uniform;
-  a.temperature = temperature;
   a.temperature_value = temperature_value;
-  a.top_k = top_k;
   a.top_k_value = top_k_value;
-  a.top_p = top_p;
   a.top_p_value = top_p_value;
-  a.min_p = min_p;
   a.min_p_value = min_p_value;
-  a.ids = ids;
-  a.logprobs = logprobs;
   a.chunk = static_cast<int32_t>(p.chunk);
   a.chunks = static_cast<int32_t>(p.chunks);
   unsigned char *ws = static_cast<unsigned char *>(workspace);
@@ -850,24 +906,39 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
   };
   a.chunk_max = reinterpret_cast<float *>(take(p.max_bytes));
   a.chunk_mass = reinterpret_cast<u64 *>(take(p.mass_bytes));
+  a.chunk_bins = reinterpret_cast<u64 *>(take(p.chunk_bins_bytes));
   a.bin_mass = reinterpret_cast<u64 *>(take(p.bin_mass_bytes));
   a.bin_count = reinterpret_cast<uint32_t *>(take(p.bin_count_bytes));
   a.ends = reinterpret_cast<RowEnds *>(take(p.ends_bytes));
   a.list = reinterpret_cast<u64 *>(take(p.list_bytes));
   a.list_count = reinterpret_cast<uint32_t *>(take(p.count_bytes));
-  const dim3 grid(static_cast<unsigned>(rows * p.chunks));
-  const dim3 block(kChunkThreads);
-  const hipStream_t s = static_cast<hipStream_t>(stream);
-  hipError_t e = launch_kernel(sample_max_kernel, grid, block, 0, s, a);
-  if (e != hipSuccess) return e;
-  e = launch_kernel(sample_weigh_kernel, grid, block, 0, s, a);
-  if (e != hipSuccess) return e;
   // numbers for all rows that cut nothing need no lists
-  if (top_k != nullptr || top_k_value > 0 || top_p != nullptr || top_p_value < 1.0 ||
-      min_p != nullptr || min_p_value > 1.0) {
-    e = launch_kernel(sample_collect_kernel, grid, block, 0, s, a);
+  const bool cuts = top_k != nullptr || top_k_value > 0 || top_p != nullptr ||
+                    top_p_value < 1.0 || min_p != nullptr || min_p_value > 1.0;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 block(kChunkThreads);
+  for (int64_t first = 0; first < rows; first += kSliceRows) {
+    const int64_t count = rows - first < kSliceRows ? rows - first : kSliceRows;
+    a.logits = logits + first * row_stride;
+    a.uniform = uniform + first;
+    a.temperature = temperature != nullptr ? temperature + first : nullptr;
+    a.top_k = top_k != nullptr ? top_k + first : nullptr;
+    a.top_p = top_p != nullptr ? top_p + first : nullptr;
+    a.min_p = min_p != nullptr ? min_p + first : nullptr;
+    a.ids = ids + first;
+    a.logprobs = logprobs != nullptr ? logprobs + first : nullptr;
+    const dim3 grid(static_cast<unsigned>(count * p.chunks));
+    hipError_t e = launch_kernel(sample_max_kernel, grid, block, 0, s, a);
+    if (e != hipSuccess) return e;
+    e = launch_kernel(sample_weigh_kernel, grid, block, 0, s, a);
+    if (e != hipSuccess) return e;
+    if (cuts) {
+      e = launch_kernel(sample_collect_kernel, grid, block, 0, s, a);
+      if (e != hipSuccess) return e;
+    }
+    e = launch_kernel(sample_draw_kernel, dim3(static_cast<unsigned>(count)),
+                      dim3(kSampleThreads), 0, s, a);
     if (e != hipSuccess) return e;
   }
-  return launch_kernel(sample_draw_kernel, dim3(static_cast<unsigned>(rows)),
-                       dim3(kSampleThreads), 0, s, a);
+  return 0;
 }
