@@ -42,15 +42,16 @@ constexpr u64 kWeightOne = u64{1} << kWeightBits;
 constexpr int64_t kSampleMaxVocab = int64_t{1} << 19;
 constexpr int kListMax = 4096;
 constexpr int kChunkThreads = 256;
-constexpr int kChunkStep = 4;  // vectors of four logits a thread loads at once
 constexpr int kChunkMin = 2048;
 constexpr int kChunkMax = 8192;
 constexpr int kChunkWorkgroups = 1024;  // wanted of a launch
+constexpr int kChunkVecs = kChunkMax / (4 * kChunkThreads);  // of four logits, a thread
 constexpr int64_t kSliceRows = 256;  // rows of a launch (the workspace holds these)
-// The bins hold the 45 units of log2 weight that count, and what the fp32
-// arithmetic of weight_bin may be off there (45 x 3 x 2^-24 units).
-constexpr float kBinRange = 45.01f;
-constexpr float kBinsPerLog2 = kSampleBins / kBinRange;
+// Log2 weights are held in steps of 1/32 (the table of fixed_weight); the bins
+// hold the 45 units in which a weight is not 0.
+constexpr int kTable = 32;
+constexpr double kLeast = -60.0 * kTable;
+constexpr double kBinsPerStep = kSampleBins / (45.0 * kTable);
 
 // Four logits behind a pointer aligned to four bytes (rows of odd length);
 // one 16-byte load all the same.
@@ -98,7 +99,7 @@ struct RowEnds {
 
 struct RowSettings {
   bool greedy;
-  double scale;   // log2(e) / T
+  double scale;   // 32 log2(e) / T
   int64_t top_k;  // <= 0: off
   double top_p;   // >= 1: off
   u64 min_w;      // smallest weight kept
@@ -109,7 +110,7 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs &a, int row
   const double t = a.temperature != nullptr ? static_cast<double>(a.temperature[row])
                                             : a.temperature_value;
   r.greedy = !(t > 0.0);
-  r.scale = 1.4426950408889634 / t;
+  r.scale = kTable * 1.4426950408889634 / t;
   r.top_k = a.top_k != nullptr ? static_cast<int64_t>(a.top_k[row]) : a.top_k_value;
   r.top_p = a.top_p != nullptr ? static_cast<double>(a.top_p[row]) : a.top_p_value;
   const double p = a.min_p != nullptr ? static_cast<double>(a.min_p[row]) : a.min_p_value;
@@ -119,44 +120,72 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs &a, int row
   return r;
 }
 
-// 2^(44 + y) rounded to an integer, y <= 0 (0 from y = -45 on).  2^f for
-// |f| <= 1/2 is the Taylor polynomial of e^(f ln 2) to the 12th power, whose
-// remainder is below 2e-16; adding 2^52 rounds to an integer and leaves it in
-// the low bits.
-__device__ __forceinline__ u64 fixed_exp2(double y) {
-  y = fmax(y, -60.0);
-  const double n = rint(y);
-  const double z = (y - n) * 0.6931471805599453;
-  double p = 1.0 / 479001600.0;
-  p = fma(p, z, 1.0 / 39916800.0);
-  p = fma(p, z, 1.0 / 3628800.0);
-  p = fma(p, z, 1.0 / 362880.0);
-  p = fma(p, z, 1.0 / 40320.0);
-  p = fma(p, z, 1.0 / 5040.0);
-  p = fma(p, z, 1.0 / 720.0);
-  p = fma(p, z, 1.0 / 120.0);
-  p = fma(p, z, 1.0 / 24.0);
-  p = fma(p, z, 1.0 / 6.0);
-  p = fma(p, z, 0.5);
-  p = fma(p, z, 1.0);
-  p = fma(p, z, 1.0);
-  const double v = ldexp(p, static_cast<int>(n) + kWeightBits) + 4503599627370496.0;
+// A row's largest logit and the scale of the differences to it.
+struct RowScale {
+  double mx;
+  double scale;
+  const double *table;  // in LDS: 2^(44 + j / 32), j < 32
+};
+
+// An infinite logit counts as 1e300: equal to another infinite one, and all
+// above the finite ones.
+__device__ __forceinline__ double logit64(float x) {
+  return fmin(static_cast<double>(x), 1e300);
+}
+
+__device__ __forceinline__ RowScale row_scale(float mx, const RowSettings &set,
+                                              const double *table) {
+  return RowScale{logit64(mx), set.scale, table};
+}
+
+// 32 times the log2 weight of logit x: 0 for the largest, never below kLeast
+// (-inf, and 0 times an infinity, end there).  A larger logit gets no less.
+__device__ __forceinline__ double log_weight(float x, const RowScale &r) {
+  return fmax((logit64(x) - r.mx) * r.scale, kLeast);
+}
+
+// Bin of a log weight: bin 0 holds the largest, kSampleBins and above have no
+// weight.
+__device__ __forceinline__ int weight_bin(double t) {
+  return static_cast<int>(t * -kBinsPerStep);
+}
+
+// 2^(44 + t / 32) rounded to an integer (0 from t / 32 = -45 on).  With n the
+// integer next to t and f = t - n, the weight is 2^floor(n / 32) times the
+// table's 2^(44 + (n mod 32) / 32) times 2^(f / 32), the Taylor polynomial of
+// e^(f ln 2 / 32) to the 5th power, whose remainder is below 3e-15.  Adding
+// 1.5 x 2^52 rounds t and leaves n in the low bits; adding 2^52 does so with
+// the weight.
+__device__ __forceinline__ u64 fixed_weight(double t, const double *table) {
+  constexpr double kLn = 0.6931471805599453 / kTable;
+  const double shifted = t + 6755399441055744.0;
+  const int n = static_cast<int>(__double_as_longlong(shifted));
+  const double f = t - (shifted - 6755399441055744.0);
+  double p = kLn * kLn * kLn * kLn * kLn / 120.0;
+  p = fma(p, f, kLn * kLn * kLn * kLn / 24.0);
+  p = fma(p, f, kLn * kLn * kLn / 6.0);
+  p = fma(p, f, kLn * kLn / 2.0);
+  p = fma(p, f, kLn);
+  p = fma(p, f, 1.0);
+  const double v = ldexp(p * table[n & (kTable - 1)], n >> 5) + 4503599627370496.0;
   return static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
 }
 
-// Bin of logit x: bin 0 holds the largest, -1 is past the last weight.  Only
-// the order matters (a larger logit is in no later bin), so fp32 does; halves
-// keep the difference of two finite logits finite.  scale2: 2 log2(e) / T.
-__device__ __forceinline__ int weight_bin(float x, float mx, float scale2) {
-  const float down = x == mx ? 0.0f : (0.5f * mx - 0.5f * x) * scale2;
-  return down < kBinRange ? min(static_cast<int>(down * kBinsPerLog2), kSampleBins - 1) : -1;
+__device__ __forceinline__ u64 fixed_weight(float x, const RowScale &r) {
+  return fixed_weight(log_weight(x, r), r.table);
 }
 
-// Weight of logit x in a row whose largest logit is mx: 2^44 for the largest
-// itself (also where it is infinite), 0 for -inf.
-__device__ __forceinline__ u64 fixed_weight(float x, float mx, double scale) {
-  const u64 w = fixed_exp2((static_cast<double>(x) - static_cast<double>(mx)) * scale);
-  return x == mx ? kWeightOne : x == -INFINITY ? 0 : w;
+// The table: 2^(j / 32) by the Taylor polynomial of e^(z ln 2), |z| <= 1/2, to
+// the 12th power (remainder below 2e-16).  A barrier has to follow.
+__device__ __forceinline__ void fill_table(double *table) {
+  const int j = threadIdx.x;
+  if (j >= kTable) return;
+  const int whole = j > kTable / 2 ? 1 : 0;
+  const double z = (static_cast<double>(j) / kTable - whole) * 0.6931471805599453;
+  double p = 1.0, term = 1.0;
+#pragma unroll 1
+  for (int k = 12; k >= 1; --k) p = fma(p * z, 1.0 / k, term);
+  table[j] = ldexp(p, whole + kWeightBits);
 }
 
 // Inclusive prefix sum over the wave's lanes.
@@ -213,7 +242,7 @@ struct SampleShared {
 // with a weight, so that their number (BY_MASS: mass) reaches `need` >= 1;
 // *mass_kept is then the mass kept.  All elements together have to reach it.
 template <bool BY_MASS>
-__device__ Cut find_cut(const float *x, int n, float mx, double scale, Cut in, u64 need,
+__device__ Cut find_cut(const float *x, int n, const RowScale &r, Cut in, u64 need,
                         SampleShared &sh, u64 *mass_kept) {
   const int tid = threadIdx.x;
   uint32_t prefix = 0, known = 0;  // the value's bits found so far
@@ -233,7 +262,7 @@ __device__ Cut find_cut(const float *x, int n, float mx, double scale, Cut in, u
       const float v = x[i];
       const uint32_t o = ordered_bits(v);
       if ((o & known) != prefix || !keeps(in, o, i)) continue;
-      const u64 w = fixed_weight(v, mx, scale);
+      const u64 w = fixed_weight(v, r);
       if (w == 0) continue;
       const uint32_t b = (o >> shift) & (bins - 1);
       atomicAdd(&sh.count[b], 1u);
@@ -314,37 +343,52 @@ __device__ __forceinline__ float row_max(const SampleArgs &a, int row) {
 // A row with a NaN or without any number yields no token.
 __device__ __forceinline__ bool no_token(float mx) { return mx != mx || mx == -INFINITY; }
 
-// Calls f(logit, index) for the chunk's logits, four neighbours to a thread,
-// with kChunkStep loads on their way.
-template <typename F>
-__device__ __forceinline__ void for_chunk(const SampleArgs &a, int row, int chunk, F f) {
-  constexpr int kSpan = 4 * kChunkThreads;
-  const float *x = a.logits + row * a.row_stride;
-  const int begin = chunk * a.chunk;
-  const int end = min(begin + a.chunk, a.vocab);
-  const int whole = begin + (end - begin) / 4 * 4;
-  for (int base = begin + 4 * static_cast<int>(threadIdx.x); base < whole;
-       base += kSpan * kChunkStep) {
-    f32x4_at4 v[kChunkStep];
+// A chunk's logits in the registers of its workgroup: vectors of four
+// neighbours, and the row's last three at most one by one.  All are loaded
+// before the first is used, ahead of whatever the kernel has to find out.
+struct Chunk {
+  f32x4_at4 v[kChunkVecs];
+  float rest;
+  int begin, whole, end;
+
+  __device__ __forceinline__ Chunk(const SampleArgs &a, int row, int chunk) {
+    const float *x = a.logits + row * a.row_stride;
+    begin = chunk * a.chunk;
+    end = min(begin + a.chunk, a.vocab);
+    whole = begin + (end - begin) / 4 * 4;
+    if (whole > begin) {  // uniform
 #pragma unroll
-    for (int j = 0; j < kChunkStep; ++j)
-      v[j] = *reinterpret_cast<const f32x4_at4 *>(x + min(base + j * kSpan, whole - 4));
-#pragma unroll
-    for (int j = 0; j < kChunkStep; ++j)
-      if (base + j * kSpan < whole) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f(v[j][i], base + j * kSpan + i);
-      }
+      for (int j = 0; j < kChunkVecs; ++j)
+        if (begin + 4 * kChunkThreads * j < whole)  // uniform
+          v[j] = *reinterpret_cast<const f32x4_at4 *>(x + min(at(j), whole - 4));
+    }
+    rest = x[min(whole + static_cast<int>(threadIdx.x), end - 1)];
   }
-  const int rest = whole + static_cast<int>(threadIdx.x);
-  if (rest < end) f(x[rest], rest);
-}
+
+  __device__ __forceinline__ int at(int j) const {
+    return begin + 4 * (kChunkThreads * j + static_cast<int>(threadIdx.x));
+  }
+
+  // f(logit, index) for each
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int j = 0; j < kChunkVecs; ++j)
+      if (at(j) < whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f(v[j][i], at(j) + i);
+      }
+    const int i = whole + static_cast<int>(threadIdx.x);
+    if (i < end) f(rest, i);
+  }
+};
 
 __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a) {
   __shared__ float s_max[kChunkThreads / kWave];
   const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
+  const Chunk logits(a, row, chunk);
   // the bins and the list of the row start empty
   u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins;
   uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins;
@@ -354,7 +398,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a)
   }
   if (chunk == 0 && tid == 0) a.list_count[row] = 0;
   float best = -INFINITY;
-  for_chunk(a, row, chunk, [&](float v, int) { best = nan_max(best, v); });
+  logits.each([&](float v, int) { best = nan_max(best, v); });
   best = wave_nan_max(best);
   if ((tid & (kWave - 1)) == 0) s_max[tid / kWave] = best;
   __syncthreads();
@@ -368,16 +412,21 @@ __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a)
 __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs a) {
   __shared__ u64 s_mass[kSampleBins];
   __shared__ uint32_t s_count[kSampleBins];
+  __shared__ double s_table[kTable];
   const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
+  const Chunk logits(a, row, chunk);
+  fill_table(s_table);
   const RowSettings set = row_settings(a, row);
   const float mx = row_max(a, row);
   if (set.greedy || no_token(mx)) return;
+  const RowScale r = row_scale(mx, set, s_table);
   if (set.top_k <= 0 && set.top_p >= 1.0) {
+    __syncthreads();
     u64 sum = 0;
-    for_chunk(a, row, chunk, [&](float v, int) {
-      const u64 w = fixed_weight(v, mx, set.scale);
+    logits.each([&](float v, int) {
+      const u64 w = fixed_weight(v, r);
       sum += w >= set.min_w ? w : 0;
     });
     u64 total;
@@ -386,18 +435,18 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
     return;
   }
   // top-k needs the numbers, top-p the masses
-  const float scale2 = static_cast<float>(2.0 * set.scale);
   const bool use_k = set.top_k > 0, use_p = set.top_p < 1.0;
   for (int i = tid; i < kSampleBins; i += kChunkThreads) {
     s_mass[i] = 0;
     s_count[i] = 0;
   }
   __syncthreads();
-  for_chunk(a, row, chunk, [&](float v, int) {
-    const int b = weight_bin(v, mx, scale2);
-    if (b < 0) return;
+  logits.each([&](float v, int) {
+    const double t = log_weight(v, r);
+    const int b = weight_bin(t);
+    if (b >= kSampleBins) return;
     if (use_k) atomicAdd(&s_count[b], 1u);
-    if (use_p) atomicAdd(&s_mass[b], fixed_weight(v, mx, set.scale));
+    if (use_p) atomicAdd(&s_mass[b], fixed_weight(t, s_table));
   });
   __syncthreads();
   u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins;
@@ -507,10 +556,13 @@ __device__ RowEnds find_ends(const SampleArgs &a, int row, const RowSettings &se
 __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArgs a) {
   __shared__ u64 s_keys[kListMax];
   __shared__ uint32_t s_count, s_at;
+  __shared__ double s_table[kTable];
   __shared__ u64 s_scan[kChunkThreads / kWave];
   const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
+  const Chunk logits(a, row, chunk);
+  fill_table(s_table);
   const RowSettings set = row_settings(a, row);
   const float mx = row_max(a, row);
   if (set.greedy || no_token(mx) || (set.top_k <= 0 && set.top_p >= 1.0)) return;
@@ -518,7 +570,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   if (chunk == 0 && tid == 0) a.ends[row] = e;
   // without a cut inside the bins (top_k of all tokens) nothing is listed
   const int first = e.last_p < 0 && e.last_k < 0 ? kSampleBins : e.first;
-  const float scale2 = static_cast<float>(2.0 * set.scale);
+  const RowScale r = row_scale(mx, set, s_table);
   // the mass of the bins above the listed ones: from the chunk's own bins
   // where they hold it (and min-p drops none of it)
   const bool summed = set.top_p < 1.0 && set.min_w == 0;
@@ -529,12 +581,13 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   }
   if (tid == 0) s_count = 0;
   __syncthreads();
-  for_chunk(a, row, chunk, [&](float v, int i) {
-    const int b = weight_bin(v, mx, scale2);
-    if (b < 0) return;
+  logits.each([&](float v, int i) {
+    const double t = log_weight(v, r);
+    const int b = weight_bin(t);
+    if (b >= kSampleBins) return;
     if (b < first) {
       if (summed) return;
-      const u64 w = fixed_weight(v, mx, set.scale);
+      const u64 w = fixed_weight(t, s_table);
       sum += w >= set.min_w ? w : 0;
     } else if (b <= e.last_p || b == e.last_k) {
       const uint32_t at = atomicAdd(&s_count, 1u);
@@ -565,6 +618,7 @@ struct DrawShared {
   u64 mass[kSampleThreads];   // of the chunks
   u64 scan[kSampleWaves];
   u64 found[2];
+  double table[kTable];
   int first[2];
 };
 
@@ -625,7 +679,7 @@ __device__ __forceinline__ u64 sort_block(u64 v, int n, u64 *keys) {
 // Positions of the sorted list (in sh.keys): K's last bin starts at e.before.
 template <int PER>
 __device__ u64 list_cut(const SampleArgs &a, int row, int n, u64 mine, const RowEnds &e,
-                        const RowSettings &set, float mx, DrawShared &sh) {
+                        const RowSettings &set, const RowScale &r, DrawShared &sh) {
   const int tid = threadIdx.x;
   if constexpr (PER == 1) {
     sort_block(mine, n, sh.keys);
@@ -643,7 +697,7 @@ __device__ u64 list_cut(const SampleArgs &a, int row, int n, u64 mine, const Row
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int at = PER * tid + i;
-    w[i] = at < n ? fixed_weight(key_value(sh.keys[at]), mx, set.scale) : 0;
+    w[i] = at < n ? fixed_weight(key_value(sh.keys[at]), r) : 0;
     sum += w[i];
   }
   u64 total;
@@ -675,13 +729,13 @@ __device__ u64 list_cut(const SampleArgs &a, int row, int n, u64 mine, const Row
 }
 
 // The cut of a row found over the whole row, as a key.
-__device__ u64 counted_cut(const float *x, int n, float mx, const RowSettings &set,
+__device__ u64 counted_cut(const float *x, int n, const RowScale &r, const RowSettings &set,
                            u64 mass_all, u64 live, SampleShared &sh) {
   Cut cut{0u, 0xffffffffu};
   if (set.top_k > 0 && static_cast<u64>(set.top_k) < live)
-    cut = find_cut<false>(x, n, mx, set.scale, cut, static_cast<u64>(set.top_k), sh, &mass_all);
+    cut = find_cut<false>(x, n, r, cut, static_cast<u64>(set.top_k), sh, &mass_all);
   if (set.top_p < 1.0)
-    cut = find_cut<true>(x, n, mx, set.scale, cut, top_p_mass(set.top_p, mass_all), sh,
+    cut = find_cut<true>(x, n, r, cut, top_p_mass(set.top_p, mass_all), sh,
                          &mass_all);
   return (static_cast<u64>(cut.value) << 32) | (0xffffffffu - cut.index);
 }
@@ -692,6 +746,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   const int row = blockIdx.x;
   const int tid = threadIdx.x;
   const float *x = a.logits + row * a.row_stride;
+  fill_table(sh.table);
   // what the earlier launches left, loaded at once (a row without cuts has
   // no ends and no list: those words are not used then)
   const u64 *chunk_mass = a.chunk_mass + static_cast<int64_t>(row) * a.chunks;
@@ -731,20 +786,22 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
     }
     return;
   }
+  __syncthreads();  // the table
+  const RowScale r = row_scale(mx, set, sh.table);
   u64 cut = 0;
   if (set.top_k > 0 || set.top_p < 1.0) {
     if (entries > kListMax) {
       u64 live = 0, sum = 0;
 #pragma unroll 1
       for (int i = tid; i < a.vocab; i += kSampleThreads) {
-        const u64 w = fixed_weight(x[i], mx, set.scale);
+        const u64 w = fixed_weight(x[i], r);
         live += w != 0 ? 1 : 0;
         sum += w;
       }
       u64 live_all, mass_all;
       block_prefix(live, sh.scan, &live_all);
       block_prefix(sum, sh.scan, &mass_all);
-      cut = counted_cut(x, a.vocab, mx, set, mass_all, live_all, sh.row);
+      cut = counted_cut(x, a.vocab, r, set, mass_all, live_all, sh.row);
       // the chunks' masses, a wave a chunk
 #pragma unroll 1
       for (int c = tid / kWave; c < a.chunks; c += kSampleWaves) {
@@ -752,7 +809,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
         u64 part = 0;
 #pragma unroll 1
         for (int i = c * a.chunk + (tid & (kWave - 1)); i < end; i += kWave) {
-          const u64 w = fixed_weight(x[i], mx, set.scale);
+          const u64 w = fixed_weight(x[i], r);
           if (w >= set.min_w && topk_key(x[i], static_cast<uint32_t>(i)) >= cut) part += w;
         }
         part = wave_prefix(part, tid & (kWave - 1));
@@ -764,12 +821,12 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
       if (tid < a.chunks) sh.mass[tid] = mass;
       const int n = static_cast<int>(entries);
       cut = n <= kSampleThreads
-                ? list_cut<1>(a, row, n, tid < n ? key : 0, e, set, mx, sh)
-                : list_cut<kListMax / kSampleThreads>(a, row, n, 0, e, set, mx, sh);
+                ? list_cut<1>(a, row, n, tid < n ? key : 0, e, set, r, sh)
+                : list_cut<kListMax / kSampleThreads>(a, row, n, 0, e, set, r, sh);
       // what the list adds to its chunks
       for (int i = tid; i < static_cast<int>(entries); i += kSampleThreads) {
         const u64 key = sh.keys[i];
-        const u64 w = fixed_weight(key_value(key), mx, set.scale);
+        const u64 w = fixed_weight(key_value(key), r);
         if (key >= cut && w >= set.min_w) atomicAdd(&sh.mass[key_index(key) / a.chunk], w);
       }
       __syncthreads();
@@ -802,7 +859,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   }
   const int mine = begin + tid * per;
   auto weight_of = [&](float logit, int i) {
-    const u64 w = fixed_weight(logit, mx, set.scale);
+    const u64 w = fixed_weight(logit, r);
     return w >= set.min_w && topk_key(logit, static_cast<uint32_t>(i)) >= cut ? w : u64{0};
   };
   u64 sum = 0;
