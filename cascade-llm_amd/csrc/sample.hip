@@ -14,7 +14,9 @@
 // not depend on their order, so neither does the token on how the row was
 // cut up.  A token below 2^-45 of the likeliest one is never drawn.
 //
-// Four launches cut a row into chunks, so that a few rows fill the device:
+// Rows of up to kShortVocab logits take one launch, a workgroup a row
+// (sample_short_kernel).  For longer ones four launches cut a row into chunks,
+// so that a few rows fill the device:
 //   1. sample_max_kernel     a chunk's largest logit
 //   2. sample_weigh_kernel   2048 bins of (x_i - max) / T, with the number
 //                            and the mass of their tokens (rows with a top-k
@@ -46,6 +48,8 @@ constexpr int kChunkMin = 2048;
 constexpr int kChunkMax = 8192;
 constexpr int kChunkWorkgroups = 1024;  // wanted of a launch
 constexpr int kChunkVecs = kChunkMax / (4 * kChunkThreads);  // of four logits, a thread
+constexpr int kShortVecs = 4;
+constexpr int64_t kShortVocab = int64_t{4} * kSampleThreads * kShortVecs;
 constexpr int64_t kSliceRows = 256;  // rows of a launch (the workspace holds these)
 // Log2 weights are held in steps of 1/32 (the table of fixed_weight); the bins
 // hold the 45 units in which a weight is not 0.
@@ -343,37 +347,39 @@ __device__ __forceinline__ float row_max(const SampleArgs &a, int row) {
 // A row with a NaN or without any number yields no token.
 __device__ __forceinline__ bool no_token(float mx) { return mx != mx || mx == -INFINITY; }
 
-// A chunk's logits in the registers of its workgroup: vectors of four
-// neighbours, and the row's last three at most one by one.  All are loaded
-// before the first is used, ahead of whatever the kernel has to find out.
+// Logits begin .. end - 1 of a row in the registers of its workgroup: VECS
+// vectors of four neighbours a thread, and the last three at most one by one.
+// All are loaded before the first is used, ahead of whatever the kernel has
+// to find out.
+template <int THREADS, int VECS>
 struct Chunk {
-  f32x4_at4 v[kChunkVecs];
+  f32x4_at4 v[VECS];
   float rest;
   int begin, whole, end;
 
-  __device__ __forceinline__ Chunk(const SampleArgs &a, int row, int chunk) {
-    const float *x = a.logits + row * a.row_stride;
-    begin = chunk * a.chunk;
-    end = min(begin + a.chunk, a.vocab);
+  __device__ __forceinline__ Chunk(const float *x, int first, int last) {
+    begin = first;
+    end = last;
     whole = begin + (end - begin) / 4 * 4;
     if (whole > begin) {  // uniform
 #pragma unroll
-      for (int j = 0; j < kChunkVecs; ++j)
-        if (begin + 4 * kChunkThreads * j < whole)  // uniform
+      for (int j = 0; j < VECS; ++j)
+        if (begin + 4 * THREADS * j < whole)  // uniform
           v[j] = *reinterpret_cast<const f32x4_at4 *>(x + min(at(j), whole - 4));
     }
     rest = x[min(whole + static_cast<int>(threadIdx.x), end - 1)];
   }
 
+  // first index of this thread's vector j
   __device__ __forceinline__ int at(int j) const {
-    return begin + 4 * (kChunkThreads * j + static_cast<int>(threadIdx.x));
+    return begin + 4 * (THREADS * j + static_cast<int>(threadIdx.x));
   }
 
   // f(logit, index) for each
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll
-    for (int j = 0; j < kChunkVecs; ++j)
+    for (int j = 0; j < VECS; ++j)
       if (at(j) < whole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) f(v[j][i], at(j) + i);
@@ -383,12 +389,19 @@ struct Chunk {
   }
 };
 
+__device__ __forceinline__ Chunk<kChunkThreads, kChunkVecs> row_chunk(const SampleArgs &a,
+                                                                      int row, int chunk) {
+  const int begin = chunk * a.chunk;
+  return Chunk<kChunkThreads, kChunkVecs>(a.logits + row * a.row_stride, begin,
+                                          min(begin + a.chunk, a.vocab));
+}
+
 __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a) {
   __shared__ float s_max[kChunkThreads / kWave];
   const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
-  const Chunk logits(a, row, chunk);
+  const auto logits = row_chunk(a, row, chunk);
   // the bins and the list of the row start empty
   u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins;
   uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins;
@@ -416,7 +429,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
   const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
-  const Chunk logits(a, row, chunk);
+  const auto logits = row_chunk(a, row, chunk);
   fill_table(s_table);
   const RowSettings set = row_settings(a, row);
   const float mx = row_max(a, row);
@@ -466,20 +479,23 @@ __device__ __forceinline__ u64 top_p_mass(double top_p, u64 mass) {
   return n < mass ? n : mass;
 }
 
-// The ends of K and P in the row's bins (every thread of 256 has eight bins).
+// The ends of K and P in the row's bins, by a workgroup of THREADS.
 // K's last bin is exact; P's is known up to what K takes of its last bin, so
 // every bin in which P could end is listed.
-__device__ RowEnds find_ends(const SampleArgs &a, int row, const RowSettings &set) {
-  constexpr int kPer = kSampleBins / kChunkThreads;
-  __shared__ u64 s_scan[kChunkThreads / kWave];
+template <int THREADS>
+__device__ RowEnds find_ends(const u64 *bin_mass, const uint32_t *bin_count,
+                             const RowSettings &set) {
+  constexpr int kPer = kSampleBins / THREADS;
+  constexpr int kWaves = THREADS / kWave;
+  __shared__ u64 s_scan[kWaves];
   __shared__ RowEnds s_ends;
   __shared__ u64 s_most;           // the most that K can weigh
   __shared__ uint32_t s_above[2];  // tokens above the first listed bin, above K's last
   __shared__ uint32_t s_upto;      // tokens up to P's last candidate
   const int tid = threadIdx.x;
   const bool use_p = set.top_p < 1.0;
-  const u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins + tid * kPer;
-  const uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins + tid * kPer;
+  const u64 *mass = bin_mass + tid * kPer;
+  const uint32_t *count = bin_count + tid * kPer;
   u64 m[kPer], msum = 0;
   uint32_t n[kPer];
   u64 nsum = 0;
@@ -491,8 +507,8 @@ __device__ RowEnds find_ends(const SampleArgs &a, int row, const RowSettings &se
     nsum += n[i];
   }
   u64 total, live;
-  const u64 m_at = block_prefix<kChunkThreads / kWave>(msum, s_scan, &total) - msum;
-  const u64 n_at = block_prefix<kChunkThreads / kWave>(nsum, s_scan, &live) - nsum;
+  const u64 m_at = block_prefix<kWaves>(msum, s_scan, &total) - msum;
+  const u64 n_at = block_prefix<kWaves>(nsum, s_scan, &live) - nsum;
   if (tid == 0) {
     s_ends = RowEnds{0, 0, total, 0, 0, 0, -1, -1};
     s_above[0] = s_above[1] = s_upto = 0;
@@ -561,12 +577,14 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
-  const Chunk logits(a, row, chunk);
+  const auto logits = row_chunk(a, row, chunk);
   fill_table(s_table);
   const RowSettings set = row_settings(a, row);
   const float mx = row_max(a, row);
   if (set.greedy || no_token(mx) || (set.top_k <= 0 && set.top_p >= 1.0)) return;
-  const RowEnds e = find_ends(a, row, set);
+  const RowEnds e = find_ends<kChunkThreads>(
+      a.bin_mass + static_cast<int64_t>(row) * kSampleBins,
+      a.bin_count + static_cast<int64_t>(row) * kSampleBins, set);
   if (chunk == 0 && tid == 0) a.ends[row] = e;
   // without a cut inside the bins (top_k of all tokens) nothing is listed
   const int first = e.last_p < 0 && e.last_k < 0 ? kSampleBins : e.first;
@@ -678,15 +696,15 @@ __device__ __forceinline__ u64 sort_block(u64 v, int n, u64 *keys) {
 // which this thread has keys tid, tid + 1024, ...  PER: keys a thread holds.
 // Positions of the sorted list (in sh.keys): K's last bin starts at e.before.
 template <int PER>
-__device__ u64 list_cut(const SampleArgs &a, int row, int n, u64 mine, const RowEnds &e,
+__device__ u64 list_cut(const u64 *list, int n, u64 mine, const RowEnds &e,
                         const RowSettings &set, const RowScale &r, DrawShared &sh) {
   const int tid = threadIdx.x;
   if constexpr (PER == 1) {
     sort_block(mine, n, sh.keys);
   } else {
-    const u64 *list = a.list + static_cast<int64_t>(row) * kListMax;
     int padded = 2;
     while (padded < n) padded *= 2;
+    // (the list may be in sh.keys already)
     for (int i = tid; i < padded; i += kSampleThreads) sh.keys[i] = i < n ? list[i] : 0;
     sort_keys(sh.keys, padded);
   }
@@ -821,8 +839,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
       if (tid < a.chunks) sh.mass[tid] = mass;
       const int n = static_cast<int>(entries);
       cut = n <= kSampleThreads
-                ? list_cut<1>(a, row, n, tid < n ? key : 0, e, set, r, sh)
-                : list_cut<kListMax / kSampleThreads>(a, row, n, 0, e, set, r, sh);
+                ? list_cut<1>(nullptr, n, tid < n ? key : 0, e, set, r, sh)
+                : list_cut<kListMax / kSampleThreads>(
+                      a.list + static_cast<int64_t>(row) * kListMax, n, 0, e, set, r, sh);
       // what the list adds to its chunks
       for (int i = tid; i < static_cast<int>(entries); i += kSampleThreads) {
         const u64 key = sh.keys[i];
@@ -884,6 +903,154 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   }
 }
 
+// A row of at most kShortVocab logits in one launch: the row stays in the
+// registers of one workgroup, its bins and its list in LDS.
+__global__ __launch_bounds__(kSampleThreads) void sample_short_kernel(SampleArgs a) {
+  __shared__ DrawShared sh;
+  __shared__ uint32_t s_count;
+  const int row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int lane = tid & (kWave - 1);
+  const int wave = tid / kWave;
+  const float *x = a.logits + row * a.row_stride;
+  const Chunk<kSampleThreads, kShortVecs> logits(x, 0, a.vocab);
+  const double uniform = static_cast<double>(a.uniform[row]);
+  const RowSettings set = row_settings(a, row);
+  fill_table(sh.table);
+  for (int b = tid; b < kSampleBins; b += kSampleThreads) {
+    sh.row.count[b] = 0;
+    sh.row.mass[b] = 0;
+  }
+  if (tid == 0) {
+    s_count = 0;
+    sh.first[0] = 0x7fffffff;
+  }
+  float mx = -INFINITY;
+  logits.each([&](float v, int) { mx = nan_max(mx, v); });
+  mx = wave_nan_max(mx);
+  float *s_max = reinterpret_cast<float *>(sh.mass);
+  if (lane == 0) s_max[wave] = mx;
+  __syncthreads();
+#pragma unroll 4
+  for (int w = 0; w < kSampleWaves; ++w) mx = nan_max(mx, s_max[w]);
+  if (no_token(mx)) {
+    if (tid == 0) {
+      a.ids[row] = -1;
+      if (a.logprobs != nullptr) a.logprobs[row] = __builtin_nanf("");
+    }
+    return;
+  }
+  if (set.greedy) {
+    int at = 0x7fffffff;
+    logits.each([&](float v, int i) { at = v == mx ? min(at, i) : at; });
+    if (at != 0x7fffffff) atomicMin(&sh.first[0], at);
+    __syncthreads();
+    if (tid == 0) {
+      a.ids[row] = sh.first[0];
+      if (a.logprobs != nullptr) a.logprobs[row] = 0.0f;
+    }
+    return;
+  }
+  const RowScale r = row_scale(mx, set, sh.table);
+  const bool use_k = set.top_k > 0, use_p = set.top_p < 1.0;
+  u64 cut = 0;
+  if (use_k || use_p) {
+    logits.each([&](float v, int) {
+      const double t = log_weight(v, r);
+      const int b = weight_bin(t);
+      if (b >= kSampleBins) return;
+      if (use_k) atomicAdd(&sh.row.count[b], 1u);
+      if (use_p) atomicAdd(&sh.row.mass[b], fixed_weight(t, sh.table));
+    });
+    __syncthreads();
+    const RowEnds e = find_ends<kSampleThreads>(sh.row.mass, sh.row.count, set);
+    if (e.last_p >= 0 || e.last_k >= 0) {
+      __syncthreads();  // the list takes the place of the bins
+      logits.each([&](float v, int i) {
+        const int b = weight_bin(log_weight(v, r));
+        if (b >= e.first && (b <= e.last_p || b == e.last_k)) {
+          const uint32_t at = atomicAdd(&s_count, 1u);
+          if (at < kListMax) sh.keys[at] = topk_key(v, static_cast<uint32_t>(i));
+        }
+      });
+      __syncthreads();
+      const int n = static_cast<int>(s_count);
+      if (n > kListMax) {
+        u64 live = 0, sum = 0;
+        logits.each([&](float v, int) {
+          const u64 w = fixed_weight(v, r);
+          live += w != 0 ? 1 : 0;
+          sum += w;
+        });
+        u64 live_all, mass_all;
+        block_prefix(live, sh.scan, &live_all);
+        block_prefix(sum, sh.scan, &mass_all);
+        cut = counted_cut(x, a.vocab, r, set, mass_all, live_all, sh.row);
+      } else if (n <= kSampleThreads) {
+        const u64 key = tid < n ? sh.keys[tid] : 0;
+        __syncthreads();  // the sort writes sh.keys
+        cut = list_cut<1>(nullptr, n, key, e, set, r, sh);
+      } else {
+        cut = list_cut<kListMax / kSampleThreads>(sh.keys, n, 0, e, set, r, sh);
+      }
+    }
+  }
+  // the draw: masses of the threads' vectors, in the order of their tokens
+  // (vector j of all threads, then vector j + 1; the rest last)
+  auto weight_of = [&](float logit, int i) {
+    const u64 w = fixed_weight(logit, r);
+    return w >= set.min_w && topk_key(logit, static_cast<uint32_t>(i)) >= cut ? w : u64{0};
+  };
+  u64 sum[kShortVecs + 1];
+#pragma unroll
+  for (int j = 0; j < kShortVecs; ++j) {
+    sum[j] = 0;
+    if (logits.at(j) < logits.whole) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[j] += weight_of(logits.v[j][i], logits.at(j) + i);
+    }
+    sum[j] = wave_prefix(sum[j], lane);
+    if (lane == kWave - 1) sh.mass[j * kSampleWaves + wave] = sum[j];
+  }
+  const int last = logits.whole + tid;
+  sum[kShortVecs] = last < logits.end ? weight_of(logits.rest, last) : 0;
+  sum[kShortVecs] = wave_prefix(sum[kShortVecs], lane);
+  if (tid == kWave - 1) sh.mass[kShortVecs * kSampleWaves] = sum[kShortVecs];
+  __syncthreads();
+  // prefix sums of the waves' masses: one a lane of the first waves
+  constexpr int kParts = kShortVecs * kSampleWaves + 1;
+  u64 total;
+  const u64 part = tid < kParts ? sh.mass[tid] : 0;
+  const u64 upto = block_prefix(part, sh.scan, &total);
+  if (tid < kParts) sh.mass[tid] = upto - part;
+  __syncthreads();
+  const double u = uniform > 0.0 ? uniform : 0.0;  // NaN too
+  const double t = u * static_cast<double>(total);
+  u64 target = t < static_cast<double>(total) ? static_cast<u64>(t) : total - 1;
+  target = target < total ? target : total - 1;
+#pragma unroll
+  for (int j = 0; j <= kShortVecs; ++j) {
+    if (j == kShortVecs && wave != 0) break;
+    const u64 base = sh.mass[j * kSampleWaves + (j < kShortVecs ? wave : 0)];
+    // this thread's share of vector j: from the lane before it on
+    u64 at = __shfl_up(sum[j], 1);
+    at = base + (lane == 0 ? 0 : at);
+    if (at <= target && target < base + sum[j]) {
+      for (int i = j < kShortVecs ? logits.at(j) : last;; ++i) {
+        const u64 w = weight_of(x[i], i);
+        if (target < at + w) {
+          a.ids[row] = i;
+          if (a.logprobs != nullptr)
+            a.logprobs[row] = static_cast<float>(
+                log(static_cast<double>(w) / static_cast<double>(total)));
+          break;
+        }
+        at += w;
+      }
+    }
+  }
+}
+
 // A row's chunks: enough of them to fill the device with few rows, as large
 // as possible otherwise (fewer sums to join).
 struct SamplePlan {
@@ -919,6 +1086,7 @@ using namespace cascade;
 
 extern "C" size_t cascade_sample_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows <= 0 || vocab <= 0 || vocab > kSampleMaxVocab || rows > 0x7fffffff) return 0;
+  if (vocab <= kShortVocab) return 256;
   const SamplePlan p = sample_plan(rows, vocab);
   return p.max_bytes + p.mass_bytes + p.chunk_bins_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes +
          p.list_bytes + p.count_bytes;
@@ -945,7 +1113,6 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
     if (reinterpret_cast<uintptr_t>(p) & 3) return CASCADE_EALIGN;
   if ((reinterpret_cast<uintptr_t>(ids) & 7) || !aligned16(workspace)) return CASCADE_EALIGN;
   if (workspace_bytes < cascade_sample_workspace_bytes(rows, vocab)) return CASCADE_EWORKSPACE;
-  const SamplePlan p = sample_plan(rows, vocab);
   SampleArgs a{};
   a.row_stride = row_stride;
   a.vocab = static_cast<int32_t>(vocab);
@@ -953,6 +1120,20 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
   a.top_k_value = top_k_value;
   a.top_p_value = top_p_value;
   a.min_p_value = min_p_value;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (vocab <= kShortVocab) {
+    a.logits = logits;
+    a.uniform = uniform;
+    a.temperature = temperature;
+    a.top_k = top_k;
+    a.top_p = top_p;
+    a.min_p = min_p;
+    a.ids = ids;
+    a.logprobs = logprobs;
+    return launch_kernel(sample_short_kernel, dim3(static_cast<unsigned>(rows)),
+                         dim3(kSampleThreads), 0, s, a);
+  }
+  const SamplePlan p = sample_plan(rows, vocab);
   a.chunk = static_cast<int32_t>(p.chunk);
   a.chunks = static_cast<int32_t>(p.chunks);
   unsigned char *ws = static_cast<unsigned char *>(workspace);
@@ -972,7 +1153,6 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
   // numbers for all rows that cut nothing need no lists
   const bool cuts = top_k != nullptr || top_k_value > 0 || top_p != nullptr ||
                     top_p_value < 1.0 || min_p != nullptr || min_p_value > 1.0;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 block(kChunkThreads);
   for (int64_t first = 0; first < rows; first += kSliceRows) {
     const int64_t count = rows - first < kSliceRows ? rows - first : kSliceRows;

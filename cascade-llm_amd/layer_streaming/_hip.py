@@ -899,7 +899,18 @@ def device_copy(dst, src, stream=None):
 
 # ------------------------------------------- paged KV cache and sampling
 # These operators take strided views, and launch on the current stream of the
-# tensors' own device (or on ``stream``).
+# tensors' own device (or on ``stream``).  At a decode step's sizes the checks
+# below would cost more than the kernels, so each wrapper first asks, in one
+# expression, whether its arguments have the ordinary form; only others go
+# through the checks one by one, which refuse them by name or say what the
+# strides of a dimension of one stand for.
+
+_BF16, _F32, _I32, _LONG, _U8 = (torch.bfloat16, torch.float32, torch.int32,
+                                 torch.int64, torch.uint8)
+# the current stream's handle by device index, without a Stream object
+_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(
+    torch._C, "_cuda_getCurrentRawStream") else (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _placed(device, name, tensor, dtype, dim=None):
@@ -926,14 +937,15 @@ def _gpu_of(name, tensor):
     return tensor.device
 
 
-def _int32_vector(device, name, tensor, count=None):
-    _placed(device, name, tensor, torch.int32, 1)
-    if count is not None and tensor.shape[0] != count:
+def _vector(device, name, tensor, dtype, count):
+    """A contiguous vector of ``count`` values."""
+
+    _placed(device, name, tensor, dtype, 1)
+    if tensor.shape[0] != count:
         raise ValueError("{} holds {} entries, expected {}".format(
             name, tensor.shape[0], count))
-    if tensor.shape[0] > 1 and tensor.stride(0) != 1:
+    if count > 1 and tensor.stride(0) != 1:
         raise ValueError("{} must be contiguous".format(name))
-    return tensor.data_ptr()
 
 
 def _strides(name, tensor):
@@ -959,13 +971,11 @@ def _apart(name, tensor):
         dim = stride * (size - 1) + dim
 
 
-def _error_word(device, error_flag):
-    if error_flag is None:
-        return 0
-    _placed(device, "error_flag", error_flag, torch.int32)
-    if error_flag.numel() < 1:
-        raise ValueError("error_flag is empty")
-    return error_flag.data_ptr()
+def _check_error_word(device, error_flag):
+    if error_flag is not None:
+        _placed(device, "error_flag", error_flag, torch.int32)
+        if error_flag.numel() < 1:
+            raise ValueError("error_flag is empty")
 
 
 def _page_pools(device, k_pages, v_pages):
@@ -987,7 +997,7 @@ def _page_pools(device, k_pages, v_pages):
     return page_stride, head_stride
 
 
-def _page_table(device, page_table):
+def _table_stride(device, page_table):
     _placed(device, "page_table", page_table, torch.int32, 2)
     if page_table.shape[1] > 1 and page_table.stride(1) != 1:
         raise ValueError("the rows of page_table must be contiguous")
@@ -995,24 +1005,74 @@ def _page_table(device, page_table):
     stride = width if sequences == 1 else page_table.stride(0)
     if stride < width:
         raise ValueError("the rows of page_table overlap")
-    return page_table.data_ptr(), stride
+    return stride
 
 
-def _call_on(device, stream, name, *args):
-    """Call an entry point whose last argument is the stream, with the
-    tensors' device current."""
+def _check_bytes(device, workspace):
+    _placed(device, "workspace", workspace, torch.uint8, 1)
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
 
-    if stream is None:
-        handle = torch.cuda.current_stream(device).cuda_stream
+
+def _call_on(index, stream, name, *args):
+    """Call an entry point whose last argument is the stream, with device
+    ``index`` current."""
+
+    handle = _current_stream(index) if stream is None else stream.cuda_stream
+    if index == torch.cuda.current_device():
+        code = getattr(_lib or load(), name)(*args, handle)
     else:
-        handle = stream.cuda_stream
-    if device.index is None or device.index == torch.cuda.current_device():
-        code = getattr(load(), name)(*args, handle)
-    else:
-        with torch.cuda.device(device):
-            code = getattr(load(), name)(*args, handle)
+        with torch.cuda.device(index):
+            code = getattr(_lib or load(), name)(*args, handle)
     if code != 0:
         _check(name, code)
+
+
+def _check_append(q, k, v, positions, k_pages, v_pages, page_table, rows, rope,
+                  q_out, error_flag):
+    """The checks of paged_append; returns the strides of q, k, v, q_out, the
+    pools and the table."""
+
+    device = _gpu_of("k", k)
+    _placed(device, "k", k, torch.bfloat16, 3)
+    _placed(device, "v", v, torch.bfloat16, 3)
+    tokens, kv_heads, dim = k.shape
+    if v.shape != k.shape:
+        raise ValueError("k and v differ in shape")
+    pool = _page_pools(device, k_pages, v_pages)
+    if (k_pages.shape[1], k_pages.shape[3]) != (kv_heads, dim):
+        raise ValueError("the pools hold {} heads of {}, the rows {} of {}".format(
+            k_pages.shape[1], k_pages.shape[3], kv_heads, dim))
+    q_strides = out_strides = (0, 0)
+    if q is not None:
+        _placed(device, "q", q, torch.bfloat16, 3)
+        if q.shape != (tokens, q.shape[1], dim):
+            raise ValueError("q and k differ in tokens or head size")
+        q_strides = _strides("q", q)
+        if q_out is not q:
+            _placed(device, "q_out", q_out, torch.bfloat16, 3)
+            if q_out.shape != q.shape:
+                raise ValueError("q_out and q differ in shape")
+        _apart("q_out", q_out)
+        out_strides = _strides("q_out", q_out)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    table_stride = _table_stride(device, page_table)
+    _vector(device, "positions", positions, torch.int32, tokens)
+    if rows is not None:
+        _vector(device, "rows", rows, torch.int32, tokens)
+    elif tokens > page_table.shape[0]:
+        raise ValueError("more tokens than page table rows (give rows)")
+    if rope is not None:
+        cos, sin = rope
+        _placed(device, "rope cos", cos, torch.bfloat16, 2)
+        _placed(device, "rope sin", sin, torch.bfloat16, 2)
+        if cos.shape != sin.shape:
+            raise ValueError("rope cos and sin differ in shape")
+        if not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError("the rope tables must be contiguous")
+    _check_error_word(device, error_flag)
+    return q_strides, _strides("k", k), _strides("v", v), out_strides, pool, table_stride
 
 
 def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
@@ -1031,61 +1091,82 @@ def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
     ``page_table`` int32 [sequences, pages of one].  An index out of range
     leaves its token out and ors PAGED_ERANGE into ``error_flag``."""
 
-    device = _gpu_of("k", k)
-    _placed(device, "k", k, torch.bfloat16, 3)
-    _placed(device, "v", v, torch.bfloat16, 3)
-    tokens, kv_heads, dim = k.shape
-    if v.shape != k.shape:
-        raise ValueError("k and v differ in shape")
-    page_stride, head_stride = _page_pools(device, k_pages, v_pages)
-    pages, pool_heads, page_size, pool_dim = k_pages.shape
-    if (pool_heads, pool_dim) != (kv_heads, dim):
-        raise ValueError("the pools hold {} heads of {}, the rows {} of {}".format(
-            pool_heads, pool_dim, kv_heads, dim))
-    q_heads = 0
-    q_args, out_args = (0, 0, 0), (0, 0, 0)
-    if q is not None:
-        _placed(device, "q", q, torch.bfloat16, 3)
-        q_heads = q.shape[1]
-        if q.shape != (tokens, q_heads, dim):
-            raise ValueError("q and k differ in tokens or head size")
-        q_args = (q.data_ptr(),) + _strides("q", q)
-        if q_out is None:
-            q_out = q
-        if q_out is not q:
-            _placed(device, "q_out", q_out, torch.bfloat16, 3)
-            if q_out.shape != q.shape:
-                raise ValueError("q_out and q differ in shape")
-        _apart("q_out", q_out)
-        out_args = (q_out.data_ptr(),) + _strides("q_out", q_out)
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    table, table_stride = _page_table(device, page_table)
+    if q is not None and q_out is None:
+        q_out = q
+    cos, sin = (None, None) if rope is None else rope
+    try:
+        index = k.get_device()
+        ks, vs, ps, ts = k.stride(), v.stride(), k_pages.stride(), page_table.stride()
+        tokens, kv_heads, dim = shape = k.shape
+        pages, pool_heads, page_size, pool_dim = k_pages.shape
+        ordinary = (
+            tokens > 0 and pages > 1 and index >= 0
+            and v.shape == shape and k_pages.shape == v_pages.shape
+            and pool_heads == kv_heads and pool_dim == dim and v_pages.stride() == ps
+            and ks[2] == vs[2] == ps[3] == ts[1] == 1 and ps[2] == dim
+            and k.dtype is _BF16 and v.dtype is _BF16 and k_pages.dtype is _BF16
+            and v_pages.dtype is _BF16 and page_table.dtype is _I32
+            and positions.dtype is _I32 and index == v.get_device()
+            == k_pages.get_device() == v_pages.get_device()
+            == page_table.get_device() == positions.get_device()
+            and positions.shape == (tokens,) and positions.is_contiguous()
+            and (tokens <= page_table.shape[0] if rows is None else (
+                rows.dtype is _I32 and rows.get_device() == index
+                and rows.shape == (tokens,) and rows.is_contiguous()))
+            and ts[0] >= page_table.shape[1]
+            and (q_out is None if q is None else (
+                q.dtype is _BF16 and q_out.dtype is _BF16
+                and index == q.get_device() == q_out.get_device()
+                and q.shape[0] == tokens and q.shape[2] == dim
+                and q.stride(2) == 1 and q_out.shape == q.shape
+                and q_out.is_contiguous()))
+            and (rope is None or (
+                cos.dtype is _BF16 and sin.dtype is _BF16
+                and index == cos.get_device() == sin.get_device()
+                and cos.dim() == 2 and cos.shape == sin.shape
+                and cos.is_contiguous() and sin.is_contiguous()))
+            and (error_flag is None or (
+                error_flag.dtype is _I32 and error_flag.get_device() == index
+                and error_flag.numel() > 0)))
+    except (AttributeError, IndexError, TypeError, ValueError, RuntimeError):
+        ordinary = False
+    if ordinary:
+        # (the stride of a dimension of one says nothing)
+        k_strides, v_strides, table_stride = ks, vs, ts[0]
+        q_strides = out_strides = (0, 0)
+        if q is not None:
+            q_strides, out_strides = q.stride(), q_out.stride()
+        if tokens == 1:
+            k_strides, v_strides = (0, ks[1]), (0, vs[1])
+            q_strides = (0, q_strides[1])
+        pool = ps
+        if kv_heads == 1:
+            k_strides, v_strides = (k_strides[0], 0), (v_strides[0], 0)
+            pool = (ps[0], page_size * dim)
+        if q is not None and q.shape[1] == 1:
+            q_strides = (q_strides[0], 0)
+    else:
+        q_strides, k_strides, v_strides, out_strides, pool, table_stride = _check_append(
+            q, k, v, positions, k_pages, v_pages, page_table, rows, rope, q_out,
+            error_flag)
+        index = k.get_device()
+        tokens, kv_heads, dim = k.shape
+        pages, _, page_size, _ = k_pages.shape
+        if tokens == 0:
+            return q_out
     sequences, max_pages = page_table.shape
-    pos = _int32_vector(device, "positions", positions, tokens)
-    row = 0 if rows is None else _int32_vector(device, "rows", rows, tokens)
-    if rows is None and tokens > sequences:
-        raise ValueError("more tokens than page table rows (give rows)")
-    cos = sin = rope_positions = rope_dim = 0
-    if rope is not None:
-        cos_t, sin_t = rope
-        _placed(device, "rope cos", cos_t, torch.bfloat16, 2)
-        _placed(device, "rope sin", sin_t, torch.bfloat16, 2)
-        if cos_t.shape != sin_t.shape:
-            raise ValueError("rope cos and sin differ in shape")
-        if not (cos_t.is_contiguous() and sin_t.is_contiguous()):
-            raise ValueError("the rope tables must be contiguous")
-        rope_positions, rope_dim = cos_t.shape[0], 2 * cos_t.shape[1]
-        cos, sin = cos_t.data_ptr(), sin_t.data_ptr()
-    error = _error_word(device, error_flag)
-    if tokens == 0:
-        return q_out
-    _call_on(device, stream, "cascade_paged_append_bf16", *q_args, k.data_ptr(),
-             *_strides("k", k), v.data_ptr(), *_strides("v", v), tokens, q_heads,
-             kv_heads, dim, pos, row, table, table_stride, sequences, max_pages,
-             cos, sin, rope_positions, rope_dim, 1 if interleaved else 0, *out_args,
-             k_pages.data_ptr(), v_pages.data_ptr(), page_stride, head_stride,
-             pages, page_size, error)
+    _call_on(
+        index, stream, "cascade_paged_append_bf16",
+        0 if q is None else q.data_ptr(), q_strides[0], q_strides[1], k.data_ptr(),
+        k_strides[0], k_strides[1], v.data_ptr(), v_strides[0], v_strides[1], tokens,
+        0 if q is None else q.shape[1], kv_heads, dim, positions.data_ptr(),
+        0 if rows is None else rows.data_ptr(), page_table.data_ptr(), table_stride,
+        sequences, max_pages, 0 if rope is None else cos.data_ptr(),
+        0 if rope is None else sin.data_ptr(), 0 if rope is None else cos.shape[0],
+        0 if rope is None else 2 * cos.shape[1], 1 if interleaved else 0,
+        0 if q is None else q_out.data_ptr(), out_strides[0], out_strides[1],
+        k_pages.data_ptr(), v_pages.data_ptr(), pool[0], pool[1], pages, page_size,
+        0 if error_flag is None else error_flag.data_ptr())
     return q_out
 
 
@@ -1100,6 +1181,34 @@ def paged_attention_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim,
     if size == 0:
         raise ValueError("unsupported paged attention shape")
     return int(size)
+
+
+def _check_attention(q, k_pages, v_pages, page_table, lengths, out, workspace,
+                     rows, error_flag):
+    """The checks of paged_decode_attention; returns the strides of q, out,
+    the pools and the table."""
+
+    device = _gpu_of("q", q)
+    _placed(device, "q", q, torch.bfloat16, 3)
+    batch, _, dim = q.shape
+    pool = _page_pools(device, k_pages, v_pages)
+    if k_pages.shape[3] != dim:
+        raise ValueError("the pools hold heads of {}, q of {}".format(
+            k_pages.shape[3], dim))
+    _placed(device, "out", out, torch.bfloat16, 3)
+    if out.shape != q.shape:
+        raise ValueError("out and q differ in shape")
+    _apart("out", out)
+    table_stride = _table_stride(device, page_table)
+    sequences = page_table.shape[0]
+    _vector(device, "lengths", lengths, torch.int32, sequences)
+    if rows is not None:
+        _vector(device, "rows", rows, torch.int32, batch)
+    elif batch > sequences:
+        raise ValueError("more rows than page table rows (give rows)")
+    _check_bytes(device, workspace)
+    _check_error_word(device, error_flag)
+    return _strides("q", q), _strides("out", out), pool, table_stride
 
 
 def paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out,
@@ -1117,40 +1226,62 @@ def paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out,
     paged_attention_workspace_bytes(...) uint8, one for calls that may
     overlap."""
 
-    device = _gpu_of("q", q)
-    _placed(device, "q", q, torch.bfloat16, 3)
-    batch, q_heads, dim = q.shape
-    page_stride, head_stride = _page_pools(device, k_pages, v_pages)
-    pages, kv_heads, page_size, pool_dim = k_pages.shape
-    if pool_dim != dim:
-        raise ValueError("the pools hold heads of {}, q of {}".format(pool_dim, dim))
-    _placed(device, "out", out, torch.bfloat16, 3)
-    if out.shape != q.shape:
-        raise ValueError("out and q differ in shape")
-    _apart("out", out)
-    table, table_stride = _page_table(device, page_table)
-    sequences, max_pages = page_table.shape
-    lens = _int32_vector(device, "lengths", lengths, sequences)
-    row = 0 if rows is None else _int32_vector(device, "rows", rows, batch)
-    if rows is None and batch > sequences:
-        raise ValueError("more rows than page table rows (give rows)")
+    try:
+        index = q.get_device()
+        qs, ps, ts = q.stride(), k_pages.stride(), page_table.stride()
+        batch, _, dim = q.shape
+        pages, kv_heads, page_size, pool_dim = k_pages.shape
+        sequences, width = page_table.shape
+        ordinary = (
+            batch > 0 and pages > 1 and index >= 0
+            and k_pages.shape == v_pages.shape and pool_dim == dim
+            and v_pages.stride() == ps and out.shape == q.shape
+            and qs[2] == ps[3] == ts[1] == 1 and ps[2] == dim
+            and q.dtype is _BF16 and k_pages.dtype is _BF16 and v_pages.dtype is _BF16
+            and out.dtype is _BF16 and page_table.dtype is _I32
+            and lengths.dtype is _I32 and workspace.dtype is _U8
+            and index == k_pages.get_device() == v_pages.get_device()
+            == out.get_device() == page_table.get_device() == lengths.get_device()
+            == workspace.get_device()
+            and lengths.shape == (sequences,) and lengths.is_contiguous()
+            and (batch <= sequences if rows is None else (
+                rows.dtype is _I32 and rows.get_device() == index
+                and rows.shape == (batch,) and rows.is_contiguous()))
+            and ts[0] >= width and out.is_contiguous()
+            and workspace.dim() == 1 and workspace.is_contiguous()
+            and (error_flag is None or (
+                error_flag.dtype is _I32 and error_flag.get_device() == index
+                and error_flag.numel() > 0)))
+    except (AttributeError, IndexError, TypeError, ValueError, RuntimeError):
+        ordinary = False
+    if ordinary:
+        # (the stride of a dimension of one says nothing)
+        q_strides = (qs[0] if batch > 1 else 0, qs[1] if q.shape[1] > 1 else 0)
+        out_strides, table_stride = out.stride(), ts[0]
+        pool = ps if kv_heads > 1 else (ps[0], page_size * dim)
+    else:
+        q_strides, out_strides, pool, table_stride = _check_attention(
+            q, k_pages, v_pages, page_table, lengths, out, workspace, rows,
+            error_flag)
+        index = q.get_device()
+        batch, _, dim = q.shape
+        pages, kv_heads, page_size, _ = k_pages.shape
+        sequences, width = page_table.shape
     if max_length is None:
-        max_length = max_pages * page_size
-    elif not 0 < max_length <= max_pages * page_size:
+        max_length = width * page_size
+    elif not 0 < max_length <= width * page_size:
         raise ValueError("max_length {} is outside the page table's {}".format(
-            max_length, max_pages * page_size))
-    _placed(device, "workspace", workspace, torch.uint8, 1)
-    if not workspace.is_contiguous():
-        raise ValueError("workspace must be contiguous")
-    error = _error_word(device, error_flag)
+            max_length, width * page_size))
     if batch == 0:
         return out
-    _call_on(device, stream, "cascade_paged_decode_attention_bf16", q.data_ptr(),
-             *_strides("q", q), k_pages.data_ptr(), v_pages.data_ptr(), page_stride,
-             head_stride, pages, page_size, table, table_stride, sequences, lens, row,
-             batch, int(max_length), q_heads, kv_heads, dim, float(scale),
-             out.data_ptr(), *_strides("out", out), workspace.data_ptr(),
-             workspace.numel(), error)
+    _call_on(
+        index, stream, "cascade_paged_decode_attention_bf16", q.data_ptr(),
+        q_strides[0], q_strides[1], k_pages.data_ptr(), v_pages.data_ptr(), pool[0],
+        pool[1], pages, page_size, page_table.data_ptr(), table_stride, sequences,
+        lengths.data_ptr(), 0 if rows is None else rows.data_ptr(), batch,
+        int(max_length), q.shape[1], kv_heads, dim, scale, out.data_ptr(),
+        out_strides[0], out_strides[1], workspace.data_ptr(), workspace.numel(),
+        0 if error_flag is None else error_flag.data_ptr())
     return out
 
 
@@ -1166,23 +1297,23 @@ def copy_pages(pages, pairs, error_flag=None, stream=None):
     device = _gpu_of("pages", pages)
     if not pages.is_contiguous():
         raise ValueError("pages must be contiguous")
-    if pages.dim() < 3:
+    shape = pages.shape
+    if len(shape) < 3:
         raise ValueError("pages must be [layers, 2, pages, ...] or [planes, pages, ...]")
-    lead = 2 if pages.dim() >= 5 else 1
-    count = pages.shape[lead]
-    planes = 1
-    for size in pages.shape[:lead]:
-        planes *= size
+    if len(shape) >= 5:
+        planes, count = shape[0] * shape[1], shape[2]
+    else:
+        planes, count = shape[0], shape[1]
     _placed(device, "pairs", pairs, torch.int32, 2)
     if pairs.shape[1] != 2 or not pairs.is_contiguous():
         raise ValueError("pairs must be contiguous [n, 2]")
-    error = _error_word(device, error_flag)
+    _check_error_word(device, error_flag)
     if pairs.shape[0] == 0 or pages.numel() == 0:
         return pages
     plane_bytes = pages.numel() * pages.element_size() // planes
-    _call_on(device, stream, "cascade_copy_pages", pages.data_ptr(), planes,
+    _call_on(device.index, stream, "cascade_copy_pages", pages.data_ptr(), planes,
              plane_bytes, count, plane_bytes // count, pairs.data_ptr(),
-             pairs.shape[0], error)
+             pairs.shape[0], 0 if error_flag is None else error_flag.data_ptr())
     return pages
 
 
@@ -1197,13 +1328,11 @@ def sample_workspace_bytes(rows, vocab):
 
 
 def _setting(device, name, value, dtype, rows):
-    """(pointer, value) of a per-row tensor or one number for all rows."""
+    """(pointer, number) of a per-row tensor or one number for all rows."""
 
     if not isinstance(value, torch.Tensor):
         return 0, value
-    _placed(device, name, value, dtype, 1)
-    if value.shape[0] != rows or (rows > 1 and value.stride(0) != 1):
-        raise ValueError("{} must be contiguous with one value a row".format(name))
+    _vector(device, name, value, dtype, rows)
     return value.data_ptr(), 0
 
 
@@ -1222,35 +1351,31 @@ def sample(logits, uniform, ids, workspace, temperature=1.0, top_k=0, top_p=1.0,
     overlap."""
 
     device = _gpu_of("logits", logits)
-    _placed(device, "logits", logits, torch.float32, 2)
+    _placed(device, "logits", logits, _F32, 2)
     rows, vocab = logits.shape
-    if vocab > 1 and logits.stride(1) != 1:
+    row_stride, last = logits.stride()
+    if vocab > 1 and last != 1:
         raise ValueError("the rows of logits must be contiguous")
-    row_stride = vocab if rows == 1 else logits.stride(0)
-    if row_stride < vocab:
+    if rows == 1:
+        row_stride = vocab
+    elif row_stride < vocab:
         raise ValueError("the rows of logits overlap")
-    for name, tensor, dtype in (("uniform", uniform, torch.float32),
-                                ("ids", ids, torch.int64),
-                                ("logprobs", logprobs, torch.float32)):
-        if tensor is None and name == "logprobs":
-            continue
-        _placed(device, name, tensor, dtype, 1)
-        if tensor.shape[0] != rows or (rows > 1 and tensor.stride(0) != 1):
-            raise ValueError("{} must be contiguous with one value a row".format(name))
-    t_ptr, t = _setting(device, "temperature", temperature, torch.float32, rows)
-    k_ptr, k = _setting(device, "top_k", top_k, torch.int32, rows)
-    p_ptr, p = _setting(device, "top_p", top_p, torch.float32, rows)
-    m_ptr, m = _setting(device, "min_p", min_p, torch.float32, rows)
-    _placed(device, "workspace", workspace, torch.uint8, 1)
-    if not workspace.is_contiguous():
-        raise ValueError("workspace must be contiguous")
+    _vector(device, "uniform", uniform, _F32, rows)
+    _vector(device, "ids", ids, _LONG, rows)
+    if logprobs is not None:
+        _vector(device, "logprobs", logprobs, _F32, rows)
+    t_ptr, t = _setting(device, "temperature", temperature, _F32, rows)
+    k_ptr, k = _setting(device, "top_k", top_k, _I32, rows)
+    p_ptr, p = _setting(device, "top_p", top_p, _F32, rows)
+    m_ptr, m = _setting(device, "min_p", min_p, _F32, rows)
+    _check_bytes(device, workspace)
     if rows == 0:
         return ids
-    _call_on(device, stream, "cascade_sample_f32", logits.data_ptr(),
-             row_stride, rows, vocab, uniform.data_ptr(), t_ptr,
-             float(t), k_ptr, int(k), p_ptr, float(p), m_ptr, float(m),
-             ids.data_ptr(), 0 if logprobs is None else logprobs.data_ptr(),
-             workspace.data_ptr(), workspace.numel())
+    _call_on(device.index, stream, "cascade_sample_f32", logits.data_ptr(),
+             row_stride, rows, vocab, uniform.data_ptr(), t_ptr, t, k_ptr, int(k),
+             p_ptr, p, m_ptr, m, ids.data_ptr(),
+             0 if logprobs is None else logprobs.data_ptr(), workspace.data_ptr(),
+             workspace.numel())
     return ids
 
 

@@ -509,3 +509,32 @@ def test_operators_on_a_stream_of_the_callers(gpu_device):
     _hip.paged_decode_attention(*args, out, ws, 0.125, stream=side)
     side.synchronize()
     assert torch.equal(out.cpu(), expected)
+
+
+def test_dimensions_of_one_with_odd_strides(gpu_device):
+    # a stride of a dimension of one is any number: nothing may depend on it
+    dev, dim = gpu_device, 64
+    g = torch.Generator().manual_seed(51)
+    pool = Pool([9], 1, dim, 16, seed=51, spare=0).to(dev)
+    storage = normal((4096,), g).to(dev)
+    q = torch.as_strided(storage, (1, 1, dim), (3, 5, 1), 512)
+    k = torch.as_strided(storage, (1, 1, dim), (7, 1, 1), 1024)
+    k_pages, v_pages = (torch.as_strided(p, (1, 1, 16, dim), (11, 13, dim, 1))
+                        for p in (pool.k, pool.v))
+    out = torch.as_strided(torch.zeros(256, dtype=torch.bfloat16, device=dev), (1, 1, dim),
+                           (9, 1, 1))
+    table = torch.as_strided(pool.table, (1, 1), (17, 19))
+    ws = workspace(1, 1, 1, dim, 16, dev)
+    _hip.paged_decode_attention(q, k_pages, v_pages, table, pool.lengths, out, ws, 0.125)
+    kk, vv, good = Pool.rows_of(pool.to("cpu"), 0, 9)
+    ref, tol = attention(q[0].cpu(), kk, vv, good, 0.125)
+    assert bool(((out[0].cpu().double() - ref).abs() <= tol).all())
+    _hip.paged_append(q, k, k, torch.tensor([9], dtype=torch.int32, device=dev), k_pages,
+                      v_pages, table, q_out=out)
+    assert torch.equal(k_pages[0, :, 9].cpu(), k[0].cpu())
+    assert torch.equal(out.cpu(), q.cpu())
+    logits = torch.as_strided(torch.randn(50, generator=g).to(dev), (1, 50), (3, 1))
+    ids = torch.empty(1, dtype=torch.int64, device=dev)
+    ws = torch.empty(_hip.sample_workspace_bytes(1, 50), dtype=torch.uint8, device=dev)
+    _hip.sample(logits, torch.zeros(1, device=dev), ids, ws, temperature=0.0)
+    assert int(ids) == int(logits.argmax())
