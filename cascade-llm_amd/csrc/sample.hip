@@ -186,20 +186,31 @@ __device__ __forceinline__ void fill_table(double *table) {
   if (j >= kTable) return;
   const int whole = j > kTable / 2 ? 1 : 0;
   const double z = (static_cast<double>(j) / kTable - whole) * 0.6931471805599453;
-  double p = 1.0, term = 1.0;
-#pragma unroll 1
-  for (int k = 12; k >= 1; --k) p = fma(p * z, 1.0 / k, term);
+  double p = 1.0;
+#pragma unroll
+  for (int k = 12; k >= 1; --k) p = fma(p * z, 1.0 / k, 1.0);
   table[j] = ldexp(p, whole + kWeightBits);
 }
 
-// Inclusive prefix sum over the wave's lanes.
-__device__ __forceinline__ u64 wave_prefix(u64 v, int lane) {
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const u64 o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
+// v plus the value that the DPP control CTRL brings in from another lane, in
+// the rows of ROWS (0 where it brings none).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_add(u64 v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xF, true);
+  return v + ((static_cast<u64>(static_cast<uint32_t>(hi)) << 32) | static_cast<uint32_t>(lo));
+}
+
+// Inclusive prefix sum over the wave's lanes (all 64 active): row_shr by 1, 2,
+// 4, 8 inside each row of 16, then lane 15 of a row into the next one
+// (row_bcast:15, rows 1 and 3) and lane 31 into the upper half (row_bcast:31).
+__device__ __forceinline__ u64 wave_prefix(u64 v) {
+  v = dpp_add<0x111, 0xF>(v);
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);
+  return dpp_add<0x143, 0xC>(v);
 }
 
 // Inclusive prefix sum over the workgroup in thread order, and its total.
@@ -208,7 +219,7 @@ template <int WAVES = kSampleWaves>
 __device__ __forceinline__ u64 block_prefix(u64 v, u64 *lds, u64 *total) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = threadIdx.x / kWave;
-  v = wave_prefix(v, lane);
+  v = wave_prefix(v);
   if (lane == kWave - 1) lds[wave] = v;
   __syncthreads();
   u64 before = 0, all = 0;
@@ -245,7 +256,7 @@ struct SampleShared {
 // The cut that keeps the fewest elements of the row, among those of `in`
 // with a weight, so that their number (BY_MASS: mass) reaches `need` >= 1;
 // *mass_kept is then the mass kept.  All elements together have to reach it.
-template <bool BY_MASS>
+template <int THREADS, bool BY_MASS>
 __device__ Cut find_cut(const float *x, int n, const RowScale &r, Cut in, u64 need,
                         SampleShared &sh, u64 *mass_kept) {
   const int tid = threadIdx.x;
@@ -256,13 +267,13 @@ __device__ Cut find_cut(const float *x, int n, const RowScale &r, Cut in, u64 ne
   for (int round = 0; round < 3; ++round) {
     const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
     const uint32_t bins = round == 2 ? 1024u : 2048u;
-    for (int b = tid; b < kSampleBins; b += kSampleThreads) {
+    for (int b = tid; b < kSampleBins; b += THREADS) {
       sh.count[b] = 0;
       sh.mass[b] = 0;
     }
     __syncthreads();
 #pragma unroll 1
-    for (int i = tid; i < n; i += kSampleThreads) {
+    for (int i = tid; i < n; i += THREADS) {
       const float v = x[i];
       const uint32_t o = ordered_bits(v);
       if ((o & known) != prefix || !keeps(in, o, i)) continue;
@@ -273,22 +284,28 @@ __device__ Cut find_cut(const float *x, int n, const RowScale &r, Cut in, u64 ne
       atomicAdd(&sh.mass[b], w);
     }
     __syncthreads();
-    // thread t scans bins 2047 - 2 t and 2046 - 2 t, from the top down
-    const int hi = kSampleBins - 1 - 2 * tid, lo = hi - 1;
-    const u64 c0 = sh.count[hi], c1 = sh.count[lo];
-    const u64 m0 = sh.mass[hi], m1 = sh.mass[lo];
-    u64 total;
-    const u64 c_end = block_prefix(c0 + c1, sh.scan, &total) + above_count;
-    const u64 m_end = block_prefix(m0 + m1, sh.scan, &total) + above_mass;
-    const u64 c_mid = c_end - c1, c_start = c_mid - c0;
-    const u64 m_mid = m_end - m1, m_start = m_mid - m0;
-    const u64 end = BY_MASS ? m_end : c_end, mid = BY_MASS ? m_mid : c_mid,
-              start = BY_MASS ? m_start : c_start;
-    if (start < need && need <= end) {
-      const bool first = need <= mid;
-      sh.found[0] = first ? hi : lo;
-      sh.found[1] = first ? c_start : c_mid;
-      sh.found[2] = first ? m_start : m_mid;
+    // thread t scans kPer bins from 2047 - kPer t on, from the top down
+    constexpr int kPer = kSampleBins / THREADS;
+    const int top = kSampleBins - 1 - kPer * tid;
+    u64 c_sum = 0, m_sum = 0, total;
+#pragma unroll 1
+    for (int j = 0; j < kPer; ++j) {
+      c_sum += sh.count[top - j];
+      m_sum += sh.mass[top - j];
+    }
+    u64 c_at = block_prefix<THREADS / kWave>(c_sum, sh.scan, &total) - c_sum + above_count;
+    u64 m_at = block_prefix<THREADS / kWave>(m_sum, sh.scan, &total) - m_sum + above_mass;
+#pragma unroll 1
+    for (int j = 0; j < kPer; ++j) {
+      const u64 c = sh.count[top - j], m = sh.mass[top - j];
+      const u64 start = BY_MASS ? m_at : c_at, end = start + (BY_MASS ? m : c);
+      if (start < need && need <= end) {
+        sh.found[0] = top - j;
+        sh.found[1] = c_at;
+        sh.found[2] = m_at;
+      }
+      c_at += c;
+      m_at += m;
     }
     __syncthreads();
     const uint32_t bin = static_cast<uint32_t>(sh.found[0]);
@@ -309,11 +326,11 @@ __device__ Cut find_cut(const float *x, int n, const RowScale &r, Cut in, u64 ne
     // the index of the take-th of them
     u64 seen = 0;
 #pragma unroll 1
-    for (int base = 0; base < n; base += kSampleThreads) {
+    for (int base = 0; base < n; base += THREADS) {
       const int i = base + tid;
       const bool hit = i < n && ordered_bits(x[i]) == prefix;
       u64 total;
-      const u64 at = seen + block_prefix(hit ? 1 : 0, sh.scan, &total);
+      const u64 at = seen + block_prefix<THREADS / kWave>(hit ? 1 : 0, sh.scan, &total);
       if (hit && at == take) sh.found[0] = i;
       seen += total;
       if (seen >= take) break;  // uniform
@@ -501,14 +518,14 @@ __device__ RowEnds find_ends(const u64 *bin_mass, const uint32_t *bin_count,
   u64 nsum = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    m[i] = mass[i];
-    n[i] = count[i];
+    m[i] = use_p ? mass[i] : 0;
+    n[i] = set.top_k > 0 ? count[i] : 0;
     msum += m[i];
     nsum += n[i];
   }
-  u64 total, live;
-  const u64 m_at = block_prefix<kWaves>(msum, s_scan, &total) - msum;
-  const u64 n_at = block_prefix<kWaves>(nsum, s_scan, &live) - nsum;
+  u64 total = 0, live = 0, m_at = 0, n_at = 0;
+  if (use_p) m_at = block_prefix<kWaves>(msum, s_scan, &total) - msum;
+  if (set.top_k > 0) n_at = block_prefix<kWaves>(nsum, s_scan, &live) - nsum;
   if (tid == 0) {
     s_ends = RowEnds{0, 0, total, 0, 0, 0, -1, -1};
     s_above[0] = s_above[1] = s_upto = 0;
@@ -630,8 +647,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
 
 struct DrawShared {
   union {
-    SampleShared row;         // the counted cut of a whole row
-    u64 keys[kListMax];       // the sorted list
+    SampleShared row;         // the counted cut of a whole row, and bins
+    u64 keys[kListMax];       // the list
   };
   u64 mass[kSampleThreads];   // of the chunks
   u64 scan[kSampleWaves];
@@ -641,11 +658,12 @@ struct DrawShared {
 };
 
 // Sorts keys[0..n) in descending order (n a power of two, at least 2).
+template <int THREADS>
 __device__ __forceinline__ void sort_keys(u64 *keys, int n) {
   for (int run = 2; run <= n; run *= 2)
     for (int gap = run / 2; gap >= 1; gap /= 2) {
       __syncthreads();
-      for (int i = threadIdx.x; i < n / 2; i += kSampleThreads) {
+      for (int i = threadIdx.x; i < n / 2; i += THREADS) {
         const int lo = 2 * i - (i & (gap - 1));
         const int hi = lo + gap;
         const u64 x = keys[lo], y = keys[hi];
@@ -658,9 +676,10 @@ __device__ __forceinline__ void sort_keys(u64 *keys, int n) {
   __syncthreads();
 }
 
-// The same for up to 1024 keys, one a thread (v; 0 past the list): runs of 64
+// The same for up to THREADS keys, one a thread (v; 0 past the list): runs of 64
 // are sorted and merged in a wave's registers, and only the steps over a
-// longer gap go through LDS.  The sorted keys end up in keys[0..1024).
+// longer gap go through LDS.  The sorted keys end up in keys[0..THREADS).
+template <int THREADS>
 __device__ __forceinline__ u64 sort_block(u64 v, int n, u64 *keys) {
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
@@ -677,7 +696,7 @@ __device__ __forceinline__ u64 sort_block(u64 v, int n, u64 *keys) {
   for (int run = 2 * kWave; run < 2 * kWave * runs; run *= 2) {
     const bool down = (tid & run) != 0;
     for (int gap = run / 2; gap >= kWave; gap /= 2) {
-      u64 *half = keys + side * kSampleThreads;
+      u64 *half = keys + side * THREADS;
       half[tid] = v;
       __syncthreads();
       const u64 other = half[tid ^ gap];
@@ -693,20 +712,20 @@ __device__ __forceinline__ u64 sort_block(u64 v, int n, u64 *keys) {
 }
 
 // The key of the last token of the row's P (or K) in its list of n keys, of
-// which this thread has keys tid, tid + 1024, ...  PER: keys a thread holds.
+// which this thread has key tid (PER = 1).  PER: keys a thread holds.
 // Positions of the sorted list (in sh.keys): K's last bin starts at e.before.
-template <int PER>
+template <int THREADS, int PER>
 __device__ u64 list_cut(const u64 *list, int n, u64 mine, const RowEnds &e,
                         const RowSettings &set, const RowScale &r, DrawShared &sh) {
   const int tid = threadIdx.x;
   if constexpr (PER == 1) {
-    sort_block(mine, n, sh.keys);
+    sort_block<THREADS>(mine, n, sh.keys);
   } else {
     int padded = 2;
     while (padded < n) padded *= 2;
     // (the list may be in sh.keys already)
-    for (int i = tid; i < padded; i += kSampleThreads) sh.keys[i] = i < n ? list[i] : 0;
-    sort_keys(sh.keys, padded);
+    for (int i = tid; i < padded; i += THREADS) sh.keys[i] = i < n ? list[i] : 0;
+    sort_keys<THREADS>(sh.keys, padded);
   }
   const int last_k = static_cast<int>(e.before + e.need_k) - 1;
   if (e.last_p < 0) return sh.keys[last_k];
@@ -719,7 +738,7 @@ __device__ u64 list_cut(const u64 *list, int n, u64 mine, const RowEnds &e,
     sum += w[i];
   }
   u64 total;
-  const u64 start = block_prefix(sum, sh.scan, &total) - sum;
+  const u64 start = block_prefix<THREADS / kWave>(sum, sh.scan, &total) - sum;
   u64 mass_k = e.total;
   if (e.last_k >= 0) {
     // mass of the list before K's last bin, and up to K's last token
@@ -747,13 +766,14 @@ __device__ u64 list_cut(const u64 *list, int n, u64 mine, const RowEnds &e,
 }
 
 // The cut of a row found over the whole row, as a key.
+template <int THREADS>
 __device__ u64 counted_cut(const float *x, int n, const RowScale &r, const RowSettings &set,
                            u64 mass_all, u64 live, SampleShared &sh) {
   Cut cut{0u, 0xffffffffu};
   if (set.top_k > 0 && static_cast<u64>(set.top_k) < live)
-    cut = find_cut<false>(x, n, r, cut, static_cast<u64>(set.top_k), sh, &mass_all);
+    cut = find_cut<THREADS, false>(x, n, r, cut, static_cast<u64>(set.top_k), sh, &mass_all);
   if (set.top_p < 1.0)
-    cut = find_cut<true>(x, n, r, cut, top_p_mass(set.top_p, mass_all), sh,
+    cut = find_cut<THREADS, true>(x, n, r, cut, top_p_mass(set.top_p, mass_all), sh,
                          &mass_all);
   return (static_cast<u64>(cut.value) << 32) | (0xffffffffu - cut.index);
 }
@@ -819,7 +839,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
       u64 live_all, mass_all;
       block_prefix(live, sh.scan, &live_all);
       block_prefix(sum, sh.scan, &mass_all);
-      cut = counted_cut(x, a.vocab, r, set, mass_all, live_all, sh.row);
+      cut = counted_cut<kSampleThreads>(x, a.vocab, r, set, mass_all, live_all, sh.row);
       // the chunks' masses, a wave a chunk
 #pragma unroll 1
       for (int c = tid / kWave; c < a.chunks; c += kSampleWaves) {
@@ -830,7 +850,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
           const u64 w = fixed_weight(x[i], r);
           if (w >= set.min_w && topk_key(x[i], static_cast<uint32_t>(i)) >= cut) part += w;
         }
-        part = wave_prefix(part, tid & (kWave - 1));
+        part = wave_prefix(part);
         if ((tid & (kWave - 1)) == kWave - 1) sh.mass[c] = part;
       }
       __syncthreads();
@@ -839,8 +859,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
       if (tid < a.chunks) sh.mass[tid] = mass;
       const int n = static_cast<int>(entries);
       cut = n <= kSampleThreads
-                ? list_cut<1>(nullptr, n, tid < n ? key : 0, e, set, r, sh)
-                : list_cut<kListMax / kSampleThreads>(
+                ? list_cut<kSampleThreads, 1>(nullptr, n, tid < n ? key : 0, e, set, r, sh)
+                : list_cut<kSampleThreads, kListMax / kSampleThreads>(
                       a.list + static_cast<int64_t>(row) * kListMax, n, 0, e, set, r, sh);
       // what the list adds to its chunks
       for (int i = tid; i < static_cast<int>(entries); i += kSampleThreads) {
@@ -905,19 +925,22 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
 
 // A row of at most kShortVocab logits in one launch: the row stays in the
 // registers of one workgroup, its bins and its list in LDS.
-__global__ __launch_bounds__(kSampleThreads) void sample_short_kernel(SampleArgs a) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
   __shared__ DrawShared sh;
+  constexpr int kWaves = THREADS / kWave;
+  __shared__ float s_max[kWaves];
   __shared__ uint32_t s_count;
   const int row = blockIdx.x;
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
   const int wave = tid / kWave;
   const float *x = a.logits + row * a.row_stride;
-  const Chunk<kSampleThreads, kShortVecs> logits(x, 0, a.vocab);
+  const Chunk<THREADS, kShortVecs> logits(x, 0, a.vocab);
   const double uniform = static_cast<double>(a.uniform[row]);
   const RowSettings set = row_settings(a, row);
   fill_table(sh.table);
-  for (int b = tid; b < kSampleBins; b += kSampleThreads) {
+  for (int b = tid; b < kSampleBins; b += THREADS) {
     sh.row.count[b] = 0;
     sh.row.mass[b] = 0;
   }
@@ -928,11 +951,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_short_kernel(SampleArgs
   float mx = -INFINITY;
   logits.each([&](float v, int) { mx = nan_max(mx, v); });
   mx = wave_nan_max(mx);
-  float *s_max = reinterpret_cast<float *>(sh.mass);
   if (lane == 0) s_max[wave] = mx;
   __syncthreads();
 #pragma unroll 4
-  for (int w = 0; w < kSampleWaves; ++w) mx = nan_max(mx, s_max[w]);
+  for (int w = 0; w < kWaves; ++w) mx = nan_max(mx, s_max[w]);
   if (no_token(mx)) {
     if (tid == 0) {
       a.ids[row] = -1;
@@ -963,7 +985,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_short_kernel(SampleArgs
       if (use_p) atomicAdd(&sh.row.mass[b], fixed_weight(t, sh.table));
     });
     __syncthreads();
-    const RowEnds e = find_ends<kSampleThreads>(sh.row.mass, sh.row.count, set);
+    const RowEnds e = find_ends<THREADS>(sh.row.mass, sh.row.count, set);
     if (e.last_p >= 0 || e.last_k >= 0) {
       __syncthreads();  // the list takes the place of the bins
       logits.each([&](float v, int i) {
@@ -983,15 +1005,15 @@ __global__ __launch_bounds__(kSampleThreads) void sample_short_kernel(SampleArgs
           sum += w;
         });
         u64 live_all, mass_all;
-        block_prefix(live, sh.scan, &live_all);
-        block_prefix(sum, sh.scan, &mass_all);
-        cut = counted_cut(x, a.vocab, r, set, mass_all, live_all, sh.row);
-      } else if (n <= kSampleThreads) {
+        block_prefix<kWaves>(live, sh.scan, &live_all);
+        block_prefix<kWaves>(sum, sh.scan, &mass_all);
+        cut = counted_cut<THREADS>(x, a.vocab, r, set, mass_all, live_all, sh.row);
+      } else if (n <= THREADS) {
         const u64 key = tid < n ? sh.keys[tid] : 0;
         __syncthreads();  // the sort writes sh.keys
-        cut = list_cut<1>(nullptr, n, key, e, set, r, sh);
+        cut = list_cut<THREADS, 1>(nullptr, n, key, e, set, r, sh);
       } else {
-        cut = list_cut<kListMax / kSampleThreads>(sh.keys, n, 0, e, set, r, sh);
+        cut = list_cut<THREADS, kListMax / THREADS>(sh.keys, n, 0, e, set, r, sh);
       }
     }
   }
@@ -1009,19 +1031,19 @@ __global__ __launch_bounds__(kSampleThreads) void sample_short_kernel(SampleArgs
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[j] += weight_of(logits.v[j][i], logits.at(j) + i);
     }
-    sum[j] = wave_prefix(sum[j], lane);
-    if (lane == kWave - 1) sh.mass[j * kSampleWaves + wave] = sum[j];
+    sum[j] = wave_prefix(sum[j]);
+    if (lane == kWave - 1) sh.mass[j * kWaves + wave] = sum[j];
   }
   const int last = logits.whole + tid;
   sum[kShortVecs] = last < logits.end ? weight_of(logits.rest, last) : 0;
-  sum[kShortVecs] = wave_prefix(sum[kShortVecs], lane);
-  if (tid == kWave - 1) sh.mass[kShortVecs * kSampleWaves] = sum[kShortVecs];
+  sum[kShortVecs] = wave_prefix(sum[kShortVecs]);
+  if (tid == kWave - 1) sh.mass[kShortVecs * kWaves] = sum[kShortVecs];
   __syncthreads();
   // prefix sums of the waves' masses: one a lane of the first waves
-  constexpr int kParts = kShortVecs * kSampleWaves + 1;
+  constexpr int kParts = kShortVecs * kWaves + 1;
   u64 total;
   const u64 part = tid < kParts ? sh.mass[tid] : 0;
-  const u64 upto = block_prefix(part, sh.scan, &total);
+  const u64 upto = block_prefix<kWaves>(part, sh.scan, &total);
   if (tid < kParts) sh.mass[tid] = upto - part;
   __syncthreads();
   const double u = uniform > 0.0 ? uniform : 0.0;  // NaN too
@@ -1031,7 +1053,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_short_kernel(SampleArgs
 #pragma unroll
   for (int j = 0; j <= kShortVecs; ++j) {
     if (j == kShortVecs && wave != 0) break;
-    const u64 base = sh.mass[j * kSampleWaves + (j < kShortVecs ? wave : 0)];
+    const u64 base = sh.mass[j * kWaves + (j < kShortVecs ? wave : 0)];
     // this thread's share of vector j: from the lane before it on
     u64 at = __shfl_up(sum[j], 1);
     at = base + (lane == 0 ? 0 : at);
@@ -1130,8 +1152,12 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
     a.min_p = min_p;
     a.ids = ids;
     a.logprobs = logprobs;
-    return launch_kernel(sample_short_kernel, dim3(static_cast<unsigned>(rows)),
-                         dim3(kSampleThreads), 0, s, a);
+    const dim3 grid(static_cast<unsigned>(rows));
+    // as few waves as hold the row: every sum waits for all of them
+    if (vocab <= 4 * 256 * kShortVecs)
+      return launch_kernel(sample_short_kernel<256>, grid, dim3(256), 0, s, a);
+    return launch_kernel(sample_short_kernel<kSampleThreads>, grid, dim3(kSampleThreads), 0,
+                         s, a);
   }
   const SamplePlan p = sample_plan(rows, vocab);
   a.chunk = static_cast<int32_t>(p.chunk);
