@@ -392,19 +392,29 @@ struct Chunk {
     return begin + 4 * (THREADS * j + static_cast<int>(threadIdx.x));
   }
 
-  // f(logit, index) for each
+  // f(logits, index of the first) for every four neighbours: f
+  // does the arithmetic of all four before it branches on any, so that their
+  // chains of fp64 instructions overlap.  The rest comes as one logit with
+  // three -inf.
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll
     for (int j = 0; j < VECS; ++j)
-      if (at(j) < whole) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f(v[j][i], at(j) + i);
-      }
+      if (at(j) < whole) f(v[j], at(j));
     const int i = whole + static_cast<int>(threadIdx.x);
-    if (i < end) f(rest, i);
+    if (i < end) f(f32x4_at4{rest, -INFINITY, -INFINITY, -INFINITY}, i);
   }
 };
+
+// Bins of four logits.
+__device__ __forceinline__ void bins_of(const f32x4_at4 &v, const RowScale &r, double (&t)[4],
+                                        int (&b)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t[i] = log_weight(v[i], r);
+    b[i] = weight_bin(t[i]);
+  }
+}
 
 __device__ __forceinline__ Chunk<kChunkThreads, kChunkVecs> row_chunk(const SampleArgs &a,
                                                                       int row, int chunk) {
@@ -428,7 +438,9 @@ __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a)
   }
   if (chunk == 0 && tid == 0) a.list_count[row] = 0;
   float best = -INFINITY;
-  logits.each([&](float v, int) { best = nan_max(best, v); });
+  logits.each([&](const f32x4_at4 &v, int) {
+    best = nan_max(nan_max(best, nan_max(v[0], v[1])), nan_max(v[2], v[3]));
+  });
   best = wave_nan_max(best);
   if ((tid & (kWave - 1)) == 0) s_max[tid / kWave] = best;
   __syncthreads();
@@ -437,6 +449,25 @@ __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a)
     for (int w = 1; w < kChunkThreads / kWave; ++w) best = nan_max(best, s_max[w]);
     a.chunk_max[static_cast<int64_t>(row) * a.chunks + chunk] = best;
   }
+}
+
+// Adds four logits to their bins: their number, and their mass.
+__device__ __forceinline__ void add_to_bins(const f32x4_at4 &v, const RowScale &r, bool use_k,
+                                            bool use_p, uint32_t *count, u64 *mass) {
+  double t[4];
+  int b[4];
+  u64 w[4];
+  bins_of(v, r, t, b);
+  if (use_p) {  // uniform
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = fixed_weight(t[i], r.table);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (b[i] < kSampleBins) {
+      if (use_k) atomicAdd(&count[b[i]], 1u);
+      if (use_p) atomicAdd(&mass[b[i]], w[i]);
+    }
 }
 
 __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs a) {
@@ -455,9 +486,12 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
   if (set.top_k <= 0 && set.top_p >= 1.0) {
     __syncthreads();
     u64 sum = 0;
-    logits.each([&](float v, int) {
-      const u64 w = fixed_weight(v, r);
-      sum += w >= set.min_w ? w : 0;
+    logits.each([&](const f32x4_at4 &v, int) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u64 w = fixed_weight(v[i], r);
+        sum += w >= set.min_w ? w : 0;
+      }
     });
     u64 total;
     block_prefix<kChunkThreads / kWave>(sum, s_mass, &total);
@@ -471,12 +505,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
     s_count[i] = 0;
   }
   __syncthreads();
-  logits.each([&](float v, int) {
-    const double t = log_weight(v, r);
-    const int b = weight_bin(t);
-    if (b >= kSampleBins) return;
-    if (use_k) atomicAdd(&s_count[b], 1u);
-    if (use_p) atomicAdd(&s_mass[b], fixed_weight(t, s_table));
+  logits.each([&](const f32x4_at4 &v, int) {
+    add_to_bins(v, r, use_k, use_p, s_count, s_mass);
   });
   __syncthreads();
   u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins;
@@ -586,6 +616,22 @@ __device__ RowEnds find_ends(const u64 *bin_mass, const uint32_t *bin_count,
   return e;
 }
 
+// Puts those of four logits that are in a listed bin (from `first` on) on a
+// list of kListMax; *count counts them all.
+__device__ __forceinline__ void list_of(const f32x4_at4 &v, int at, const int (&b)[4], int first,
+                                        const RowEnds &e, u64 *list, uint32_t *count) {
+  bool in[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) in[i] = b[i] >= first && (b[i] <= e.last_p || b[i] == e.last_k);
+  if (!(in[0] || in[1] || in[2] || in[3])) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (in[i]) {
+      const uint32_t n = atomicAdd(count, 1u);
+      if (n < kListMax) list[n] = topk_key(v[i], static_cast<uint32_t>(at + i));
+    }
+}
+
 __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArgs a) {
   __shared__ u64 s_keys[kListMax];
   __shared__ uint32_t s_count, s_at;
@@ -616,18 +662,19 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   }
   if (tid == 0) s_count = 0;
   __syncthreads();
-  logits.each([&](float v, int i) {
-    const double t = log_weight(v, r);
-    const int b = weight_bin(t);
-    if (b >= kSampleBins) return;
-    if (b < first) {
-      if (summed) return;
-      const u64 w = fixed_weight(t, s_table);
-      sum += w >= set.min_w ? w : 0;
-    } else if (b <= e.last_p || b == e.last_k) {
-      const uint32_t at = atomicAdd(&s_count, 1u);
-      if (at < kListMax) s_keys[at] = topk_key(v, static_cast<uint32_t>(i));
+  logits.each([&](const f32x4_at4 &v, int at) {
+    double t[4];
+    int b[4];
+    bins_of(v, r, t, b);
+    const int least = min(min(b[0], b[1]), min(b[2], b[3]));
+    if (!summed && least < first) {
+      u64 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = fixed_weight(t[i], s_table);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += b[i] < first && w[i] >= set.min_w ? w[i] : 0;
     }
+    list_of(v, at, b, first, e, s_keys, &s_count);
   });
   u64 total;
   block_prefix<kChunkThreads / kWave>(sum, s_scan, &total);
@@ -949,7 +996,9 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
     sh.first[0] = 0x7fffffff;
   }
   float mx = -INFINITY;
-  logits.each([&](float v, int) { mx = nan_max(mx, v); });
+  logits.each([&](const f32x4_at4 &v, int) {
+    mx = nan_max(nan_max(mx, nan_max(v[0], v[1])), nan_max(v[2], v[3]));
+  });
   mx = wave_nan_max(mx);
   if (lane == 0) s_max[wave] = mx;
   __syncthreads();
@@ -964,7 +1013,10 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
   }
   if (set.greedy) {
     int at = 0x7fffffff;
-    logits.each([&](float v, int i) { at = v == mx ? min(at, i) : at; });
+    logits.each([&](const f32x4_at4 &v, int first) {
+#pragma unroll
+      for (int i = 3; i >= 0; --i) at = v[i] == mx ? min(at, first + i) : at;
+    });
     if (at != 0x7fffffff) atomicMin(&sh.first[0], at);
     __syncthreads();
     if (tid == 0) {
@@ -977,32 +1029,30 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
   const bool use_k = set.top_k > 0, use_p = set.top_p < 1.0;
   u64 cut = 0;
   if (use_k || use_p) {
-    logits.each([&](float v, int) {
-      const double t = log_weight(v, r);
-      const int b = weight_bin(t);
-      if (b >= kSampleBins) return;
-      if (use_k) atomicAdd(&sh.row.count[b], 1u);
-      if (use_p) atomicAdd(&sh.row.mass[b], fixed_weight(t, sh.table));
+    logits.each([&](const f32x4_at4 &v, int) {
+      add_to_bins(v, r, use_k, use_p, sh.row.count, sh.row.mass);
     });
     __syncthreads();
     const RowEnds e = find_ends<THREADS>(sh.row.mass, sh.row.count, set);
     if (e.last_p >= 0 || e.last_k >= 0) {
       __syncthreads();  // the list takes the place of the bins
-      logits.each([&](float v, int i) {
-        const int b = weight_bin(log_weight(v, r));
-        if (b >= e.first && (b <= e.last_p || b == e.last_k)) {
-          const uint32_t at = atomicAdd(&s_count, 1u);
-          if (at < kListMax) sh.keys[at] = topk_key(v, static_cast<uint32_t>(i));
-        }
+      logits.each([&](const f32x4_at4 &v, int at) {
+        double t[4];
+        int b[4];
+        bins_of(v, r, t, b);
+        list_of(v, at, b, e.first, e, sh.keys, &s_count);
       });
       __syncthreads();
       const int n = static_cast<int>(s_count);
       if (n > kListMax) {
         u64 live = 0, sum = 0;
-        logits.each([&](float v, int) {
-          const u64 w = fixed_weight(v, r);
-          live += w != 0 ? 1 : 0;
-          sum += w;
+        logits.each([&](const f32x4_at4 &v, int) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const u64 w = fixed_weight(v[i], r);
+            live += w != 0 ? 1 : 0;
+            sum += w;
+          }
         });
         u64 live_all, mass_all;
         block_prefix<kWaves>(live, sh.scan, &live_all);
