@@ -23,7 +23,9 @@
 //                            or top-p), or the chunk's mass (other rows)
 //   3. sample_collect_kernel the bins in which K and P end, from those sums;
 //                            their tokens go to a list, the mass of the
-//                            bins above is kept by chunk
+//                            bins above is kept by chunk.  A K of at most
+//                            kShortK tokens is listed whole, which spares
+//                            its row the masses.
 //   4. sample_draw_kernel    one workgroup a row: sorts the list, finds the
 //                            two ends in it, draws a chunk and then its token
 // A row whose list would be longer than kListMax (ends in runs of equal
@@ -43,6 +45,7 @@ constexpr int kWeightBits = 44;
 constexpr u64 kWeightOne = u64{1} << kWeightBits;
 constexpr int64_t kSampleMaxVocab = int64_t{1} << 19;
 constexpr int kListMax = 4096;
+constexpr int kShortK = 1024;  // K up to this size is listed whole
 constexpr int kChunkThreads = 256;
 constexpr int kChunkMin = 2048;
 constexpr int kChunkMax = 8192;
@@ -103,6 +106,8 @@ struct RowEnds {
 
 struct RowSettings {
   bool greedy;
+  bool use_k;     // there is a top-k
+  bool use_p;     // the bins' masses are needed: a top-p, and no short K
   double scale;   // 32 log2(e) / T
   int64_t top_k;  // <= 0: off
   double top_p;   // >= 1: off
@@ -121,6 +126,8 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs &a, int row
   r.min_w = p > 0.0 ? static_cast<u64>(ceil(fmin(p, 1.0) * static_cast<double>(kWeightOne)))
                     : u64{0};
   if (p > 1.0) r.top_k = 1;  // none reaches it: the likeliest alone stays
+  r.use_k = r.top_k > 0;
+  r.use_p = r.top_p < 1.0 && !(r.use_k && r.top_k <= kShortK);
   return r;
 }
 
@@ -483,7 +490,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
   const float mx = row_max(a, row);
   if (set.greedy || no_token(mx)) return;
   const RowScale r = row_scale(mx, set, s_table);
-  if (set.top_k <= 0 && set.top_p >= 1.0) {
+  if (!set.use_k && !set.use_p) {
     __syncthreads();
     u64 sum = 0;
     logits.each([&](const f32x4_at4 &v, int) {
@@ -499,7 +506,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
     return;
   }
   // top-k needs the numbers, top-p the masses
-  const bool use_k = set.top_k > 0, use_p = set.top_p < 1.0;
+  const bool use_k = set.use_k, use_p = set.use_p;
   for (int i = tid; i < kSampleBins; i += kChunkThreads) {
     s_mass[i] = 0;
     s_count[i] = 0;
@@ -526,13 +533,28 @@ __device__ __forceinline__ u64 top_p_mass(double top_p, u64 mass) {
   return n < mass ? n : mass;
 }
 
-// The ends of K and P in the row's bins, by a workgroup of THREADS.
-// K's last bin is exact; P's is known up to what K takes of its last bin, so
-// every bin in which P could end is listed.
+// A thread's share of the bins, neighbours.
 template <int THREADS>
-__device__ RowEnds find_ends(const u64 *bin_mass, const uint32_t *bin_count,
-                             const RowSettings &set) {
-  constexpr int kPer = kSampleBins / THREADS;
+struct BinShare {
+  static constexpr int kPer = kSampleBins / THREADS;
+  u64 mass[kPer];
+  uint32_t count[kPer];
+
+  __device__ __forceinline__ BinShare(const u64 *bin_mass, const uint32_t *bin_count) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      mass[i] = bin_mass[threadIdx.x * kPer + i];
+      count[i] = bin_count[threadIdx.x * kPer + i];
+    }
+  }
+};
+
+// The ends of K and P in the row's bins, by a workgroup of THREADS.  K's last
+// bin is exact; P's is known up to what K takes of its last bin, so every bin
+// in which P could end is listed.  A short K is listed from bin 0 on.
+template <int THREADS>
+__device__ RowEnds find_ends(const BinShare<THREADS> &bins, const RowSettings &set) {
+  constexpr int kPer = BinShare<THREADS>::kPer;
   constexpr int kWaves = THREADS / kWave;
   __shared__ u64 s_scan[kWaves];
   __shared__ RowEnds s_ends;
@@ -540,44 +562,38 @@ __device__ RowEnds find_ends(const u64 *bin_mass, const uint32_t *bin_count,
   __shared__ uint32_t s_above[2];  // tokens above the first listed bin, above K's last
   __shared__ uint32_t s_upto;      // tokens up to P's last candidate
   const int tid = threadIdx.x;
-  const bool use_p = set.top_p < 1.0;
-  const u64 *mass = bin_mass + tid * kPer;
-  const uint32_t *count = bin_count + tid * kPer;
-  u64 m[kPer], msum = 0;
-  uint32_t n[kPer];
-  u64 nsum = 0;
+  const bool short_k = set.use_k && set.top_k <= kShortK;
+  u64 msum = 0, nsum = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    m[i] = use_p ? mass[i] : 0;
-    n[i] = set.top_k > 0 ? count[i] : 0;
-    msum += m[i];
-    nsum += n[i];
+    msum += bins.mass[i];
+    nsum += bins.count[i];
   }
   u64 total = 0, live = 0, m_at = 0, n_at = 0;
-  if (use_p) m_at = block_prefix<kWaves>(msum, s_scan, &total) - msum;
-  if (set.top_k > 0) n_at = block_prefix<kWaves>(nsum, s_scan, &live) - nsum;
+  if (set.use_p) m_at = block_prefix<kWaves>(msum, s_scan, &total) - msum;
+  if (set.use_k) n_at = block_prefix<kWaves>(nsum, s_scan, &live) - nsum;
   if (tid == 0) {
     s_ends = RowEnds{0, 0, total, 0, 0, 0, -1, -1};
     s_above[0] = s_above[1] = s_upto = 0;
   }
   __syncthreads();
-  const bool use_k = set.top_k > 0 && static_cast<u64>(set.top_k) < live;
+  const bool use_k = set.use_k && (short_k || static_cast<u64>(set.top_k) < live);
   u64 k_least = total, k_most = total;
   if (use_k) {
-    const u64 need = static_cast<u64>(set.top_k);
+    const u64 need = min(static_cast<u64>(set.top_k), live);
     u64 ma = m_at, na = n_at;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (na < need && need <= na + n[i]) {
+      if (na < need && need <= na + bins.count[i]) {
         s_ends.above_k = ma;
         s_ends.need_k = static_cast<uint32_t>(need - na);
         s_ends.last_k = tid * kPer + i;
         s_ends.first = tid * kPer + i;
         s_above[1] = static_cast<uint32_t>(na);
-        s_most = ma + m[i];
+        s_most = ma + bins.mass[i];
       }
-      ma += m[i];
-      na += n[i];
+      ma += bins.mass[i];
+      na += bins.count[i];
     }
     __syncthreads();
     k_most = s_most;
@@ -585,27 +601,31 @@ __device__ RowEnds find_ends(const u64 *bin_mass, const uint32_t *bin_count,
     k_least = min(s_ends.above_k + 1, k_most);
   }
   __syncthreads();
-  if (use_p) {
+  if (set.use_p) {
     const u64 least = top_p_mass(set.top_p, k_least), most = top_p_mass(set.top_p, k_most);
     u64 ma = m_at, na = n_at;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (ma < least && least <= ma + m[i]) {
+      if (ma < least && least <= ma + bins.mass[i]) {
         s_ends.first = tid * kPer + i;
         s_ends.above_p = ma;
         s_above[0] = static_cast<uint32_t>(na);
       }
-      if (ma < most && most <= ma + m[i]) {
+      if (ma < most && most <= ma + bins.mass[i]) {
         s_ends.last_p = tid * kPer + i;
-        s_upto = static_cast<uint32_t>(na + n[i]);
+        s_upto = static_cast<uint32_t>(na + bins.count[i]);
       }
-      ma += m[i];
-      na += n[i];
+      ma += bins.mass[i];
+      na += bins.count[i];
     }
   }
   __syncthreads();
   RowEnds e = s_ends;
-  if (use_p && use_k) {
+  if (short_k) {
+    e.first = 0;
+    e.before = s_above[1];
+    e.last_p = e.last_k;
+  } else if (set.use_p && use_k) {
     if (e.last_p >= e.last_k) {  // one run of bins: first .. last_k
       e.before = s_above[1] - s_above[0];
       e.last_p = e.last_k;
@@ -641,24 +661,31 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
   const auto logits = row_chunk(a, row, chunk);
+  const BinShare<kChunkThreads> bins(a.bin_mass + static_cast<int64_t>(row) * kSampleBins,
+                                     a.bin_count + static_cast<int64_t>(row) * kSampleBins);
+  // the chunk's own bins (not written, nor used, where there is no top-p)
+  constexpr int kPer = BinShare<kChunkThreads>::kPer;
+  const u64 *chunk_bins =
+      a.chunk_bins + (static_cast<int64_t>(row) * a.chunks + chunk) * kSampleBins;
+  u64 own[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) own[i] = chunk_bins[tid * kPer + i];
   fill_table(s_table);
   const RowSettings set = row_settings(a, row);
   const float mx = row_max(a, row);
-  if (set.greedy || no_token(mx) || (set.top_k <= 0 && set.top_p >= 1.0)) return;
-  const RowEnds e = find_ends<kChunkThreads>(
-      a.bin_mass + static_cast<int64_t>(row) * kSampleBins,
-      a.bin_count + static_cast<int64_t>(row) * kSampleBins, set);
+  if (set.greedy || no_token(mx) || (!set.use_k && !set.use_p)) return;
+  const RowEnds e = find_ends(bins, set);
   if (chunk == 0 && tid == 0) a.ends[row] = e;
   // without a cut inside the bins (top_k of all tokens) nothing is listed
   const int first = e.last_p < 0 && e.last_k < 0 ? kSampleBins : e.first;
   const RowScale r = row_scale(mx, set, s_table);
   // the mass of the bins above the listed ones: from the chunk's own bins
   // where they hold it (and min-p drops none of it)
-  const bool summed = set.top_p < 1.0 && set.min_w == 0;
+  const bool summed = set.use_p && set.min_w == 0;
   u64 sum = 0;
   if (summed) {
-    const u64 *bins = a.chunk_bins + (static_cast<int64_t>(row) * a.chunks + chunk) * kSampleBins;
-    for (int i = tid; i < first; i += kChunkThreads) sum += bins[i];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += tid * kPer + i < first ? own[i] : 0;
   }
   if (tid == 0) s_count = 0;
   __syncthreads();
@@ -775,7 +802,7 @@ __device__ u64 list_cut(const u64 *list, int n, u64 mine, const RowEnds &e,
     sort_keys<THREADS>(sh.keys, padded);
   }
   const int last_k = static_cast<int>(e.before + e.need_k) - 1;
-  if (e.last_p < 0) return sh.keys[last_k];
+  if (!(set.top_p < 1.0)) return sh.keys[last_k];
   // prefix sums of the weights, PER neighbours a thread
   u64 w[PER], sum = 0;
 #pragma unroll
@@ -798,7 +825,7 @@ __device__ u64 list_cut(const u64 *list, int n, u64 mine, const RowEnds &e,
       if (at == last_k) sh.found[1] = upto;
     }
     __syncthreads();
-    mass_k = e.above_k + (sh.found[1] - sh.found[0]);
+    mass_k = e.first == 0 ? sh.found[1] : e.above_k + (sh.found[1] - sh.found[0]);
     __syncthreads();
   }
   const u64 need = top_p_mass(set.top_p, mass_k);
@@ -874,7 +901,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   __syncthreads();  // the table
   const RowScale r = row_scale(mx, set, sh.table);
   u64 cut = 0;
-  if (set.top_k > 0 || set.top_p < 1.0) {
+  if (set.use_k || set.use_p) {
     if (entries > kListMax) {
       u64 live = 0, sum = 0;
 #pragma unroll 1
@@ -1026,14 +1053,14 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
     return;
   }
   const RowScale r = row_scale(mx, set, sh.table);
-  const bool use_k = set.top_k > 0, use_p = set.top_p < 1.0;
+  const bool use_k = set.use_k, use_p = set.use_p;
   u64 cut = 0;
   if (use_k || use_p) {
     logits.each([&](const f32x4_at4 &v, int) {
       add_to_bins(v, r, use_k, use_p, sh.row.count, sh.row.mass);
     });
     __syncthreads();
-    const RowEnds e = find_ends<THREADS>(sh.row.mass, sh.row.count, set);
+    const RowEnds e = find_ends(BinShare<THREADS>(sh.row.mass, sh.row.count), set);
     if (e.last_p >= 0 || e.last_k >= 0) {
       __syncthreads();  // the list takes the place of the bins
       logits.each([&](const f32x4_at4 &v, int at) {
