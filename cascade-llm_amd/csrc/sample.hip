@@ -112,6 +112,7 @@ struct RowSettings {
   int64_t top_k;  // <= 0: off
   double top_p;   // >= 1: off
   u64 min_w;      // smallest weight kept
+  int min_bin;    // from this bin on no token has it
 };
 
 __device__ __forceinline__ RowSettings row_settings(const SampleArgs &a, int row) {
@@ -126,6 +127,12 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs &a, int row
   r.min_w = p > 0.0 ? static_cast<u64>(ceil(fmin(p, 1.0) * static_cast<double>(kWeightOne)))
                     : u64{0};
   if (p > 1.0) r.top_k = 1;  // none reaches it: the likeliest alone stays
+  // (a bin of margin for log2f)
+  r.min_bin = p > 0.0 ? static_cast<int>(fminf(-log2f(static_cast<float>(fmin(p, 1.0))) *
+                                                   static_cast<float>(kTable * kBinsPerStep) +
+                                               2.0f,
+                                           static_cast<float>(kSampleBins)))
+                      : kSampleBins;
   r.use_k = r.top_k > 0;
   r.use_p = r.top_p < 1.0 && !(r.use_k && r.top_k <= kShortK);
   return r;
@@ -494,9 +501,15 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
     __syncthreads();
     u64 sum = 0;
     logits.each([&](const f32x4_at4 &v, int) {
+      double t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = log_weight(v[i], r);
+      if (set.min_w != 0 &&
+          weight_bin(fmax(fmax(t[0], t[1]), fmax(t[2], t[3]))) >= set.min_bin)
+        return;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const u64 w = fixed_weight(v[i], r);
+        const u64 w = fixed_weight(t[i], s_table);
         sum += w >= set.min_w ? w : 0;
       }
     });
@@ -533,25 +546,35 @@ __device__ __forceinline__ u64 top_p_mass(double top_p, u64 mass) {
   return n < mass ? n : mass;
 }
 
-// A thread's share of the bins, neighbours.
+// A thread's share of the bins, neighbours: what the row's settings need.
 template <int THREADS>
 struct BinShare {
   static constexpr int kPer = kSampleBins / THREADS;
   u64 mass[kPer];
   uint32_t count[kPer];
 
-  __device__ __forceinline__ BinShare(const u64 *bin_mass, const uint32_t *bin_count) {
+  __device__ __forceinline__ BinShare(const u64 *bin_mass, const uint32_t *bin_count,
+                                      const RowSettings &set) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      mass[i] = bin_mass[threadIdx.x * kPer + i];
-      count[i] = bin_count[threadIdx.x * kPer + i];
+      mass[i] = 0;
+      count[i] = 0;
+    }
+    if (set.use_p) {  // uniform
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) mass[i] = bin_mass[threadIdx.x * kPer + i];
+    }
+    if (set.use_k) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) count[i] = bin_count[threadIdx.x * kPer + i];
     }
   }
 };
 
 // The ends of K and P in the row's bins, by a workgroup of THREADS.  K's last
 // bin is exact; P's is known up to what K takes of its last bin, so every bin
-// in which P could end is listed.  A short K is listed from bin 0 on.
+// in which P could end is listed.  A short K that a top-p follows is listed from
+// bin 0 on.
 template <int THREADS>
 __device__ RowEnds find_ends(const BinShare<THREADS> &bins, const RowSettings &set) {
   constexpr int kPer = BinShare<THREADS>::kPer;
@@ -621,7 +644,7 @@ __device__ RowEnds find_ends(const BinShare<THREADS> &bins, const RowSettings &s
   }
   __syncthreads();
   RowEnds e = s_ends;
-  if (short_k) {
+  if (short_k && set.top_p < 1.0) {
     e.first = 0;
     e.before = s_above[1];
     e.last_p = e.last_k;
@@ -661,27 +684,30 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
   const auto logits = row_chunk(a, row, chunk);
-  const BinShare<kChunkThreads> bins(a.bin_mass + static_cast<int64_t>(row) * kSampleBins,
-                                     a.bin_count + static_cast<int64_t>(row) * kSampleBins);
-  // the chunk's own bins (not written, nor used, where there is no top-p)
-  constexpr int kPer = BinShare<kChunkThreads>::kPer;
-  const u64 *chunk_bins =
-      a.chunk_bins + (static_cast<int64_t>(row) * a.chunks + chunk) * kSampleBins;
-  u64 own[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) own[i] = chunk_bins[tid * kPer + i];
-  fill_table(s_table);
   const RowSettings set = row_settings(a, row);
+  if (set.greedy || (!set.use_k && !set.use_p)) return;
+  const BinShare<kChunkThreads> bins(a.bin_mass + static_cast<int64_t>(row) * kSampleBins,
+                                     a.bin_count + static_cast<int64_t>(row) * kSampleBins,
+                                     set);
+  // the mass of the bins above the listed ones: from the chunk's own bins
+  // where they hold it (and min-p drops none of it)
+  constexpr int kPer = BinShare<kChunkThreads>::kPer;
+  const bool summed = set.use_p && set.min_w == 0;
+  u64 own[kPer];
+  if (summed) {
+    const u64 *chunk_bins =
+        a.chunk_bins + (static_cast<int64_t>(row) * a.chunks + chunk) * kSampleBins;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) own[i] = chunk_bins[tid * kPer + i];
+  }
+  fill_table(s_table);
   const float mx = row_max(a, row);
-  if (set.greedy || no_token(mx) || (!set.use_k && !set.use_p)) return;
+  if (no_token(mx)) return;
   const RowEnds e = find_ends(bins, set);
   if (chunk == 0 && tid == 0) a.ends[row] = e;
   // without a cut inside the bins (top_k of all tokens) nothing is listed
   const int first = e.last_p < 0 && e.last_k < 0 ? kSampleBins : e.first;
   const RowScale r = row_scale(mx, set, s_table);
-  // the mass of the bins above the listed ones: from the chunk's own bins
-  // where they hold it (and min-p drops none of it)
-  const bool summed = set.use_p && set.min_w == 0;
   u64 sum = 0;
   if (summed) {
 #pragma unroll
@@ -694,7 +720,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
     int b[4];
     bins_of(v, r, t, b);
     const int least = min(min(b[0], b[1]), min(b[2], b[3]));
-    if (!summed && least < first) {
+    if (!summed && least < min(first, set.min_bin)) {
       u64 w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = fixed_weight(t[i], s_table);
@@ -1060,7 +1086,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
       add_to_bins(v, r, use_k, use_p, sh.row.count, sh.row.mass);
     });
     __syncthreads();
-    const RowEnds e = find_ends(BinShare<THREADS>(sh.row.mass, sh.row.count), set);
+    const RowEnds e = find_ends(BinShare<THREADS>(sh.row.mass, sh.row.count, set), set);
     if (e.last_p >= 0 || e.last_k >= 0) {
       __syncthreads();  // the list takes the place of the bins
       logits.each([&](const f32x4_at4 &v, int at) {
