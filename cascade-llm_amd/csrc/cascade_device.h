@@ -258,6 +258,35 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
   return best;
 }
 
+// Inclusive prefix sums over the wave's lanes (all 64 active): row_shr by 1, 2,
+// 4, 8 inside each row of 16, then lane 15 of a row into the next one
+// (row_bcast:15, rows 1 and 3) and lane 31 into the upper half (row_bcast:31).
+// dpp_add: v plus the value that CTRL brings in from another lane, in the
+// rows of ROWS (0 where it brings none).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
+}
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp_add(unsigned long long v) {
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+      0, static_cast<int>(v), CTRL, ROWS, 0xF, true));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+      0, static_cast<int>(v >> 32), CTRL, ROWS, 0xF, true));
+  return v + ((static_cast<unsigned long long>(hi) << 32) | lo);
+}
+
+template <typename T>
+__device__ __forceinline__ T wave_prefix(T v) {
+  v = dpp_add<0x111, 0xF>(v);
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);
+  return dpp_add<0x143, 0xC>(v);
+}
+
 // ---------------------------------------------------------------------------
 // Top-k keys. A (value, index) pair maps to one uint64 whose unsigned order
 // is "value descending, then index ascending", so selecting the k largest

@@ -157,7 +157,7 @@ struct PagedAttnArgs {
   int64_t out_token, out_head;
   int32_t *error;
   // split runs (SPLIT kernels): see "Runs"
-  int32_t target;   // runs wanted
+  double per_target;  // 1 / runs wanted
   int32_t *plan;    // [batch][2]: first run of a batch row, and how many
   float *part_ml;   // [run][q_heads][2]: maximum (log2 units), sum
   float *part_acc;  // [run][q_heads][D]
@@ -203,8 +203,8 @@ __device__ __forceinline__ PagedRow paged_row(const PagedAttnArgs &a, int b, boo
 // Runs.  The lengths are on the device, so the launch is sized for any of
 // them and each workgroup finds its own piece of work: the blocks of 32
 // positions of all batch rows are cut into runs of `size` blocks,
-//   size = max(kPagedMinRun, ceil(blocks of all rows / target)),
-// a multiple of the workgroup's waves, and row b gets max(1, ceil(blocks_b /
+//   size = max(kPagedMinRun, floor(blocks of all rows / target) + 1),
+// rounded up to the workgroup's waves, and row b gets max(1, ceil(blocks_b /
 // size)) runs, numbered through the batch.  There are at most target + batch
 // runs whatever the lengths, all but a row's last of one size, so a ragged
 // batch and a single long sequence both fill the device.  Every wave works
@@ -215,51 +215,52 @@ struct PagedRun {
   int len;
   int first;  // blocks [first, end) of the row
   int end;
-  int index;  // number of the row's first run
   int count;  // runs of the row
 };
 
+__device__ __forceinline__ int blocks_of(int len) {
+  return (len + kPagedBlock - 1) / kPagedBlock;
+}
+
+// The run's place; `first` (one wave of the launch) also flags what is out of
+// range and writes the plan for the launch that joins the runs.
 __device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, int lane,
-                                             bool flag) {
-  uint64_t blocks = 0;
-  for (int base = 0; base < a.batch; base += kWave)
-    blocks += static_cast<uint32_t>((paged_row(a, base + lane, flag).len + kPagedBlock - 1) /
-                                    kPagedBlock);
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) blocks += __shfl_xor(blocks, d);
-  uint64_t want = (blocks + a.target - 1) / a.target;
-  want = (want + kPagedWaves - 1) / kPagedWaves * kPagedWaves;
-  // (no row has more than 2^26 blocks)
-  const int size = static_cast<int>(
-      min(max(want, static_cast<uint64_t>(kPagedMinRun)), uint64_t{1} << 26));
+                                             bool first) {
+  // the first 64 rows stay in registers
+  const PagedRow head = paged_row(a, lane, first);
+  unsigned long long blocks = static_cast<uint32_t>(blocks_of(head.len));
+  for (int base = kWave; base < a.batch; base += kWave)
+    blocks += static_cast<uint32_t>(blocks_of(paged_row(a, base + lane, first).len));
+  blocks = lane_u64(wave_prefix(blocks), kWave - 1);
+  // more than blocks / target, in fp64 (no row has more than 2^26 blocks)
+  const int want = static_cast<int>(
+      fmin(static_cast<double>(blocks) * a.per_target, 67108864.0 - kPagedWaves)) + 1;
+  const int size = max((want + kPagedWaves - 1) / kPagedWaves * kPagedWaves, kPagedMinRun);
+  PagedRun out{-1, -1, 0, 0, 0, 0};
   int before = 0;
   for (int base = 0; base < a.batch; base += kWave) {
-    const PagedRow r = paged_row(a, base + lane, false);
-    const int nb = (r.len + kPagedBlock - 1) / kPagedBlock;
-    const int mine = r.row < 0 ? 0 : max(1, (nb + size - 1) / size);
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int o = __shfl_up(upto, d);
-      if (lane >= d) upto += o;
+    const PagedRow r = base == 0 ? head : paged_row(a, base + lane, false);
+    const int mine = r.row < 0 ? 0 : max(1, (blocks_of(r.len) + size - 1) / size);
+    const int upto = before + wave_prefix(mine);
+    if (first && base + lane < a.batch) {
+      a.plan[2 * (base + lane)] = upto - mine;
+      a.plan[2 * (base + lane) + 1] = mine;
     }
-    upto += before;
     const uint64_t past = __ballot(upto > run);
-    if (past != 0) {
+    if (out.b < 0 && past != 0) {
       const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      PagedRun out;
       out.b = base + at;
-      out.row = __shfl(r.row, at);
-      out.len = __shfl(r.len, at);
-      out.count = __shfl(mine, at);
-      out.index = __shfl(upto, at) - out.count;
-      out.first = (run - out.index) * size;
-      out.end = min(out.first + size, (out.len + kPagedBlock - 1) / kPagedBlock);
-      return out;
+      out.row = __builtin_amdgcn_readlane(static_cast<int>(r.row), at);
+      out.len = __builtin_amdgcn_readlane(r.len, at);
+      out.count = __builtin_amdgcn_readlane(mine, at);
+      const int place = run - (__builtin_amdgcn_readlane(upto, at) - out.count);
+      out.first = place * size;
+      out.end = min(out.first + size, blocks_of(out.len));
+      if (!first) return out;
     }
-    before = __shfl(upto, kWave - 1);
+    before = __builtin_amdgcn_readlane(upto, kWave - 1);
   }
-  return PagedRun{-1, -1, 0, 0, 0, 0, 0};
+  return out;
 }
 
 // Workgroup (run, KV head), or (batch row, KV head) without SPLIT; each wave
@@ -276,12 +277,14 @@ __device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, in
 // a block whose rows are all left out keeps it and adds nothing; a sequence
 // with no row at all ends with a zero sum and writes zeros.
 template <int D, bool SPLIT>
-__global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
+__global__ __launch_bounds__(kPagedWaves *kWave, 4) void paged_attention_kernel(
     PagedAttnArgs a) {
   constexpr int DV = D / 16;  // dims a lane holds of a V row
   constexpr int KC = D / 32;  // 32-dim chunks
   __shared__ float s_ml[kPagedWaves][kPagedGroup][2];
   __shared__ float s_acc[kPagedWaves][kPagedGroup][D];
+  __shared__ u32x4 s_q[KC][kWave];
+  static_assert(KC <= kPagedWaves, "a chunk of q a wave");
   const int g = static_cast<int>(blockIdx.x) % a.kv_heads;
   const int run = static_cast<int>(blockIdx.x) / a.kv_heads;
   const int G = a.group;
@@ -301,10 +304,6 @@ __global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
     first = r.first;
     end = r.end;
     count = r.count;
-    if (run == r.index && g == 0 && tid == 0) {
-      a.plan[2 * b] = run;
-      a.plan[2 * b + 1] = count;
-    }
   } else {
     b = run;
     const PagedRow r = paged_row(a, b, g == 0 && tid == 0);
@@ -320,13 +319,14 @@ __global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
   const uint16_t *vb = a.v_pages + g * a.head_stride;
   const int page_mask = (1 << a.page_shift) - 1;
 
-  u32x4 qop[KC];
-#pragma unroll
-  for (int c = 0; c < KC; ++c)
-    qop[c] = c16 < G ? *reinterpret_cast<const u32x4 *>(
-                           a.q + b * a.q_token + (g * G + c16) * a.q_head +
-                           32 * c + 8 * g4)
-                     : u32x4{0u, 0u, 0u, 0u};
+  // the q operands, a chunk a wave, kept in LDS: 16 registers less are what
+  // lets four waves share a SIMD
+  if (wave < KC)
+    s_q[wave][lane] = c16 < G ? *reinterpret_cast<const u32x4 *>(
+                                    a.q + b * a.q_token + (g * G + c16) * a.q_head +
+                                    32 * wave + 8 * g4)
+                              : u32x4{0u, 0u, 0u, 0u};
+  __syncthreads();
   const uint32_t head_mask = c16 < G ? 0xffffffffu : 0u;
 
   float m = -FLT_MAX, l = 0.0f;
@@ -341,13 +341,17 @@ __global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
     kpage = table[min(blk * kPagedBlock + 8 * (c16 >> 2), last) >> a.page_shift];
     vpage = table[min(blk * kPagedBlock + 8 * g4, last) >> a.page_shift];
   };
-  int kpage = 0, vpage = 0;
-  if (first + wave < end) pages_of(first + wave, kpage, vpage);
-  for (int blk = first + wave; blk < end; blk += kPagedWaves) {
+  // One block's rows in registers.
+  struct Rows {
+    u32x4 k[2][KC];
+    uint32_t v[8][DV / 2];
+    bool bad;  // the V group's page is none of the pool's
+  };
+  auto load = [&](int blk, int kpage, int vpage, Rows &x) __attribute__((always_inline)) {
     const int r0 = blk * kPagedBlock;
-    const bool vbad = vpage < 0 || vpage >= a.num_pages;
+    x.bad = vpage < 0 || vpage >= a.num_pages;
     if (kpage < 0 || kpage >= a.num_pages) kpage = 0;
-    if (vbad) {
+    if (x.bad) {
       vpage = 0;
       flag_range(a.error);
     }
@@ -355,41 +359,54 @@ __global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
     const uint16_t *kp = kb + kpage * a.page_stride +
                          (((r0 + 8 * (c16 >> 2)) & page_mask) + (c16 & 3)) * D + 8 * g4;
     const uint16_t *vp = vb + vpage * a.page_stride + ((r0 + 8 * g4) & page_mask) * D + DV * c16;
-    u32x4 kt[2][KC];
-    uint32_t vt[8][DV / 2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
       for (int c = 0; c < KC; ++c)
-        kt[hf][c] = __builtin_nontemporal_load(
+        x.k[hf][c] = __builtin_nontemporal_load(
             reinterpret_cast<const u32x4 *>(kp + 4 * hf * D + 32 * c));
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if constexpr (DV == 8) {
-        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vp + j * D));
+        const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vp + j * D));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vt[j][i] = x[i];
+        for (int i = 0; i < 4; ++i) x.v[j][i] = w[i];
       } else {
-        const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(vp + j * D));
-        vt[j][0] = x[0];
-        vt[j][1] = x[1];
+        const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(vp + j * D));
+        x.v[j][0] = w[0];
+        x.v[j][1] = w[1];
       }
     }
-    // the next block's pages, while this one's rows are on their way
-    if (blk + kPagedWaves < end) pages_of(blk + kPagedWaves, kpage, vpage);
+  };
+  auto step = [&](int blk, Rows &x) __attribute__((always_inline)) {
+    const int r0 = blk * kPagedBlock;
+    asm volatile("" ::: "memory");  // s_q is read again in each step
     f32x4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      s0 = mfma_16x16x32_bf16(kt[0][c], qop[c], s0);
-      s1 = mfma_16x16x32_bf16(kt[1][c], qop[c], s1);
+      const u32x4 qop = s_q[c][lane];
+      s0 = mfma_16x16x32_bf16(x.k[0][c], qop, s0);
+      s1 = mfma_16x16x32_bf16(x.k[1][c], qop, s1);
     }
     float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
     float bmax = -INFINITY;
+    const bool cut = r0 + kPagedBlock > len || __any(x.bad);  // uniform
+    if (cut) {
+      // rows past the end, or of a page outside the pool, take no part
+      // whatever they hold: 0 times a NaN of theirs would be one
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      s[j] = r0 + 8 * g4 + j < len && !vbad ? s[j] * a.scale_log2 : -INFINITY;
-      bmax = fmaxf(bmax, s[j]);
+      for (int j = 0; j < 8; ++j) {
+        const bool out = x.bad || r0 + 8 * g4 + j >= len;
+        s[j] = out ? -INFINITY : s[j] * a.scale_log2;
+#pragma unroll
+        for (int i = 0; i < DV / 2; ++i) x.v[j][i] = out ? 0u : x.v[j][i];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] *= a.scale_log2;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bmax = fmaxf(bmax, s[j]);
     bmax = xor32_max(xor16_max(bmax));
     const float mnew = fmaxf(m, bmax);
     const float alpha = paged_exp2(m - mnew);
@@ -409,25 +426,24 @@ __global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
 #pragma unroll
       for (int e = 0; e < DV; ++e) o[e] *= alpha;
     }
-    if (r0 + kPagedBlock > len || __any(vbad)) {
-      // rows past the end, or of another sequence's page, take no part
-      // whatever they hold: 0 times a NaN would be one
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool out = vbad || r0 + 8 * g4 + j >= len;
-#pragma unroll
-        for (int i = 0; i < DV / 2; ++i) vt[j][i] = out ? 0u : vt[j][i];
-      }
-    }
 #pragma unroll
     for (int e = 0; e < DV; ++e) {
       const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
       u32x4 vop;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        vop[i] = __builtin_amdgcn_perm(vt[2 * i + 1][e >> 1], vt[2 * i][e >> 1], sel);
+        vop[i] = __builtin_amdgcn_perm(x.v[2 * i + 1][e >> 1], x.v[2 * i][e >> 1], sel);
       o[e] = mfma_16x16x32_bf16(vop, pop, o[e]);
     }
+  };
+  int kpage = 0, vpage = 0;
+  if (first + wave < end) pages_of(first + wave, kpage, vpage);
+  for (int blk = first + wave; blk < end; blk += kPagedWaves) {
+    Rows x;
+    load(blk, kpage, vpage, x);
+    // the next block's pages, while this one's rows are on their way
+    if (blk + kPagedWaves < end) pages_of(blk + kPagedWaves, kpage, vpage);
+    step(blk, x);
   }
 
   l = xor32_sum(xor16_sum(l));
@@ -472,54 +488,57 @@ __global__ __launch_bounds__(kPagedWaves *kWave) void paged_attention_kernel(
 
 // Joins the runs of one (batch row, query head):
 //   out = sum_r 2^(m_r - M) acc_r / sum_r 2^(m_r - M) l_r,  M = max_r m_r.
-// Wave-sized slices of the workgroup take every kMergeSlices-th run each, in
-// order, and add up in LDS.  Rows of one run were written already.
-constexpr int kPagedMergeThreads = 512;
+// A slice of D / 4 threads (four dims each) takes every kSlices-th run with a
+// running maximum of its own, so that no load waits for another, and the
+// slices join in LDS in a fixed order.  Rows of one run were written already.
+constexpr int kPagedMergeThreads = 256;
 
 template <int D>
 __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(PagedAttnArgs a) {
-  constexpr int kSlices = kPagedMergeThreads / D;
-  __shared__ float s_max[kPagedMergeThreads / kWave];
-  __shared__ float s_acc[kSlices][D];
-  __shared__ float s_den[kSlices];
+  constexpr int kSlices = kPagedMergeThreads * 4 / D;
+  __shared__ f32x4 s_acc[kSlices][D / 4];
+  __shared__ float s_ml[kSlices][2];
   const int heads = a.kv_heads * a.group;
   const int b = static_cast<int>(blockIdx.x) / heads;
   const int h = static_cast<int>(blockIdx.x) % heads;
-  const int tid = threadIdx.x;
-  if (paged_row(a, b, false).row < 0) return;
+  const int slice = threadIdx.x / (D / 4);
+  const int d = threadIdx.x % (D / 4);
   const int index = a.plan[2 * b], count = a.plan[2 * b + 1];
-  if (count <= 1) return;
+  if (count <= 1) return;  // a padding row, or written already
   const int64_t base = static_cast<int64_t>(index) * heads + h;
-  float mm = -FLT_MAX;
-  for (int r = tid; r < count; r += kPagedMergeThreads)
-    mm = fmaxf(mm, a.part_ml[2 * (base + static_cast<int64_t>(r) * heads)]);
-  mm = wave_max(mm);
-  if ((tid & (kWave - 1)) == 0) s_max[tid / kWave] = mm;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kPagedMergeThreads / kWave; ++w) mm = fmaxf(mm, s_max[w]);
-  const int slice = tid / D;
-  const int d = tid % D;
-  float den = 0.0f, acc = 0.0f;
+  float m = -FLT_MAX, den = 0.0f;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int r = slice; r < count; r += kSlices) {
     const int64_t slot = base + static_cast<int64_t>(r) * heads;
-    const float w = paged_exp2(a.part_ml[2 * slot] - mm);
-    den = fmaf(w, a.part_ml[2 * slot + 1], den);
-    acc = fmaf(w, a.part_acc[slot * D + d], acc);
+    const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * slot);
+    const f32x4 v = *reinterpret_cast<const f32x4 *>(a.part_acc + slot * D + 4 * d);
+    const float mnew = fmaxf(m, ml.x);
+    const float keep = paged_exp2(m - mnew), w = paged_exp2(ml.x - mnew);
+    m = mnew;
+    den = fmaf(w, ml.y, den * keep);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = fmaf(w, v[i], acc[i] * keep);
   }
   s_acc[slice][d] = acc;
-  if (d == 0) s_den[slice] = den;
-  __syncthreads();
-  if (slice == 0) {
-#pragma unroll
-    for (int k = 1; k < kSlices; ++k) {
-      acc += s_acc[k][d];
-      den += s_den[k];
-    }
-    a.out[b * a.out_token + h * a.out_head + d] =
-        f32_to_bf16(den == 0.0f ? 0.0f : acc / den);
+  if (d == 0) {
+    s_ml[slice][0] = m;
+    s_ml[slice][1] = den;
   }
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  const int dim = threadIdx.x;
+  float mm = -FLT_MAX;
+#pragma unroll
+  for (int k = 0; k < kSlices; ++k) mm = fmaxf(mm, s_ml[k][0]);
+  float sum = 0.0f, r = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kSlices; ++k) {
+    const float w = paged_exp2(s_ml[k][0] - mm);
+    sum = fmaf(w, s_ml[k][1], sum);
+    r = fmaf(w, s_acc[k][dim / 4][dim % 4], r);
+  }
+  a.out[b * a.out_token + h * a.out_head + dim] = f32_to_bf16(sum == 0.0f ? 0.0f : r / sum);
 }
 
 // Whether a launch splits, and its sizes.  Rows of at most one shortest run
@@ -776,7 +795,7 @@ extern "C" int cascade_paged_decode_attention_bf16(
                : launch_kernel(paged_attention_kernel<64, false>, grid, block, 0, s, a);
   }
   unsigned char *ws = static_cast<unsigned char *>(workspace);
-  a.target = static_cast<int32_t>(p.target);
+  a.per_target = 1.0 / static_cast<double>(p.target);
   a.plan = reinterpret_cast<int32_t *>(ws);
   a.part_ml = reinterpret_cast<float *>(ws + p.plan_bytes);
   a.part_acc = reinterpret_cast<float *>(ws + p.plan_bytes + p.ml_bytes);

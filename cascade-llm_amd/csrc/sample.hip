@@ -206,27 +206,6 @@ __device__ __forceinline__ void fill_table(double *table) {
   table[j] = ldexp(p, whole + kWeightBits);
 }
 
-// v plus the value that the DPP control CTRL brings in from another lane, in
-// the rows of ROWS (0 where it brings none).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ u64 dpp_add(u64 v) {
-  const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, true);
-  const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xF, true);
-  return v + ((static_cast<u64>(static_cast<uint32_t>(hi)) << 32) | static_cast<uint32_t>(lo));
-}
-
-// Inclusive prefix sum over the wave's lanes (all 64 active): row_shr by 1, 2,
-// 4, 8 inside each row of 16, then lane 15 of a row into the next one
-// (row_bcast:15, rows 1 and 3) and lane 31 into the upper half (row_bcast:31).
-__device__ __forceinline__ u64 wave_prefix(u64 v) {
-  v = dpp_add<0x111, 0xF>(v);
-  v = dpp_add<0x112, 0xF>(v);
-  v = dpp_add<0x114, 0xF>(v);
-  v = dpp_add<0x118, 0xF>(v);
-  v = dpp_add<0x142, 0xA>(v);
-  return dpp_add<0x143, 0xC>(v);
-}
-
 // Inclusive prefix sum over the workgroup in thread order, and its total.
 // Two barriers; `lds` may be reused after the second.
 template <int WAVES = kSampleWaves>
