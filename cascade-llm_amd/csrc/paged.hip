@@ -170,7 +170,7 @@ constexpr int kPagedBlock = 32;  // positions a wave step
 constexpr int kPagedGroup = 16;  // MFMA columns
 constexpr int kPagedMinRun = 4;  // blocks
 constexpr int kPagedMaxBatch = 1024;  // of a split launch
-constexpr int kPagedTarget = 1024;    // workgroups wanted of one
+constexpr int kPagedTarget = 2048;    // workgroups wanted of one
 constexpr size_t kPagedAlign = 256;
 
 __device__ __forceinline__ float paged_exp2(float x) {
@@ -271,8 +271,8 @@ __device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, in
 //   O += V_blk^T P   D / 16 tiles, K = the 32 positions
 // Lane (c, g4) = (l % 16, l / 16) owns the scores of head c at rows
 // 8 g4 .. 8 g4 + 7 (the row order inside a K tile is chosen for that), which
-// is its piece of the P operand.  V rows are loaded whole (16 lanes a row,
-// dims DV c .. DV c + DV - 1 with DV = D / 16) and transposed in registers.
+// is its piece of the P operand.  K rows are transposed through LDS, V rows
+// (16 lanes a row, dims DV c .. DV c + DV - 1 with DV = D / 16) in registers.
 // Scores carry scale * log2(e).  The running maximum starts at -FLT_MAX, so
 // a block whose rows are all left out keeps it and adds nothing; a sequence
 // with no row at all ends with a zero sum and writes zeros.
@@ -281,8 +281,13 @@ __global__ __launch_bounds__(kPagedWaves *kWave, 4) void paged_attention_kernel(
     PagedAttnArgs a) {
   constexpr int DV = D / 16;  // dims a lane holds of a V row
   constexpr int KC = D / 32;  // 32-dim chunks
+  constexpr int CH = D / 8;   // 16-byte chunks of a row
   __shared__ float s_ml[kPagedWaves][kPagedGroup][2];
-  __shared__ float s_acc[kPagedWaves][kPagedGroup][D];
+  // a wave's K block, and in the end its output (both 64 D bytes)
+  __shared__ union {
+    u32x4 k[kPagedBlock * CH];
+    float acc[kPagedGroup][D];
+  } s_wave[kPagedWaves];
   __shared__ u32x4 s_q[KC][kWave];
   static_assert(KC <= kPagedWaves, "a chunk of q a wave");
   const int g = static_cast<int>(blockIdx.x) % a.kv_heads;
@@ -334,45 +339,60 @@ __global__ __launch_bounds__(kPagedWaves *kWave, 4) void paged_attention_kernel(
 #pragma unroll
   for (int e = 0; e < DV; ++e) o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // A lane reads K rows of group c16 / 4 of eight of a block and V rows of
-  // group g4; a group lies in one page.  Groups past the end take the last
-  // row's page: its rows are memory of the pool whatever they hold.
-  auto pages_of = [&](int blk, int &kpage, int &vpage) {
-    kpage = table[min(blk * kPagedBlock + 8 * (c16 >> 2), last) >> a.page_shift];
-    vpage = table[min(blk * kPagedBlock + 8 * g4, last) >> a.page_shift];
+  // Rows come in whole, 16 lanes a row (8 for K rows of 64 dims), so that a
+  // load covers runs of 128 bytes or more.  A lane's V rows are group g4 of
+  // eight of a block, which lies in one page; groups past the end take the
+  // last row's page: its rows are memory of the pool whatever they hold.
+  auto page_of = [&](int blk) {
+    return table[min(blk * kPagedBlock + 8 * g4, last) >> a.page_shift];
   };
-  // One block's rows in registers.
+  // One block's rows in registers: V of rows 8 g4 + j, dims DV c16 ..; K as
+  // laid out by k_slot.
   struct Rows {
-    u32x4 k[2][KC];
+    u32x4 k[D / 16];
     uint32_t v[8][DV / 2];
-    bool bad;  // the V group's page is none of the pool's
+    bool bad;  // the group's page is none of the pool's
   };
-  auto load = [&](int blk, int kpage, int vpage, Rows &x) __attribute__((always_inline)) {
-    const int r0 = blk * kPagedBlock;
-    x.bad = vpage < 0 || vpage >= a.num_pages;
-    if (kpage < 0 || kpage >= a.num_pages) kpage = 0;
+  // K rows go through LDS to become MFMA operands.  Row r keeps its chunk ch at
+  // slot CH r + (ch ^ key(r)), where the keys of the 16 rows of an operand
+  // (of the eight of one parity, for 64 dims: two rows share the banks)
+  // differ: neither the writes nor the reads meet in a bank.
+  auto k_slot = [](int r, int ch) {
+    const int key = D == 128 ? 4 * (r >> 3) + (r & 3) : 2 * (r >> 3) + ((r >> 1) & 1);
+    return CH * r + (ch ^ key);
+  };
+  auto load = [&](int blk, int page, Rows &x) __attribute__((always_inline)) {
+    x.bad = page < 0 || page >= a.num_pages;
     if (x.bad) {
-      vpage = 0;
+      page = 0;
       flag_range(a.error);
     }
-    // K tile row i is block row 8 (i / 4) + i % 4 + 4 hf
-    const uint16_t *kp = kb + kpage * a.page_stride +
-                         (((r0 + 8 * (c16 >> 2)) & page_mask) + (c16 & 3)) * D + 8 * g4;
-    const uint16_t *vp = vb + vpage * a.page_stride + ((r0 + 8 * g4) & page_mask) * D + DV * c16;
+    const int64_t at = page * a.page_stride + ((blk * kPagedBlock + 8 * g4) & page_mask) * D;
+    if constexpr (D == 128) {
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
+      for (int j = 0; j < 8; ++j)
+        x.k[j] = __builtin_nontemporal_load(
+            reinterpret_cast<const u32x4 *>(kb + at + j * D + 8 * c16));
+    } else {
+      // group i of eight rows, eight lanes a row
 #pragma unroll
-      for (int c = 0; c < KC; ++c)
-        x.k[hf][c] = __builtin_nontemporal_load(
-            reinterpret_cast<const u32x4 *>(kp + 4 * hf * D + 32 * c));
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(at), 16 * i);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(at >> 32), 16 * i);
+        const int64_t group = static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+        x.k[i] = __builtin_nontemporal_load(
+            reinterpret_cast<const u32x4 *>(kb + group + 8 * lane));
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
+      const uint16_t *vp = vb + at + j * D + DV * c16;
       if constexpr (DV == 8) {
-        const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vp + j * D));
+        const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vp));
 #pragma unroll
         for (int i = 0; i < 4; ++i) x.v[j][i] = w[i];
       } else {
-        const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(vp + j * D));
+        const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(vp));
         x.v[j][0] = w[0];
         x.v[j][1] = w[1];
       }
@@ -380,13 +400,28 @@ __global__ __launch_bounds__(kPagedWaves *kWave, 4) void paged_attention_kernel(
   };
   auto step = [&](int blk, Rows &x) __attribute__((always_inline)) {
     const int r0 = blk * kPagedBlock;
-    asm volatile("" ::: "memory");  // s_q is read again in each step
+    u32x4 *sk = s_wave[wave].k;
+    // the slots are worked out again in each step, and s_q is read again:
+    // kept in registers they would cost the fourth wave of a SIMD
+    int ln = lane;
+    asm volatile("" : "+v"(ln)::"memory");
+    const int lc = ln & 15, lg = ln >> 4;
+    if constexpr (D == 128) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sk[k_slot(8 * lg + j, lc)] = x.k[j];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sk[k_slot(8 * i + (ln >> 3), ln & 7)] = x.k[i];
+    }
+    asm volatile("" ::: "memory");
+    // K tile row i is block row 8 (i / 4) + i % 4 + 4 hf
+    const int krow = 8 * (lc >> 2) + (lc & 3);
     f32x4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      const u32x4 qop = s_q[c][lane];
-      s0 = mfma_16x16x32_bf16(x.k[0][c], qop, s0);
-      s1 = mfma_16x16x32_bf16(x.k[1][c], qop, s1);
+      const u32x4 qop = s_q[c][ln];
+      s0 = mfma_16x16x32_bf16(sk[k_slot(krow, 4 * c + lg)], qop, s0);
+      s1 = mfma_16x16x32_bf16(sk[k_slot(krow + 4, 4 * c + lg)], qop, s1);
     }
     float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
     float bmax = -INFINITY;
@@ -436,13 +471,12 @@ __global__ __launch_bounds__(kPagedWaves *kWave, 4) void paged_attention_kernel(
       o[e] = mfma_16x16x32_bf16(vop, pop, o[e]);
     }
   };
-  int kpage = 0, vpage = 0;
-  if (first + wave < end) pages_of(first + wave, kpage, vpage);
+  int page = first + wave < end ? page_of(first + wave) : 0;
   for (int blk = first + wave; blk < end; blk += kPagedWaves) {
     Rows x;
-    load(blk, kpage, vpage, x);
+    load(blk, page, x);
     // the next block's pages, while this one's rows are on their way
-    if (blk + kPagedWaves < end) pages_of(blk + kPagedWaves, kpage, vpage);
+    if (blk + kPagedWaves < end) page = page_of(blk + kPagedWaves);
     step(blk, x);
   }
 
@@ -452,7 +486,7 @@ __global__ __launch_bounds__(kPagedWaves *kWave, 4) void paged_attention_kernel(
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int e = 0; e < DV; ++e) s_acc[wave][c16][DV * (4 * g4 + r) + e] = o[e][r];
+      for (int e = 0; e < DV; ++e) s_wave[wave].acc[c16][DV * (4 * g4 + r) + e] = o[e][r];
     if (g4 == 0) {
       s_ml[wave][c16][0] = m;
       s_ml[wave][c16][1] = l;
@@ -470,7 +504,7 @@ __global__ __launch_bounds__(kPagedWaves *kWave, 4) void paged_attention_kernel(
     for (int w = 0; w < kPagedWaves; ++w) {
       const float wt = paged_exp2(s_ml[w][h][0] - mm);
       den = fmaf(wt, s_ml[w][h][1], den);
-      r = fmaf(wt, s_acc[w][h][d], r);
+      r = fmaf(wt, s_wave[w].acc[h][d], r);
     }
     if (!SPLIT || count == 1) {
       a.out[b * a.out_token + (g * G + h) * a.out_head + d] =
