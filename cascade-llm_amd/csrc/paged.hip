@@ -165,7 +165,9 @@ struct PagedAttnArgs {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kPagedWaves = 4;
+constexpr int kPagedWaves = 4;   // of a workgroup that takes a run
+constexpr int kWholeWaves = 8;   // of one that takes a whole row
+constexpr int kWholeBlocks = 16;  // rows of at most this many blocks are not split
 constexpr int kPagedBlock = 32;  // positions a wave step
 constexpr int kPagedGroup = 16;  // MFMA columns
 constexpr int kPagedMinRun = 4;  // blocks
@@ -264,7 +266,7 @@ __device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, in
 }
 
 // Workgroup (run, KV head), or (batch row, KV head) without SPLIT; each wave
-// runs an online softmax over every fourth block of 32 positions and the
+// runs an online softmax over every WAVES-th block of 32 positions and the
 // waves merge in LDS.  The products are v_mfma_f32_16x16x32_bf16 with the
 // query heads of the KV head as columns (zeros past group):
 //   S = K_blk q^T    two 16-row tiles x D / 32 chunks
@@ -277,19 +279,20 @@ __device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, in
 // a block whose rows are all left out keeps it and adds nothing; a sequence
 // with no row at all ends with a zero sum and writes zeros.
 template <int D, bool SPLIT>
-__global__ __launch_bounds__(kPagedWaves *kWave, 4) void paged_attention_kernel(
-    PagedAttnArgs a) {
+__global__ __launch_bounds__((SPLIT ? kPagedWaves : kWholeWaves) * kWave, 4) void
+paged_attention_kernel(PagedAttnArgs a) {
+  constexpr int WAVES = SPLIT ? kPagedWaves : kWholeWaves;
   constexpr int DV = D / 16;  // dims a lane holds of a V row
   constexpr int KC = D / 32;  // 32-dim chunks
   constexpr int CH = D / 8;   // 16-byte chunks of a row
-  __shared__ float s_ml[kPagedWaves][kPagedGroup][2];
+  __shared__ float s_ml[WAVES][kPagedGroup][2];
   // a wave's K block, and in the end its output (both 64 D bytes)
   __shared__ union {
     u32x4 k[kPagedBlock * CH];
     float acc[kPagedGroup][D];
-  } s_wave[kPagedWaves];
+  } s_wave[WAVES];
   __shared__ u32x4 s_q[KC][kWave];
-  static_assert(KC <= kPagedWaves, "a chunk of q a wave");
+  static_assert(KC <= WAVES, "a chunk of q a wave");
   const int g = static_cast<int>(blockIdx.x) % a.kv_heads;
   const int run = static_cast<int>(blockIdx.x) / a.kv_heads;
   const int G = a.group;
@@ -472,11 +475,11 @@ __global__ __launch_bounds__(kPagedWaves *kWave, 4) void paged_attention_kernel(
     }
   };
   int page = first + wave < end ? page_of(first + wave) : 0;
-  for (int blk = first + wave; blk < end; blk += kPagedWaves) {
+  for (int blk = first + wave; blk < end; blk += WAVES) {
     Rows x;
     load(blk, page, x);
     // the next block's pages, while this one's rows are on their way
-    if (blk + kPagedWaves < end) page = page_of(blk + kPagedWaves);
+    if (blk + WAVES < end) page = page_of(blk + WAVES);
     step(blk, x);
   }
 
@@ -493,15 +496,15 @@ __global__ __launch_bounds__(kPagedWaves *kWave, 4) void paged_attention_kernel(
     }
   }
   __syncthreads();
-  for (int i = tid; i < G * D; i += kPagedWaves * kWave) {
+  for (int i = tid; i < G * D; i += WAVES * kWave) {
     const int h = i / D;
     const int d = i % D;
     float mm = -FLT_MAX;
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) mm = fmaxf(mm, s_ml[w][h][0]);
+    for (int w = 0; w < WAVES; ++w) mm = fmaxf(mm, s_ml[w][h][0]);
     float den = 0.0f, r = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float wt = paged_exp2(s_ml[w][h][0] - mm);
       den = fmaf(wt, s_ml[w][h][1], den);
       r = fmaf(wt, s_wave[w].acc[h][d], r);
@@ -575,8 +578,11 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(PagedAt
   a.out[b * a.out_token + h * a.out_head + dim] = f32_to_bf16(sum == 0.0f ? 0.0f : r / sum);
 }
 
-// Whether a launch splits, and its sizes.  Rows of at most one shortest run
-// need none; past kPagedMaxBatch rows every wave's walk over the lengths would
+// Whether a launch splits, and its sizes.  Rows of at most kWholeBlocks blocks
+// take one workgroup of eight waves each, which costs less than a second
+// launch (512 positions, 8 KV heads: 1 row 6.8 us against 7.6 split, 64 rows
+// 16.4 against 20.3; at 1000 positions 12.5 against 7.7 and 28.9 against
+// 30.1).  Past kPagedMaxBatch rows every wave's walk over the lengths would
 // cost more than the balance is worth, and the rows fill the device.
 struct PagedPlan {
   bool split;
@@ -589,7 +595,7 @@ static PagedPlan paged_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, in
                             int64_t max_length) {
   PagedPlan p{};
   const int64_t blocks = (max_length + kPagedBlock - 1) / kPagedBlock;
-  p.split = blocks > kPagedMinRun && batch <= kPagedMaxBatch;
+  p.split = blocks > kWholeBlocks && batch <= kPagedMaxBatch;
   if (!p.split) return p;
   p.target = (kPagedTarget + kv_heads - 1) / kv_heads;
   p.runs = p.target + batch;
@@ -827,7 +833,7 @@ extern "C" int cascade_paged_decode_attention_bf16(
   a.batch = static_cast<int32_t>(batch);
   a.kv_heads = static_cast<int32_t>(n_kv_heads);
   const PagedPlan p = paged_plan(batch, n_q_heads, n_kv_heads, head_dim, max_length);
-  const dim3 block(kPagedWaves * kWave);
+  const dim3 block((p.split ? kPagedWaves : kWholeWaves) * kWave);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (!p.split) {
     const dim3 grid(static_cast<unsigned>(batch * n_kv_heads));
