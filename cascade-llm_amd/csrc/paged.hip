@@ -161,6 +161,7 @@ struct PagedAttnArgs {
   int32_t *plan;    // [batch][2]: first run of a batch row, and how many
   float *part_ml;   // [run][q_heads][2]: maximum (log2 units), sum
   float *part_acc;  // [run][q_heads][D]
+  int32_t runs;     // that the workspace holds
 };
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -541,7 +542,9 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(PagedAt
   const int slice = threadIdx.x / (D / 4);
   const int d = threadIdx.x % (D / 4);
   const int index = a.plan[2 * b], count = a.plan[2 * b + 1];
-  if (count <= 1) return;  // a padding row, or written already
+  // a padding row, or written already (or, past the workspace, a plan that
+  // another call has overwritten)
+  if (count <= 1 || index < 0 || count > a.runs - index) return;
   const int64_t base = static_cast<int64_t>(index) * heads + h;
   float m = -FLT_MAX, den = 0.0f;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -661,6 +664,9 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyPagesArgs 
   }
 }
 
+// Threads that one launch can have.
+constexpr int64_t kMaxThreads = 0xffffffff;
+
 static bool page_shift_of(int64_t page_size, int32_t *shift) {
   if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1))) return false;
   *shift = __builtin_ctzll(static_cast<unsigned long long>(page_size));
@@ -699,6 +705,10 @@ extern "C" int cascade_paged_append_bf16(
       n_kv_heads > 1024 || !page_shift_of(page_size, &a.page_shift) ||
       max_pages * page_size > 0x7fffffff)
     return CASCADE_ESHAPE;
+  const int64_t units = (n_q_heads + 2 * n_kv_heads) * (head_dim / 16);
+  int64_t threads = (units + kWave - 1) / kWave * kWave;
+  if (threads > kAppendThreads) threads = kAppendThreads;
+  if (tokens > kMaxThreads / threads) return CASCADE_ESHAPE;
   if (rope_dim < 0 || rope_dim > head_dim || (rope_dim & 15)) return CASCADE_ESHAPE;
   if (rope_dim > 0 &&
       (rope_cos == nullptr || rope_sin == nullptr || rope_positions <= 0))
@@ -751,11 +761,8 @@ extern "C" int cascade_paged_append_bf16(
   a.kv_heads = static_cast<int32_t>(n_kv_heads);
   a.dim = static_cast<int32_t>(head_dim);
   a.error = error_flag;
-  const int64_t units = (n_q_heads + 2 * n_kv_heads) * (head_dim / 16);
-  const int64_t threads = (units + kWave - 1) / kWave * kWave;
   return launch_kernel(paged_append_kernel, dim3(static_cast<unsigned>(tokens)),
-                       dim3(static_cast<unsigned>(threads < kAppendThreads ? threads
-                                                                           : kAppendThreads)),
+                       dim3(static_cast<unsigned>(threads)),
                        0, static_cast<hipStream_t>(stream), a);
 }
 
@@ -768,7 +775,9 @@ extern "C" size_t cascade_paged_attention_workspace_bytes(int64_t batch,
       n_q_heads / n_kv_heads > kPagedGroup || (head_dim != 64 && head_dim != 128) ||
       max_length <= 0 || max_length > 0x7fffffff - 64)
     return 0;
-  const PagedPlan p = paged_plan(batch, n_q_heads, n_kv_heads, head_dim, max_length);
+  // enough for fewer rows too: a launch of more than kPagedMaxBatch needs none
+  const PagedPlan p = paged_plan(batch < kPagedMaxBatch ? batch : kPagedMaxBatch, n_q_heads,
+                                 n_kv_heads, head_dim, max_length);
   return kPagedAlign + p.plan_bytes + p.ml_bytes + p.acc_bytes;
 }
 
@@ -790,7 +799,8 @@ extern "C" int cascade_paged_decode_attention_bf16(
     return CASCADE_EINVAL;
   PagedAttnArgs a{};
   if ((head_dim != 64 && head_dim != 128) || n_q_heads <= 0 || n_q_heads % n_kv_heads ||
-      n_q_heads / n_kv_heads > kPagedGroup || n_kv_heads > 0xffff || batch * n_q_heads > 0x7fffffff ||
+      n_q_heads / n_kv_heads > kPagedGroup || n_kv_heads > 0xffff ||
+      batch > kMaxThreads / (kWholeWaves * kWave) / n_kv_heads ||
       !page_shift_of(page_size, &a.page_shift) || max_length > 0x7fffffff - 64)
     return CASCADE_ESHAPE;
   if (table_stride < (max_length + page_size - 1) / page_size ||
@@ -807,8 +817,8 @@ extern "C" int cascade_paged_decode_attention_bf16(
                              page_head_stride, out_token_stride, out_head_stride};
   for (int64_t s : strides)
     if (!stride_ok(s)) return CASCADE_EALIGN;
-  if (workspace_bytes < cascade_paged_attention_workspace_bytes(
-                            batch, n_q_heads, n_kv_heads, head_dim, max_length))
+  const PagedPlan p = paged_plan(batch, n_q_heads, n_kv_heads, head_dim, max_length);
+  if (workspace_bytes < kPagedAlign + p.plan_bytes + p.ml_bytes + p.acc_bytes)
     return CASCADE_EWORKSPACE;
   a.q = static_cast<const uint16_t *>(q);
   a.q_token = q_token_stride;
@@ -832,7 +842,6 @@ extern "C" int cascade_paged_decode_attention_bf16(
   a.error = error_flag;
   a.batch = static_cast<int32_t>(batch);
   a.kv_heads = static_cast<int32_t>(n_kv_heads);
-  const PagedPlan p = paged_plan(batch, n_q_heads, n_kv_heads, head_dim, max_length);
   const dim3 block((p.split ? kPagedWaves : kWholeWaves) * kWave);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (!p.split) {
@@ -842,6 +851,7 @@ extern "C" int cascade_paged_decode_attention_bf16(
                : launch_kernel(paged_attention_kernel<64, false>, grid, block, 0, s, a);
   }
   unsigned char *ws = static_cast<unsigned char *>(workspace);
+  a.runs = static_cast<int32_t>(p.runs);
   a.per_target = 1.0 / static_cast<double>(p.target);
   a.plan = reinterpret_cast<int32_t *>(ws);
   a.part_ml = reinterpret_cast<float *>(ws + p.plan_bytes);
@@ -885,7 +895,7 @@ extern "C" int cascade_copy_pages(void *pages, int64_t planes, int64_t plane_byt
   if (a.pieces > INT64_MAX / planes / count) return CASCADE_EINVAL;
   a.total = a.pieces * planes * count;
   a.error = error_flag;
-  const int64_t blocks = a.total < (1 << 24) ? a.total : (1 << 24);
+  const int64_t blocks = a.total < (1 << 22) ? a.total : (1 << 22);
   return launch_kernel(copy_pages_kernel, dim3(static_cast<unsigned>(blocks)),
                        dim3(kCopyThreads), 0, static_cast<hipStream_t>(stream), a);
 }

@@ -120,7 +120,7 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs &a, int row
   const double t = a.temperature != nullptr ? static_cast<double>(a.temperature[row])
                                             : a.temperature_value;
   r.greedy = !(t > 0.0);
-  r.scale = kTable * 1.4426950408889634 / t;
+  r.scale = fmin(kTable * 1.4426950408889634 / t, 1e300);  // 0 times it stays 0
   r.top_k = a.top_k != nullptr ? static_cast<int64_t>(a.top_k[row]) : a.top_k_value;
   r.top_p = a.top_p != nullptr ? static_cast<double>(a.top_p[row]) : a.top_p_value;
   const double p = a.min_p != nullptr ? static_cast<double>(a.min_p[row]) : a.min_p_value;
@@ -889,7 +889,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
     __syncthreads();
     if (has) atomicMin(&sh.first[0], tid);
     __syncthreads();
-    const int begin = sh.first[0] * a.chunk;
+    const int begin = min(sh.first[0], a.chunks - 1) * a.chunk;
     const int end = min(begin + a.chunk, a.vocab);
     for (int i = begin + tid; i < end; i += kSampleThreads)
       if (x[i] == mx) {
@@ -963,7 +963,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
     sh.found[1] = target - (upto - mass);
   }
   __syncthreads();
-  const int begin = static_cast<int>(sh.found[0]) * a.chunk;
+  const int begin = static_cast<int>(min(sh.found[0], static_cast<u64>(a.chunks - 1))) * a.chunk;
   const int end = min(begin + a.chunk, a.vocab);
   target = sh.found[1];
   // neighbouring tokens to a thread, so that one prefix sum orders them all
@@ -988,7 +988,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   u64 at = block_prefix(sum, sh.scan, &all) - sum;
   if (at <= target && target < at + sum) {
     // this thread's: its tokens again, one by one
-    for (int i = mine;; ++i) {
+    for (int i = mine; i < end; ++i) {
       const u64 w = weight_of(x[i], i);
       if (target < at + w) {
         a.ids[row] = i;
@@ -1140,7 +1140,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
     u64 at = __shfl_up(sum[j], 1);
     at = base + (lane == 0 ? 0 : at);
     if (at <= target && target < base + sum[j]) {
-      for (int i = j < kShortVecs ? logits.at(j) : last;; ++i) {
+      for (int i = j < kShortVecs ? logits.at(j) : last; i < a.vocab; ++i) {
         const u64 w = weight_of(x[i], i);
         if (target < at + w) {
           a.ids[row] = i;
@@ -1159,7 +1159,9 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
 // as possible otherwise (fewer sums to join).
 struct SamplePlan {
   int64_t chunk, chunks;
-  size_t max_bytes, mass_bytes, chunk_bins_bytes, bin_mass_bytes, bin_count_bytes, ends_bytes, list_bytes, count_bytes;
+  size_t max_bytes, mass_bytes, chunk_bins_bytes, bin_mass_bytes, bin_count_bytes, ends_bytes,
+      list_bytes, count_bytes;
+  size_t bytes;  // of all of them
 };
 
 static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
@@ -1181,6 +1183,8 @@ static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
   p.ends_bytes = rounded(r * sizeof(RowEnds));
   p.list_bytes = rounded(r * kListMax * sizeof(u64));
   p.count_bytes = rounded(r * sizeof(uint32_t));
+  p.bytes = p.max_bytes + p.mass_bytes + p.chunk_bins_bytes + p.bin_mass_bytes +
+            p.bin_count_bytes + p.ends_bytes + p.list_bytes + p.count_bytes;
   return p;
 }
 
@@ -1191,9 +1195,13 @@ using namespace cascade;
 extern "C" size_t cascade_sample_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows <= 0 || vocab <= 0 || vocab > kSampleMaxVocab || rows > 0x7fffffff) return 0;
   if (vocab <= kShortVocab) return 256;
-  const SamplePlan p = sample_plan(rows, vocab);
-  return p.max_bytes + p.mass_bytes + p.chunk_bins_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes +
-         p.list_bytes + p.count_bytes;
+  // enough for fewer rows too, which may be cut into more chunks
+  size_t most = 0;
+  for (int64_t r = rows < kSliceRows ? rows : kSliceRows; r >= 1; --r) {
+    const size_t bytes = sample_plan(r, vocab).bytes;
+    most = bytes > most ? bytes : most;
+  }
+  return most;
 }
 
 extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64_t rows,
@@ -1216,7 +1224,10 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
   for (const void *p : words)
     if (reinterpret_cast<uintptr_t>(p) & 3) return CASCADE_EALIGN;
   if ((reinterpret_cast<uintptr_t>(ids) & 7) || !aligned16(workspace)) return CASCADE_EALIGN;
-  if (workspace_bytes < cascade_sample_workspace_bytes(rows, vocab)) return CASCADE_EWORKSPACE;
+  const bool short_rows = vocab <= kShortVocab;
+  if (short_rows && rows > 0xffffffff / kSampleThreads) return CASCADE_ESHAPE;
+  const SamplePlan p = short_rows ? SamplePlan{} : sample_plan(rows, vocab);
+  if (workspace_bytes < (short_rows ? size_t{256} : p.bytes)) return CASCADE_EWORKSPACE;
   SampleArgs a{};
   a.row_stride = row_stride;
   a.vocab = static_cast<int32_t>(vocab);
@@ -1225,7 +1236,7 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
   a.top_p_value = top_p_value;
   a.min_p_value = min_p_value;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (vocab <= kShortVocab) {
+  if (short_rows) {
     a.logits = logits;
     a.uniform = uniform;
     a.temperature = temperature;
@@ -1241,7 +1252,6 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
     return launch_kernel(sample_short_kernel<kSampleThreads>, grid, dim3(kSampleThreads), 0,
                          s, a);
   }
-  const SamplePlan p = sample_plan(rows, vocab);
   a.chunk = static_cast<int32_t>(p.chunk);
   a.chunks = static_cast<int32_t>(p.chunks);
   unsigned char *ws = static_cast<unsigned char *>(workspace);

@@ -289,6 +289,11 @@ class PagedKVCache:
         count = kv_cache.sequence_length()
         if count == 0:
             return
+        if kv_cache.buffer.device != self.buffer.device:
+            raise ValueError("the caches live on {} and {}".format(
+                kv_cache.buffer.device, self.buffer.device))
+        if kv_cache.lengths != [count] * kv_cache.layer_count:
+            raise ValueError("the layers of the cache differ in length")
         if (kv_cache.layer_count, kv_cache.num_kv_heads, kv_cache.head_dim) != (
                 self.layer_count, self.num_kv_heads, self.head_dim):
             raise ValueError("the caches differ in layers, heads or head size")

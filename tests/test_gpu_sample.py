@@ -142,6 +142,43 @@ def test_whole_vocabularies(gpu_device, vocab):
         assert torch.equal(a, ids.cpu())
 
 
+@pytest.mark.parametrize("vocab", [900, 5000, 20000])
+def test_extreme_temperatures(gpu_device, vocab):
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randn(3, vocab, generator=g)
+    uniform = torch.rand(3, generator=g)
+    # the smallest numbers above 0: the largest logit, drawn with certainty
+    for t in (5e-324, 1e-310, 1e-40):
+        ids, logprobs = draw(logits, uniform, gpu_device, temperature=t)
+        assert torch.equal(ids, logits.argmax(-1)) and bool((logprobs == 0).all())
+        ids, _ = draw(logits, uniform, gpu_device, temperature=t, top_k=20, top_p=0.9)
+        assert torch.equal(ids, logits.argmax(-1))
+    # an infinite one: every token that is not masked alike
+    logits[:, ::3] = -math.inf
+    live = [i for i in range(vocab) if i % 3]
+    ids, logprobs = draw(logits, uniform, gpu_device, temperature=math.inf)
+    for r in range(3):
+        assert int(ids[r]) == live[int(float(uniform[r]) * len(live))]
+        assert abs(float(logprobs[r]) + math.log(len(live))) <= 2.0 ** -24 * math.log(len(live))
+
+
+def test_rows_past_one_slice(gpu_device):
+    # more rows than one launch's workspace holds, of the longer kind
+    g = torch.Generator().manual_seed(77)
+    rows, vocab = 300, 17000
+    logits = torch.randn(rows, vocab, generator=g) * 2
+    uniform = torch.rand(rows, generator=g)
+    settings = dict(temperature=0.5 + torch.rand(rows, generator=g), top_k=30, top_p=0.9)
+    ids, logprobs = draw(logits, uniform, gpu_device, **settings)
+    for first in (0, 100, 250, 299):
+        part = {k: v[first:first + 1] if isinstance(v, torch.Tensor) else v
+                for k, v in settings.items()}
+        one, lp = draw(logits[first:first + 1], uniform[first:first + 1], gpu_device, **part)
+        assert one[0] == ids[first] and lp[0] == logprobs[first]
+        mine = {k: v[0].item() if isinstance(v, torch.Tensor) else v for k, v in part.items()}
+        assert int(one[0]) == plain(logits[first], uniform[first], **mine)[0]
+
+
 def test_frequencies(gpu_device):
     # evenly spaced uniforms: each token's count is its probability, to one
     # draw either way

@@ -148,6 +148,12 @@ def test_load_refuses_another_geometry(cache):
     other.append(0, torch.zeros(1, 1, 3, 32), torch.zeros(1, 1, 3, 32))
     with pytest.raises(ValueError):
         cache.load(cache.add(), other)
+    # one layer behind the others
+    other = SimpleKVCache(2, 1, 16, device="cpu")
+    other.append(0, torch.zeros(1, 1, 3, 16), torch.zeros(1, 1, 3, 16))
+    with pytest.raises(ValueError):
+        cache.load(0, other)
+    assert cache.length(0) == 0
     empty = SimpleKVCache(2, 1, 32, device="cpu")
     cache.load(0, empty)  # nothing to copy
 
@@ -193,7 +199,8 @@ def append_args(**changes):
     (1003, dict(page_size=4)), (1003, dict(page_size=2048, page_stride=1 << 20,
                                            head_stride=1 << 19)),
     (1003, dict(rope_dim=136)), (1003, dict(rope_dim=24)), (1003, dict(rope_dim=-16)),
-    (1003, dict(max_pages=1 << 28, table_stride=1 << 28)), (1002, dict(k=24)),
+    (1003, dict(max_pages=1 << 28, table_stride=1 << 28)),
+    (1003, dict(tokens=1 << 25)), (1002, dict(k=24)),
     (1002, dict(q_out=8)), (1002, dict(cos=20)), (1002, dict(kt=1028)),
     (1002, dict(qh=-128)), (1002, dict(positions=18)), (1002, dict(error=17))])
 def test_append_entry_point_refuses(code, changes):
@@ -216,7 +223,7 @@ def attention_args(**changes):
     (1001, dict(batch=0)), (1001, dict(kv=0)), (1001, dict(max_length=0)),
     (1001, dict(max_length=161)), (1001, dict(page_stride=16 * 128)),
     (1001, dict(sequences=0)), (1003, dict(dim=96)), (1003, dict(heads=9)),
-    (1003, dict(heads=34)), (1003, dict(page_size=48)), (1002, dict(q=20)),
+    (1003, dict(heads=34)), (1003, dict(page_size=48)), (1003, dict(batch=1 << 24)), (1002, dict(q=20)),
     (1002, dict(out=8)), (1002, dict(qt=1020)), (1002, dict(lengths=18)),
     (1002, dict(workspace=8)), (1004, dict(workspace_bytes=8))])
 def test_attention_entry_point_refuses(code, changes):
@@ -249,7 +256,7 @@ def test_copy_entry_point_refuses(code, changes):
     (1001, dict(workspace=None)), (1001, dict(rows=0)), (1001, dict(vocab=0)),
     (1001, dict(row_stride=99)), (1001, dict(t=-1.0)), (1001, dict(t=float("nan"))),
     (1001, dict(p=float("nan"))), (1001, dict(p=-0.5)), (1001, dict(m=-0.5)),
-    (1003, dict(vocab=(1 << 19) + 1, row_stride=1 << 20)), (1002, dict(ids=12)),
+    (1003, dict(vocab=(1 << 19) + 1, row_stride=1 << 20)), (1003, dict(rows=1 << 23)), (1002, dict(ids=12)),
     (1002, dict(logits=18)), (1002, dict(workspace=8)), (1004, dict(workspace_bytes=8))])
 def test_sample_entry_point_refuses(code, changes):
     names = dict(logits=16, row_stride=100, rows=2, vocab=100, uniform=16, t_ptr=None, t=1.0,
@@ -257,6 +264,17 @@ def test_sample_entry_point_refuses(code, changes):
                  workspace=16, workspace_bytes=1 << 30, stream=None)
     names.update(changes)
     assert _hip.load().cascade_sample_f32(*names.values()) == code
+
+
+def test_workspaces_serve_smaller_calls_too():
+    # sized once for the largest call: fewer rows never need more
+    size = _hip.paged_attention_workspace_bytes
+    for limit in (1, 500, 5000, 1 << 20):
+        needs = [size(b, 32, 8, 128, limit) for b in (1, 2, 7, 64, 1000, 1024, 1025, 5000)]
+        assert needs == sorted(needs)
+    for vocab in (100, 16385, 20000, 128256, 1 << 19):
+        needs = [_hip.sample_workspace_bytes(r, vocab) for r in range(1, 300)]
+        assert needs == sorted(needs)
 
 
 def test_sample_workspace_shapes():
