@@ -13,6 +13,11 @@ and, after the prefill, decodes by replaying one captured HIP graph per
 token (layer_streaming.DecodeGraph; needs --vocab-mode resident).  Its
 decode_token_latencies_ms lists the replays; the first decode step runs
 eagerly while the graph is captured (decode_graph_setup_ms).
+
+--temperature (not in the reference, which takes the top-1 of the logits)
+draws each token instead, over the whole vocabulary: --sample-top-k,
+--sample-top-p and --sample-min-p restrict the draw (layer_streaming.sample),
+--sample-seed fixes its random numbers.  The default, 0, is greedy.
 """
 
 import argparse
@@ -37,6 +42,8 @@ from layer_streaming import (  # noqa: E402
     VocabStreamingRuntime,
     build_llama31_8b_plan,
     create_weight_store,
+    sample,
+    sample_workspace_bytes,
 )
 
 
@@ -64,12 +71,58 @@ def parse_args(argv=None):
                         help="weights resident in HBM; decode by replaying one "
                              "captured HIP graph per token (needs --vocab-mode "
                              "resident)")
+    parser.add_argument("--temperature", type=float, default=0.0,
+                        help="draw tokens at this temperature (0: greedy)")
+    parser.add_argument("--sample-top-k", type=int, default=0,
+                        help="draw from this many most likely tokens (0: all)")
+    parser.add_argument("--sample-top-p", type=float, default=1.0,
+                        help="draw from the likeliest tokens of this total "
+                             "probability")
+    parser.add_argument("--sample-min-p", type=float, default=0.0,
+                        help="draw from tokens at least this likely, relative "
+                             "to the likeliest")
+    parser.add_argument("--sample-seed", type=int, default=0)
     args = parser.parse_args(argv)
     if args.checkpoint is None and not args.random_init:
         parser.error("either --checkpoint or --random-init is required")
     if args.decode_graph and args.vocab_mode != "resident":
         parser.error("--decode-graph needs --vocab-mode resident")
+    if args.decode_graph and args.temperature != 0:
+        parser.error("--decode-graph decodes greedily (--temperature 0)")
+    for name in ("temperature", "sample_top_k", "sample_top_p", "sample_min_p"):
+        if not getattr(args, name) >= 0:
+            parser.error("--{} must not be negative".format(name.replace("_", "-")))
     return args
+
+
+class _NextToken:
+    """The next input id ([1, 1] int64 on the device) from a finished step:
+    the top-1 of its logits, or a draw from them."""
+
+    def __init__(self, args, device):
+        self.settings = None
+        if args.temperature == 0:
+            return
+        self.settings = {"temperature": args.temperature, "top_k": args.sample_top_k,
+                         "top_p": args.sample_top_p, "min_p": args.sample_min_p}
+        # one number a token, drawn ahead
+        generator = torch.Generator().manual_seed(args.sample_seed)
+        self.uniform = torch.rand(args.max_new_tokens, generator=generator).to(device)
+        self.drawn = 0
+        self.workspace = None
+
+    def __call__(self, state):
+        if self.settings is None:
+            return state.topk_indices[..., 0]
+        logits = state.logits[:, -1]
+        if self.workspace is None:
+            self.workspace = torch.empty(sample_workspace_bytes(*logits.shape),
+                                         dtype=torch.uint8, device=logits.device)
+        ids = torch.empty(1, dtype=torch.int64, device=logits.device)
+        sample(logits, self.uniform[self.drawn:self.drawn + 1], ids, self.workspace,
+               **self.settings)
+        self.drawn += 1
+        return ids.view(1, 1)
 
 
 def main(argv=None):
@@ -113,7 +166,9 @@ def main(argv=None):
     if plan.vocab is not None:
         vocab_runtime = VocabStreamingRuntime(plan, store, runtime)
     executor = Llama31DecodeExecutor(config, resident, vocab_runtime=vocab_runtime,
-                                     top_k=args.top_k)
+                                     top_k=args.top_k,
+                                     return_full_logits=args.temperature != 0)
+    next_token_of = _NextToken(args, device)
     if tokenizer is not None:
         input_ids = tokenizer(args.prompt, return_tensors="pt",
                               add_special_tokens=True).input_ids.to(device)
@@ -128,7 +183,7 @@ def main(argv=None):
         state = executor.begin(input_ids)
         state = runtime.run(executor, state)
         state = executor.finish(state)
-        next_token = state.topk_indices[..., 0]
+        next_token = next_token_of(state)
         generated.append(next_token)
         eager_steps = args.max_new_tokens - 1
         if args.decode_graph and args.max_new_tokens >= 3:
@@ -150,7 +205,7 @@ def main(argv=None):
             state = executor.begin(next_token)
             state = runtime.run(executor, state)
             state = executor.finish(state)
-            next_token = state.topk_indices[..., 0]
+            next_token = next_token_of(state)
             # the token is on the device once the caller's stream is done;
             # a device-wide synchronise would also wait for the copies the
             # streamed runtime already runs for the next token
@@ -169,6 +224,7 @@ def main(argv=None):
         "granularity": args.granularity,
         "vocab_mode": args.vocab_mode,
         "top_k": args.top_k,
+        "temperature": args.temperature,
         "prompt_tokens": int(input_ids.numel()),
         "generated_tokens": args.max_new_tokens,
         "generated_ids": generated_ids[0].tolist(),
