@@ -51,6 +51,7 @@ constexpr int kChunkMin = 2048;
 constexpr int kChunkMax = 8192;
 constexpr int kChunkWorkgroups = 1024;  // wanted of a launch
 constexpr int kChunkVecs = kChunkMax / (4 * kChunkThreads);  // of four logits, a thread
+constexpr int kFewThreads = 512;  // of the draw from the smallest chunks
 constexpr int kShortVecs = 4;
 constexpr int64_t kShortVocab = int64_t{4} * kSampleThreads * kShortVecs;
 constexpr int64_t kSliceRows = 256;  // rows of a launch (the workspace holds these)
@@ -858,7 +859,8 @@ __device__ u64 counted_cut(const float *x, int n, const RowScale &r, const RowSe
 }
 
 // One workgroup a row.
-__global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs a) {
+template <int THREADS, int CHUNK>
+__global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
   __shared__ DrawShared sh;
   const int row = blockIdx.x;
   const int tid = threadIdx.x;
@@ -891,7 +893,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
     __syncthreads();
     const int begin = min(sh.first[0], a.chunks - 1) * a.chunk;
     const int end = min(begin + a.chunk, a.vocab);
-    for (int i = begin + tid; i < end; i += kSampleThreads)
+    for (int i = begin + tid; i < end; i += THREADS)
       if (x[i] == mx) {
         atomicMin(&sh.first[1], i);
         break;
@@ -910,18 +912,18 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
     if (entries > kListMax) {
       u64 live = 0, sum = 0;
 #pragma unroll 1
-      for (int i = tid; i < a.vocab; i += kSampleThreads) {
+      for (int i = tid; i < a.vocab; i += THREADS) {
         const u64 w = fixed_weight(x[i], r);
         live += w != 0 ? 1 : 0;
         sum += w;
       }
       u64 live_all, mass_all;
-      block_prefix(live, sh.scan, &live_all);
-      block_prefix(sum, sh.scan, &mass_all);
-      cut = counted_cut<kSampleThreads>(x, a.vocab, r, set, mass_all, live_all, sh.row);
+      block_prefix<THREADS / kWave>(live, sh.scan, &live_all);
+      block_prefix<THREADS / kWave>(sum, sh.scan, &mass_all);
+      cut = counted_cut<THREADS>(x, a.vocab, r, set, mass_all, live_all, sh.row);
       // the chunks' masses, a wave a chunk
 #pragma unroll 1
-      for (int c = tid / kWave; c < a.chunks; c += kSampleWaves) {
+      for (int c = tid / kWave; c < a.chunks; c += (THREADS / kWave)) {
         const int end = min((c + 1) * a.chunk, a.vocab);
         u64 part = 0;
 #pragma unroll 1
@@ -937,12 +939,12 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
     } else if (entries > 0) {
       if (tid < a.chunks) sh.mass[tid] = mass;
       const int n = static_cast<int>(entries);
-      cut = n <= kSampleThreads
-                ? list_cut<kSampleThreads, 1>(nullptr, n, tid < n ? key : 0, e, set, r, sh)
-                : list_cut<kSampleThreads, kListMax / kSampleThreads>(
+      cut = n <= THREADS
+                ? list_cut<THREADS, 1>(nullptr, n, tid < n ? key : 0, e, set, r, sh)
+                : list_cut<THREADS, kListMax / THREADS>(
                       a.list + static_cast<int64_t>(row) * kListMax, n, 0, e, set, r, sh);
       // what the list adds to its chunks
-      for (int i = tid; i < static_cast<int>(entries); i += kSampleThreads) {
+      for (int i = tid; i < static_cast<int>(entries); i += THREADS) {
         const u64 key = sh.keys[i];
         const u64 w = fixed_weight(key_value(key), r);
         if (key >= cut && w >= set.min_w) atomicAdd(&sh.mass[key_index(key) / a.chunk], w);
@@ -953,7 +955,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   }
   // the draw: a chunk, then a token in it
   u64 total;
-  const u64 upto = block_prefix(mass, sh.scan, &total);
+  const u64 upto = block_prefix<THREADS / kWave>(mass, sh.scan, &total);
   u = u > 0.0 ? u : 0.0;  // NaN too
   const double t = u * static_cast<double>(total);
   u64 target = t < static_cast<double>(total) ? static_cast<u64>(t) : total - 1;
@@ -967,8 +969,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   const int end = min(begin + a.chunk, a.vocab);
   target = sh.found[1];
   // neighbouring tokens to a thread, so that one prefix sum orders them all
-  constexpr int kPer = kChunkMax / kSampleThreads;
-  const int per = a.chunk / kSampleThreads;
+  constexpr int kPer = CHUNK / THREADS;
+  const int per = a.chunk / THREADS;
   float v[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
@@ -985,7 +987,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
   for (int j = 0; j < kPer; ++j)
     if (j < per) sum += weight_of(v[j], mine + j);
   u64 all;
-  u64 at = block_prefix(sum, sh.scan, &all) - sum;
+  u64 at = block_prefix<THREADS / kWave>(sum, sh.scan, &all) - sum;
   if (at <= target && target < at + sum) {
     // this thread's: its tokens again, one by one
     for (int i = mine; i < end; ++i) {
@@ -1101,17 +1103,26 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
   }
   // the draw: masses of the threads' vectors, in the order of their tokens
   // (vector j of all threads, then vector j + 1; the rest last)
+  auto in_cut = [&](float logit, int i) {
+    return topk_key(logit, static_cast<uint32_t>(i)) >= cut;
+  };
   auto weight_of = [&](float logit, int i) {
     const u64 w = fixed_weight(logit, r);
-    return w >= set.min_w && topk_key(logit, static_cast<uint32_t>(i)) >= cut ? w : u64{0};
+    return w >= set.min_w && in_cut(logit, i) ? w : u64{0};
   };
   u64 sum[kShortVecs + 1];
 #pragma unroll
   for (int j = 0; j < kShortVecs; ++j) {
     sum[j] = 0;
     if (logits.at(j) < logits.whole) {
+      // (a cut leaves most vectors nothing)
+      bool any = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[j] += weight_of(logits.v[j][i], logits.at(j) + i);
+      for (int i = 0; i < 4; ++i) any |= in_cut(logits.v[j][i], logits.at(j) + i);
+      if (any) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[j] += weight_of(logits.v[j][i], logits.at(j) + i);
+      }
     }
     sum[j] = wave_prefix(sum[j]);
     if (lane == kWave - 1) sh.mass[j * kWaves + wave] = sum[j];
@@ -1291,8 +1302,12 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
       e = launch_kernel(sample_collect_kernel, grid, block, 0, s, a);
       if (e != hipSuccess) return e;
     }
-    e = launch_kernel(sample_draw_kernel, dim3(static_cast<unsigned>(count)),
-                      dim3(kSampleThreads), 0, s, a);
+    const dim3 rows_grid(static_cast<unsigned>(count));
+    e = p.chunk == kChunkMin
+            ? launch_kernel(sample_draw_kernel<kFewThreads, kChunkMin>, rows_grid,
+                            dim3(kFewThreads), 0, s, a)
+            : launch_kernel(sample_draw_kernel<kSampleThreads, kChunkMax>, rows_grid,
+                            dim3(kSampleThreads), 0, s, a);
     if (e != hipSuccess) return e;
   }
   return 0;
