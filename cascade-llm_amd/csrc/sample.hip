@@ -85,7 +85,8 @@ struct SampleArgs {
   int32_t chunks;
   float *chunk_max;  // [rows][chunks]: the largest logit, NaN if there is one
   u64 *chunk_mass;  // [rows][chunks]
-  u64 *chunk_bins;  // [rows][chunks][kSampleBins]: rows with a top-p
+  u64 *chunk_bins;  // [rows][chunks][kSampleBins]: rows with a top-p; null
+                    // for small chunks, whose bins would outweigh them
   u64 *bin_mass;    // [rows][kSampleBins]
   uint32_t *bin_count;
   struct RowEnds *ends;  // [rows]
@@ -515,7 +516,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
   for (int i = tid; i < kSampleBins; i += kChunkThreads) {
     if (s_count[i] != 0) atomicAdd(&count[i], s_count[i]);
     if (s_mass[i] != 0) atomicAdd(&mass[i], s_mass[i]);
-    if (use_p) bins[i] = s_mass[i];
+    if (use_p && a.chunk_bins != nullptr) bins[i] = s_mass[i];
   }
 }
 
@@ -672,7 +673,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   // the mass of the bins above the listed ones: from the chunk's own bins
   // where they hold it (and min-p drops none of it)
   constexpr int kPer = BinShare<kChunkThreads>::kPer;
-  const bool summed = set.use_p && set.min_w == 0;
+  const bool summed = set.use_p && set.min_w == 0 && a.chunk_bins != nullptr;
   u64 own[kPer];
   if (summed) {
     const u64 *chunk_bins =
@@ -1188,7 +1189,7 @@ static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
   const size_t r = static_cast<size_t>(rows);
   p.max_bytes = rounded(r * p.chunks * sizeof(float));
   p.mass_bytes = rounded(r * p.chunks * sizeof(u64));
-  p.chunk_bins_bytes = r * p.chunks * kSampleBins * sizeof(u64);
+  p.chunk_bins_bytes = p.chunk < kChunkMax ? 0 : r * p.chunks * kSampleBins * sizeof(u64);
   p.bin_mass_bytes = rounded(r * kSampleBins * sizeof(u64));
   p.bin_count_bytes = rounded(r * kSampleBins * sizeof(uint32_t));
   p.ends_bytes = rounded(r * sizeof(RowEnds));
@@ -1273,7 +1274,8 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
   };
   a.chunk_max = reinterpret_cast<float *>(take(p.max_bytes));
   a.chunk_mass = reinterpret_cast<u64 *>(take(p.mass_bytes));
-  a.chunk_bins = reinterpret_cast<u64 *>(take(p.chunk_bins_bytes));
+  a.chunk_bins =
+      p.chunk_bins_bytes != 0 ? reinterpret_cast<u64 *>(take(p.chunk_bins_bytes)) : nullptr;
   a.bin_mass = reinterpret_cast<u64 *>(take(p.bin_mass_bytes));
   a.bin_count = reinterpret_cast<uint32_t *>(take(p.bin_count_bytes));
   a.ends = reinterpret_cast<RowEnds *>(take(p.ends_bytes));
