@@ -20,14 +20,14 @@
 //   1. sample_max_kernel     a chunk's largest logit
 //   2. sample_weigh_kernel   2048 bins of (x_i - max) / T, with the number
 //                            and the mass of their tokens (rows with a top-k
-//                            or top-p), or the chunk's mass (other rows)
+//                            or top-p), or the masses of parts (other rows)
 //   3. sample_collect_kernel the bins in which K and P end, from those sums;
 //                            their tokens go to a list, the mass of the
-//                            bins above is kept by chunk.  A K of at most
+//                            bins above is kept by parts of 2048.  A K of at most
 //                            kShortK tokens is listed whole, which spares
 //                            its row the masses.
 //   4. sample_draw_kernel    one workgroup a row: sorts the list, finds the
-//                            two ends in it, draws a chunk and then its token
+//                            two ends in it, draws a part and then its token
 // A row whose list would be longer than kListMax (ends in runs of equal
 // logits) is instead cut by the last launch alone, which counts 11 bits of
 // the ordered logits at a time over the row.
@@ -48,10 +48,13 @@ constexpr int kListMax = 4096;
 constexpr int kShortK = 1024;  // K up to this size is listed whole
 constexpr int kChunkThreads = 256;
 constexpr int kChunkMin = 2048;
+constexpr int kPart = 2048;  // tokens of a chunk whose mass is kept: the draw walks one
 constexpr int kChunkMax = 8192;
 constexpr int kChunkWorkgroups = 1024;  // wanted of a launch
 constexpr int kChunkVecs = kChunkMax / (4 * kChunkThreads);  // of four logits, a thread
-constexpr int kFewThreads = 512;  // of the draw from the smallest chunks
+constexpr int kChunkParts = kChunkMax / kPart;
+constexpr int kFewThreads = 512;  // of a draw whose list is short
+constexpr int64_t kFewK = 480;    // K up to this is one
 constexpr int kShortVecs = 4;
 constexpr int64_t kShortVocab = int64_t{4} * kSampleThreads * kShortVecs;
 constexpr int64_t kSliceRows = 256;  // rows of a launch (the workspace holds these)
@@ -84,9 +87,8 @@ struct SampleArgs {
   int32_t chunk;
   int32_t chunks;
   float *chunk_max;  // [rows][chunks]: the largest logit, NaN if there is one
-  u64 *chunk_mass;  // [rows][chunks]
-  u64 *chunk_bins;  // [rows][chunks][kSampleBins]: rows with a top-p; null
-                    // for small chunks, whose bins would outweigh them
+  int32_t parts;    // of a row: ceil(vocab / kPart)
+  u64 *part_mass;   // [rows][parts]
   u64 *bin_mass;    // [rows][kSampleBins]
   uint32_t *bin_count;
   struct RowEnds *ends;  // [rows]
@@ -387,7 +389,8 @@ struct Chunk {
     return begin + 4 * (THREADS * j + static_cast<int>(threadIdx.x));
   }
 
-  // f(logits, index of the first) for every four neighbours: f
+  // f(logits, index of the first, part) for every four neighbours, part being
+  // the kPart tokens of the chunk that they belong to: f
   // does the arithmetic of all four before it branches on any, so that their
   // chains of fp64 instructions overlap.  The rest comes as one logit with
   // three -inf.
@@ -395,9 +398,9 @@ struct Chunk {
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll
     for (int j = 0; j < VECS; ++j)
-      if (at(j) < whole) f(v[j], at(j));
+      if (at(j) < whole) f(v[j], at(j), 4 * THREADS * j / kPart);
     const int i = whole + static_cast<int>(threadIdx.x);
-    if (i < end) f(f32x4_at4{rest, -INFINITY, -INFINITY, -INFINITY}, i);
+    if (i < end) f(f32x4_at4{rest, -INFINITY, -INFINITY, -INFINITY}, i, (i - begin) / kPart);
   }
 };
 
@@ -433,7 +436,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a)
   }
   if (chunk == 0 && tid == 0) a.list_count[row] = 0;
   float best = -INFINITY;
-  logits.each([&](const f32x4_at4 &v, int) {
+  logits.each([&](const f32x4_at4 &v, int, int) {
     best = nan_max(nan_max(best, nan_max(v[0], v[1])), nan_max(v[2], v[3]));
   });
   best = wave_nan_max(best);
@@ -443,6 +446,26 @@ __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs a)
 #pragma unroll
     for (int w = 1; w < kChunkThreads / kWave; ++w) best = nan_max(best, s_max[w]);
     a.chunk_max[static_cast<int64_t>(row) * a.chunks + chunk] = best;
+  }
+}
+
+// Writes the masses of the chunk's parts from its threads' shares of them.
+__device__ __forceinline__ void store_parts(const SampleArgs &a, int row, int chunk,
+                                            const u64 (&sum)[kChunkParts], u64 *lds) {
+  constexpr int kWaves = kChunkThreads / kWave;
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < kChunkParts; ++k) {
+    const u64 wave = wave_prefix(sum[k]);
+    if ((tid & (kWave - 1)) == kWave - 1) lds[k * kWaves + tid / kWave] = wave;
+  }
+  __syncthreads();
+  const int part = chunk * (a.chunk / kPart) + tid;
+  if (tid < a.chunk / kPart && part < a.parts) {
+    u64 total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += lds[tid * kWaves + w];
+    a.part_mass[static_cast<int64_t>(row) * a.parts + part] = total;
   }
 }
 
@@ -480,23 +503,24 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
   const RowScale r = row_scale(mx, set, s_table);
   if (!set.use_k && !set.use_p) {
     __syncthreads();
-    u64 sum = 0;
-    logits.each([&](const f32x4_at4 &v, int) {
+    u64 sum[kChunkParts] = {};
+    logits.each([&](const f32x4_at4 &v, int, int part) {
       double t[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) t[i] = log_weight(v[i], r);
       if (set.min_w != 0 &&
           weight_bin(fmax(fmax(t[0], t[1]), fmax(t[2], t[3]))) >= set.min_bin)
         return;
+      u64 four = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const u64 w = fixed_weight(t[i], s_table);
-        sum += w >= set.min_w ? w : 0;
+        four += w >= set.min_w ? w : 0;
       }
+#pragma unroll
+      for (int k = 0; k < kChunkParts; ++k) sum[k] += part == k ? four : 0;
     });
-    u64 total;
-    block_prefix<kChunkThreads / kWave>(sum, s_mass, &total);
-    if (tid == 0) a.chunk_mass[static_cast<int64_t>(row) * a.chunks + chunk] = total;
+    store_parts(a, row, chunk, sum, s_mass);
     return;
   }
   // top-k needs the numbers, top-p the masses
@@ -506,17 +530,15 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
     s_count[i] = 0;
   }
   __syncthreads();
-  logits.each([&](const f32x4_at4 &v, int) {
+  logits.each([&](const f32x4_at4 &v, int, int) {
     add_to_bins(v, r, use_k, use_p, s_count, s_mass);
   });
   __syncthreads();
   u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins;
   uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins;
-  u64 *bins = a.chunk_bins + (static_cast<int64_t>(row) * a.chunks + chunk) * kSampleBins;
   for (int i = tid; i < kSampleBins; i += kChunkThreads) {
     if (s_count[i] != 0) atomicAdd(&count[i], s_count[i]);
     if (s_mass[i] != 0) atomicAdd(&mass[i], s_mass[i]);
-    if (use_p && a.chunk_bins != nullptr) bins[i] = s_mass[i];
   }
 }
 
@@ -660,7 +682,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   __shared__ u64 s_keys[kListMax];
   __shared__ uint32_t s_count, s_at;
   __shared__ double s_table[kTable];
-  __shared__ u64 s_scan[kChunkThreads / kWave];
+  __shared__ u64 s_sum[kChunkParts * (kChunkThreads / kWave)];
   const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
@@ -670,17 +692,6 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   const BinShare<kChunkThreads> bins(a.bin_mass + static_cast<int64_t>(row) * kSampleBins,
                                      a.bin_count + static_cast<int64_t>(row) * kSampleBins,
                                      set);
-  // the mass of the bins above the listed ones: from the chunk's own bins
-  // where they hold it (and min-p drops none of it)
-  constexpr int kPer = BinShare<kChunkThreads>::kPer;
-  const bool summed = set.use_p && set.min_w == 0 && a.chunk_bins != nullptr;
-  u64 own[kPer];
-  if (summed) {
-    const u64 *chunk_bins =
-        a.chunk_bins + (static_cast<int64_t>(row) * a.chunks + chunk) * kSampleBins;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) own[i] = chunk_bins[tid * kPer + i];
-  }
   fill_table(s_table);
   const float mx = row_max(a, row);
   if (no_token(mx)) return;
@@ -689,29 +700,26 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
   // without a cut inside the bins (top_k of all tokens) nothing is listed
   const int first = e.last_p < 0 && e.last_k < 0 ? kSampleBins : e.first;
   const RowScale r = row_scale(mx, set, s_table);
-  u64 sum = 0;
-  if (summed) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += tid * kPer + i < first ? own[i] : 0;
-  }
+  u64 sum[kChunkParts] = {};  // of the bins above the listed ones
   if (tid == 0) s_count = 0;
   __syncthreads();
-  logits.each([&](const f32x4_at4 &v, int at) {
+  logits.each([&](const f32x4_at4 &v, int at, int part) {
     double t[4];
     int b[4];
     bins_of(v, r, t, b);
     const int least = min(min(b[0], b[1]), min(b[2], b[3]));
-    if (!summed && least < min(first, set.min_bin)) {
-      u64 w[4];
+    if (least < min(first, set.min_bin)) {
+      u64 w[4], four = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = fixed_weight(t[i], s_table);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += b[i] < first && w[i] >= set.min_w ? w[i] : 0;
+      for (int i = 0; i < 4; ++i) four += b[i] < first && w[i] >= set.min_w ? w[i] : 0;
+#pragma unroll
+      for (int k = 0; k < kChunkParts; ++k) sum[k] += part == k ? four : 0;
     }
     list_of(v, at, b, first, e, s_keys, &s_count);
   });
-  u64 total;
-  block_prefix<kChunkThreads / kWave>(sum, s_scan, &total);
+  store_parts(a, row, chunk, sum, s_sum);  // (a barrier: the list is whole)
   const uint32_t mine = s_count;
   if (mine != 0) {
     // the list's order does not matter: the draw sorts it.  A row of more
@@ -723,7 +731,6 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(SampleArg
     if (mine <= kListMax && at <= kListMax - mine)
       for (uint32_t i = tid; i < mine; i += kChunkThreads) list[at + i] = s_keys[i];
   }
-  if (tid == 0) a.chunk_mass[static_cast<int64_t>(row) * a.chunks + chunk] = total;
 }
 
 struct DrawShared {
@@ -860,7 +867,7 @@ __device__ u64 counted_cut(const float *x, int n, const RowScale &r, const RowSe
 }
 
 // One workgroup a row.
-template <int THREADS, int CHUNK>
+template <int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
   __shared__ DrawShared sh;
   const int row = blockIdx.x;
@@ -869,8 +876,8 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
   fill_table(sh.table);
   // what the earlier launches left, loaded at once (a row without cuts has
   // no ends and no list: those words are not used then)
-  const u64 *chunk_mass = a.chunk_mass + static_cast<int64_t>(row) * a.chunks;
-  u64 mass = tid < a.chunks ? chunk_mass[tid] : 0;
+  const u64 *part_mass = a.part_mass + static_cast<int64_t>(row) * a.parts;
+  u64 mass = tid < a.parts ? part_mass[tid] : 0;
   const RowEnds e = a.ends[row];
   const uint32_t entries = a.list_count[row];
   const u64 key = a.list[static_cast<int64_t>(row) * kListMax + tid];
@@ -922,13 +929,13 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
       block_prefix<THREADS / kWave>(live, sh.scan, &live_all);
       block_prefix<THREADS / kWave>(sum, sh.scan, &mass_all);
       cut = counted_cut<THREADS>(x, a.vocab, r, set, mass_all, live_all, sh.row);
-      // the chunks' masses, a wave a chunk
+      // the parts' masses, a wave a part
 #pragma unroll 1
-      for (int c = tid / kWave; c < a.chunks; c += (THREADS / kWave)) {
-        const int end = min((c + 1) * a.chunk, a.vocab);
+      for (int c = tid / kWave; c < a.parts; c += (THREADS / kWave)) {
+        const int end = min((c + 1) * kPart, a.vocab);
         u64 part = 0;
 #pragma unroll 1
-        for (int i = c * a.chunk + (tid & (kWave - 1)); i < end; i += kWave) {
+        for (int i = c * kPart + (tid & (kWave - 1)); i < end; i += kWave) {
           const u64 w = fixed_weight(x[i], r);
           if (w >= set.min_w && topk_key(x[i], static_cast<uint32_t>(i)) >= cut) part += w;
         }
@@ -936,25 +943,25 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
         if ((tid & (kWave - 1)) == kWave - 1) sh.mass[c] = part;
       }
       __syncthreads();
-      if (tid < a.chunks) mass = sh.mass[tid];
+      if (tid < a.parts) mass = sh.mass[tid];
     } else if (entries > 0) {
-      if (tid < a.chunks) sh.mass[tid] = mass;
+      if (tid < a.parts) sh.mass[tid] = mass;
       const int n = static_cast<int>(entries);
       cut = n <= THREADS
                 ? list_cut<THREADS, 1>(nullptr, n, tid < n ? key : 0, e, set, r, sh)
                 : list_cut<THREADS, kListMax / THREADS>(
                       a.list + static_cast<int64_t>(row) * kListMax, n, 0, e, set, r, sh);
-      // what the list adds to its chunks
+      // what the list adds to its parts
       for (int i = tid; i < static_cast<int>(entries); i += THREADS) {
         const u64 key = sh.keys[i];
         const u64 w = fixed_weight(key_value(key), r);
-        if (key >= cut && w >= set.min_w) atomicAdd(&sh.mass[key_index(key) / a.chunk], w);
+        if (key >= cut && w >= set.min_w) atomicAdd(&sh.mass[key_index(key) / kPart], w);
       }
       __syncthreads();
-      if (tid < a.chunks) mass = sh.mass[tid];
+      if (tid < a.parts) mass = sh.mass[tid];
     }
   }
-  // the draw: a chunk, then a token in it
+  // the draw: a part, then a token in it
   u64 total;
   const u64 upto = block_prefix<THREADS / kWave>(mass, sh.scan, &total);
   u = u > 0.0 ? u : 0.0;  // NaN too
@@ -966,27 +973,25 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
     sh.found[1] = target - (upto - mass);
   }
   __syncthreads();
-  const int begin = static_cast<int>(min(sh.found[0], static_cast<u64>(a.chunks - 1))) * a.chunk;
-  const int end = min(begin + a.chunk, a.vocab);
+  const int begin = static_cast<int>(min(sh.found[0], static_cast<u64>(a.parts - 1))) * kPart;
+  const int end = min(begin + kPart, a.vocab);
   target = sh.found[1];
   // neighbouring tokens to a thread, so that one prefix sum orders them all
-  constexpr int kPer = CHUNK / THREADS;
-  const int per = a.chunk / THREADS;
+  constexpr int kPer = kPart / THREADS;
+  const int mine = begin + tid * kPer;
   float v[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    const int i = begin + tid * per + j;
-    v[j] = j < per && i < end ? x[i] : -INFINITY;
+    const float logit = x[min(mine + j, end - 1)];
+    v[j] = mine + j < end ? logit : -INFINITY;
   }
-  const int mine = begin + tid * per;
   auto weight_of = [&](float logit, int i) {
     const u64 w = fixed_weight(logit, r);
     return w >= set.min_w && topk_key(logit, static_cast<uint32_t>(i)) >= cut ? w : u64{0};
   };
   u64 sum = 0;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j)
-    if (j < per) sum += weight_of(v[j], mine + j);
+  for (int j = 0; j < kPer; ++j) sum += weight_of(v[j], mine + j);
   u64 all;
   u64 at = block_prefix<THREADS / kWave>(sum, sh.scan, &all) - sum;
   if (at <= target && target < at + sum) {
@@ -1031,7 +1036,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
     sh.first[0] = 0x7fffffff;
   }
   float mx = -INFINITY;
-  logits.each([&](const f32x4_at4 &v, int) {
+  logits.each([&](const f32x4_at4 &v, int, int) {
     mx = nan_max(nan_max(mx, nan_max(v[0], v[1])), nan_max(v[2], v[3]));
   });
   mx = wave_nan_max(mx);
@@ -1048,7 +1053,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
   }
   if (set.greedy) {
     int at = 0x7fffffff;
-    logits.each([&](const f32x4_at4 &v, int first) {
+    logits.each([&](const f32x4_at4 &v, int first, int) {
 #pragma unroll
       for (int i = 3; i >= 0; --i) at = v[i] == mx ? min(at, first + i) : at;
     });
@@ -1064,14 +1069,14 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
   const bool use_k = set.use_k, use_p = set.use_p;
   u64 cut = 0;
   if (use_k || use_p) {
-    logits.each([&](const f32x4_at4 &v, int) {
+    logits.each([&](const f32x4_at4 &v, int, int) {
       add_to_bins(v, r, use_k, use_p, sh.row.count, sh.row.mass);
     });
     __syncthreads();
     const RowEnds e = find_ends(BinShare<THREADS>(sh.row.mass, sh.row.count, set), set);
     if (e.last_p >= 0 || e.last_k >= 0) {
       __syncthreads();  // the list takes the place of the bins
-      logits.each([&](const f32x4_at4 &v, int at) {
+      logits.each([&](const f32x4_at4 &v, int at, int) {
         double t[4];
         int b[4];
         bins_of(v, r, t, b);
@@ -1081,7 +1086,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
       const int n = static_cast<int>(s_count);
       if (n > kListMax) {
         u64 live = 0, sum = 0;
-        logits.each([&](const f32x4_at4 &v, int) {
+        logits.each([&](const f32x4_at4 &v, int, int) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const u64 w = fixed_weight(v[i], r);
@@ -1171,8 +1176,9 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
 // as possible otherwise (fewer sums to join).
 struct SamplePlan {
   int64_t chunk, chunks;
-  size_t max_bytes, mass_bytes, chunk_bins_bytes, bin_mass_bytes, bin_count_bytes, ends_bytes,
-      list_bytes, count_bytes;
+  int64_t parts;
+  size_t max_bytes, mass_bytes, bin_mass_bytes, bin_count_bytes, ends_bytes, list_bytes,
+      count_bytes;
   size_t bytes;  // of all of them
 };
 
@@ -1181,22 +1187,21 @@ static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
   if (rows > kSliceRows) rows = kSliceRows;  // more rows go slice by slice
   const int64_t want = (kChunkWorkgroups + rows - 1) / rows;
   p.chunk = (vocab + want - 1) / want;
-  p.chunk = (p.chunk + kSampleThreads - 1) / kSampleThreads * kSampleThreads;
+  p.chunk = (p.chunk + kPart - 1) / kPart * kPart;
   if (p.chunk < kChunkMin) p.chunk = kChunkMin;
   if (p.chunk > kChunkMax) p.chunk = kChunkMax;
   p.chunks = (vocab + p.chunk - 1) / p.chunk;
   auto rounded = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
   const size_t r = static_cast<size_t>(rows);
   p.max_bytes = rounded(r * p.chunks * sizeof(float));
-  p.mass_bytes = rounded(r * p.chunks * sizeof(u64));
-  p.chunk_bins_bytes = p.chunk < kChunkMax ? 0 : r * p.chunks * kSampleBins * sizeof(u64);
+  p.parts = (vocab + kPart - 1) / kPart;
+  p.mass_bytes = rounded(r * p.parts * sizeof(u64));
   p.bin_mass_bytes = rounded(r * kSampleBins * sizeof(u64));
   p.bin_count_bytes = rounded(r * kSampleBins * sizeof(uint32_t));
   p.ends_bytes = rounded(r * sizeof(RowEnds));
   p.list_bytes = rounded(r * kListMax * sizeof(u64));
   p.count_bytes = rounded(r * sizeof(uint32_t));
-  p.bytes = p.max_bytes + p.mass_bytes + p.chunk_bins_bytes + p.bin_mass_bytes +
-            p.bin_count_bytes + p.ends_bytes + p.list_bytes + p.count_bytes;
+  p.bytes = p.max_bytes + p.mass_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes + p.list_bytes + p.count_bytes;
   return p;
 }
 
@@ -1273,9 +1278,8 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
     return part;
   };
   a.chunk_max = reinterpret_cast<float *>(take(p.max_bytes));
-  a.chunk_mass = reinterpret_cast<u64 *>(take(p.mass_bytes));
-  a.chunk_bins =
-      p.chunk_bins_bytes != 0 ? reinterpret_cast<u64 *>(take(p.chunk_bins_bytes)) : nullptr;
+  a.parts = static_cast<int32_t>(p.parts);
+  a.part_mass = reinterpret_cast<u64 *>(take(p.mass_bytes));
   a.bin_mass = reinterpret_cast<u64 *>(take(p.bin_mass_bytes));
   a.bin_count = reinterpret_cast<uint32_t *>(take(p.bin_count_bytes));
   a.ends = reinterpret_cast<RowEnds *>(take(p.ends_bytes));
@@ -1284,6 +1288,9 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
   // numbers for all rows that cut nothing need no lists
   const bool cuts = top_k != nullptr || top_k_value > 0 || top_p != nullptr ||
                     top_p_value < 1.0 || min_p != nullptr || min_p_value > 1.0;
+  // a list of at most a key a thread is sorted in registers; more threads make
+  // every sum dearer
+  const bool few = top_k == nullptr && top_k_value <= kFewK;
   const dim3 block(kChunkThreads);
   for (int64_t first = 0; first < rows; first += kSliceRows) {
     const int64_t count = rows - first < kSliceRows ? rows - first : kSliceRows;
@@ -1305,10 +1312,9 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
       if (e != hipSuccess) return e;
     }
     const dim3 rows_grid(static_cast<unsigned>(count));
-    e = p.chunk == kChunkMin
-            ? launch_kernel(sample_draw_kernel<kFewThreads, kChunkMin>, rows_grid,
-                            dim3(kFewThreads), 0, s, a)
-            : launch_kernel(sample_draw_kernel<kSampleThreads, kChunkMax>, rows_grid,
+    e = few ? launch_kernel(sample_draw_kernel<kFewThreads>, rows_grid, dim3(kFewThreads), 0,
+                            s, a)
+            : launch_kernel(sample_draw_kernel<kSampleThreads>, rows_grid,
                             dim3(kSampleThreads), 0, s, a);
     if (e != hipSuccess) return e;
   }
