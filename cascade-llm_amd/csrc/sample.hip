@@ -50,7 +50,10 @@ constexpr int kChunkThreads = 256;
 constexpr int kChunkMin = 2048;
 constexpr int kPart = 2048;  // tokens of a chunk whose mass is kept: the draw walks one
 constexpr int kChunkMax = 8192;
-constexpr int kChunkWorkgroups = 1024;  // wanted of a launch
+// Workgroups wanted of a launch: more of them find the row's bins and add to
+// them for fewer tokens each (16 rows of 128256 with a top-p: 31.9 us with 256
+// wanted, 34.6 with 512, 41.4 with 1024).
+constexpr int kChunkWorkgroups = 256;
 constexpr int kChunkVecs = kChunkMax / (4 * kChunkThreads);  // of four logits, a thread
 constexpr int kChunkParts = kChunkMax / kPart;
 constexpr int kFewThreads = 512;  // of a draw whose list is short
@@ -526,8 +529,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
   // top-k needs the numbers, top-p the masses
   const bool use_k = set.use_k, use_p = set.use_p;
   for (int i = tid; i < kSampleBins; i += kChunkThreads) {
-    s_mass[i] = 0;
-    s_count[i] = 0;
+    if (use_p) s_mass[i] = 0;
+    if (use_k) s_count[i] = 0;
   }
   __syncthreads();
   logits.each([&](const f32x4_at4 &v, int, int) {
@@ -537,8 +540,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(SampleArgs 
   u64 *mass = a.bin_mass + static_cast<int64_t>(row) * kSampleBins;
   uint32_t *count = a.bin_count + static_cast<int64_t>(row) * kSampleBins;
   for (int i = tid; i < kSampleBins; i += kChunkThreads) {
-    if (s_count[i] != 0) atomicAdd(&count[i], s_count[i]);
-    if (s_mass[i] != 0) atomicAdd(&mass[i], s_mass[i]);
+    if (use_k && s_count[i] != 0) atomicAdd(&count[i], s_count[i]);
+    if (use_p && s_mass[i] != 0) atomicAdd(&mass[i], s_mass[i]);
   }
 }
 
