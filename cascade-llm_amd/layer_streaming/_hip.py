@@ -907,7 +907,9 @@ def device_copy(dst, src, stream=None):
 
 _BF16, _F32, _I32, _LONG, _U8 = (torch.bfloat16, torch.float32, torch.int32,
                                  torch.int64, torch.uint8)
-# the current stream's handle by device index, without a Stream object
+# the current device, and the current stream's handle by device index, without
+# the Python around them (the device is initialised: its tensors are here)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _current_stream = torch._C._cuda_getCurrentRawStream if hasattr(
     torch._C, "_cuda_getCurrentRawStream") else (
         lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -1019,11 +1021,12 @@ def _call_on(index, stream, name, *args):
     ``index`` current."""
 
     handle = _current_stream(index) if stream is None else stream.cuda_stream
-    if index == torch.cuda.current_device():
-        code = getattr(_lib or load(), name)(*args, handle)
+    fn = getattr(_lib or load(), name)
+    if index == _current_device():
+        code = fn(*args, handle)
     else:
         with torch.cuda.device(index):
-            code = getattr(_lib or load(), name)(*args, handle)
+            code = fn(*args, handle)
     if code != 0:
         _check(name, code)
 
