@@ -142,6 +142,58 @@ def test_whole_vocabularies(gpu_device, vocab):
         assert torch.equal(a, ids.cpu())
 
 
+@pytest.mark.parametrize("vocab", [3, 1027, 4095, 4096, 4097, 8190, 16383, 16384, 16385, 16389,
+                                   18433, 40961])
+def test_row_lengths_around_the_kernels_tiles(gpu_device, vocab):
+    # one launch up to 16384 logits, by 256 threads up to 4096; chunks of 2048
+    # beyond; the last three logits of an odd row stand alone
+    print("sample", vocab, flush=True)
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randn(4, vocab, generator=g) * 1.5
+    logits[1, -1] += 9.0
+    logits[2, :-2] = -math.inf
+    uniform = torch.rand(4, generator=g)
+    for settings in (dict(temperature=1.3), dict(top_p=0.97), dict(top_k=1500, top_p=0.9),
+                     dict(top_k=1025), dict(top_k=1024, top_p=0.999, min_p=0.001),
+                     dict(temperature=0.0), dict(min_p=0.3)):
+        check(logits, uniform, gpu_device, **settings)
+
+
+def test_lists_of_every_length(gpu_device):
+    # logits that differ by less than a bin: whole rows of candidates, sorted
+    # in registers, in LDS, or (past 4096) replaced by counting
+    g = torch.Generator().manual_seed(5)
+    for vocab, near in ((3000, 200), (3000, 300), (6000, 600), (9000, 1100), (16000, 3000),
+                        (16000, 5000), (30000, 400), (30000, 700), (30000, 1500),
+                        (30000, 4000), (30000, 4200)):
+        print("list of", near, "in", vocab, flush=True)
+        logits = torch.randn(2, vocab, generator=g) - 20.0
+        for r in range(2):
+            at = torch.randperm(vocab, generator=g)[:near]
+            logits[r, at] = 1.0 + torch.rand(near, generator=g) * 0.004
+        uniform = torch.rand(2, generator=g)
+        for settings in (dict(top_p=0.6), dict(top_k=near // 2), dict(top_k=near - 1, top_p=0.7),
+                         dict(top_k=torch.tensor([near // 3, 7], dtype=torch.int32),
+                              top_p=0.5)):
+            check(logits, uniform, gpu_device, **settings)
+
+
+def test_on_a_stream_of_the_callers(gpu_device):
+    g = torch.Generator().manual_seed(6)
+    for vocab in (3000, 50000):
+        logits = (torch.randn(3, vocab, generator=g) * 2).to(gpu_device)
+        uniform = torch.rand(3, generator=g).to(gpu_device)
+        ws = torch.empty(_hip.sample_workspace_bytes(3, vocab), dtype=torch.uint8,
+                         device=gpu_device)
+        one, other = (torch.zeros(3, dtype=torch.int64, device=gpu_device) for _ in range(2))
+        _hip.sample(logits, uniform, one, ws, top_k=30, top_p=0.9)
+        side = torch.cuda.Stream(gpu_device)
+        side.wait_stream(torch.cuda.current_stream(gpu_device))
+        _hip.sample(logits, uniform, other, ws, top_k=30, top_p=0.9, stream=side)
+        side.synchronize()
+        assert torch.equal(one, other)
+
+
 @pytest.mark.parametrize("vocab", [900, 5000, 20000])
 def test_extreme_temperatures(gpu_device, vocab):
     g = torch.Generator().manual_seed(vocab)
