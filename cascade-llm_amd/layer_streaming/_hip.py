@@ -1096,57 +1096,61 @@ def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
 
     if q is not None and q_out is None:
         q_out = q
+    q_strides = out_strides = (0, 0)
+    q_heads = half = rope_positions = 0
     cos, sin = (None, None) if rope is None else rope
     try:
         index = k.get_device()
-        ks, vs, ps, ts = k.stride(), v.stride(), k_pages.stride(), page_table.stride()
+        k_strides, v_strides, pool = k.stride(), v.stride(), k_pages.stride()
+        table_stride, table_last = page_table.stride()
         tokens, kv_heads, dim = shape = k.shape
-        pages, pool_heads, page_size, pool_dim = k_pages.shape
+        pages, pool_heads, page_size, pool_dim = pool_shape = k_pages.shape
+        sequences, max_pages = page_table.shape
         ordinary = (
             tokens > 0 and pages > 1 and index >= 0
-            and v.shape == shape and k_pages.shape == v_pages.shape
-            and pool_heads == kv_heads and pool_dim == dim and v_pages.stride() == ps
-            and ks[2] == vs[2] == ps[3] == ts[1] == 1 and ps[2] == dim
+            and v.shape == shape and v_pages.shape == pool_shape
+            and pool_heads == kv_heads and pool_dim == dim and v_pages.stride() == pool
+            and k_strides[2] == v_strides[2] == pool[3] == table_last == 1
+            and pool[2] == dim and table_stride >= max_pages
             and k.dtype is _BF16 and v.dtype is _BF16 and k_pages.dtype is _BF16
             and v_pages.dtype is _BF16 and page_table.dtype is _I32
             and positions.dtype is _I32 and index == v.get_device()
             == k_pages.get_device() == v_pages.get_device()
             == page_table.get_device() == positions.get_device()
             and positions.shape == (tokens,) and positions.is_contiguous()
-            and (tokens <= page_table.shape[0] if rows is None else (
+            and (tokens <= sequences if rows is None else (
                 rows.dtype is _I32 and rows.get_device() == index
                 and rows.shape == (tokens,) and rows.is_contiguous()))
-            and ts[0] >= page_table.shape[1]
-            and (q_out is None if q is None else (
-                q.dtype is _BF16 and q_out.dtype is _BF16
-                and index == q.get_device() == q_out.get_device()
-                and q.shape[0] == tokens and q.shape[2] == dim
-                and q.stride(2) == 1 and q_out.shape == q.shape
-                and q_out.is_contiguous()))
-            and (rope is None or (
-                cos.dtype is _BF16 and sin.dtype is _BF16
-                and index == cos.get_device() == sin.get_device()
-                and cos.dim() == 2 and cos.shape == sin.shape
-                and cos.is_contiguous() and sin.is_contiguous()))
             and (error_flag is None or (
                 error_flag.dtype is _I32 and error_flag.get_device() == index
                 and error_flag.numel() > 0)))
+        if q is not None:
+            q_tokens, q_heads, q_dim = shape = q.shape
+            q_strides, out_strides = q.stride(), (q_heads * dim, dim)
+            ordinary = (
+                ordinary and q_tokens == tokens and q_dim == dim and q_strides[2] == 1
+                and q_out.shape == shape and q_out.is_contiguous()
+                and q.dtype is _BF16 and q_out.dtype is _BF16
+                and index == q.get_device() == q_out.get_device())
+        elif q_out is not None:
+            ordinary = False
+        if rope is not None:
+            rope_positions, half = shape = cos.shape
+            ordinary = (
+                ordinary and sin.shape == shape and cos.is_contiguous()
+                and sin.is_contiguous() and cos.dtype is _BF16 and sin.dtype is _BF16
+                and index == cos.get_device() == sin.get_device())
     except (AttributeError, IndexError, TypeError, ValueError, RuntimeError):
         ordinary = False
     if ordinary:
         # (the stride of a dimension of one says nothing)
-        k_strides, v_strides, table_stride = ks, vs, ts[0]
-        q_strides = out_strides = (0, 0)
-        if q is not None:
-            q_strides, out_strides = q.stride(), q_out.stride()
         if tokens == 1:
-            k_strides, v_strides = (0, ks[1]), (0, vs[1])
+            k_strides, v_strides = (0, k_strides[1]), (0, v_strides[1])
             q_strides = (0, q_strides[1])
-        pool = ps
         if kv_heads == 1:
             k_strides, v_strides = (k_strides[0], 0), (v_strides[0], 0)
-            pool = (ps[0], page_size * dim)
-        if q is not None and q.shape[1] == 1:
+            pool = (pool[0], page_size * dim)
+        if q_heads == 1:
             q_strides = (q_strides[0], 0)
     else:
         q_strides, k_strides, v_strides, out_strides, pool, table_stride = _check_append(
@@ -1155,21 +1159,22 @@ def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
         index = k.get_device()
         tokens, kv_heads, dim = k.shape
         pages, _, page_size, _ = k_pages.shape
+        sequences, max_pages = page_table.shape
+        q_heads = 0 if q is None else q.shape[1]
+        rope_positions, half = (0, 0) if rope is None else cos.shape
         if tokens == 0:
             return q_out
-    sequences, max_pages = page_table.shape
     _call_on(
         index, stream, "cascade_paged_append_bf16",
         0 if q is None else q.data_ptr(), q_strides[0], q_strides[1], k.data_ptr(),
         k_strides[0], k_strides[1], v.data_ptr(), v_strides[0], v_strides[1], tokens,
-        0 if q is None else q.shape[1], kv_heads, dim, positions.data_ptr(),
+        q_heads, kv_heads, dim, positions.data_ptr(),
         0 if rows is None else rows.data_ptr(), page_table.data_ptr(), table_stride,
         sequences, max_pages, 0 if rope is None else cos.data_ptr(),
-        0 if rope is None else sin.data_ptr(), 0 if rope is None else cos.shape[0],
-        0 if rope is None else 2 * cos.shape[1], 1 if interleaved else 0,
-        0 if q is None else q_out.data_ptr(), out_strides[0], out_strides[1],
-        k_pages.data_ptr(), v_pages.data_ptr(), pool[0], pool[1], pages, page_size,
-        0 if error_flag is None else error_flag.data_ptr())
+        0 if rope is None else sin.data_ptr(), rope_positions, 2 * half,
+        1 if interleaved else 0, 0 if q is None else q_out.data_ptr(), out_strides[0],
+        out_strides[1], k_pages.data_ptr(), v_pages.data_ptr(), pool[0], pool[1], pages,
+        page_size, 0 if error_flag is None else error_flag.data_ptr())
     return q_out
 
 
@@ -1231,15 +1236,17 @@ def paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out,
 
     try:
         index = q.get_device()
-        qs, ps, ts = q.stride(), k_pages.stride(), page_table.stride()
-        batch, _, dim = q.shape
-        pages, kv_heads, page_size, pool_dim = k_pages.shape
+        q_strides, pool = q.stride(), k_pages.stride()
+        table_stride, table_last = page_table.stride()
+        batch, q_heads, dim = shape = q.shape
+        pages, kv_heads, page_size, pool_dim = pool_shape = k_pages.shape
         sequences, width = page_table.shape
         ordinary = (
             batch > 0 and pages > 1 and index >= 0
-            and k_pages.shape == v_pages.shape and pool_dim == dim
-            and v_pages.stride() == ps and out.shape == q.shape
-            and qs[2] == ps[3] == ts[1] == 1 and ps[2] == dim
+            and v_pages.shape == pool_shape and pool_dim == dim
+            and v_pages.stride() == pool and out.shape == shape
+            and q_strides[2] == pool[3] == table_last == 1 and pool[2] == dim
+            and table_stride >= width
             and q.dtype is _BF16 and k_pages.dtype is _BF16 and v_pages.dtype is _BF16
             and out.dtype is _BF16 and page_table.dtype is _I32
             and lengths.dtype is _I32 and workspace.dtype is _U8
@@ -1250,7 +1257,7 @@ def paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out,
             and (batch <= sequences if rows is None else (
                 rows.dtype is _I32 and rows.get_device() == index
                 and rows.shape == (batch,) and rows.is_contiguous()))
-            and ts[0] >= width and out.is_contiguous()
+            and out.is_contiguous()
             and workspace.dim() == 1 and workspace.is_contiguous()
             and (error_flag is None or (
                 error_flag.dtype is _I32 and error_flag.get_device() == index
@@ -1259,15 +1266,16 @@ def paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out,
         ordinary = False
     if ordinary:
         # (the stride of a dimension of one says nothing)
-        q_strides = (qs[0] if batch > 1 else 0, qs[1] if q.shape[1] > 1 else 0)
-        out_strides, table_stride = out.stride(), ts[0]
-        pool = ps if kv_heads > 1 else (ps[0], page_size * dim)
+        q_strides = (q_strides[0] if batch > 1 else 0, q_strides[1] if q_heads > 1 else 0)
+        out_strides = (q_heads * dim, dim)
+        if kv_heads == 1:
+            pool = (pool[0], page_size * dim)
     else:
         q_strides, out_strides, pool, table_stride = _check_attention(
             q, k_pages, v_pages, page_table, lengths, out, workspace, rows,
             error_flag)
         index = q.get_device()
-        batch, _, dim = q.shape
+        batch, q_heads, dim = q.shape
         pages, kv_heads, page_size, _ = k_pages.shape
         sequences, width = page_table.shape
     if max_length is None:
@@ -1282,7 +1290,7 @@ def paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out,
         q_strides[0], q_strides[1], k_pages.data_ptr(), v_pages.data_ptr(), pool[0],
         pool[1], pages, page_size, page_table.data_ptr(), table_stride, sequences,
         lengths.data_ptr(), 0 if rows is None else rows.data_ptr(), batch,
-        int(max_length), q.shape[1], kv_heads, dim, scale, out.data_ptr(),
+        int(max_length), q_heads, kv_heads, dim, scale, out.data_ptr(),
         out_strides[0], out_strides[1], workspace.data_ptr(), workspace.numel(),
         0 if error_flag is None else error_flag.data_ptr())
     return out

@@ -511,15 +511,18 @@ def test_operators_on_a_stream_of_the_callers(gpu_device):
     assert torch.equal(out.cpu(), expected)
 
 
-def test_dimensions_of_one_with_odd_strides(gpu_device):
+@pytest.mark.parametrize("spare", [0, 2])
+def test_dimensions_of_one_with_odd_strides(gpu_device, spare):
     # a stride of a dimension of one is any number: nothing may depend on it
     dev, dim = gpu_device, 64
     g = torch.Generator().manual_seed(51)
-    pool = Pool([9], 1, dim, 16, seed=51, spare=0).to(dev)
+    pool = Pool([9], 1, dim, 16, seed=51, spare=spare).to(dev)
+    pages = 1 + spare
     storage = normal((4096,), g).to(dev)
     q = torch.as_strided(storage, (1, 1, dim), (3, 5, 1), 512)
     k = torch.as_strided(storage, (1, 1, dim), (7, 1, 1), 1024)
-    k_pages, v_pages = (torch.as_strided(p, (1, 1, 16, dim), (11, 13, dim, 1))
+    page_stride = 11 if pages == 1 else 16 * dim
+    k_pages, v_pages = (torch.as_strided(p, (pages, 1, 16, dim), (page_stride, 13, dim, 1))
                         for p in (pool.k, pool.v))
     out = torch.as_strided(torch.zeros(256, dtype=torch.bfloat16, device=dev), (1, 1, dim),
                            (9, 1, 1))
@@ -531,7 +534,7 @@ def test_dimensions_of_one_with_odd_strides(gpu_device):
     assert bool(((out[0].cpu().double() - ref).abs() <= tol).all())
     _hip.paged_append(q, k, k, torch.tensor([9], dtype=torch.int32, device=dev), k_pages,
                       v_pages, table, q_out=out)
-    assert torch.equal(k_pages[0, :, 9].cpu(), k[0].cpu())
+    assert torch.equal(k_pages[int(pool.table[0, 0]), :, 9].cpu(), k[0].cpu())
     assert torch.equal(out.cpu(), q.cpu())
     logits = torch.as_strided(torch.randn(50, generator=g).to(dev), (1, 50), (3, 1))
     ids = torch.empty(1, dtype=torch.int64, device=dev)
