@@ -157,7 +157,7 @@ struct PagedAttnArgs {
   int64_t out_token, out_head;
   int32_t *error;
   // split runs (SPLIT kernels): see "Runs"
-  double per_target;  // 1 / runs wanted
+  double per_round, per_two;  // 1 / runs wanted, in one round and in two
   int32_t *plan;    // [batch][2]: first run of a batch row, and how many
   float *part_ml;   // [run][q_heads][2]: maximum (log2 units), sum
   float *part_acc;  // [run][q_heads][D]
@@ -173,7 +173,9 @@ constexpr int kPagedBlock = 32;  // positions a wave step
 constexpr int kPagedGroup = 16;  // MFMA columns
 constexpr int kPagedMinRun = 4;  // blocks
 constexpr int kPagedMaxBatch = 1024;  // of a split launch
-constexpr int kPagedTarget = 2048;    // workgroups wanted of one
+// Workgroups that the device holds at a time (256 CUs with four and with six).
+constexpr int64_t kPagedSlots128 = 1024, kPagedSlots64 = 1536;
+constexpr double kPagedLongRun = 100.0;  // blocks
 constexpr size_t kPagedAlign = 256;
 
 __device__ __forceinline__ float paged_exp2(float x) {
@@ -206,12 +208,17 @@ __device__ __forceinline__ PagedRow paged_row(const PagedAttnArgs &a, int b, boo
 // Runs.  The lengths are on the device, so the launch is sized for any of
 // them and each workgroup finds its own piece of work: the blocks of 32
 // positions of all batch rows are cut into runs of `size` blocks,
-//   size = max(kPagedMinRun, floor(blocks of all rows / target) + 1),
+//   size = max(kPagedMinRun, floor(blocks of all rows / wanted) + 1),
 // rounded up to the workgroup's waves, and row b gets max(1, ceil(blocks_b /
-// size)) runs, numbered through the batch.  There are at most target + batch
+// size)) runs, numbered through the batch.  There are at most wanted + batch
 // runs whatever the lengths, all but a row's last of one size, so a ragged
 // batch and a single long sequence both fill the device.  Every wave works
 // this out for itself from the lengths (64 rows at a time), with no barrier.
+// Wanted is one round of workgroups where rows get three runs or more; two
+// rounds otherwise, and where one makes runs of more than 100 blocks: uneven
+// ends then cost more than a second start (8 KV heads of 128: 3 sequences of
+// up to 20000 positions 22.4 us in one round and 25.8 in two, 16 of 4096 27.8
+// and 30.0, 64 of 2000 52.9 and 49.7, 64 of 16384 327 and 320).
 struct PagedRun {
   int b;      // batch row; -1: no such run
   int64_t row;
@@ -236,8 +243,9 @@ __device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, in
     blocks += static_cast<uint32_t>(blocks_of(paged_row(a, base + lane, first).len));
   blocks = lane_u64(wave_prefix(blocks), kWave - 1);
   // more than blocks / target, in fp64 (no row has more than 2^26 blocks)
-  const int want = static_cast<int>(
-      fmin(static_cast<double>(blocks) * a.per_target, 67108864.0 - kPagedWaves)) + 1;
+  double per_run = static_cast<double>(blocks) * a.per_round;
+  if (per_run > kPagedLongRun) per_run = static_cast<double>(blocks) * a.per_two;
+  const int want = static_cast<int>(fmin(per_run, 67108864.0 - kPagedWaves)) + 1;
   const int size = max((want + kPagedWaves - 1) / kPagedWaves * kPagedWaves, kPagedMinRun);
   PagedRun out{-1, -1, 0, 0, 0, 0};
   int before = 0;
@@ -589,8 +597,8 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(PagedAt
 // cost more than the balance is worth, and the rows fill the device.
 struct PagedPlan {
   bool split;
-  int64_t target;
-  int64_t runs;  // at most
+  int64_t round, two;  // runs wanted, in one round and in two
+  int64_t runs;        // at most
   size_t plan_bytes, ml_bytes, acc_bytes;
 };
 
@@ -600,8 +608,16 @@ static PagedPlan paged_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, in
   const int64_t blocks = (max_length + kPagedBlock - 1) / kPagedBlock;
   p.split = blocks > kWholeBlocks && batch <= kPagedMaxBatch;
   if (!p.split) return p;
-  p.target = (kPagedTarget + kv_heads - 1) / kv_heads;
-  p.runs = p.target + batch;
+  const int64_t slots =
+      ((dim == 128 ? kPagedSlots128 : kPagedSlots64) + kv_heads - 1) / kv_heads;
+  // (half a run a row is lost to the last runs)
+  auto wanted = [batch](int64_t runs) {
+    return runs - batch / 2 > runs / 2 ? runs - batch / 2 : (runs + 1) / 2;
+  };
+  p.two = wanted(2 * slots);
+  p.round = wanted(slots);
+  if (3 * batch > p.round) p.round = p.two;
+  p.runs = p.two + batch;
   const int64_t most = batch * ((blocks + kPagedMinRun - 1) / kPagedMinRun);
   if (p.runs > most) p.runs = most;
   auto rounded = [](int64_t bytes) {
@@ -852,7 +868,8 @@ extern "C" int cascade_paged_decode_attention_bf16(
   }
   unsigned char *ws = static_cast<unsigned char *>(workspace);
   a.runs = static_cast<int32_t>(p.runs);
-  a.per_target = 1.0 / static_cast<double>(p.target);
+  a.per_round = 1.0 / static_cast<double>(p.round);
+  a.per_two = 1.0 / static_cast<double>(p.two);
   a.plan = reinterpret_cast<int32_t *>(ws);
   a.part_ml = reinterpret_cast<float *>(ws + p.plan_bytes);
   a.part_acc = reinterpret_cast<float *>(ws + p.plan_bytes + p.ml_bytes);
