@@ -19,6 +19,7 @@ ordered by the caller.
 """
 
 import heapq
+import operator
 
 import torch
 
@@ -104,7 +105,7 @@ class PagedKVCache:
         page that other sequences share is copied first.  Raises without any
         change when a row or the pool is too small."""
 
-        rows, count = list(rows), int(count)
+        rows, count = [operator.index(row) for row in rows], int(count)
         if count < 1:
             raise ValueError("count must be positive")
         if len(set(rows)) != len(rows):

@@ -143,6 +143,16 @@ def test_refusals_change_nothing(cache):
                                      device="cpu"), **bad))
 
 
+def test_rows_given_as_tensor_elements(cache):
+    a, b = cache.add(), cache.add()
+    cache.extend(torch.tensor([a, b]), 39)
+    consistent(cache)
+    with pytest.raises(ValueError):  # two tensors, one sequence
+        cache.extend(torch.tensor([b, b]))
+    consistent(cache)
+    assert cache.length(b) == 39
+
+
 def test_load_refuses_another_geometry(cache):
     other = SimpleKVCache(2, 1, 32, device="cpu")
     other.append(0, torch.zeros(1, 1, 3, 32), torch.zeros(1, 1, 3, 32))
