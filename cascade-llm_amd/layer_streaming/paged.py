@@ -11,8 +11,9 @@ pages, the page table and the lengths, and the kernels of libcascade_hip
 read them there: ``append`` (cascade_paged_append_bf16), ``attend``
 (cascade_paged_decode_attention_bf16) and the copies of ``extend`` and
 ``compact`` (cascade_copy_pages).  Table, lengths and pools never move, so a
-captured graph of a decode step serves every later step: ``extend`` (outside
-the graph) makes room and updates them in place.
+captured graph of a decode step serves every later step: ``extend`` makes room and
+updates them in place.  It, and whatever else assigns pages, refuses to run
+while a graph is captured: a replay would bring its pages back.
 
 Work is enqueued on the current stream; calls on several streams have to be
 ordered by the caller.
@@ -106,6 +107,7 @@ class PagedKVCache:
         change when a row or the pool is too small."""
 
         rows, count = [operator.index(row) for row in rows], int(count)
+        self._outside_graph()
         if count < 1:
             raise ValueError("count must be positive")
         if len(set(rows)) != len(rows):
@@ -147,6 +149,7 @@ class PagedKVCache:
         """``count`` new sequences with the pages of ``row``; returns their
         rows.  Nothing is copied until one of them is extended."""
 
+        self._outside_graph()
         pages = self._of(row)
         if sum(p is None for p in self._pages) < count:
             raise RuntimeError("all {} sequences are in use".format(self.max_sequences))
@@ -165,6 +168,7 @@ class PagedKVCache:
     def truncate(self, row, length):
         """Drop the positions of a sequence from ``length`` on."""
 
+        self._outside_graph()
         pages = self._of(row)
         length = int(length)
         if not 0 <= length <= self._lengths[row]:
@@ -177,6 +181,7 @@ class PagedKVCache:
     def free(self, row):
         """End a sequence; pages that no other one holds become free."""
 
+        self._outside_graph()
         self._of(row)
         self._drop(row, 0)
         self._lengths[row] = 0
@@ -187,6 +192,7 @@ class PagedKVCache:
         """Move the pages in use to the front of the pool (so that its tail
         can be given up, or copied out); returns how many moved."""
 
+        self._outside_graph()
         used = [p for p in range(self.num_pages) if self._refs[p]]
         # a page at or behind `len(used)` moves into a free one before it:
         # no page is both a source and a destination
@@ -210,6 +216,10 @@ class PagedKVCache:
         if not 0 <= row < self.max_sequences or self._pages[row] is None:
             raise ValueError("there is no sequence {}".format(row))
         return self._pages[row]
+
+    def _outside_graph(self):
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("pages cannot be assigned while a graph is captured")
 
     def _take(self):
         page = heapq.heappop(self._free)

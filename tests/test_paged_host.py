@@ -153,6 +153,21 @@ def test_rows_given_as_tensor_elements(cache):
     assert cache.length(b) == 39
 
 
+def test_no_page_is_assigned_under_capture(cache, monkeypatch):
+    a = cache.add()
+    cache.extend([a], 20)
+    b = cache.fork(a)[0]
+    cache.free(a)
+    monkeypatch.setattr(cache, "device", torch.device("cuda"))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call in (lambda: cache.extend([b]), lambda: cache.fork(b), lambda: cache.free(b),
+                 lambda: cache.truncate(b, 3), cache.compact):
+        with pytest.raises(RuntimeError, match="captured"):
+            call()
+    consistent(cache)
+    assert cache.length(b) == 20
+
+
 def test_load_refuses_another_geometry(cache):
     other = SimpleKVCache(2, 1, 32, device="cpu")
     other.append(0, torch.zeros(1, 1, 3, 32), torch.zeros(1, 1, 3, 32))
