@@ -63,6 +63,7 @@ class PagedKVCache:
         self.buffer = torch.empty(
             (self.layer_count, 2, self.num_pages, self.num_kv_heads, page_size,
              self.head_dim), dtype=torch.bfloat16, device=self.device)
+        self.device = self.buffer.device  # with its index: the current one may change
         self.page_table = torch.full((self.max_sequences, self.max_pages), -1,
                                      dtype=torch.int32, device=self.device)
         self.lengths = torch.zeros(self.max_sequences, dtype=torch.int32,

@@ -496,6 +496,15 @@ def test_captured_step_replays(gpu_device):
     cache.check()
 
 
+def test_cache_keeps_the_device_of_its_pool():
+    cache = PagedKVCache(2, 1, 16, layer_count=1, num_kv_heads=1, head_dim=64, page_size=8)
+    assert cache.device == cache.buffer.device == torch.device("cuda", 0)
+    assert cache.page_table.device == cache.device
+    row = cache.add()
+    cache.extend([row], 9)
+    assert cache.page_table.tolist() == [[0, 1]] and cache.lengths.tolist() == [9]
+
+
 def test_operators_on_a_stream_of_the_callers(gpu_device):
     dev = gpu_device
     pool = Pool([500, 3], 2, 64, 16, seed=41)
