@@ -730,7 +730,7 @@ extern "C" int cascade_paged_append_bf16(
   AppendArgs a{};
   if (head_dim < 16 || head_dim > 1024 || (head_dim & 15) || n_q_heads > 1024 ||
       n_kv_heads > 1024 || !page_shift_of(page_size, &a.page_shift) ||
-      max_pages * page_size > 0x7fffffff)
+      max_pages > 0x7fffffff / page_size)
     return CASCADE_ESHAPE;
   const int64_t units = (n_q_heads + 2 * n_kv_heads) * (head_dim / 16);
   int64_t threads = (units + kWave - 1) / kWave * kWave;
@@ -845,6 +845,7 @@ extern "C" int cascade_paged_decode_attention_bf16(
   for (int64_t s : strides)
     if (!stride_ok(s)) return CASCADE_EALIGN;
   const PagedPlan p = paged_plan(batch, n_q_heads, n_kv_heads, head_dim, max_length);
+  if (p.split && batch > kMaxThreads / kPagedMergeThreads / n_q_heads) return CASCADE_ESHAPE;
   if (workspace_bytes < kPagedAlign + p.plan_bytes + p.ml_bytes + p.acc_bytes)
     return CASCADE_EWORKSPACE;
   a.q = static_cast<const uint16_t *>(q);

@@ -1089,8 +1089,8 @@ def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
     or row marks padding, of which nothing is written.  ``rope``: (cos, sin)
     tables, bf16 [positions, r / 2]; the first r dims of a head turn, in pairs
     (i, i + r / 2) or, ``interleaved``, (2 i, 2 i + 1).  None copies the rows
-    as they are.  ``q_out`` (q itself by default) receives the rotated q rows
-    and is returned.  Pools are [pages, kv_heads, page_size, dim] views,
+    as they are.  ``q_out`` (q itself by default; none of its rows may be
+    another's q, k or v) receives the rotated q rows and is returned.  Pools are [pages, kv_heads, page_size, dim] views,
     ``page_table`` int32 [sequences, pages of one].  An index out of range
     leaves its token out and ors PAGED_ERANGE into ``error_flag``."""
 
@@ -1231,7 +1231,7 @@ def paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out,
     holds).  An empty sequence gives zeros.  Positions on a page outside the
     pool are left out and flagged, as are longer lengths and larger rows
     (PAGED_ERANGE in ``error_flag``).  ``workspace``:
-    paged_attention_workspace_bytes(...) uint8, one for calls that may
+    paged_attention_workspace_bytes(...) uint8, one each for calls that may
     overlap."""
 
     try:
@@ -1358,7 +1358,7 @@ def sample(logits, uniform, ids, workspace, temperature=1.0, top_k=0, top_p=1.0,
     logit; top_k 0, top_p 1 and min_p 0 are off.  ``logprobs`` (fp32 [rows])
     receives the log-probability the token was drawn with.  A row with a NaN,
     or with every token at -inf, yields -1 (and NaN).  ``workspace``:
-    sample_workspace_bytes(rows, vocab) uint8, one for calls that may
+    sample_workspace_bytes(rows, vocab) uint8, one each for calls that may
     overlap."""
 
     device = _gpu_of("logits", logits)
@@ -1383,7 +1383,8 @@ def sample(logits, uniform, ids, workspace, temperature=1.0, top_k=0, top_p=1.0,
     if rows == 0:
         return ids
     _call_on(device.index, stream, "cascade_sample_f32", logits.data_ptr(),
-             row_stride, rows, vocab, uniform.data_ptr(), t_ptr, t, k_ptr, int(k),
+             row_stride, rows, vocab, uniform.data_ptr(), t_ptr, t, k_ptr,
+             max(0, min(int(k), 1 << 31)),  # (one past 64 bits would wrap)
              p_ptr, p, m_ptr, m, ids.data_ptr(),
              0 if logprobs is None else logprobs.data_ptr(), workspace.data_ptr(),
              workspace.numel())

@@ -105,6 +105,15 @@ def test_uniform_outside_is_taken_as_the_nearest_inside(gpu_device):
     assert ids.tolist() == [0, 399, 399, 399, 0]
 
 
+def test_top_k_past_64_bits_is_off(gpu_device):
+    g = torch.Generator().manual_seed(19)
+    logits, uniform = torch.randn(8, 500, generator=g), torch.rand(8, generator=g)
+    off = draw(logits, uniform, gpu_device)
+    assert len(set(off[0].tolist())) > 1
+    for top_k in (1 << 40, (1 << 64) + 1, -1, 1 - (1 << 64)):
+        assert torch.equal(draw(logits, uniform, gpu_device, top_k=top_k)[0], off[0])
+
+
 def test_settings_per_row(gpu_device):
     g = torch.Generator().manual_seed(10)
     rows, vocab = 23, 4097

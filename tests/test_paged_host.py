@@ -225,6 +225,7 @@ def append_args(**changes):
                                            head_stride=1 << 19)),
     (1003, dict(rope_dim=136)), (1003, dict(rope_dim=24)), (1003, dict(rope_dim=-16)),
     (1003, dict(max_pages=1 << 28, table_stride=1 << 28)),
+    (1003, dict(max_pages=1 << 60, table_stride=1 << 60)),
     (1003, dict(tokens=1 << 25)), (1002, dict(k=24)),
     (1002, dict(q_out=8)), (1002, dict(cos=20)), (1002, dict(kt=1028)),
     (1002, dict(qh=-128)), (1002, dict(positions=18)), (1002, dict(error=17))])
@@ -248,6 +249,8 @@ def attention_args(**changes):
     (1001, dict(batch=0)), (1001, dict(kv=0)), (1001, dict(max_length=0)),
     (1001, dict(max_length=161)), (1001, dict(page_stride=16 * 128)),
     (1001, dict(sequences=0)), (1003, dict(dim=96)), (1003, dict(heads=9)),
+    (1003, dict(batch=1024, kv=8000, heads=128000, page_stride=8000 * 16 * 128,
+                max_length=16000, table_stride=1000)),
     (1003, dict(heads=34)), (1003, dict(page_size=48)), (1003, dict(batch=1 << 24)), (1002, dict(q=20)),
     (1002, dict(out=8)), (1002, dict(qt=1020)), (1002, dict(lengths=18)),
     (1002, dict(workspace=8)), (1004, dict(workspace_bytes=8))])
