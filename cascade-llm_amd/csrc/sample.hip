@@ -321,9 +321,9 @@ __device__ Cut find_cut(const float *x, int n, const RowScale &r, Cut in, u64 ne
   const u64 w = equal_mass / equal;
   const u64 take = BY_MASS ? (need - above_mass + w - 1) / w : need - above_count;
   *mass_kept = above_mass + take * w;
-  Cut cut{prefix, 0xffffffffu};
+  Cut cut{prefix, prefix == in.value ? in.index : 0xffffffffu};
   if (take < equal) {
-    // the index of the take-th of them
+    // the index of the take-th of them (`in` leaves out later ones at most)
     u64 seen = 0;
 #pragma unroll 1
     for (int base = 0; base < n; base += THREADS) {

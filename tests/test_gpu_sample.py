@@ -187,6 +187,21 @@ def test_lists_of_every_length(gpu_device):
             check(logits, uniform, gpu_device, **settings)
 
 
+@pytest.mark.parametrize("vocab,equal", [(6000, 5000), (30000, 5000), (30000, 30000)])
+def test_cuts_among_more_equals_than_a_list_holds(gpu_device, vocab, equal):
+    # both cuts end among the same equal logits: top-p's must not bring back
+    # those that top-k left out
+    print("sample", equal, "equal of", vocab, flush=True)
+    g = torch.Generator().manual_seed(equal + vocab)
+    logits = torch.randn(4, vocab, generator=g) - 20.0
+    for r in range(4):
+        logits[r, torch.randperm(vocab, generator=g)[:equal]] = 1.0
+    uniform = torch.rand(4, generator=g)
+    for settings in (dict(top_k=1, top_p=0.95), dict(top_k=2000, top_p=0.9999999),
+                     dict(top_k=2000, top_p=0.3), dict(top_k=4500, top_p=0.5, min_p=0.5)):
+        check(logits, uniform, gpu_device, **settings)
+
+
 def test_on_a_stream_of_the_callers(gpu_device):
     g = torch.Generator().manual_seed(6)
     for vocab in (3000, 50000):
