@@ -31,6 +31,13 @@
 // A row whose list would be longer than kListMax (ends in runs of equal
 // logits) is instead cut by the last launch alone, which counts 11 bits of
 // the ordered logits at a time over the row.
+// One top-k of at most kTopK for all rows takes two launches instead:
+//   1. sample_top_kernel     lists a chunk's top_k largest, by bins under the
+//                            chunk's own largest
+//   2. sample_top_draw_kernel  one workgroup a row: the row's top_k largest
+//                            out of these lists, sorted, cut and drawn from
+#include <algorithm>
+
 #include "cascade_device.h"
 #include "cascade_internal.h"
 
@@ -60,6 +67,12 @@ constexpr int kFewThreads = 512;  // of a draw whose list is short
 constexpr int64_t kFewK = 480;    // K up to this is one
 constexpr int kShortVecs = 4;
 constexpr int64_t kShortVocab = int64_t{4} * kSampleThreads * kShortVecs;
+// One K up to this for all rows takes two launches (128256 logits, top-p 0.95,
+// K = 40: 1 row 12.9 us against 18.9, 64 rows 20.2 against 36.3; K = 100: 17.4
+// against 19.8 and 25.3 against 39.3).  Past it the draw holds the keys of many
+// lists no longer (K = 128: 1 row 23.9 against 19.8).
+constexpr int kTopK = 112;
+constexpr int kTopCap = 4 * kTopK;  // keys of a chunk's list
 constexpr int64_t kSliceRows = 256;  // rows of a launch (the workspace holds these)
 // Log2 weights are held in steps of 1/32 (the table of fixed_weight); the bins
 // hold the 45 units in which a weight is not 0.
@@ -95,7 +108,7 @@ struct SampleArgs {
   u64 *bin_mass;    // [rows][kSampleBins]
   uint32_t *bin_count;
   struct RowEnds *ends;  // [rows]
-  u64 *list;             // [rows][kListMax] keys
+  u64 *list;             // [rows][kListMax] keys, or [rows][chunks][kTopCap]
   uint32_t *list_count;  // [rows]
 };
 
@@ -672,7 +685,8 @@ __device__ RowEnds find_ends(const BinShare<THREADS> &bins, const RowSettings &s
 }
 
 // Puts those of four logits that are in a listed bin (from `first` on) on a
-// list of kListMax; *count counts them all.
+// list of CAP; *count counts them all.
+template <uint32_t CAP = kListMax>
 __device__ __forceinline__ void list_of(const f32x4_at4 &v, int at, const int (&b)[4], int first,
                                         const RowEnds &e, u64 *list, uint32_t *count) {
   bool in[4];
@@ -683,7 +697,7 @@ __device__ __forceinline__ void list_of(const f32x4_at4 &v, int at, const int (&
   for (int i = 0; i < 4; ++i)
     if (in[i]) {
       const uint32_t n = atomicAdd(count, 1u);
-      if (n < kListMax) list[n] = topk_key(v[i], static_cast<uint32_t>(at + i));
+      if (n < CAP) list[n] = topk_key(v[i], static_cast<uint32_t>(at + i));
     }
 }
 
@@ -878,110 +892,100 @@ __device__ u64 counted_cut(const float *x, int n, const RowScale &r, const RowSe
   return (static_cast<u64>(cut.value) << 32) | (0xffffffffu - cut.index);
 }
 
-// One workgroup a row.  Bound by the barriers of its sort and sums: 12.4 us with
-// lists of up to a thousand keys (64 rows), 6.4 with one of 40 (512 threads sort
-// and sum over half the waves: 8.6 with 1024), 5.4 with none.
+// The cut of a row whose list would be too long, and the masses of the row's
+// parts under it in sh.mass.
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
-  __shared__ DrawShared sh;
-  const int row = blockIdx.x;
+__device__ __forceinline__ u64 counted_row(const SampleArgs &a, const float *x,
+                                           const RowScale &r, const RowSettings &set,
+                                           DrawShared &sh) {
   const int tid = threadIdx.x;
-  const float *x = a.logits + row * a.row_stride;
-  fill_table(sh.table);
-  // what the earlier launches left, loaded at once (a row without cuts has
-  // no ends and no list: those words are not used then)
-  const u64 *part_mass = a.part_mass + static_cast<int64_t>(row) * a.parts;
-  u64 mass = tid < a.parts ? part_mass[tid] : 0;
-  const RowEnds e = a.ends[row];
-  const uint32_t entries = a.list_count[row];
-  const u64 key = a.list[static_cast<int64_t>(row) * kListMax + tid];
-  double u = static_cast<double>(a.uniform[row]);
-  const RowSettings set = row_settings(a, row);
-  const float mx = row_max(a, row);
-  if (no_token(mx)) {
-    if (tid == 0) {
-      a.ids[row] = -1;
-      if (a.logprobs != nullptr) a.logprobs[row] = __builtin_nanf("");
-    }
-    return;
-  }
-  if (set.greedy) {
-    // the first chunk that has the largest logit, its first token that has it
-    const bool has = tid < a.chunks &&
-                     a.chunk_max[static_cast<int64_t>(row) * a.chunks + tid] == mx;
-    if (tid == 0) sh.first[0] = sh.first[1] = 0x7fffffff;
-    __syncthreads();
-    if (has) atomicMin(&sh.first[0], tid);
-    __syncthreads();
-    const int begin = min(sh.first[0], a.chunks - 1) * a.chunk;
-    const int end = min(begin + a.chunk, a.vocab);
-    for (int i = begin + tid; i < end; i += THREADS)
-      if (x[i] == mx) {
-        atomicMin(&sh.first[1], i);
-        break;
-      }
-    __syncthreads();
-    if (tid == 0) {
-      a.ids[row] = sh.first[1];
-      if (a.logprobs != nullptr) a.logprobs[row] = 0.0f;
-    }
-    return;
-  }
-  __syncthreads();  // the table
-  const RowScale r = row_scale(mx, set, sh.table);
-  u64 cut = 0;
-  if (set.use_k || set.use_p) {
-    if (entries > kListMax) {
-      u64 live = 0, sum = 0;
+  u64 live = 0, sum = 0;
 #pragma unroll 1
-      for (int i = tid; i < a.vocab; i += THREADS) {
-        const u64 w = fixed_weight(x[i], r);
-        live += w != 0 ? 1 : 0;
-        sum += w;
-      }
-      u64 live_all, mass_all;
-      block_prefix<THREADS / kWave>(live, sh.scan, &live_all);
-      block_prefix<THREADS / kWave>(sum, sh.scan, &mass_all);
-      cut = counted_cut<THREADS>(x, a.vocab, r, set, mass_all, live_all, sh.row);
-      // the parts' masses, a wave a part
-#pragma unroll 1
-      for (int c = tid / kWave; c < a.parts; c += (THREADS / kWave)) {
-        const int end = min((c + 1) * kPart, a.vocab);
-        u64 part = 0;
-#pragma unroll 1
-        for (int i = c * kPart + (tid & (kWave - 1)); i < end; i += kWave) {
-          const u64 w = fixed_weight(x[i], r);
-          if (w >= set.min_w && topk_key(x[i], static_cast<uint32_t>(i)) >= cut) part += w;
-        }
-        part = wave_prefix(part);
-        if ((tid & (kWave - 1)) == kWave - 1) sh.mass[c] = part;
-      }
-      __syncthreads();
-      if (tid < a.parts) mass = sh.mass[tid];
-    } else if (entries > 0) {
-      if (tid < a.parts) sh.mass[tid] = mass;
-      const int n = static_cast<int>(entries);
-      cut = n <= THREADS
-                ? list_cut<THREADS, 1>(nullptr, n, tid < n ? key : 0, e, set, r, sh)
-                : list_cut<THREADS, kListMax / THREADS>(
-                      a.list + static_cast<int64_t>(row) * kListMax, n, 0, e, set, r, sh);
-      // what the list adds to its parts
-      for (int i = tid; i < static_cast<int>(entries); i += THREADS) {
-        const u64 key = sh.keys[i];
-        const u64 w = fixed_weight(key_value(key), r);
-        if (key >= cut && w >= set.min_w) atomicAdd(&sh.mass[key_index(key) / kPart], w);
-      }
-      __syncthreads();
-      if (tid < a.parts) mass = sh.mass[tid];
-    }
+  for (int i = tid; i < a.vocab; i += THREADS) {
+    const u64 w = fixed_weight(x[i], r);
+    live += w != 0 ? 1 : 0;
+    sum += w;
   }
-  // the draw: a part, then a token in it
-  u64 total;
-  const u64 upto = block_prefix<THREADS / kWave>(mass, sh.scan, &total);
+  u64 live_all, mass_all;
+  block_prefix<THREADS / kWave>(live, sh.scan, &live_all);
+  block_prefix<THREADS / kWave>(sum, sh.scan, &mass_all);
+  const u64 cut = counted_cut<THREADS>(x, a.vocab, r, set, mass_all, live_all, sh.row);
+  // a wave a part
+#pragma unroll 1
+  for (int c = tid / kWave; c < a.parts; c += (THREADS / kWave)) {
+    const int end = min((c + 1) * kPart, a.vocab);
+    u64 part = 0;
+#pragma unroll 1
+    for (int i = c * kPart + (tid & (kWave - 1)); i < end; i += kWave) {
+      const u64 w = fixed_weight(x[i], r);
+      if (w >= set.min_w && topk_key(x[i], static_cast<uint32_t>(i)) >= cut) part += w;
+    }
+    part = wave_prefix(part);
+    if ((tid & (kWave - 1)) == kWave - 1) sh.mass[c] = part;
+  }
+  __syncthreads();
+  return cut;
+}
+
+// The mass that `uniform` points at, of `total`.
+__device__ __forceinline__ u64 target_of(float uniform, u64 total) {
+  double u = static_cast<double>(uniform);
   u = u > 0.0 ? u : 0.0;  // NaN too
   const double t = u * static_cast<double>(total);
-  u64 target = t < static_cast<double>(total) ? static_cast<u64>(t) : total - 1;
-  target = target < total ? target : total - 1;
+  const u64 target = t < static_cast<double>(total) ? static_cast<u64>(t) : total - 1;
+  return target < total ? target : total - 1;
+}
+
+// Writes a row's token of weight w.
+__device__ __forceinline__ void store_token(const SampleArgs &a, int row, int64_t token, u64 w,
+                                            u64 total) {
+  a.ids[row] = token;
+  if (a.logprobs != nullptr)
+    a.logprobs[row] =
+        static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total)));
+}
+
+__device__ __forceinline__ void store_no_token(const SampleArgs &a, int row) {
+  if (threadIdx.x != 0) return;
+  a.ids[row] = -1;
+  if (a.logprobs != nullptr) a.logprobs[row] = __builtin_nanf("");
+}
+
+// The first of the row's largest logits: in the first chunk that has it.
+template <int THREADS>
+__device__ __forceinline__ void store_largest(const SampleArgs &a, int row, const float *x,
+                                              float mx, int *first) {
+  const int tid = threadIdx.x;
+  const bool has = tid < a.chunks &&
+                   a.chunk_max[static_cast<int64_t>(row) * a.chunks + tid] == mx;
+  if (tid == 0) first[0] = first[1] = 0x7fffffff;
+  __syncthreads();
+  if (has) atomicMin(&first[0], tid);
+  __syncthreads();
+  const int begin = min(first[0], a.chunks - 1) * a.chunk;
+  const int end = min(begin + a.chunk, a.vocab);
+  for (int i = begin + tid; i < end; i += THREADS)
+    if (x[i] == mx) {
+      atomicMin(&first[1], i);
+      break;
+    }
+  __syncthreads();
+  if (tid == 0) {
+    a.ids[row] = first[1];
+    if (a.logprobs != nullptr) a.logprobs[row] = 0.0f;
+  }
+}
+
+// The draw from a row of which thread c has the mass of part c: a part, then
+// a token in it.
+template <int THREADS>
+__device__ __forceinline__ void draw_token(const SampleArgs &a, int row, const float *x,
+                                           float uniform, u64 mass, u64 cut, const RowScale &r,
+                                           const RowSettings &set, DrawShared &sh) {
+  const int tid = threadIdx.x;
+  u64 total;
+  const u64 upto = block_prefix<THREADS / kWave>(mass, sh.scan, &total);
+  u64 target = target_of(uniform, total);
   if (upto - mass <= target && target < upto) {
     sh.found[0] = static_cast<u64>(tid);
     sh.found[1] = target - (upto - mass);
@@ -1013,15 +1017,286 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
     for (int i = mine; i < end; ++i) {
       const u64 w = weight_of(x[i], i);
       if (target < at + w) {
-        a.ids[row] = i;
-        if (a.logprobs != nullptr)
-          a.logprobs[row] = static_cast<float>(
-              log(static_cast<double>(w) / static_cast<double>(total)));
+        store_token(a, row, i, w, total);
         break;
       }
       at += w;
     }
   }
+}
+
+// One workgroup a row.  Bound by the barriers of its sort and sums: 12.4 us with
+// lists of up to a thousand keys (64 rows), 6.4 with one of 40 (512 threads sort
+// and sum over half the waves: 8.6 with 1024), 5.4 with none.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
+  __shared__ DrawShared sh;
+  const int row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const float *x = a.logits + row * a.row_stride;
+  fill_table(sh.table);
+  // what the earlier launches left, loaded at once (a row without cuts has
+  // no ends and no list: those words are not used then)
+  const u64 *part_mass = a.part_mass + static_cast<int64_t>(row) * a.parts;
+  u64 mass = tid < a.parts ? part_mass[tid] : 0;
+  const RowEnds e = a.ends[row];
+  const uint32_t entries = a.list_count[row];
+  const u64 key = a.list[static_cast<int64_t>(row) * kListMax + tid];
+  const float uniform = a.uniform[row];
+  const RowSettings set = row_settings(a, row);
+  const float mx = row_max(a, row);
+  if (no_token(mx)) return store_no_token(a, row);
+  if (set.greedy) return store_largest<THREADS>(a, row, x, mx, sh.first);
+  __syncthreads();  // the table
+  const RowScale r = row_scale(mx, set, sh.table);
+  u64 cut = 0;
+  if (set.use_k || set.use_p) {
+    if (entries > kListMax) {
+      cut = counted_row<THREADS>(a, x, r, set, sh);
+      if (tid < a.parts) mass = sh.mass[tid];
+    } else if (entries > 0) {
+      if (tid < a.parts) sh.mass[tid] = mass;
+      const int n = static_cast<int>(entries);
+      cut = n <= THREADS
+                ? list_cut<THREADS, 1>(nullptr, n, tid < n ? key : 0, e, set, r, sh)
+                : list_cut<THREADS, kListMax / THREADS>(
+                      a.list + static_cast<int64_t>(row) * kListMax, n, 0, e, set, r, sh);
+      // what the list adds to its parts
+      for (int i = tid; i < static_cast<int>(entries); i += THREADS) {
+        const u64 key = sh.keys[i];
+        const u64 w = fixed_weight(key_value(key), r);
+        if (key >= cut && w >= set.min_w) atomicAdd(&sh.mass[key_index(key) / kPart], w);
+      }
+      __syncthreads();
+      if (tid < a.parts) mass = sh.mass[tid];
+    }
+  }
+  draw_token<THREADS>(a, row, x, uniform, mass, cut, r, set, sh);
+}
+
+// Where the top_k of the tokens in `count` (LDS; there is one at least) end.
+struct CountEnd {
+  int bin;
+  uint32_t above;  // tokens in the bins above it
+  uint32_t need;   // and taken of it
+};
+
+struct CountShared {
+  int scan[kSampleWaves];
+  int bin, above;
+};
+
+template <int THREADS>
+__device__ __forceinline__ CountEnd count_end(const uint32_t *count, int64_t top_k,
+                                              CountShared &sh) {
+  constexpr int kPer = kSampleBins / THREADS;
+  const int tid = threadIdx.x;
+  int c[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    c[i] = static_cast<int>(count[tid * kPer + i]);
+    sum += c[i];
+  }
+  const int upto = wave_prefix(sum);
+  if ((tid & (kWave - 1)) == kWave - 1) sh.scan[tid / kWave] = upto;
+  __syncthreads();
+  int at = upto - sum, all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / kWave; ++w) {
+    if (w < tid / kWave) at += sh.scan[w];
+    all += sh.scan[w];
+  }
+  const int need = static_cast<int>(min(top_k, static_cast<int64_t>(all)));
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (at < need && need <= at + c[i]) {
+      sh.bin = tid * kPer + i;
+      sh.above = at;
+    }
+    at += c[i];
+  }
+  __syncthreads();
+  return CountEnd{sh.bin, static_cast<uint32_t>(sh.above),
+                  static_cast<uint32_t>(need - sh.above)};
+}
+
+// A workgroup a chunk: its largest logit, and a list of the tokens in the bins
+// (under that logit) of its top_k largest, which hold the row's.
+__global__ __launch_bounds__(kChunkThreads) void sample_top_kernel(SampleArgs a) {
+  __shared__ uint32_t s_bins[kSampleBins];
+  __shared__ u64 s_keys[kTopCap];
+  __shared__ float s_max[kChunkThreads / kWave];
+  __shared__ CountShared s_end;
+  __shared__ uint32_t s_count;
+  const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
+  const int row = static_cast<int>(blockIdx.x) / a.chunks;
+  const int tid = threadIdx.x;
+  const auto logits = row_chunk(a, row, chunk);
+  const RowSettings set = row_settings(a, row);
+  for (int i = tid; i < kSampleBins; i += kChunkThreads) s_bins[i] = 0;
+  if (tid == 0) s_count = 0;
+  float best = -INFINITY;
+  logits.each([&](const f32x4_at4 &v, int, int) {
+    best = nan_max(nan_max(best, nan_max(v[0], v[1])), nan_max(v[2], v[3]));
+  });
+  best = wave_nan_max(best);
+  if ((tid & (kWave - 1)) == 0) s_max[tid / kWave] = best;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kChunkThreads / kWave; ++w) best = nan_max(best, s_max[w]);
+  if (tid == 0) a.chunk_max[static_cast<int64_t>(row) * a.chunks + chunk] = best;
+  uint32_t *listed = a.bin_count + static_cast<int64_t>(row) * kSampleBins + chunk;
+  if (set.greedy || no_token(best)) {  // uniform
+    if (tid == 0) *listed = 0;
+    return;
+  }
+  const RowScale r = row_scale(best, set, nullptr);
+  // the largest of every four neighbours are enough to count: where top_k of
+  // them end, top_k tokens have been passed
+  auto four_bin = [&](const f32x4_at4 &v) {
+    return weight_bin(log_weight(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), r));
+  };
+  logits.each([&](const f32x4_at4 &v, int, int) {
+    const int b = four_bin(v);
+    if (b < kSampleBins) atomicAdd(&s_bins[b], 1u);
+  });
+  __syncthreads();
+  const CountEnd end = count_end<kChunkThreads>(s_bins, set.top_k, s_end);
+  // fewer fours than top_k: at most kTopCap tokens, all listed
+  const int last = end.above + end.need < set.top_k ? kSampleBins - 1 : end.bin;
+  const RowEnds e{0, 0, 0, 0, 0, 0, last, last};
+  logits.each([&](const f32x4_at4 &v, int at, int) {
+    if (four_bin(v) > last) return;
+    double t[4];
+    int b[4];
+    bins_of(v, r, t, b);
+    list_of<kTopCap>(v, at, b, 0, e, s_keys, &s_count);
+  });
+  __syncthreads();
+  // more than kTopCap: the draw counts over the row
+  const int n = static_cast<int>(s_count);
+  if (tid == 0) *listed = s_count;
+  u64 *list = a.list + (static_cast<int64_t>(row) * a.chunks + chunk) * kTopCap;
+  for (int i = tid; i < min(n, kTopCap); i += kChunkThreads) list[i] = s_keys[i];
+}
+
+// One workgroup a row: bins of the chunks' lists under the row's largest logit
+// give its top_k, which are sorted and cut as in the draw above.  At most kTopK
+// tokens are left, and each finds the mass before it by itself.
+constexpr int kTopHeld = 8;   // lists of which a wave holds the first keys: one a
+constexpr int kTopTwo = 56;  // lane, and from this top_k on (ties come on top) two
+
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_top_draw_kernel(SampleArgs a) {
+  static_assert(kTopK <= THREADS, "a token a thread");
+  constexpr int kWaves = THREADS / kWave;
+  __shared__ DrawShared sh;
+  __shared__ CountShared s_end;
+  __shared__ uint32_t s_count, s_over;
+  const int row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int lane = tid & (kWave - 1);
+  const int wave = tid / kWave;
+  const float *x = a.logits + row * a.row_stride;
+  const uint32_t *listed = a.bin_count + static_cast<int64_t>(row) * kSampleBins;
+  const u64 *list = a.list + static_cast<int64_t>(row) * a.chunks * kTopCap;
+  const bool two = a.top_k_value >= kTopTwo;
+  u64 held[kTopHeld], more[kTopHeld];
+  int count[kTopHeld];
+#pragma unroll
+  for (int j = 0; j < kTopHeld; ++j) {
+    const int c = min(wave + kWaves * j, a.chunks - 1);
+    count[j] = wave + kWaves * j < a.chunks ? static_cast<int>(listed[c]) : 0;
+    held[j] = list[c * kTopCap + lane];
+    if (two) more[j] = list[c * kTopCap + kWave + lane];
+  }
+  const float uniform = a.uniform[row];
+  const RowSettings set = row_settings(a, row);
+  const float mx = row_max(a, row);
+  fill_table(sh.table);
+  if (no_token(mx)) return store_no_token(a, row);
+  if (set.greedy) return store_largest<THREADS>(a, row, x, mx, sh.first);
+  for (int i = tid; i < kSampleBins; i += THREADS) sh.row.count[i] = 0;
+  if (tid == 0) s_count = s_over = 0;
+  __syncthreads();
+  const RowScale r = row_scale(mx, set, sh.table);
+  // f(key) for every listed token
+  auto each = [&](auto f) {
+    auto rest = [&](int c, int first, int n) {
+#pragma unroll 1
+      for (int i = first + lane; i < min(n, kTopCap); i += kWave) f(list[c * kTopCap + i]);
+    };
+#pragma unroll
+    for (int j = 0; j < kTopHeld; ++j)
+      if (lane < count[j]) f(held[j]);
+    if (two) {  // uniform
+#pragma unroll
+      for (int j = 0; j < kTopHeld; ++j)
+        if (kWave + lane < count[j]) f(more[j]);
+    }
+    const int known = two ? 2 * kWave : kWave;
+#pragma unroll
+    for (int j = 0; j < kTopHeld; ++j)
+      if (count[j] > known) rest(wave + kWaves * j, known, count[j]);
+#pragma unroll 1
+    for (int c = wave + kWaves * kTopHeld; c < a.chunks; c += kWaves)
+      rest(c, 0, static_cast<int>(listed[c]));
+  };
+#pragma unroll
+  for (int j = 0; j < kTopHeld; ++j)
+    if (count[j] > kTopCap) s_over = 1;
+  for (int c = kWaves * kTopHeld + tid; c < a.chunks; c += THREADS)
+    if (listed[c] > kTopCap) s_over = 1;
+  each([&](u64 key) {
+    const int b = weight_bin(log_weight(key_value(key), r));
+    if (b < kSampleBins) atomicAdd(&sh.row.count[b], 1u);
+  });
+  __syncthreads();
+  bool over = s_over != 0;
+  if (!over) {
+    const CountEnd end = count_end<THREADS>(sh.row.count, set.top_k, s_end);
+    each([&](u64 key) {  // (the list takes the place of the bins)
+      if (weight_bin(log_weight(key_value(key), r)) > end.bin) return;
+      const uint32_t n = atomicAdd(&s_count, 1u);
+      if (n < kListMax) sh.keys[n] = key;
+    });
+    __syncthreads();
+    const int n = static_cast<int>(s_count);
+    over = n > kListMax;
+    if (!over) {
+      const RowEnds e{0, 0, 0, end.need, end.above, 0, end.bin, end.bin};
+      u64 cut;
+      if (n <= THREADS) {
+        const u64 key = tid < n ? sh.keys[tid] : 0;
+        __syncthreads();  // the sort writes sh.keys
+        cut = list_cut<THREADS, 1>(nullptr, n, key, e, set, r, sh);
+      } else {
+        cut = list_cut<THREADS, kListMax / THREADS>(sh.keys, n, 0, e, set, r, sh);
+      }
+      // (sorted: the tokens that are left are the first)
+      const int left = static_cast<int>(end.above + end.need);
+      const u64 key = tid < left ? sh.keys[tid] : 0;
+      u64 w = tid < left && key >= cut ? fixed_weight(key_value(key), r) : 0;
+      w = w >= set.min_w ? w : 0;
+      if (tid < left) sh.mass[tid] = w;
+      __syncthreads();
+      if (tid >= left) return;
+      const uint32_t index = static_cast<uint32_t>(key_index(key));
+      u64 total = 0, before = 0;
+#pragma unroll 8
+      for (int i = 0; i < left; ++i) {
+        const u64 other = sh.mass[i];
+        total += other;
+        before += static_cast<uint32_t>(key_index(sh.keys[i])) < index ? other : 0;
+      }
+      const u64 target = target_of(uniform, total);
+      if (before <= target && target < before + w) store_token(a, row, index, w, total);
+      return;
+    }
+    __syncthreads();  // (the count takes the place of the list)
+  }
+  const u64 cut = counted_row<THREADS>(a, x, r, set, sh);
+  draw_token<THREADS>(a, row, x, uniform, tid < a.parts ? sh.mass[tid] : 0, cut, r, set, sh);
 }
 
 // A row of at most kShortVocab logits in one launch: the row stays in the
@@ -1041,7 +1316,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
   const int wave = tid / kWave;
   const float *x = a.logits + row * a.row_stride;
   const Chunk<THREADS, kShortVecs> logits(x, 0, a.vocab);
-  const double uniform = static_cast<double>(a.uniform[row]);
+  const float uniform = a.uniform[row];
   const RowSettings set = row_settings(a, row);
   fill_table(sh.table);
   for (int b = tid; b < kSampleBins; b += THREADS) {
@@ -1061,13 +1336,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
   __syncthreads();
 #pragma unroll 4
   for (int w = 0; w < kWaves; ++w) mx = nan_max(mx, s_max[w]);
-  if (no_token(mx)) {
-    if (tid == 0) {
-      a.ids[row] = -1;
-      if (a.logprobs != nullptr) a.logprobs[row] = __builtin_nanf("");
-    }
-    return;
-  }
+  if (no_token(mx)) return store_no_token(a, row);
   if (set.greedy) {
     int at = 0x7fffffff;
     logits.each([&](const f32x4_at4 &v, int first, int) {
@@ -1162,10 +1431,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
   const u64 upto = block_prefix<kWaves>(part, sh.scan, &total);
   if (tid < kParts) sh.mass[tid] = upto - part;
   __syncthreads();
-  const double u = uniform > 0.0 ? uniform : 0.0;  // NaN too
-  const double t = u * static_cast<double>(total);
-  u64 target = t < static_cast<double>(total) ? static_cast<u64>(t) : total - 1;
-  target = target < total ? target : total - 1;
+  const u64 target = target_of(uniform, total);
 #pragma unroll
   for (int j = 0; j <= kShortVecs; ++j) {
     if (j == kShortVecs && wave != 0) break;
@@ -1177,10 +1443,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
       for (int i = j < kShortVecs ? logits.at(j) : last; i < a.vocab; ++i) {
         const u64 w = weight_of(x[i], i);
         if (target < at + w) {
-          a.ids[row] = i;
-          if (a.logprobs != nullptr)
-            a.logprobs[row] = static_cast<float>(
-                log(static_cast<double>(w) / static_cast<double>(total)));
+          store_token(a, row, i, w, total);
           break;
         }
         at += w;
@@ -1216,7 +1479,8 @@ static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
   p.bin_mass_bytes = rounded(r * kSampleBins * sizeof(u64));
   p.bin_count_bytes = rounded(r * kSampleBins * sizeof(uint32_t));
   p.ends_bytes = rounded(r * sizeof(RowEnds));
-  p.list_bytes = rounded(r * kListMax * sizeof(u64));
+  p.list_bytes = rounded(
+      r * std::max<int64_t>(kListMax, p.chunks * kTopCap) * sizeof(u64));
   p.count_bytes = rounded(r * sizeof(uint32_t));
   p.bytes = p.max_bytes + p.mass_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes + p.list_bytes + p.count_bytes;
   return p;
@@ -1308,6 +1572,7 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
   // a list of at most a key a thread is sorted in registers; more threads make
   // every sum dearer
   const bool few = top_k == nullptr && top_k_value <= kFewK;
+  const bool top = top_k == nullptr && top_k_value > 0 && top_k_value <= kTopK;
   const dim3 block(kChunkThreads);
   for (int64_t first = 0; first < rows; first += kSliceRows) {
     const int64_t count = rows - first < kSliceRows ? rows - first : kSliceRows;
@@ -1320,6 +1585,15 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
     a.ids = ids + first;
     a.logprobs = logprobs != nullptr ? logprobs + first : nullptr;
     const dim3 grid(static_cast<unsigned>(count * p.chunks));
+    const dim3 rows_grid(static_cast<unsigned>(count));
+    if (top) {
+      hipError_t e = launch_kernel(sample_top_kernel, grid, block, 0, s, a);
+      if (e != hipSuccess) return e;
+      e = launch_kernel(sample_top_draw_kernel<kFewThreads>, rows_grid, dim3(kFewThreads), 0,
+                        s, a);
+      if (e != hipSuccess) return e;
+      continue;
+    }
     hipError_t e = launch_kernel(sample_max_kernel, grid, block, 0, s, a);
     if (e != hipSuccess) return e;
     e = launch_kernel(sample_weigh_kernel, grid, block, 0, s, a);
@@ -1328,7 +1602,6 @@ extern "C" int cascade_sample_f32(const float *logits, int64_t row_stride, int64
       e = launch_kernel(sample_collect_kernel, grid, block, 0, s, a);
       if (e != hipSuccess) return e;
     }
-    const dim3 rows_grid(static_cast<unsigned>(count));
     e = few ? launch_kernel(sample_draw_kernel<kFewThreads>, rows_grid, dim3(kFewThreads), 0,
                             s, a)
             : launch_kernel(sample_draw_kernel<kSampleThreads>, rows_grid,

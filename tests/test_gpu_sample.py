@@ -202,6 +202,64 @@ def test_cuts_among_more_equals_than_a_list_holds(gpu_device, vocab, equal):
         check(logits, uniform, gpu_device, **settings)
 
 
+@pytest.mark.parametrize("vocab", [16385, 20002, 128256, 1 << 19])
+def test_short_top_k_of_long_rows(gpu_device, vocab):
+    # one top_k of at most 112: lists of the chunks' largest, more than 64 of
+    # them for the longest rows; 113 takes the other way
+    print("sample", vocab, flush=True)
+    g = torch.Generator().manual_seed(vocab + 1)
+    logits = torch.randn(6, vocab, generator=g) * 2.5
+    logits[1] = logits[1].to(torch.bfloat16).float()  # many ties
+    logits[2, :-5] = -math.inf                        # fewer tokens than top_k
+    logits[3, 2048:] = -100.0                         # one chunk has them all, and
+    logits[3, 300:] -= 1000.0                         # few have a weight
+    logits[4] = logits[4].clamp(max=0.0) * 0.01
+    logits[4, ::7] = -0.0
+    logits[5, vocab // 2] = math.inf
+    uniform = torch.tensor([0.3, 0.999, 0.6, 0.0, 0.45, 0.8])
+    for top_k in (1, 40, 112) if vocab > 200000 else (1, 2, 40, 55, 56, 64, 65, 112, 113):
+        check(logits, uniform, gpu_device, temperature=0.8, top_k=top_k, top_p=0.95)
+    for settings in (dict(top_k=100, min_p=0.2), dict(top_k=3, min_p=1.5),
+                     dict(top_k=112, top_p=0.0), dict(temperature=0.0, top_k=40),
+                     dict(temperature=50.0, top_k=90, top_p=0.7)):
+        if vocab > 200000:  # (the plain form sorts in Python)
+            break
+        check(logits, uniform, gpu_device, **settings)
+    temperature = torch.tensor([0.0, 1.0, 0.0, 0.5, 0.0, 2.0])
+    check(logits, uniform, gpu_device, temperature=temperature, top_k=20,
+          top_p=torch.tensor([0.5, 1.0, 0.1, 0.9, 1.0, 0.3]))
+    logits[0, vocab - 1] = math.nan
+    logits[1] = -math.inf
+    ids, logprobs = draw(logits, uniform, gpu_device, top_k=7)
+    assert ids[:2].tolist() == [-1, -1] and bool(logprobs[:2].isnan().all())
+    assert bool((ids[2:] >= 0).all())
+
+
+@pytest.mark.parametrize("vocab,near", [(30000, 100), (30000, 300), (30000, 700),
+                                        (30000, 4200), (30000, 30000), (61440, 3000),
+                                        (61440, 5000)])
+def test_short_top_k_among_equals(gpu_device, vocab, near):
+    # `near` tokens in one bin: the chunks' lists are longer than top_k, or
+    # than they can be; so is the row's
+    print("sample", near, "in", vocab, flush=True)
+    g = torch.Generator().manual_seed(near)
+    logits = torch.randn(3, vocab, generator=g) - 20.0
+    for r in range(3):
+        at = torch.randperm(vocab, generator=g)[:near]
+        logits[r, at] = 1.0 if r == 2 else 1.0 + torch.rand(near, generator=g) * 0.004
+    uniform = torch.rand(3, generator=g)
+    for settings in (dict(top_k=1), dict(top_k=40), dict(top_k=112, top_p=0.6),
+                     dict(top_k=99, min_p=0.9), dict(top_k=112, temperature=0.5)):
+        check(logits, uniform, gpu_device, **settings)
+
+
+def test_short_top_k_of_many_rows(gpu_device):
+    # the rows of two slices, chunks of 8192
+    g = torch.Generator().manual_seed(77)
+    logits, uniform = torch.randn(300, 17000, generator=g) * 3, torch.rand(300, generator=g)
+    check(logits, uniform, gpu_device, temperature=0.9, top_k=40, top_p=0.9)
+
+
 def test_on_a_stream_of_the_callers(gpu_device):
     g = torch.Generator().manual_seed(6)
     for vocab in (3000, 50000):
