@@ -68,8 +68,8 @@ constexpr int64_t kFewK = 480;    // K up to this is one
 constexpr int kShortVecs = 4;
 constexpr int64_t kShortVocab = int64_t{4} * kSampleThreads * kShortVecs;
 // One K up to this for all rows takes two launches (128256 logits, top-p 0.95,
-// K = 40: 1 row 12.9 us against 18.9, 64 rows 20.2 against 36.3; K = 100: 17.4
-// against 19.8 and 25.3 against 39.3).  Past it the draw holds the keys of many
+// K = 40: 1 row 12.1 us against 18.9, 64 rows 17.5 against 36.3; K = 100: 16.5
+// against 19.8 and 21.3 against 39.3).  Past it the draw holds the keys of many
 // lists no longer (K = 128: 1 row 23.9 against 19.8).
 constexpr int kTopK = 112;
 constexpr int kTopCap = 4 * kTopK;  // keys of a chunk's list
@@ -685,8 +685,7 @@ __device__ RowEnds find_ends(const BinShare<THREADS> &bins, const RowSettings &s
 }
 
 // Puts those of four logits that are in a listed bin (from `first` on) on a
-// list of CAP; *count counts them all.
-template <uint32_t CAP = kListMax>
+// list of kListMax; *count counts them all.
 __device__ __forceinline__ void list_of(const f32x4_at4 &v, int at, const int (&b)[4], int first,
                                         const RowEnds &e, u64 *list, uint32_t *count) {
   bool in[4];
@@ -697,7 +696,7 @@ __device__ __forceinline__ void list_of(const f32x4_at4 &v, int at, const int (&
   for (int i = 0; i < 4; ++i)
     if (in[i]) {
       const uint32_t n = atomicAdd(count, 1u);
-      if (n < CAP) list[n] = topk_key(v[i], static_cast<uint32_t>(at + i));
+      if (n < kListMax) list[n] = topk_key(v[i], static_cast<uint32_t>(at + i));
     }
 }
 
@@ -1027,7 +1026,8 @@ __device__ __forceinline__ void draw_token(const SampleArgs &a, int row, const f
 
 // One workgroup a row.  Bound by the barriers of its sort and sums: 12.4 us with
 // lists of up to a thousand keys (64 rows), 6.4 with one of 40 (512 threads sort
-// and sum over half the waves: 8.6 with 1024), 5.4 with none.
+// and sum over half the waves: 8.6 with 1024; both before such rows took
+// sample_top_draw_kernel), 5.4 with none.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
   __shared__ DrawShared sh;
@@ -1120,17 +1120,30 @@ __device__ __forceinline__ CountEnd count_end(const uint32_t *count, int64_t top
                   static_cast<uint32_t>(need - sh.above)};
 }
 
+constexpr int kTopFours = 160;  // vectors that a wave gathers
+
+__device__ __forceinline__ int lanes_below(uint64_t which) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(which >> 32),
+                                   __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(which), 0));
+}
+
 // A workgroup a chunk: its largest logit, and a list of the tokens in the bins
-// (under that logit) of its top_k largest, which hold the row's.
+// (under that logit) of its top_k largest, which hold the row's.  Bound by
+// latency for one row of 128256 (4.4 us) and by its reads for 64 (11.3 us with
+// top-k 40, where the largest logits alone take 6.5); with every lane listing
+// its own tokens, an atomic behind the other, 5.7 and 13.8.
 __global__ __launch_bounds__(kChunkThreads) void sample_top_kernel(SampleArgs a) {
   __shared__ uint32_t s_bins[kSampleBins];
-  __shared__ u64 s_keys[kTopCap];
+  __shared__ f32x4_at4 s_four[kChunkThreads / kWave][kTopFours];
+  __shared__ int s_at[kChunkThreads / kWave][kTopFours];
   __shared__ float s_max[kChunkThreads / kWave];
   __shared__ CountShared s_end;
   __shared__ uint32_t s_count;
   const int chunk = static_cast<int>(blockIdx.x) % a.chunks;
   const int row = static_cast<int>(blockIdx.x) / a.chunks;
   const int tid = threadIdx.x;
+  const int lane = tid & (kWave - 1);
+  const int wave = tid / kWave;
   const auto logits = row_chunk(a, row, chunk);
   const RowSettings set = row_settings(a, row);
   for (int i = tid; i < kSampleBins; i += kChunkThreads) s_bins[i] = 0;
@@ -1140,7 +1153,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_top_kernel(SampleArgs a)
     best = nan_max(nan_max(best, nan_max(v[0], v[1])), nan_max(v[2], v[3]));
   });
   best = wave_nan_max(best);
-  if ((tid & (kWave - 1)) == 0) s_max[tid / kWave] = best;
+  if (lane == 0) s_max[wave] = best;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kChunkThreads / kWave; ++w) best = nan_max(best, s_max[w]);
@@ -1164,25 +1177,45 @@ __global__ __launch_bounds__(kChunkThreads) void sample_top_kernel(SampleArgs a)
   const CountEnd end = count_end<kChunkThreads>(s_bins, set.top_k, s_end);
   // fewer fours than top_k: at most kTopCap tokens, all listed
   const int last = end.above + end.need < set.top_k ? kSampleBins - 1 : end.bin;
-  const RowEnds e{0, 0, 0, 0, 0, 0, last, last};
+  // a wave gathers its fours that hold such a token, so that its lanes take a
+  // logit of these each
+  int fours = 0;
   logits.each([&](const f32x4_at4 &v, int at, int) {
-    if (four_bin(v) > last) return;
-    double t[4];
-    int b[4];
-    bins_of(v, r, t, b);
-    list_of<kTopCap>(v, at, b, 0, e, s_keys, &s_count);
+    const bool in = four_bin(v) <= last;
+    const uint64_t which = __ballot(in);
+    // (a lane that had no four before this one has not counted them)
+    fours = __builtin_amdgcn_readfirstlane(fours);
+    const int n = fours + lanes_below(which);
+    if (in && n < kTopFours) {
+      s_four[wave][n] = v;
+      s_at[wave][n] = at;
+    }
+    fours += __popcll(which);
   });
-  __syncthreads();
-  // more than kTopCap: the draw counts over the row
-  const int n = static_cast<int>(s_count);
-  if (tid == 0) *listed = s_count;
+  fours = __builtin_amdgcn_readfirstlane(fours);
   u64 *list = a.list + (static_cast<int64_t>(row) * a.chunks + chunk) * kTopCap;
-  for (int i = tid; i < min(n, kTopCap); i += kChunkThreads) list[i] = s_keys[i];
+  for (int first = 0; first < 4 * min(fours, kTopFours); first += kWave) {
+    const int i = first + lane;
+    const bool mine = i < 4 * min(fours, kTopFours);
+    const float v = mine ? s_four[wave][i / 4][i % 4] : -INFINITY;
+    const bool in = weight_bin(log_weight(v, r)) <= last;
+    const uint64_t which = __ballot(in);
+    uint32_t base = 0;
+    if (lane == 0) base = atomicAdd(&s_count, static_cast<uint32_t>(__popcll(which)));
+    const uint32_t n = __builtin_amdgcn_readfirstlane(base) + lanes_below(which);
+    if (in && n < kTopCap)
+      list[n] = topk_key(v, static_cast<uint32_t>(s_at[wave][i / 4] + i % 4));
+  }
+  // more than fit: the draw counts over the row
+  if (lane == 0 && fours > kTopFours) atomicAdd(&s_count, kTopCap + 1);
+  __syncthreads();
+  if (tid == 0) *listed = s_count;
 }
 
 // One workgroup a row: bins of the chunks' lists under the row's largest logit
 // give its top_k, which are sorted and cut as in the draw above.  At most kTopK
-// tokens are left, and each finds the mass before it by itself.
+// tokens are left, and each finds the mass before it by itself.  Bound by its
+// barriers: 7.8 us for 63 lists of top-k 40 or 64 rows of 16 lists.
 constexpr int kTopHeld = 8;   // lists of which a wave holds the first keys: one a
 constexpr int kTopTwo = 56;  // lane, and from this top_k on (ties come on top) two
 
