@@ -1257,7 +1257,7 @@ __global__ __launch_bounds__(THREADS) void sample_top_draw_kernel(SampleArgs a) 
   auto each = [&](auto f) {
     auto rest = [&](int c, int first, int n) {
 #pragma unroll 1
-      for (int i = first + lane; i < min(n, kTopCap); i += kWave) f(list[c * kTopCap + i]);
+      for (int i = first + lane; i < n; i += kWave) f(list[c * kTopCap + i]);
     };
 #pragma unroll
     for (int j = 0; j < kTopHeld; ++j)
@@ -1273,11 +1273,15 @@ __global__ __launch_bounds__(THREADS) void sample_top_draw_kernel(SampleArgs a) 
       if (count[j] > known) rest(wave + kWaves * j, known, count[j]);
 #pragma unroll 1
     for (int c = wave + kWaves * kTopHeld; c < a.chunks; c += kWaves)
-      rest(c, 0, static_cast<int>(listed[c]));
+      if (listed[c] <= kTopCap) rest(c, 0, static_cast<int>(listed[c]));
   };
+  // a list that did not fit has holes: its keys are nothing to work with
 #pragma unroll
   for (int j = 0; j < kTopHeld; ++j)
-    if (count[j] > kTopCap) s_over = 1;
+    if (count[j] > kTopCap) {
+      s_over = 1;
+      count[j] = 0;
+    }
   for (int c = kWaves * kTopHeld + tid; c < a.chunks; c += THREADS)
     if (listed[c] > kTopCap) s_over = 1;
   each([&](u64 key) {

@@ -253,6 +253,27 @@ def test_short_top_k_among_equals(gpu_device, vocab, near):
         check(logits, uniform, gpu_device, **settings)
 
 
+def test_what_the_workspace_held_is_not_read(gpu_device):
+    # bytes that are keys of large logits, numbers of tokens and masses; lists
+    # that are written in part
+    g = torch.Generator().manual_seed(78)
+    for vocab, near in ((30000, 30000), (150000, 150000), (30000, 900), (9000, 5000)):
+        print("sample", near, "in", vocab, flush=True)
+        logits = torch.randn(2, vocab, generator=g) - 20.0
+        logits[:, :near] = 1.0
+        uniform = torch.rand(2, generator=g).to(gpu_device)
+        on_device = logits.to(gpu_device)
+        for settings in (dict(top_k=40, top_p=0.9), dict(top_k=300), dict(top_p=0.6), dict()):
+            found = []
+            for byte in (0, 0xC5, 0x3F, 0xFF):
+                ids = torch.empty(2, dtype=torch.int64, device=gpu_device)
+                ws = torch.full((_hip.sample_workspace_bytes(2, vocab),), byte,
+                                dtype=torch.uint8, device=gpu_device)
+                _hip.sample(on_device, uniform, ids, ws, **settings)
+                found.append(ids.tolist())
+            assert all(ids == found[0] for ids in found), (settings, found)
+
+
 def test_short_top_k_of_many_rows(gpu_device):
     # the rows of two slices, chunks of 8192
     g = torch.Generator().manual_seed(77)
