@@ -274,6 +274,36 @@ def test_what_the_workspace_held_is_not_read(gpu_device):
             assert all(ids == found[0] for ids in found), (settings, found)
 
 
+def test_captured_draws_replay(gpu_device):
+    # both forms of long rows in one graph, and another graph, share a workspace
+    dev, vocab = gpu_device, 50000
+    g = torch.Generator().manual_seed(79)
+    logits, uniform = torch.zeros(3, vocab, device=dev), torch.zeros(3, device=dev)
+    ws = torch.empty(_hip.sample_workspace_bytes(3, vocab), dtype=torch.uint8, device=dev)
+    forms = (dict(top_k=40, top_p=0.9), dict(top_k=500, top_p=0.95, min_p=0.01), dict())
+    ids = [torch.zeros(3, dtype=torch.int64, device=dev) for _ in forms]
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        _hip.sample(logits, uniform, ids[0], ws)
+    torch.cuda.current_stream(dev).wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph, which in zip(graphs, ((0, 1), (2, 0))):
+        with torch.cuda.graph(graph):
+            for i in which:
+                _hip.sample(logits, uniform, ids[i], ws, **forms[i])
+    for replay in range(4):
+        logits.copy_((torch.randn(3, vocab, generator=g) * 3).to(dev))
+        uniform.copy_(torch.rand(3, generator=g).to(dev))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize(dev)
+        for i, form in enumerate(forms):
+            eager = torch.zeros(3, dtype=torch.int64, device=dev)
+            _hip.sample(logits, uniform, eager, ws, **form)
+            assert torch.equal(ids[i], eager), (replay, form)
+
+
 def test_short_top_k_of_many_rows(gpu_device):
     # the rows of two slices, chunks of 8192
     g = torch.Generator().manual_seed(77)
