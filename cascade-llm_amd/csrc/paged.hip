@@ -184,6 +184,26 @@ __device__ __forceinline__ float paged_exp2(float x) {
   return __builtin_amdgcn_exp2f(x);
 }
 
+// Two weights as sums of two bf16 values each, for the product with V: one
+// value alone, 2^-8 off, shows next to the rounding of the result where V's
+// rows cancel.  The upper parts are cut off just below the weights (a factor
+// of 1 - 2^-24 leaves no normal fp32 number as it is), so that the lower ones,
+// which fp32 holds exactly, are positive: a zero or a negative one would turn
+// an infinite value of V into a NaN.  Of a weight in [2^e, 2^(e+1)) the lower
+// part is at most 2^(e-7), and its rounding, half a step, 2^(e-16).  The second
+// product hides behind the loads (64 ragged sequences of up to 16384 positions
+// 318 us, 317 with one; 32769 positions 28.8 and 28.6).
+struct SplitWeights {
+  uint32_t upper, lower;
+};
+
+__device__ __forceinline__ SplitWeights split_weights(float a, float b) {
+  constexpr float kBelow = 1.0f - 0x1p-24f;
+  const uint32_t upper = __builtin_amdgcn_perm(__float_as_uint(b * kBelow),
+                                               __float_as_uint(a * kBelow), 0x07060302u);
+  return {upper, pack_bf16x2(a - lo_bf16(upper), b - hi_bf16(upper))};
+}
+
 // Table row and length of batch row b.  row < 0: nothing to do.
 struct PagedRow {
   int64_t row;
@@ -281,7 +301,7 @@ __device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, in
 // waves merge in LDS.  The products are v_mfma_f32_16x16x32_bf16 with the
 // query heads of the KV head as columns (zeros past group):
 //   S = K_blk q^T    two 16-row tiles x D / 32 chunks
-//   O += V_blk^T P   D / 16 tiles, K = the 32 positions
+//   O += V_blk^T P   D / 16 tiles, K = the 32 positions, for either part of P
 // Lane (c, g4) = (l % 16, l / 16) owns the scores of head c at rows
 // 8 g4 .. 8 g4 + 7 (the row order inside a K tile is chosen for that), which
 // is its piece of the P operand.  K rows are transposed through LDS, V rows
@@ -474,10 +494,13 @@ paged_attention_kernel(PagedAttnArgs a) {
       psum += p[j];
     }
     l = fmaf(l, alpha, psum);
-    u32x4 pop;
+    u32x4 pop, rest;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      pop[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]) & head_mask;
+    for (int i = 0; i < 4; ++i) {
+      const SplitWeights w = split_weights(p[2 * i], p[2 * i + 1]);
+      pop[i] = w.upper & head_mask;
+      rest[i] = w.lower & head_mask;
+    }
     if (alpha != 1.0f) {
 #pragma unroll
       for (int e = 0; e < DV; ++e) o[e] *= alpha;
@@ -489,6 +512,7 @@ paged_attention_kernel(PagedAttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         vop[i] = __builtin_amdgcn_perm(x.v[2 * i + 1][e >> 1], x.v[2 * i][e >> 1], sel);
+      o[e] = mfma_16x16x32_bf16(vop, rest, o[e]);
       o[e] = mfma_16x16x32_bf16(vop, pop, o[e]);
     }
   };
