@@ -854,7 +854,10 @@ __device__ u64 list_cut(const u64 *list, int n, u64 mine, const RowEnds &e,
   const u64 start = block_prefix<THREADS / kWave>(sum, sh.scan, &total) - sum;
   u64 mass_k = e.total;
   if (e.last_k >= 0) {
-    // mass of the list before K's last bin, and up to K's last token
+    // mass of the list before K's last bin, and up to K's last token.  Where
+    // the bins have masses the list may lack those between P's last candidate
+    // and K's last bin, also if it starts at bin 0: what lies above K's last bin
+    // is known from the bins.  Without masses (a short K) the list has all.
     u64 upto = start;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -864,7 +867,7 @@ __device__ u64 list_cut(const u64 *list, int n, u64 mine, const RowEnds &e,
       if (at == last_k) sh.found[1] = upto;
     }
     __syncthreads();
-    mass_k = e.first == 0 ? sh.found[1] : e.above_k + (sh.found[1] - sh.found[0]);
+    mass_k = set.use_p ? e.above_k + (sh.found[1] - sh.found[0]) : sh.found[1];
     __syncthreads();
   }
   const u64 need = top_p_mass(set.top_p, mass_k);
