@@ -938,13 +938,17 @@ __device__ __forceinline__ u64 target_of(float uniform, u64 total) {
   return target < total ? target : total - 1;
 }
 
-// Writes a row's token of weight w.
-__device__ __forceinline__ void store_token(const SampleArgs &a, int row, int64_t token, u64 w,
-                                            u64 total) {
+// Writes a row's token, of logit x.  Its log-probability is the log weight
+// itself and not the logarithm of the rounded weight, of which an unlikely
+// token's has few bits left; the sum's rounding is below vocab 2^-45.
+__device__ __forceinline__ void store_token(const SampleArgs &a, int row, int64_t token, float x,
+                                            const RowScale &r, u64 total) {
+  constexpr double kLn = 0.6931471805599453;
   a.ids[row] = token;
   if (a.logprobs != nullptr)
-    a.logprobs[row] =
-        static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total)));
+    a.logprobs[row] = static_cast<float>(
+        log_weight(x, r) * (kLn / kTable) -
+        log(static_cast<double>(total) / static_cast<double>(kWeightOne)));
 }
 
 __device__ __forceinline__ void store_no_token(const SampleArgs &a, int row) {
@@ -1019,7 +1023,7 @@ __device__ __forceinline__ void draw_token(const SampleArgs &a, int row, const f
     for (int i = mine; i < end; ++i) {
       const u64 w = weight_of(x[i], i);
       if (target < at + w) {
-        store_token(a, row, i, w, total);
+        store_token(a, row, i, x[i], r, total);
         break;
       }
       at += w;
@@ -1330,7 +1334,8 @@ __global__ __launch_bounds__(THREADS) void sample_top_draw_kernel(SampleArgs a) 
         before += static_cast<uint32_t>(key_index(sh.keys[i])) < index ? other : 0;
       }
       const u64 target = target_of(uniform, total);
-      if (before <= target && target < before + w) store_token(a, row, index, w, total);
+      if (before <= target && target < before + w)
+        store_token(a, row, index, key_value(key), r, total);
       return;
     }
     __syncthreads();  // (the count takes the place of the list)
@@ -1483,7 +1488,7 @@ __global__ __launch_bounds__(THREADS) void sample_short_kernel(SampleArgs a) {
       for (int i = j < kShortVecs ? logits.at(j) : last; i < a.vocab; ++i) {
         const u64 w = weight_of(x[i], i);
         if (target < at + w) {
-          store_token(a, row, i, w, total);
+          store_token(a, row, i, x[i], r, total);
           break;
         }
         at += w;

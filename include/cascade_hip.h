@@ -433,7 +433,8 @@ int cascade_topk_f32(const float *logits, int64_t rows, int64_t top_k,
  *   the lowest indices);  P = the shortest run of K, largest first, whose mass
  *   reaches top_p * mass(K);  S = the i of P with w_i >= min_p (the likeliest
  *   always stays);  ids[r] = the first i of S, by index, at which the mass
- *   of S exceeds uniform * mass(S);  logprobs[r] (nullable) = log(w_i / mass(S)).
+ *   of S exceeds uniform * mass(S);  logprobs[r] (nullable) = log(w_i / mass(S)),
+ *   with the w_i of that line not rounded.
  * Each setting is a device array with a value per row or, where that is
  * null, the value given for all.  T <= 0 takes the largest logit (lowest
  * index, log-probability 0); top_k <= 0, top_p >= 1 and min_p <= 0 are off.
