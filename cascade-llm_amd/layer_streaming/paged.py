@@ -111,6 +111,8 @@ class PagedKVCache:
         self._outside_graph()
         if count < 1:
             raise ValueError("count must be positive")
+        if not rows:
+            return
         if len(set(rows)) != len(rows):
             raise ValueError("a sequence occurs twice")
         # pages to take, and shared last pages; of the sequences that share
