@@ -1299,8 +1299,11 @@ def paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out,
 def copy_pages(pages, pairs, error_flag=None, stream=None):
     """Copy page pairs[i, 0] over page pairs[i, 1] in every plane of ``pages``.
 
-    ``pages``: a contiguous pool [layers, 2, pages, ...] (or [planes, pages,
-    ...] with ``pages.dim()`` 4 or less); ``pairs``: int32 [n, 2].  The pairs
+    ``pages``: a contiguous pool [layers, 2, pages, ...], or [planes, pages,
+    ...] with ``pages.dim()`` 4 or less: one layer's [2, pages, kv_heads,
+    page_size, dim] is given as ``pages.flatten(2)``, and a single [pages,
+    kv_heads, page_size, dim] as ``pages[None].flatten(2)``.  Five dimensions
+    that may be one layer's are refused.  ``pairs``: int32 [n, 2].  The pairs
     are copied in no order: no destination may occur twice or be another
     pair's source.  A negative page marks padding; one outside the pool
     leaves its pair out and flags PAGED_ERANGE.  Returns ``pages``."""
@@ -1312,6 +1315,10 @@ def copy_pages(pages, pairs, error_flag=None, stream=None):
     if len(shape) < 3:
         raise ValueError("pages must be [layers, 2, pages, ...] or [planes, pages, ...]")
     if len(shape) >= 5:
+        if shape[1] != 2 or (len(shape) == 5 and shape[0] == 2):
+            raise ValueError("pages {} are not [layers, 2, pages, ...], or may be one "
+                             "layer's [2, pages, ...]: give pages.flatten(2) for those, or "
+                             "pages.flatten(0, 1).flatten(2)".format(list(shape)))
         planes, count = shape[0] * shape[1], shape[2]
     else:
         planes, count = shape[0], shape[1]

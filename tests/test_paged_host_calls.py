@@ -37,3 +37,42 @@ def test_the_caches_workspace_serves_every_limit(max_length, page_size):
     held = cache._attention_workspace(3, 8).numel()
     for limit in (1, max_length, capacity):
         assert held >= _hip.paged_attention_workspace_bytes(3, 8, 2, 64, limit)
+
+
+@pytest.fixture
+def copies(monkeypatch):
+    """copy_pages on the CPU up to its launch: (planes, plane bytes, pages,
+    page bytes) of each."""
+
+    calls = []
+    monkeypatch.setattr(_hip, "_gpu_of", lambda name, tensor: tensor.device)
+    monkeypatch.setattr(
+        _hip, "_call_on", lambda index, stream, name, at, *sizes: calls.append(sizes[:4]))
+    return calls
+
+
+PAIRS = torch.tensor([[0, 1]], dtype=torch.int32)
+
+
+def test_copy_pages_refuses_one_layers_pools(copies):
+    # [2, pages, kv_heads, page_size, dim] is no [layers, 2, pages, ...]: its
+    # KV heads would pass for pages.  With two pages it looks like two layers
+    for pages in (4, 3, 2):
+        cache = small_cache(num_pages=pages)
+        with pytest.raises(ValueError, match="flatten"):
+            _hip.copy_pages(cache.buffer[0], PAIRS)
+    with pytest.raises(ValueError):
+        _hip.copy_pages(torch.zeros(2, 3, 4, 2, 8, 64), PAIRS)
+    assert not copies
+
+
+def test_copy_pages_reads_planes(copies):
+    cache = small_cache(layer_count=3)
+    page = 2 * 8 * 64 * 2
+    _hip.copy_pages(cache.buffer, PAIRS)
+    _hip.copy_pages(cache.buffer.flatten(0, 1).flatten(2), PAIRS)
+    _hip.copy_pages(cache.buffer[0].flatten(2), PAIRS)
+    _hip.copy_pages(torch.zeros(3, 2, 4, 16, 64, dtype=torch.bfloat16), PAIRS)
+    _hip.copy_pages(cache.k_pages(1)[None].flatten(2), PAIRS)
+    assert copies == [(6, 4 * page, 4, page)] * 2 + [(2, 4 * page, 4, page)] + [
+        (6, 4 * 2048, 4, 2048), (1, 4 * page, 4, page)]
