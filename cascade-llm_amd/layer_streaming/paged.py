@@ -36,7 +36,8 @@ class PagedKVCache:
     ``buffer``: bf16 [layers, 2 (K, V), num_pages, kv_heads, page_size,
     head_dim].  ``page_table`` (int32 [max_sequences, pages of one], -1 where
     there is no page) and ``lengths`` (int32 [max_sequences]) are on the
-    device.  A sequence is named by its table row.
+    device.  A sequence is named by its table row.  ``head_dim``: a multiple
+    of 16 of up to 1024; ``attend`` takes 64 and 128.
     """
 
     def __init__(self, num_pages, max_sequences, max_length, layer_count=32,
@@ -51,6 +52,8 @@ class PagedKVCache:
         page_size = int(page_size)
         if not 8 <= page_size <= 1024 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two of 8 to 1024")
+        if not 16 <= int(head_dim) <= 1024 or int(head_dim) % 16:
+            raise ValueError("head_dim must be a multiple of 16 of 16 to 1024")
         self.num_pages = int(num_pages)
         self.max_sequences = int(max_sequences)
         self.page_size = page_size
@@ -275,10 +278,14 @@ class PagedKVCache:
 
     def attend(self, layer, q, out, rows=None, scale=None, workspace=None,
                max_length=None):
-        """``paged_decode_attention`` over one layer's pages; ``scale``
-        defaults to head_dim ** -0.5, ``workspace`` to one that the cache
-        keeps (give one of your own to calls that may overlap)."""
+        """``paged_decode_attention`` over one layer's pages (heads of 64 or
+        128); ``scale`` defaults to head_dim ** -0.5, ``workspace`` to one
+        that the cache keeps (give one of your own to calls that may
+        overlap)."""
 
+        if self.head_dim not in (64, 128):
+            raise ValueError("attention takes heads of 64 or 128, these have {}".format(
+                self.head_dim))
         limit = self.max_length if max_length is None else max_length
         if workspace is None:
             workspace = self._attention_workspace(q.shape[0], q.shape[1])

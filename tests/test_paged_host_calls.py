@@ -76,3 +76,17 @@ def test_copy_pages_reads_planes(copies):
     _hip.copy_pages(cache.k_pages(1)[None].flatten(2), PAIRS)
     assert copies == [(6, 4 * page, 4, page)] * 2 + [(2, 4 * page, 4, page)] + [
         (6, 4 * 2048, 4, 2048), (1, 4 * page, 4, page)]
+
+
+@pytest.mark.parametrize("head_dim", [0, 8, 72, 1040, -64])
+def test_head_sizes_that_no_operator_takes_are_refused(head_dim):
+    with pytest.raises(ValueError):
+        small_cache(head_dim=head_dim)
+
+
+def test_attend_names_head_sizes_it_does_not_take():
+    # append and the copies take them: the refusal is attend's
+    cache = small_cache(head_dim=96)
+    q = torch.zeros(1, 4, 96, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="64 or 128"):
+        cache.attend(0, q, torch.zeros_like(q))
