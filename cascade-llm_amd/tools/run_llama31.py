@@ -17,7 +17,8 @@ eagerly while the graph is captured (decode_graph_setup_ms).
 --temperature (not in the reference, which takes the top-1 of the logits)
 draws each token instead, over the whole vocabulary: --sample-top-k,
 --sample-top-p and --sample-min-p restrict the draw (layer_streaming.sample),
---sample-seed fixes its random numbers.  The default, 0, is greedy.
+--sample-seed fixes its random numbers.  The default, 0, is greedy; settings
+of a draw without --temperature are refused.
 """
 
 import argparse
@@ -71,8 +72,8 @@ def parse_args(argv=None):
                         help="weights resident in HBM; decode by replaying one "
                              "captured HIP graph per token (needs --vocab-mode "
                              "resident)")
-    parser.add_argument("--temperature", type=float, default=0.0,
-                        help="draw tokens at this temperature (0: greedy)")
+    parser.add_argument("--temperature", type=float, default=None,
+                        help="draw tokens at this temperature (0, the default: greedy)")
     parser.add_argument("--sample-top-k", type=int, default=0,
                         help="draw from this many most likely tokens (0: all)")
     parser.add_argument("--sample-top-p", type=float, default=1.0,
@@ -87,6 +88,11 @@ def parse_args(argv=None):
         parser.error("either --checkpoint or --random-init is required")
     if args.decode_graph and args.vocab_mode != "resident":
         parser.error("--decode-graph needs --vocab-mode resident")
+    if args.temperature is None:
+        if args.sample_top_k != 0 or not args.sample_top_p >= 1 or args.sample_min_p != 0:
+            parser.error("--sample-top-k, --sample-top-p and --sample-min-p need "
+                         "--temperature")
+        args.temperature = 0.0
     if args.decode_graph and args.temperature != 0:
         parser.error("--decode-graph decodes greedily (--temperature 0)")
     for name in ("temperature", "sample_top_k", "sample_top_p", "sample_min_p"):
