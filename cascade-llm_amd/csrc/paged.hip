@@ -310,8 +310,8 @@ __device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, in
 // a block whose rows are all left out keeps it and adds nothing; a sequence
 // with no row at all ends with a zero sum and writes zeros.
 // Bound by HBM: 64 ragged sequences of up to 16384 positions (8 KV heads of
-// 128) 314 us at 6.3 TB/s, where a plain read of those bytes takes 285; one of
-// 32769 positions 24.3 us (21.1), the lookups before the first rows and the
+// 128) 316 us at 6.2 TB/s, where a plain read of those bytes takes 285; one of
+// 32769 positions 25.1 us (21.1), the lookups before the first rows and the
 // join behind the last ones showing.  Four waves on a SIMD (at most 128
 // registers, hence the q operands in LDS) hide the loads better than a second
 // register set of rows with two waves does (351 against 347 us for the first,
@@ -678,8 +678,7 @@ struct CopyPagesArgs {
 };
 
 constexpr int kCopyThreads = 256;
-constexpr int kCopyVecs = 1;  // 16-byte vectors a thread and piece
-constexpr int64_t kCopyPiece = int64_t{kCopyThreads} * kCopyVecs * 16;
+constexpr int64_t kCopyPiece = int64_t{kCopyThreads} * 16;  // a 16-byte vector a thread
 
 // One workgroup copies a piece of 4 KiB of one page of one plane.  Bound by
 // HBM: 257 pages of 128 KiB in 8 planes take 92 us (5.8 TB/s read and
@@ -701,17 +700,11 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyPagesArgs 
     unsigned char *plane_base = a.base + plane * a.plane_bytes;
     const unsigned char *from = plane_base + src * a.page_bytes;
     unsigned char *to = plane_base + dst * a.page_bytes;
-    u32x4 x[kCopyVecs];
-#pragma unroll
-    for (int i = 0; i < kCopyVecs; ++i) {
-      const int64_t at = piece * kCopyPiece + (int64_t{i} * kCopyThreads + threadIdx.x) * 16;
-      if (at < a.page_bytes) x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from + at));
-    }
-#pragma unroll
-    for (int i = 0; i < kCopyVecs; ++i) {
-      const int64_t at = piece * kCopyPiece + (int64_t{i} * kCopyThreads + threadIdx.x) * 16;
-      if (at < a.page_bytes) __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4 *>(to + at));
-    }
+    const int64_t at = piece * kCopyPiece + threadIdx.x * 16;
+    if (at < a.page_bytes)
+      __builtin_nontemporal_store(
+          __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from + at)),
+          reinterpret_cast<u32x4 *>(to + at));
   }
 }
 

@@ -63,8 +63,16 @@ constexpr int kChunkMax = 8192;
 constexpr int kChunkWorkgroups = 256;
 constexpr int kChunkVecs = kChunkMax / (4 * kChunkThreads);  // of four logits, a thread
 constexpr int kChunkParts = kChunkMax / kPart;
-constexpr int kFewThreads = 512;  // of a draw whose list is short
-constexpr int64_t kFewK = 480;    // K up to this is one
+// Threads of a draw whose list is short, and the K up to which it is: 512 sort
+// as many keys in registers and have half the waves to wait for, more keys go
+// through LDS (128256 logits, top-p 0.95, 512 against 1024 threads: K = 113 19.7
+// and 21.4 us for a row, 38.3 and 40.2 for 64; K = 480 21.2 and 23.2, 40.8 and
+// 42.9; K = 520 33.3 and 24.3, 53.0 and 44.2).  A K of 480 leaves room for ties.
+// Rows without a top-k count as short: P ends in a bin or two (64 rows, top-p
+// 0.5 45.0 and 46.6, 0.99 52.1 and 54.2), which hold more than 512 keys only
+// where that many logits nearly equal each other (700 of them 56.1 and 47.4).
+constexpr int kFewThreads = 512;
+constexpr int64_t kFewK = 480;
 constexpr int kShortVecs = 4;
 constexpr int64_t kShortVocab = int64_t{4} * kSampleThreads * kShortVecs;
 // One K up to this for all rows takes two launches (128256 logits, top-p 0.95,
@@ -1032,9 +1040,7 @@ __device__ __forceinline__ void draw_token(const SampleArgs &a, int row, const f
 }
 
 // One workgroup a row.  Bound by the barriers of its sort and sums: 12.4 us with
-// lists of up to a thousand keys (64 rows), 6.4 with one of 40 (512 threads sort
-// and sum over half the waves: 8.6 with 1024; both before such rows took
-// sample_top_draw_kernel), 5.4 with none.
+// lists of up to a thousand keys (64 rows), 5.4 with none.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleArgs a) {
   __shared__ DrawShared sh;
@@ -1527,7 +1533,8 @@ static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
   p.list_bytes = rounded(
       r * std::max<int64_t>(kListMax, p.chunks * kTopCap) * sizeof(u64));
   p.count_bytes = rounded(r * sizeof(uint32_t));
-  p.bytes = p.max_bytes + p.mass_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes + p.list_bytes + p.count_bytes;
+  p.bytes = p.max_bytes + p.mass_bytes + p.bin_mass_bytes + p.bin_count_bytes + p.ends_bytes +
+            p.list_bytes + p.count_bytes;
   return p;
 }
 

@@ -1090,9 +1090,10 @@ def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
     tables, bf16 [positions, r / 2]; the first r dims of a head turn, in pairs
     (i, i + r / 2) or, ``interleaved``, (2 i, 2 i + 1).  None copies the rows
     as they are.  ``q_out`` (q itself by default; none of its rows may be
-    another's q, k or v) receives the rotated q rows and is returned.  Pools are [pages, kv_heads, page_size, dim] views,
-    ``page_table`` int32 [sequences, pages of one].  An index out of range
-    leaves its token out and ors PAGED_ERANGE into ``error_flag``."""
+    another's q, k or v) receives the rotated q rows and is returned.  Pools
+    are [pages, kv_heads, page_size, dim] views, ``page_table`` int32
+    [sequences, pages of one].  An index out of range leaves its token out
+    and ors PAGED_ERANGE into ``error_flag``."""
 
     if q is not None and q_out is None:
         q_out = q

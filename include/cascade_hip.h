@@ -438,6 +438,8 @@ int cascade_topk_f32(const float *logits, int64_t rows, int64_t top_k,
  * Each setting is a device array with a value per row or, where that is
  * null, the value given for all.  T <= 0 takes the largest logit (lowest
  * index, log-probability 0); top_k <= 0, top_p >= 1 and min_p <= 0 are off.
+ * (One value for all that is NaN, or negative where it is not top_k, is
+ * refused; in an array a NaN temperature is greedy, other NaNs are off.)
  * Weights are fp64 rounded to multiples of 2^-44 of the largest and summed
  * exactly.  -inf is never drawn; a row with a NaN, or of nothing but -inf,
  * yields id -1 and a NaN log-probability.  The workspace
