@@ -1513,10 +1513,12 @@ struct SamplePlan {
   size_t bytes;  // of all of them
 };
 
+static int64_t chunks_wanted(int64_t rows) { return (kChunkWorkgroups + rows - 1) / rows; }
+
 static SamplePlan sample_plan(int64_t rows, int64_t vocab) {
   SamplePlan p{};
   if (rows > kSliceRows) rows = kSliceRows;  // more rows go slice by slice
-  const int64_t want = (kChunkWorkgroups + rows - 1) / rows;
+  const int64_t want = chunks_wanted(rows);
   p.chunk = (vocab + want - 1) / want;
   p.chunk = (p.chunk + kPart - 1) / kPart * kPart;
   if (p.chunk < kChunkMin) p.chunk = kChunkMin;
@@ -1545,11 +1547,15 @@ using namespace cascade;
 extern "C" size_t cascade_sample_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows <= 0 || vocab <= 0 || vocab > kSampleMaxVocab || rows > 0x7fffffff) return 0;
   if (vocab <= kShortVocab) return 256;
-  // enough for fewer rows too, which may be cut into more chunks
+  // enough for fewer rows too, which may be cut into more chunks, and for fewer
+  // logits: their chunks are most where a smaller size of chunk ends
   size_t most = 0;
   for (int64_t r = rows < kSliceRows ? rows : kSliceRows; r >= 1; --r) {
-    const size_t bytes = sample_plan(r, vocab).bytes;
-    most = bytes > most ? bytes : most;
+    most = std::max(most, sample_plan(r, vocab).bytes);
+    for (int64_t chunk = kChunkMin; chunk < kChunkMax; chunk += kPart) {
+      const int64_t end = chunks_wanted(r) * chunk;
+      if (end > kShortVocab && end < vocab) most = std::max(most, sample_plan(r, end).bytes);
+    }
   }
   return most;
 }

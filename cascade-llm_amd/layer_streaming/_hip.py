@@ -1337,7 +1337,8 @@ def copy_pages(pages, pairs, error_flag=None, stream=None):
 
 
 def sample_workspace_bytes(rows, vocab):
-    """Workspace bytes of sample for up to ``rows`` rows of ``vocab`` logits."""
+    """Workspace bytes of sample for up to ``rows`` rows of up to ``vocab``
+    logits."""
 
     size = load().cascade_sample_workspace_bytes(int(rows), int(vocab))
     if size == 0:

@@ -443,10 +443,10 @@ int cascade_topk_f32(const float *logits, int64_t rows, int64_t top_k,
  * Weights are fp64 rounded to multiples of 2^-44 of the largest and summed
  * exactly.  -inf is never drawn; a row with a NaN, or of nothing but -inf,
  * yields id -1 and a NaN log-probability.  The workspace
- * (cascade_sample_workspace_bytes, 0 for an unsupported shape) needs no
- * zero-fill and holds nothing between calls.  Stands beside the greedy
- * torch.topk(...)[..., 0] of the reference's token loop
- * (tools/run_llama31.py:105-121), which has no sampling.                   */
+ * (cascade_sample_workspace_bytes for up to as many rows and logits, 0 for an
+ * unsupported shape) needs no zero-fill and holds nothing between calls.
+ * Stands beside the greedy torch.topk(...)[..., 0] of the reference's token
+ * loop (tools/run_llama31.py:105-121), which has no sampling.               */
 size_t cascade_sample_workspace_bytes(int64_t rows, int64_t vocab);
 int cascade_sample_f32(const float *logits, int64_t row_stride, int64_t rows,
                        int64_t vocab, const float *uniform,
