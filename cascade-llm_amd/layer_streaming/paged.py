@@ -296,10 +296,11 @@ class PagedKVCache:
             max_length=limit, error_flag=self.error)
 
     def _attention_workspace(self, batch, q_heads):
-        # for any limit that a call may give: what a table row holds
+        # for any limit that a call may give: what a table row holds, and the
+        # operator takes
+        limit = min(self.max_pages * self.page_size, 0x7fffffff - 64)
         need = _hip.paged_attention_workspace_bytes(
-            max(batch, 1), q_heads, self.num_kv_heads, self.head_dim,
-            self.max_pages * self.page_size)
+            max(batch, 1), q_heads, self.num_kv_heads, self.head_dim, limit)
         if not self._workspaces or self._workspaces[-1].numel() < need:
             self._workspaces.append(
                 torch.empty(need, dtype=torch.uint8, device=self.device))

@@ -90,3 +90,11 @@ def test_attend_names_head_sizes_it_does_not_take():
     q = torch.zeros(1, 4, 96, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="64 or 128"):
         cache.attend(0, q, torch.zeros_like(q))
+
+
+def test_the_caches_workspace_of_the_longest_sequences():
+    # the last page of the longest row ends past what attention takes
+    longest = 2 ** 31 - 1 - 64
+    cache = small_cache(max_length=longest, page_size=1024, max_sequences=1)
+    held = cache._attention_workspace(3, 8).numel()
+    assert held >= _hip.paged_attention_workspace_bytes(3, 8, 2, 64, longest)
