@@ -23,7 +23,8 @@ struct AppendArgs {
   const uint16_t *q, *k, *v;  // token t, head h at t * token + h * head
   int64_t q_token, q_head, k_token, k_head, v_token, v_head;
   const int32_t *positions;
-  const int32_t *rows;  // nullable: token t belongs to table row t
+  const int32_t *turns;  // nullable: the rope tables' row, where not the position
+  const int32_t *rows;   // nullable: token t belongs to table row t
   const int32_t *table;
   int64_t table_stride;
   int64_t sequences;
@@ -57,9 +58,10 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs
   const int64_t pos = a.positions[t];
   const int64_t row = a.rows != nullptr ? a.rows[t] : t;
   if (pos < 0 || row < 0) return;  // a padding token
+  const int64_t turn_row = a.turns != nullptr ? a.turns[t] : pos;
   const int64_t slot_page = pos >> a.page_shift;
   bool ok = row < a.sequences && slot_page < a.max_pages &&
-            (a.rope_dim == 0 || pos < a.rope_positions);
+            (a.rope_dim == 0 || (turn_row >= 0 && turn_row < a.rope_positions));
   const int64_t page = ok ? a.table[row * a.table_stride + slot_page] : -1;
   ok = page >= 0 && page < a.num_pages;
   if (!ok) {
@@ -96,8 +98,8 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs
     u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + d0));
     u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + d1));
     if (turn) {
-      const u32x4 c = *reinterpret_cast<const u32x4 *>(a.cos + pos * half + 8 * part);
-      const u32x4 s = *reinterpret_cast<const u32x4 *>(a.sin + pos * half + 8 * part);
+      const u32x4 c = *reinterpret_cast<const u32x4 *>(a.cos + turn_row * half + 8 * part);
+      const u32x4 s = *reinterpret_cast<const u32x4 *>(a.sin + turn_row * half + 8 * part);
       if (a.interleaved) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -545,12 +547,13 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyPagesArgs 
 
 using namespace cascade;
 
-extern "C" int cascade_paged_append_bf16(
+extern "C" int cascade_paged_append_turned_bf16(
     const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
     int64_t k_token_stride, int64_t k_head_stride, const void *v,
     int64_t v_token_stride, int64_t v_head_stride, int64_t tokens,
     int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
-    const int32_t *positions, const int32_t *rows, const int32_t *page_table,
+    const int32_t *positions, const int32_t *turns, const int32_t *rows,
+    const int32_t *page_table,
     int64_t table_stride, int64_t sequences, int64_t max_pages,
     const void *rope_cos, const void *rope_sin, int64_t rope_positions,
     int64_t rope_dim, int interleaved, void *q_out, int64_t q_out_token_stride,
@@ -585,6 +588,7 @@ extern "C" int cascade_paged_append_bf16(
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(rope_cos) ||
       !aligned16(rope_sin) || !aligned16(q_out) || !aligned16(k_pages) ||
       !aligned16(v_pages) || (reinterpret_cast<uintptr_t>(positions) & 3) ||
+      (reinterpret_cast<uintptr_t>(turns) & 3) ||
       (reinterpret_cast<uintptr_t>(rows) & 3) ||
       (reinterpret_cast<uintptr_t>(page_table) & 3) ||
       (reinterpret_cast<uintptr_t>(error_flag) & 3))
@@ -605,6 +609,7 @@ extern "C" int cascade_paged_append_bf16(
   a.v_token = v_token_stride;
   a.v_head = v_head_stride;
   a.positions = positions;
+  a.turns = turns;
   a.rows = rows;
   a.table = page_table;
   a.table_stride = table_stride;
@@ -630,6 +635,27 @@ extern "C" int cascade_paged_append_bf16(
   return launch_kernel(paged_append_kernel, dim3(static_cast<unsigned>(tokens)),
                        dim3(static_cast<unsigned>(threads)),
                        0, static_cast<hipStream_t>(stream), a);
+}
+
+extern "C" int cascade_paged_append_bf16(
+    const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
+    int64_t k_token_stride, int64_t k_head_stride, const void *v,
+    int64_t v_token_stride, int64_t v_head_stride, int64_t tokens,
+    int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+    const int32_t *positions, const int32_t *rows, const int32_t *page_table,
+    int64_t table_stride, int64_t sequences, int64_t max_pages,
+    const void *rope_cos, const void *rope_sin, int64_t rope_positions,
+    int64_t rope_dim, int interleaved, void *q_out, int64_t q_out_token_stride,
+    int64_t q_out_head_stride, void *k_pages, void *v_pages, int64_t page_stride,
+    int64_t page_head_stride, int64_t num_pages, int64_t page_size,
+    int32_t *error_flag, void *stream) {
+  return cascade_paged_append_turned_bf16(
+      q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v,
+      v_token_stride, v_head_stride, tokens, n_q_heads, n_kv_heads, head_dim, positions,
+      nullptr, rows, page_table, table_stride, sequences, max_pages, rope_cos, rope_sin,
+      rope_positions, rope_dim, interleaved, q_out, q_out_token_stride, q_out_head_stride,
+      k_pages, v_pages, page_stride, page_head_stride, num_pages, page_size, error_flag,
+      stream);
 }
 
 extern "C" size_t cascade_paged_attention_workspace_bytes(int64_t batch,

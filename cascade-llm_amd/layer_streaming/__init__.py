@@ -8,9 +8,15 @@ nothing here falls back to other device code.
 
 from ._hip import (
     copy_pages,
+    gate_up_swiglu_w4,
+    linear_w4,
+    linear_w4_workspace_bytes,
     paged_append,
     paged_attention_workspace_bytes,
     paged_decode_attention,
+    paged_tree_accept,
+    paged_tree_attention,
+    paged_tree_attention_workspace_bytes,
     sample,
     sample_workspace_bytes,
 )
@@ -32,7 +38,9 @@ from .plan import (
     build_llama31_8b_plan,
 )
 from .runtime import DoubleBufferRuntime, ResidentDeviceArena, ResidentTransformerRuntime
+from .tree import tree_masks
 from .vocab import VocabStreamingRuntime, merge_topk
+from .w4 import W4Matrix
 from .weight_store import (
     FullPinnedWeightStore,
     PinnedStagingWeightStore,
@@ -59,14 +67,22 @@ __all__ = [
     "TransferUnit",
     "VocabPlan",
     "VocabStreamingRuntime",
+    "W4Matrix",
     "WeightStoreMode",
     "build_llama31_8b_plan",
     "copy_pages",
     "create_weight_store",
+    "gate_up_swiglu_w4",
+    "linear_w4",
+    "linear_w4_workspace_bytes",
     "merge_topk",
     "paged_append",
     "paged_attention_workspace_bytes",
     "paged_decode_attention",
+    "paged_tree_accept",
+    "paged_tree_attention",
+    "paged_tree_attention_workspace_bytes",
     "sample",
     "sample_workspace_bytes",
+    "tree_masks",
 ]

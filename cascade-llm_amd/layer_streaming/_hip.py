@@ -13,11 +13,14 @@ entry point raises :class:`HipLibraryError`.
 """
 
 import ctypes
+import operator
 import os
 import threading
 import weakref
 
 import torch
+
+from .w4 import W4Matrix
 
 __all__ = [
     "HipLibraryError",
@@ -112,6 +115,12 @@ _SIGNATURES = {
          _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _INT, _P, _I64, _I64,
          _P, _P, _I64, _I64, _I64, _I64, _P, _P],
     ),
+    "cascade_paged_append_turned_bf16": (
+        _INT,
+        [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64,
+         _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _INT, _P, _I64,
+         _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _P],
+    ),
     "cascade_paged_attention_workspace_bytes": (
         _SZ, [_I64, _I64, _I64, _I64, _I64]),
     "cascade_paged_decode_attention_bf16": (
@@ -121,6 +130,32 @@ _SIGNATURES = {
     ),
     "cascade_copy_pages": (
         _INT, [_P, _I64, _I64, _I64, _I64, _P, _I64, _P, _P]),
+    "cascade_paged_tree_attention_workspace_bytes": (
+        _SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "cascade_paged_tree_attention_bf16": (
+        _INT,
+        [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64,
+         _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _F, _P, _I64,
+         _I64, _P, _SZ, _P, _P],
+    ),
+    "cascade_paged_tree_accept": (
+        _INT,
+        [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64,
+         _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P],
+    ),
+    "cascade_linear_w4_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "cascade_linear_w4_bf16": (
+        _INT,
+        [_P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P,
+         _SZ, _P],
+    ),
+    "cascade_linear_w4_f32out_bf16": (
+        _INT,
+        [_P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _SZ, _P]),
+    "cascade_gate_up_swiglu_w4_bf16": (
+        _INT,
+        [_P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64,
+         _P]),
     "cascade_sample_workspace_bytes": (_SZ, [_I64, _I64]),
     "cascade_sample_f32": (
         _INT,
@@ -151,7 +186,7 @@ _SIGNATURES = {
     "cascade_time_next_launch": (_INT, [_U64, _U64]),
 }
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 ESHAPE = 1003  # CASCADE_ESHAPE
 # fused decode attention: sync buffer size and the bits it ors into the
 # caller's error word (include/cascade_hip.h)
@@ -1032,7 +1067,7 @@ def _call_on(index, stream, name, *args):
 
 
 def _check_append(q, k, v, positions, k_pages, v_pages, page_table, rows, rope,
-                  q_out, error_flag):
+                  q_out, rope_at, error_flag):
     """The checks of paged_append; returns the strides of q, k, v, q_out, the
     pools and the table."""
 
@@ -1074,13 +1109,15 @@ def _check_append(q, k, v, positions, k_pages, v_pages, page_table, rows, rope,
             raise ValueError("rope cos and sin differ in shape")
         if not (cos.is_contiguous() and sin.is_contiguous()):
             raise ValueError("the rope tables must be contiguous")
+    if rope_at is not None:
+        _vector(device, "rope_at", rope_at, torch.int32, tokens)
     _check_error_word(device, error_flag)
     return q_strides, _strides("k", k), _strides("v", v), out_strides, pool, table_stride
 
 
 def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
                  rope=None, interleaved=False, q_out=None, error_flag=None,
-                 stream=None):
+                 stream=None, rope_at=None):
     """Rotate projected rows by their positions and write K and V into pages.
 
     ``q`` [tokens, heads, dim] (or None), ``k`` and ``v`` [tokens, kv_heads,
@@ -1089,8 +1126,10 @@ def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
     or row marks padding, of which nothing is written.  ``rope``: (cos, sin)
     tables, bf16 [positions, r / 2]; the first r dims of a head turn, in pairs
     (i, i + r / 2) or, ``interleaved``, (2 i, 2 i + 1).  None copies the rows
-    as they are.  ``q_out`` (q itself by default; none of its rows may be
-    another's q, k or v) receives the rotated q rows and is returned.  Pools
+    as they are; ``rope_at`` (int32 [tokens]) gives the tables' rows where they
+    are not the positions (a drafted tree's depths).  ``q_out`` (q itself by
+    default; none of its rows may be another's q, k or v) receives the rotated
+    q rows and is returned.  Pools
     are [pages, kv_heads, page_size, dim] views, ``page_table`` int32
     [sequences, pages of one].  An index out of range leaves its token out
     and ors PAGED_ERANGE into ``error_flag``."""
@@ -1122,6 +1161,9 @@ def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
             and (tokens <= sequences if rows is None else (
                 rows.dtype is _I32 and rows.get_device() == index
                 and rows.shape == (tokens,) and rows.is_contiguous()))
+            and (rope_at is None or (
+                rope_at.dtype is _I32 and rope_at.get_device() == index
+                and rope_at.shape == (tokens,) and rope_at.is_contiguous()))
             and (error_flag is None or (
                 error_flag.dtype is _I32 and error_flag.get_device() == index
                 and error_flag.numel() > 0)))
@@ -1156,7 +1198,7 @@ def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
     else:
         q_strides, k_strides, v_strides, out_strides, pool, table_stride = _check_append(
             q, k, v, positions, k_pages, v_pages, page_table, rows, rope, q_out,
-            error_flag)
+            rope_at, error_flag)
         index = k.get_device()
         tokens, kv_heads, dim = k.shape
         pages, _, page_size, _ = k_pages.shape
@@ -1165,17 +1207,22 @@ def paged_append(q, k, v, positions, k_pages, v_pages, page_table, rows=None,
         rope_positions, half = (0, 0) if rope is None else cos.shape
         if tokens == 0:
             return q_out
-    _call_on(
-        index, stream, "cascade_paged_append_bf16",
+    rotated = (
         0 if q is None else q.data_ptr(), q_strides[0], q_strides[1], k.data_ptr(),
         k_strides[0], k_strides[1], v.data_ptr(), v_strides[0], v_strides[1], tokens,
-        q_heads, kv_heads, dim, positions.data_ptr(),
+        q_heads, kv_heads, dim, positions.data_ptr())
+    placed = (
         0 if rows is None else rows.data_ptr(), page_table.data_ptr(), table_stride,
         sequences, max_pages, 0 if rope is None else cos.data_ptr(),
         0 if rope is None else sin.data_ptr(), rope_positions, 2 * half,
         1 if interleaved else 0, 0 if q is None else q_out.data_ptr(), out_strides[0],
         out_strides[1], k_pages.data_ptr(), v_pages.data_ptr(), pool[0], pool[1], pages,
         page_size, 0 if error_flag is None else error_flag.data_ptr())
+    if rope_at is None:
+        _call_on(index, stream, "cascade_paged_append_bf16", *rotated, *placed)
+    else:
+        _call_on(index, stream, "cascade_paged_append_turned_bf16", *rotated,
+                 rope_at.data_ptr(), *placed)
     return q_out
 
 
@@ -1336,6 +1383,227 @@ def copy_pages(pages, pairs, error_flag=None, stream=None):
     return pages
 
 
+def _count(name, value, low, high):
+    """An integer of a range."""
+
+    value = operator.index(value)
+    if not low <= value <= high:
+        raise ValueError("{} {} is outside [{}, {}]".format(name, value, low, high))
+    return value
+
+
+def paged_tree_attention_workspace_bytes(trees, max_tree, n_q_heads, n_kv_heads,
+                                         head_dim, max_length):
+    """Workspace bytes of paged_tree_attention for up to ``trees`` trees of up
+    to ``max_tree`` nodes over sequences of up to ``max_length`` positions."""
+
+    size = load().cascade_paged_tree_attention_workspace_bytes(
+        int(trees), int(max_tree), int(n_q_heads), int(n_kv_heads), int(head_dim),
+        int(max_length))
+    if size == 0:
+        raise ValueError("unsupported tree attention shape")
+    return int(size)
+
+
+def _check_tree_attention(q, starts, masks, k_pages, v_pages, page_table, lengths,
+                          out, workspace, rows, error_flag):
+    """The checks of paged_tree_attention; returns the strides of q, out, the
+    pools and the table."""
+
+    device = _gpu_of("q", q)
+    _placed(device, "q", q, torch.bfloat16, 3)
+    tokens, _, dim = q.shape
+    _placed(device, "starts", starts, torch.int32, 1)
+    trees = starts.shape[0] - 1
+    if trees < 0:
+        raise ValueError("starts holds one entry more than there are trees")
+    _vector(device, "starts", starts, torch.int32, trees + 1)
+    _vector(device, "masks", masks, torch.int64, tokens)
+    pool = _page_pools(device, k_pages, v_pages)
+    if k_pages.shape[3] != dim:
+        raise ValueError("the pools hold heads of {}, q of {}".format(
+            k_pages.shape[3], dim))
+    _placed(device, "out", out, torch.bfloat16, 3)
+    if out.shape != q.shape:
+        raise ValueError("out and q differ in shape")
+    _apart("out", out)
+    table_stride = _table_stride(device, page_table)
+    sequences = page_table.shape[0]
+    _vector(device, "lengths", lengths, torch.int32, sequences)
+    if rows is not None:
+        _vector(device, "rows", rows, torch.int32, trees)
+    elif trees > sequences:
+        raise ValueError("more trees than page table rows (give rows)")
+    _check_bytes(device, workspace)
+    _check_error_word(device, error_flag)
+    return _strides("q", q), _strides("out", out), pool, table_stride
+
+
+def paged_tree_attention(q, starts, masks, k_pages, v_pages, page_table, lengths,
+                         out, workspace, scale, rows=None, max_tree=64,
+                         max_length=None, error_flag=None, stream=None):
+    """GQA attention of drafted trees' nodes over their sequences' pages.
+
+    ``q`` and ``out`` [tokens, heads, dim]; tree b has the rows ``starts[b]``
+    .. ``starts[b + 1]`` - 1 (int32 [trees + 1]; up to ``max_tree`` of them, 64
+    at most) and is the last of the ``lengths[r]`` positions of page table row
+    r = ``rows[b]`` (b without ``rows``; negative: padding).  A node reads
+    all positions before its tree, and of the tree the nodes j whose bit j is
+    set in its ``masks`` (int64 [tokens], see tree_masks).  A node that sees
+    nothing gives zeros; rows of no tree stay as they are.  Lengths count the
+    tree's nodes and are at most ``max_length`` (default: what a table row
+    holds).  A tree out of range is left out and flagged, as are positions on a
+    page outside the pool (PAGED_ERANGE in ``error_flag``).  ``workspace``:
+    paged_tree_attention_workspace_bytes(...) uint8, one each for calls that may
+    overlap."""
+
+    try:
+        index = q.get_device()
+        q_strides, pool = q.stride(), k_pages.stride()
+        table_stride, table_last = page_table.stride()
+        tokens, q_heads, dim = shape = q.shape
+        trees = starts.shape[0] - 1
+        pages, kv_heads, page_size, pool_dim = pool_shape = k_pages.shape
+        sequences, width = page_table.shape
+        ordinary = (
+            tokens > 0 and trees > 0 and pages > 1 and index >= 0
+            and v_pages.shape == pool_shape and pool_dim == dim
+            and v_pages.stride() == pool and out.shape == shape
+            and q_strides[2] == pool[3] == table_last == 1 and pool[2] == dim
+            and table_stride >= width
+            and q.dtype is _BF16 and k_pages.dtype is _BF16 and v_pages.dtype is _BF16
+            and out.dtype is _BF16 and page_table.dtype is _I32
+            and starts.dtype is _I32 and masks.dtype is _LONG
+            and lengths.dtype is _I32 and workspace.dtype is _U8
+            and index == k_pages.get_device() == v_pages.get_device()
+            == out.get_device() == page_table.get_device() == lengths.get_device()
+            == workspace.get_device() == starts.get_device() == masks.get_device()
+            and starts.dim() == 1 and starts.is_contiguous()
+            and masks.shape == (tokens,) and masks.is_contiguous()
+            and lengths.shape == (sequences,) and lengths.is_contiguous()
+            and (trees <= sequences if rows is None else (
+                rows.dtype is _I32 and rows.get_device() == index
+                and rows.shape == (trees,) and rows.is_contiguous()))
+            and out.is_contiguous()
+            and workspace.dim() == 1 and workspace.is_contiguous()
+            and (error_flag is None or (
+                error_flag.dtype is _I32 and error_flag.get_device() == index
+                and error_flag.numel() > 0)))
+    except (AttributeError, IndexError, TypeError, ValueError, RuntimeError):
+        ordinary = False
+    if ordinary:
+        # (the stride of a dimension of one says nothing)
+        q_strides = (q_strides[0] if tokens > 1 else 0, q_strides[1] if q_heads > 1 else 0)
+        out_strides = (q_heads * dim, dim)
+        if kv_heads == 1:
+            pool = (pool[0], page_size * dim)
+    else:
+        q_strides, out_strides, pool, table_stride = _check_tree_attention(
+            q, starts, masks, k_pages, v_pages, page_table, lengths, out, workspace,
+            rows, error_flag)
+        index = q.get_device()
+        tokens, q_heads, dim = q.shape
+        trees = starts.shape[0] - 1
+        pages, kv_heads, page_size, _ = k_pages.shape
+        sequences, width = page_table.shape
+    max_tree = _count("max_tree", max_tree, 1, 64)
+    if max_length is None:
+        max_length = width * page_size
+    elif not 0 < max_length <= width * page_size:
+        raise ValueError("max_length {} is outside the page table's {}".format(
+            max_length, width * page_size))
+    if tokens == 0 or trees == 0:
+        return out
+    _call_on(
+        index, stream, "cascade_paged_tree_attention_bf16", q.data_ptr(),
+        q_strides[0], q_strides[1], tokens, starts.data_ptr(), masks.data_ptr(), trees,
+        max_tree, k_pages.data_ptr(), v_pages.data_ptr(), pool[0], pool[1], pages,
+        page_size, page_table.data_ptr(), table_stride, sequences, lengths.data_ptr(),
+        0 if rows is None else rows.data_ptr(), int(max_length), q_heads, kv_heads, dim,
+        scale, out.data_ptr(), out_strides[0], out_strides[1], workspace.data_ptr(),
+        workspace.numel(), 0 if error_flag is None else error_flag.data_ptr())
+    return out
+
+
+def paged_tree_accept(starts, ids, parents, targets, path, counts, next_ids,
+                      pages=None, page_table=None, lengths=None, rows=None,
+                      error_flag=None, stream=None):
+    """Follow the drawn tokens through drafted trees, and keep the K and V rows
+    of the nodes on their paths.
+
+    Tree b has the rows ``starts[b]`` .. ``starts[b + 1]`` - 1 (int32 [trees +
+    1]); of each row ``ids`` (int64 [tokens]) is the node's own token,
+    ``parents`` (int32 [tokens]) its parent's place in the tree, before its
+    own, and ``targets`` (int64 [tokens]) the token drawn there.  From node 0 on, the
+    path goes to the first child whose own token is the one drawn.  ``path``
+    (int32 [trees, max_tree], max_tree <= 64) lists its nodes, -1 behind them;
+    ``counts`` (int32 [trees]) their number, ``next_ids`` (int64 [trees]) the
+    token drawn at the last.  No nodes, a negative ``rows[b]`` and a tree out
+    of range: 0 and -1.
+
+    ``pages``: a contiguous pool [layers, 2, pages, kv_heads, page_size, dim]
+    whose rows of the path move to the front of the tree, the j-th node's to
+    position lengths[r] - n + j of page table row r = ``rows[b]`` (b without
+    ``rows``; no row twice) with n nodes.  Rows, lengths and pages out of range
+    are left out and flagged (PAGED_ERANGE in ``error_flag``).  Returns
+    ``path``."""
+
+    device = _gpu_of("starts", starts)
+    _placed(device, "starts", starts, _I32, 1)
+    trees = starts.shape[0] - 1
+    if trees < 0:
+        raise ValueError("starts holds one entry more than there are trees")
+    _vector(device, "starts", starts, _I32, trees + 1)
+    _placed(device, "ids", ids, _LONG, 1)
+    tokens = ids.shape[0]
+    _vector(device, "ids", ids, _LONG, tokens)
+    _vector(device, "parents", parents, _I32, tokens)
+    _vector(device, "targets", targets, _LONG, tokens)
+    _placed(device, "path", path, _I32, 2)
+    if path.shape[0] != trees or not path.is_contiguous():
+        raise ValueError("path must be contiguous [{}, max_tree]".format(trees))
+    max_tree = _count("path's width", path.shape[1], 1, 64)
+    _vector(device, "counts", counts, _I32, trees)
+    _vector(device, "next_ids", next_ids, _LONG, trees)
+    if rows is not None:
+        _vector(device, "rows", rows, _I32, trees)
+    _check_error_word(device, error_flag)
+    planes = plane_bytes = count = kv_heads = page_size = row_bytes = 0
+    table_stride = sequences = width = 0
+    if pages is not None:
+        _placed(device, "pages", pages, _BF16, 6)
+        if not pages.is_contiguous() or pages.shape[1] != 2:
+            raise ValueError("pages must be contiguous [layers, 2, pages, kv_heads, "
+                             "page_size, dim]")
+        layers, _, count, kv_heads, page_size, dim = pages.shape
+        planes, row_bytes = 2 * layers, 2 * dim
+        plane_bytes = count * kv_heads * page_size * row_bytes
+        table_stride = _table_stride(device, page_table)
+        sequences, width = page_table.shape
+        _vector(device, "lengths", lengths, _I32, sequences)
+        if rows is None and trees > sequences:
+            raise ValueError("more trees than page table rows (give rows)")
+    elif page_table is not None or lengths is not None:
+        raise ValueError("page_table and lengths without pages")
+    if trees == 0:
+        return path
+    if tokens == 0:
+        path.fill_(-1)
+        counts.zero_()
+        next_ids.fill_(-1)
+        return path
+    _call_on(
+        device.index, stream, "cascade_paged_tree_accept", starts.data_ptr(),
+        ids.data_ptr(), parents.data_ptr(), targets.data_ptr(), tokens, trees, max_tree,
+        path.data_ptr(), counts.data_ptr(), next_ids.data_ptr(),
+        0 if pages is None else pages.data_ptr(), planes, plane_bytes, count, kv_heads,
+        page_size, row_bytes, 0 if pages is None else page_table.data_ptr(),
+        table_stride, sequences, width, 0 if pages is None else lengths.data_ptr(),
+        0 if rows is None else rows.data_ptr(),
+        0 if error_flag is None else error_flag.data_ptr())
+    return path
+
+
 def sample_workspace_bytes(rows, vocab):
     """Workspace bytes of sample for up to ``rows`` rows of up to ``vocab``
     logits."""
@@ -1398,6 +1666,119 @@ def sample(logits, uniform, ids, workspace, temperature=1.0, top_k=0, top_p=1.0,
              0 if logprobs is None else logprobs.data_ptr(), workspace.data_ptr(),
              workspace.numel())
     return ids
+
+
+# ------------------------------------------------------------- 4-bit weights
+
+
+def linear_w4_workspace_bytes(rows, n, k):
+    """Workspace bytes of linear_w4 for ``rows`` rows of ``k`` values times a
+    matrix of ``n`` rows (may be 0: none is needed)."""
+
+    return int(load().cascade_linear_w4_workspace_bytes(int(rows), int(n), int(k)))
+
+
+def _row_stride(device, name, tensor, dtype, shape):
+    """The row stride of a [rows, columns] view with contiguous rows."""
+
+    _placed(device, name, tensor, dtype, 2)
+    if shape is not None and tensor.shape != shape:
+        raise ValueError("{} has shape {}, expected {}".format(
+            name, tuple(tensor.shape), tuple(shape)))
+    rows, columns = tensor.shape
+    stride, last = tensor.stride()
+    if columns > 1 and last != 1:
+        raise ValueError("the rows of {} must be contiguous".format(name))
+    if rows == 1:
+        return columns
+    return stride
+
+
+def _w4_matrix(name, matrix):
+    if not isinstance(matrix, W4Matrix):
+        raise TypeError("{} must be a W4Matrix".format(name))
+
+
+def _w4_pointers(device, name, matrix, k):
+    if matrix.packed.device != device:
+        raise ValueError("{} must live on {}, got {}".format(
+            name, device, matrix.packed.device))
+    if matrix.k != k:
+        raise ValueError("{} has {} columns, x {}".format(name, matrix.k, k))
+    return (matrix.packed.data_ptr(), matrix.scales.data_ptr(),
+            0 if matrix.zeros is None else matrix.zeros.data_ptr())
+
+
+def _w4_rows(x, out, dtype, n):
+    """Checks x and out of a 4-bit product; returns (device, m, k, strides)."""
+
+    device = _gpu_of("x", x)
+    x_stride = _row_stride(device, "x", x, _BF16, None)
+    m, k = x.shape
+    y_stride = _row_stride(device, "out", out, dtype, (m, n))
+    if m > 1 and y_stride < n:
+        raise ValueError("the rows of out overlap")
+    if m and x.data_ptr() == out.data_ptr():
+        raise ValueError("out may not be x")
+    if m == 1:
+        x_stride = (k + 7) // 8 * 8
+    return device, m, k, x_stride, y_stride
+
+
+def linear_w4(x, matrix, out, residual=None, workspace=None, stream=None):
+    """out = x W^T (+ residual) for a W4Matrix [n, k].
+
+    ``x`` bf16 [rows, k] (row stride a multiple of 8), ``out`` [rows, n] bf16,
+    or fp32 for rows that are not rounded (logits; without residual), ``residual`` bf16
+    [rows, n], which may be ``out``.  Sums are fp32, with one rounding at the
+    end.  ``workspace``: linear_w4_workspace_bytes(rows, n, k) uint8, one each for
+    calls that may overlap; None where that is 0."""
+
+    _w4_matrix("matrix", matrix)
+    logits = isinstance(out, torch.Tensor) and out.dtype is _F32
+    device, m, k, x_stride, y_stride = _w4_rows(x, out, _F32 if logits else _BF16,
+                                                matrix.n)
+    packed, scales, zeros = _w4_pointers(device, "matrix", matrix, k)
+    residual_stride = 0
+    if residual is not None:
+        if logits:
+            raise ValueError("fp32 rows take no residual")
+        residual_stride = _row_stride(device, "residual", residual, _BF16, out.shape)
+    if workspace is not None:
+        _check_bytes(device, workspace)
+    if m == 0:
+        return out
+    space = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+    if logits:
+        _call_on(device.index, stream, "cascade_linear_w4_f32out_bf16", x.data_ptr(),
+                 x_stride, packed, scales, zeros, m, matrix.n, k, matrix.group,
+                 out.data_ptr(), y_stride, *space)
+    else:
+        _call_on(device.index, stream, "cascade_linear_w4_bf16", x.data_ptr(),
+                 x_stride, packed, scales, zeros, m, matrix.n, k, matrix.group,
+                 0 if residual is None else residual.data_ptr(), residual_stride,
+                 out.data_ptr(), y_stride, *space)
+    return out
+
+
+def gate_up_swiglu_w4(x, gate, up, out, stream=None):
+    """out = silu(x Wg^T) * (x Wu^T) for two W4Matrix [n, k] of one group size,
+    both with zero points or neither; ``x`` bf16 [rows, k], ``out`` bf16
+    [rows, n].  Sums are fp32, with one rounding at the end."""
+
+    _w4_matrix("gate", gate)
+    _w4_matrix("up", up)
+    device, m, k, x_stride, y_stride = _w4_rows(x, out, _BF16, gate.n)
+    gate_pointers = _w4_pointers(device, "gate", gate, k)
+    up_pointers = _w4_pointers(device, "up", up, k)
+    if (up.n, up.group, up.zeros is None) != (gate.n, gate.group, gate.zeros is None):
+        raise ValueError("gate and up differ in rows, group size or zero points")
+    if m == 0:
+        return out
+    _call_on(device.index, stream, "cascade_gate_up_swiglu_w4_bf16", x.data_ptr(),
+             x_stride, *gate_pointers, *up_pointers, m, gate.n, k, gate.group,
+             out.data_ptr(), y_stride)
+    return out
 
 
 # ------------------------------------------------------------ copy pipeline

@@ -9,7 +9,8 @@ its copies, and a page is copied only when one of them writes to it.
 The host decides which page holds what (this class); the device holds the
 pages, the page table and the lengths, and the kernels of libcascade_hip
 read them there: ``append`` (cascade_paged_append_bf16), ``attend``
-(cascade_paged_decode_attention_bf16) and the copies of ``extend`` and
+(cascade_paged_decode_attention_bf16), ``attend_tree`` and ``accept`` of drafted
+trees (cascade_paged_tree_attention_bf16, _accept) and the copies of ``extend`` and
 ``compact`` (cascade_copy_pages).  Table, lengths and pools never move, so a
 captured graph of a decode step serves every later step: ``extend`` makes room and
 updates them in place.  It, and whatever else assigns pages, refuses to run
@@ -268,13 +269,13 @@ class PagedKVCache:
         return self.buffer[layer, 1]
 
     def append(self, layer, q, k, v, positions, rows=None, rope=None,
-               interleaved=False, q_out=None):
+               interleaved=False, q_out=None, rope_at=None):
         """``paged_append`` into one layer's pages."""
 
         return _hip.paged_append(
             q, k, v, positions, self.buffer[layer, 0], self.buffer[layer, 1],
             self.page_table, rows=rows, rope=rope, interleaved=interleaved,
-            q_out=q_out, error_flag=self.error)
+            q_out=q_out, error_flag=self.error, rope_at=rope_at)
 
     def attend(self, layer, q, out, rows=None, scale=None, workspace=None,
                max_length=None):
@@ -295,12 +296,47 @@ class PagedKVCache:
             self.head_dim ** -0.5 if scale is None else scale, rows=rows,
             max_length=limit, error_flag=self.error)
 
+    def attend_tree(self, layer, q, starts, masks, out, rows=None, scale=None,
+                    workspace=None, max_tree=64, max_length=None):
+        """``paged_tree_attention`` over one layer's pages (heads of 64 or 128):
+        ``extend`` the sequences by their trees' nodes and ``append`` them
+        first.  ``scale`` and ``workspace`` as for ``attend``."""
+
+        if self.head_dim not in (64, 128):
+            raise ValueError("attention takes heads of 64 or 128, these have {}".format(
+                self.head_dim))
+        limit = self.max_length if max_length is None else max_length
+        if workspace is None:
+            workspace = self._workspace(_hip.paged_tree_attention_workspace_bytes(
+                max(starts.shape[0] - 1, 1), max_tree, q.shape[1], self.num_kv_heads,
+                self.head_dim, self._most_positions()))
+        return _hip.paged_tree_attention(
+            q, starts, masks, self.buffer[layer, 0], self.buffer[layer, 1],
+            self.page_table, self.lengths, out, workspace,
+            self.head_dim ** -0.5 if scale is None else scale, rows=rows,
+            max_tree=max_tree, max_length=limit, error_flag=self.error)
+
+    def accept(self, starts, ids, parents, targets, path, counts, next_ids, rows=None):
+        """``paged_tree_accept`` in every layer's pages.  The sequences keep
+        their length: ``truncate`` them to that of their past and
+        ``counts`` once the host knows these."""
+
+        return _hip.paged_tree_accept(
+            starts, ids, parents, targets, path, counts, next_ids, pages=self.buffer,
+            page_table=self.page_table, lengths=self.lengths, rows=rows,
+            error_flag=self.error)
+
+    def _most_positions(self):
+        # any limit that a call may give: what a table row holds, and the
+        # operators take
+        return min(self.max_pages * self.page_size, 0x7fffffff - 64)
+
     def _attention_workspace(self, batch, q_heads):
-        # for any limit that a call may give: what a table row holds, and the
-        # operator takes
-        limit = min(self.max_pages * self.page_size, 0x7fffffff - 64)
-        need = _hip.paged_attention_workspace_bytes(
-            max(batch, 1), q_heads, self.num_kv_heads, self.head_dim, limit)
+        return self._workspace(_hip.paged_attention_workspace_bytes(
+            max(batch, 1), q_heads, self.num_kv_heads, self.head_dim,
+            self._most_positions()))
+
+    def _workspace(self, need):
         if not self._workspaces or self._workspaces[-1].numel() < need:
             self._workspaces.append(
                 torch.empty(need, dtype=torch.uint8, device=self.device))

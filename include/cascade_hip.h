@@ -39,8 +39,13 @@ extern "C" {
    cascade_gemm_workspace_bytes added.  6: the paged KV cache
    (cascade_paged_append_bf16, cascade_paged_decode_attention_bf16,
    cascade_paged_attention_workspace_bytes, cascade_copy_pages) and sampling
-   (cascade_sample_f32, cascade_sample_workspace_bytes) added. */
-#define CASCADE_ABI_VERSION 6
+   (cascade_sample_f32, cascade_sample_workspace_bytes) added.  7: drafted
+   trees (cascade_paged_append_turned_bf16, cascade_paged_tree_attention_bf16,
+   cascade_paged_tree_attention_workspace_bytes, cascade_paged_tree_accept)
+   and products with 4-bit weights (cascade_linear_w4_bf16,
+   cascade_linear_w4_f32out_bf16, cascade_linear_w4_workspace_bytes,
+   cascade_gate_up_swiglu_w4_bf16) added. */
+#define CASCADE_ABI_VERSION 7
 
 /* Argument errors (no work enqueued). */
 #define CASCADE_EINVAL 1001     /* null pointer, bad size or count */
@@ -355,6 +360,23 @@ int cascade_paged_append_bf16(
     int64_t q_out_head_stride, void *k_pages, void *v_pages, int64_t page_stride,
     int64_t page_head_stride, int64_t num_pages, int64_t page_size,
     int32_t *error_flag, void *stream);
+/* The same with row turns[t] of the rope tables for token t (turns null:
+ * positions[t]), for tokens whose place in the text is not their place in
+ * the cache, as a drafted tree's.  A turns[t] outside the tables leaves the
+ * token out whole and is flagged.                                          */
+int cascade_paged_append_turned_bf16(
+    const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
+    int64_t k_token_stride, int64_t k_head_stride, const void *v,
+    int64_t v_token_stride, int64_t v_head_stride, int64_t tokens,
+    int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+    const int32_t *positions, const int32_t *turns, const int32_t *rows,
+    const int32_t *page_table,
+    int64_t table_stride, int64_t sequences, int64_t max_pages,
+    const void *rope_cos, const void *rope_sin, int64_t rope_positions,
+    int64_t rope_dim, int interleaved, void *q_out, int64_t q_out_token_stride,
+    int64_t q_out_head_stride, void *k_pages, void *v_pages, int64_t page_stride,
+    int64_t page_head_stride, int64_t num_pages, int64_t page_size,
+    int32_t *error_flag, void *stream);
 /* GQA attention of one query token a sequence: batch row b reads positions
  * [0, lengths[r]) of table row r = rows[b] (rows null: r = b):
  *   out[b, h] = bf16(softmax(q[b, h] . K_g^T * scale) . V_g), g = h / G,
@@ -392,6 +414,123 @@ int cascade_copy_pages(void *pages, int64_t planes, int64_t plane_bytes,
                        int64_t num_pages, int64_t page_bytes,
                        const int32_t *pairs, int64_t count, int32_t *error_flag,
                        void *stream);
+
+/* -------------------------------------------------------- drafted trees
+ * One step that scores several drafted tokens of each sequence.  A draft is a
+ * tree of up to 64 tokens: node 0 is the token drawn last, which no other
+ * node precedes, every other one continues its parent.  Tree b has the rows
+ * starts[b] .. starts[b + 1] - 1 of the step's `tokens` rows (starts: device
+ * int32 [trees + 1]) and belongs to row r = rows[b] of the page table (rows
+ * null: r = b), whose lengths[r] counts the tree's tokens: node i lies at
+ * position lengths[r] - n + i of the n nodes' sequence (write it there with
+ * cascade_paged_append_turned_bf16, at the rope row of its depth).  A negative
+ * row is padding.  A tree whose starts run backwards, outside [0, tokens] or
+ * over max_tree nodes (1..64), whose row is >= sequences, or whose length is
+ * over max_length or below its number of nodes is flagged and left out whole.
+ * No counterpart in the reference, which decodes one token at a time
+ * (tools/run_llama31.py:105-121).
+ *
+ * GQA attention of every node: node i of tree b reads all positions before
+ * the tree, and node j's where bit j of masks[starts[b] + i] is set (device
+ * int64 [tokens]; a tree's are each node's ancestors and the node itself; bits
+ * from n on say nothing):
+ *   out[t, h] = bf16(softmax(q[t, h] . K_g^T * scale) . V_g), g = h / G,
+ * G = n_q_heads / n_kv_heads <= 16, head_dim 64 or 128.  A node that sees
+ * nothing gives zeros.  What a node does not see takes no part whatever it
+ * holds, infinities and NaN among it.  Rows of no tree, of padding and of
+ * trees left out stay as they are.  Positions on a page outside [0,
+ * num_pages) are left out as if masked, and flagged.  The workspace needs no
+ * zero-fill and holds nothing between calls; calls that may overlap need one
+ * each.  Does for trees what cascade_paged_decode_attention_bf16 does for
+ * single tokens.                                                           */
+size_t cascade_paged_tree_attention_workspace_bytes(int64_t trees,
+                                                    int64_t max_tree,
+                                                    int64_t n_q_heads,
+                                                    int64_t n_kv_heads,
+                                                    int64_t head_dim,
+                                                    int64_t max_length);
+int cascade_paged_tree_attention_bf16(
+    const void *q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+    const int32_t *starts, const int64_t *masks, int64_t trees, int64_t max_tree,
+    const void *k_pages, const void *v_pages, int64_t page_stride,
+    int64_t page_head_stride, int64_t num_pages, int64_t page_size,
+    const int32_t *page_table, int64_t table_stride, int64_t sequences,
+    const int32_t *lengths, const int32_t *rows, int64_t max_length,
+    int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim, float scale,
+    void *out, int64_t out_token_stride, int64_t out_head_stride, void *workspace,
+    size_t workspace_bytes, int32_t *error_flag, void *stream);
+/* Follows the drawn tokens through every tree: from node 0 on, the next node
+ * is the first child c of the current one (parents[c], an index in the tree,
+ * is the current node, and c lies behind it) whose ids[c] is targets of the
+ * current node, the token drawn there.  path[b, :] (int32 [trees, max_tree])
+ * lists the nodes in order and -1 behind them, counts[b] is their number,
+ * next_ids[b] the token drawn at the last of them, which no node holds.  A
+ * negative target continues nowhere.  No nodes, padding and a tree whose
+ * starts are out of range: count 0, next -1.  ids, targets: device int64
+ * [tokens]; parents: int32 [tokens].
+ * pages, where not null, are `planes` planes (the K and V pools of every
+ * layer, page p of plane j at pages + j * plane_bytes + p * the bytes of
+ * n_kv_heads * page_size rows of row_bytes, a multiple of 16): the path's
+ * rows move to the front of the tree, the j-th node's to position
+ * lengths[r] - n + j.  The cache's length is then that of the past and the
+ * count.  A row or length out of range moves nothing of the tree, a page
+ * out of range leaves out the rows that it concerns; both are flagged.      */
+int cascade_paged_tree_accept(
+    const int32_t *starts, const int64_t *ids, const int32_t *parents,
+    const int64_t *targets, int64_t tokens, int64_t trees, int64_t max_tree,
+    int32_t *path, int32_t *counts, int64_t *next_ids, void *pages,
+    int64_t planes, int64_t plane_bytes, int64_t num_pages, int64_t n_kv_heads,
+    int64_t page_size, int64_t row_bytes, const int32_t *page_table,
+    int64_t table_stride, int64_t sequences, int64_t max_pages,
+    const int32_t *lengths, const int32_t *rows, int32_t *error_flag,
+    void *stream);
+
+/* ------------------------------------------------------- 4-bit weights
+ * Products of up to any number of rows with a matrix of 4-bit values q and a
+ * bf16 scale for each `group` (32, 64 or 128) consecutive columns of a row:
+ *   W[i, k] = scale[i, k / group] * (q[i, k] - zero[i, k / group]),
+ * zero an integer of 0..15, 8 everywhere where zeros is null.  n rows of K
+ * columns, K a multiple of 8.
+ * packed: tiles of 16 rows and 128 columns, 1 KiB each, tile (i, k) at (i *
+ *   ceil(K / 128) + k) KiB, the matrix padded with any values to whole tiles.
+ *   In a tile the 16 bytes at 16 l hold row l % 16: dword j the columns
+ *   32 j + 8 (l / 16) + 0 .. 7, column 2 a + h of these in the bits from (16 h
+ *   + 4 a + 3) mod 32 on (all eight, half by half, and rotated left by 3).
+ * scales: bf16 [ceil(n / 16)][ceil(K / group)][16], zeros: uint8, alike; what
+ *   lies past row n is read and has to be finite.
+ * Sums are fp32, one rounding at the end: y[r] = bf16(x[r] . W^T +
+ * residual[r]) (residual nullable; y may be the residual, not x).  Strides are
+ * in elements, x's a multiple of 8.  Values of x of 2^120 and more, infinities
+ * and NaN give NaN or infinite rows where finite ones may be meant; other rows
+ * stay as they are.  No counterpart in the reference, whose weights are bf16;
+ * stands beside cascade_gemv_residual_bf16 and cascade_gemm_residual_ws_bf16.
+ * The workspace (cascade_linear_w4_workspace_bytes; 0: none, null is accepted)
+ * needs no zero-fill and holds nothing between calls; calls that may overlap
+ * need one each.                                                           */
+size_t cascade_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int cascade_linear_w4_bf16(const void *x, int64_t x_stride, const void *packed,
+                           const void *scales, const void *zeros, int64_t m,
+                           int64_t n, int64_t k, int64_t group,
+                           const void *residual, int64_t residual_stride,
+                           void *y, int64_t y_stride, void *workspace,
+                           size_t workspace_bytes, void *stream);
+/* The same to fp32 rows that are not rounded (logits). */
+int cascade_linear_w4_f32out_bf16(const void *x, int64_t x_stride,
+                                  const void *packed, const void *scales,
+                                  const void *zeros, int64_t m, int64_t n,
+                                  int64_t k, int64_t group, float *y,
+                                  int64_t y_stride, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+/* y[r] = bf16(silu(x[r] . Wg^T) * (x[r] . Wu^T)), both matrices [n_half, K]
+ * with one group size, both with zeros or neither; one rounding.            */
+int cascade_gate_up_swiglu_w4_bf16(const void *x, int64_t x_stride,
+                                   const void *gate_packed,
+                                   const void *gate_scales,
+                                   const void *gate_zeros,
+                                   const void *up_packed, const void *up_scales,
+                                   const void *up_zeros, int64_t m,
+                                   int64_t n_half, int64_t k, int64_t group,
+                                   void *y, int64_t y_stride, void *stream);
 
 /* ------------------------------------------------------ LM head + top-k
  * One vocabulary chunk: logits[r] = W[r] . h (fp32, not rounded to bf16) for
