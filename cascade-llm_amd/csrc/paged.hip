@@ -177,7 +177,8 @@ paged_attention_kernel(PagedAttnArgs a) {
   int b, len, first, end, count = 1;
   int64_t row;
   if constexpr (SPLIT) {
-    const PagedRun r = find_run(a, run, lane, blockIdx.x == 0 && wave == 0);
+    const PagedRun r = find_run(a, run, lane, blockIdx.x == 0 && wave == 0,
+                                [&](int i, bool flag) { return paged_row(a, i, flag); });
     if (r.b < 0) return;
     b = r.b;
     row = r.row;

@@ -134,13 +134,15 @@ __device__ __forceinline__ int blocks_of(int len) {
 
 // The run's place; `first` (one wave of the launch) also flags what is out of
 // range and writes the plan for the launch that joins the runs.
+// row_of(b, flag): batch row b.
+template <typename RowOf>
 __device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, int lane,
-                                             bool first) {
+                                             bool first, RowOf row_of) {
   // the first 64 rows stay in registers
-  const PagedRow head = paged_row(a, lane, first);
+  const PagedRow head = row_of(lane, first);
   unsigned long long blocks = static_cast<uint32_t>(blocks_of(head.len));
   for (int base = kWave; base < a.batch; base += kWave)
-    blocks += static_cast<uint32_t>(blocks_of(paged_row(a, base + lane, first).len));
+    blocks += static_cast<uint32_t>(blocks_of(row_of(base + lane, first).len));
   blocks = lane_u64(wave_prefix(blocks), kWave - 1);
   // more than blocks / target, in fp64 (no row has more than 2^26 blocks)
   double per_run = static_cast<double>(blocks) * a.per_round;
@@ -150,7 +152,7 @@ __device__ __forceinline__ PagedRun find_run(const PagedAttnArgs &a, int run, in
   PagedRun out{-1, -1, 0, 0, 0, 0};
   int before = 0;
   for (int base = 0; base < a.batch; base += kWave) {
-    const PagedRow r = base == 0 ? head : paged_row(a, base + lane, false);
+    const PagedRow r = base == 0 ? head : row_of(base + lane, false);
     const int mine = r.row < 0 ? 0 : max(1, (blocks_of(r.len) + size - 1) / size);
     const int upto = before + wave_prefix(mine);
     if (first && base + lane < a.batch) {

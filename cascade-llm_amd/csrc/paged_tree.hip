@@ -6,6 +6,8 @@
 // last n of the lengths[row] positions of its sequence: "past" below is what
 // lies before it.  As everywhere over pages, device-held indices are checked
 // before they form an address.
+#include <type_traits>
+
 #include "paged_device.h"
 
 namespace cascade {
@@ -17,6 +19,8 @@ struct TreeArgs : PagedAttnArgs {
   const int64_t *masks;
   int64_t tokens;
   int32_t max_tree;
+  int32_t col_groups;      // workgroups that share a run of a KV head
+  uint32_t group_inverse;  // column / group = column * group_inverse >> 16
 };
 
 struct Tree {
@@ -44,59 +48,570 @@ __device__ __forceinline__ Tree tree_of(const int32_t *starts, const int32_t *ro
 }
 
 // ------------------------------------------------------------- attention
-// One wave a (node, query head): an online softmax, one position at a time.
-template <int D>
-__global__ __launch_bounds__(kWave) void tree_attention_kernel(TreeArgs a) {
-  constexpr int E = D / kWave;
-  const int64_t b = blockIdx.z;
-  const int node = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  Tree t = tree_of(a.starts, a.rows, a.tokens, a.max_tree, b, lane == 0 ? a.error : nullptr);
-  if (t.row < 0 || node >= t.nodes) return;
-  if (t.row >= a.sequences) {
-    if (lane == 0) flag_range(a.error);
-    return;
-  }
-  const int len = a.lengths[t.row];
+// The rows of a tree, if it and its sequence are in range.
+__device__ __forceinline__ PagedRow tree_row(const TreeArgs &a, int b, bool flag) {
+  PagedRow r{-1, 0};
+  if (b >= a.batch) return r;
+  int32_t *error = flag ? a.error : nullptr;
+  const Tree t = tree_of(a.starts, a.rows, a.tokens, a.max_tree, b, error);
+  if (t.row < 0 || t.nodes == 0) return r;
+  const int32_t len = t.row < a.sequences ? a.lengths[t.row] : -1;
   if (len < t.nodes || len > a.max_length) {
-    if (lane == 0) flag_range(a.error);
-    return;
+    flag_range(error);
+    return r;
   }
-  const int past = len - t.nodes;
-  const int64_t token = t.first + node;
-  const uint64_t mask = static_cast<uint64_t>(a.masks[token]);
-  const int64_t kv = h / a.group;
-  float q[E], acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = bf16_to_f32(a.q[token * a.q_token + h * a.q_head + E * lane + e]);
-    acc[e] = 0.0f;
-  }
-  float m = -FLT_MAX, l = 0.0f;
-  for (int p = 0; p < len; ++p) {
-    if (p >= past && !((mask >> (p - past)) & 1)) continue;
-    const int page = a.table[t.row * a.table_stride + (p >> a.page_shift)];
-    if (page < 0 || page >= a.num_pages) {
-      if (lane == 0) flag_range(a.error);
-      continue;
+  r.row = t.row;
+  r.len = len;
+  return r;
+}
+
+// Lane l's 16 bytes at base + voff land at LDS byte lds + 16 l (dma_lds16 for
+// a base of 64 bits).
+__device__ __forceinline__ void dma_lds16_from(uint64_t base, uint32_t voff, uint32_t lds) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base >> 32));
+  const uint64_t at = (static_cast<uint64_t>(hi) << 32) | lo;
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(at)
+               : "memory", "m0");
+}
+
+template <int DIM, int CT_, int WC_, int WP_>
+struct TreeShape {
+  static constexpr int D = DIM, CT = CT_, WC = WC_, WP = WP_;
+  static constexpr int WAVES = WC * WP;
+  static constexpr int COLS = 16 * CT * WC;  // of a workgroup
+  static constexpr int KC = D / 32;          // 32-dim chunks
+  static constexpr int DV = D / 16;          // dims a lane holds of a V row
+  static constexpr int ROW = 2 * D;          // bytes
+  static constexpr int TILE = kPagedBlock * ROW;
+  static constexpr int SLOT = 2 * TILE;      // K and V of a block
+  static constexpr int LOADS = SLOT / 1024 / WC;  // of a wave
+  static constexpr int FIT = 160 * 1024 / (WP * SLOT);
+  static constexpr int DEPTH = FIT < 4 ? FIT : 4;  // slots
+  static constexpr int SUMS = WAVES * 16 * (D * 4 + CT * 8);
+  static constexpr int LDS = DEPTH * WP * SLOT > SUMS ? DEPTH * WP * SLOT : SUMS;
+  static_assert(DEPTH >= 2 && LDS <= 160 * 1024 && LOADS >= 1, "shape");
+};
+
+// The columns of 16 query rows in a wave.
+template <int DV>
+struct TreeColumns {
+  float m, l;
+  f32x4 o[DV];
+};
+
+// The halves of a pair of bf16 values that are infinities or NaN, as a mask.
+__device__ __forceinline__ uint32_t special_of(uint32_t pair) {
+  return ((pair & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) |
+         ((pair & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+
+// One workgroup takes the columns (node, query head of the KV head) of a tree
+// and a run of its sequence's blocks of 32 positions.  WP groups of waves take
+// turns at the blocks; a group's K and V rows come into LDS once (loads that
+// go there directly, K rows swizzled as the operands read them), and its
+// WC waves multiply them with 16 CT columns each: scores, online softmax
+// and the product with V on the matrix cores as in paged_attention_kernel.
+template <typename T, bool SPLIT>
+__global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeArgs a) {
+  constexpr int D = T::D, CT = T::CT, WC = T::WC, WP = T::WP;
+  constexpr int KC = T::KC, DV = T::DV, ROW = T::ROW;
+  __shared__ __attribute__((aligned(16))) unsigned char s_mem[T::LDS];
+  __shared__ int s_special;
+  const int tid = threadIdx.x;
+  const int lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int wc = wave % WC, wp = wave / WC;
+  const int c16 = lane & 15, g4 = lane >> 4;
+  const int kv = static_cast<int>(blockIdx.x) % a.kv_heads;
+  const int rest = static_cast<int>(blockIdx.x) / a.kv_heads;
+  const int cg = rest % a.col_groups, run = rest / a.col_groups;
+  int b = run, len, first = 0, end, count = 1;
+  int64_t row;
+  {
+    const bool flags = blockIdx.x == 0 && wave == 0;
+    auto row_of = [&](int i, bool flag) { return tree_row(a, i, flag); };
+    if constexpr (SPLIT) {
+      const PagedRun r = find_run(a, run, lane, flags, row_of);
+      if (r.b < 0) return;
+      b = r.b;
+      row = r.row;
+      len = r.len;
+      first = r.first;
+      end = r.end;
+      count = r.count;
+    } else {
+      const PagedRow r = tree_row(a, b, kv == 0 && cg == 0 && tid == 0);
+      if (r.row < 0) return;
+      row = r.row;
+      len = r.len;
+      end = blocks_of(len);
     }
-    const int64_t at = page * a.page_stride + kv * a.head_stride +
-                       static_cast<int64_t>(p & ((1 << a.page_shift) - 1)) * D + E * lane;
-    float s = 0.0f;
+  }
+  row = __builtin_amdgcn_readfirstlane(static_cast<int>(row));
+  len = __builtin_amdgcn_readfirstlane(len);
+  b = __builtin_amdgcn_readfirstlane(b);
+  first = __builtin_amdgcn_readfirstlane(first);
+  end = __builtin_amdgcn_readfirstlane(end);
+  const int token0 = __builtin_amdgcn_readfirstlane(a.starts[b]);
+  const int nodes = __builtin_amdgcn_readfirstlane(a.starts[b + 1]) - token0;
+  const int cols = nodes * a.group;
+  const int col0 = cg * T::COLS;
+  if (col0 >= cols) return;
+  const int mine = col0 + 16 * CT * wc;  // the wave's first column
+  const int past = len - nodes, last = len - 1;
+  typedef const __attribute__((address_space(4))) int32_t *ConstTable;
+  const ConstTable table = (ConstTable)(reinterpret_cast<uintptr_t>(a.table) +
+                                        4 * static_cast<uint64_t>(row * a.table_stride));
+  const uint64_t kb = reinterpret_cast<uint64_t>(a.k_pages + kv * a.head_stride);
+  const uint64_t vb = reinterpret_cast<uint64_t>(a.v_pages + kv * a.head_stride);
+  const int page_mask = (1 << a.page_shift) - 1;
+  const uint32_t lds = lds_address(s_mem);
+  const uint32_t ring = wp * T::DEPTH * T::SLOT;
+
+  // A lane's place in a load of 1 KiB: its row, and its 16 bytes of it.  Row r
+  // of a block keeps its chunk ch at ch ^ key(r), where the keys of the 16 rows
+  // of an operand differ (of the eight of one parity, for 64 dims: two rows
+  // share the banks).
+  constexpr int CH = D / 8;
+  const int lrow = lane / CH, lch = lane % CH;
+  const uint32_t v_off = lane * 16;
+  struct Pages {
+    int of[4];  // of the block's groups of eight positions
+    uint32_t bad;
+  };
+  auto lookup = [&](int blk) {
+    Pages p;
+    p.bad = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], bf16_to_f32(a.k_pages[at + e]), s);
-    s = wave_sum(s) * a.scale_log2;
-    const float mnew = fmaxf(m, s);
-    const float keep = paged_exp2(m - mnew), w = paged_exp2(s - mnew);
-    m = mnew;
-    l = fmaf(l, keep, w);
+    for (int g = 0; g < 4; ++g) {
+      const int page = table[min(blk * kPagedBlock + 8 * g, last) >> a.page_shift];
+      const bool good = page >= 0 && page < a.num_pages;
+      p.of[g] = good ? page : 0;
+      p.bad |= good ? 0u : 1u << g;
+    }
+    return p;
+  };
+  auto issue = [&](int blk, const Pages &p, int slot) __attribute__((always_inline)) {
+    const uint32_t to = lds + ring + slot * T::SLOT;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      acc[e] = fmaf(w, bf16_to_f32(a.v_pages[at + e]), acc[e] * keep);
+    for (int i = 0; i < T::LOADS; ++i) {
+      const int idx = wc + WC * i;  // K's loads, then V's
+      const bool is_v = idx >= T::SLOT / 2048;
+      const int part = idx % (T::SLOT / 2048);
+      const int grp = D == 128 ? part >> 1 : part;
+      const int half = D == 128 ? part & 1 : 0;
+      const int64_t at = static_cast<int64_t>(grp == 0 ? p.of[0] : grp == 1 ? p.of[1] : grp == 2 ? p.of[2] : p.of[3]) * a.page_stride +
+                         ((blk * kPagedBlock + 8 * grp) & page_mask) * D;
+      const uint32_t key = D == 128 ? 4 * grp + lrow : 2 * grp + ((lrow >> 1) & 1);
+      const uint32_t off = is_v ? v_off : lrow * ROW + ((lch ^ key) << 4);
+      dma_lds16_from((is_v ? vb : kb) + 2 * static_cast<uint64_t>(at) + half * 1024, off,
+                     to + idx * 1024);
+    }
+  };
+  const int groups_of = (end - first + WP - 1) / WP;  // steps of the workgroup
+  // (past the run's end its last block again, which takes no part)
+  auto block_of = [&](int step) { return min(first + step * WP + wp, end - 1); };
+  Pages next = lookup(block_of(0));
+  uint32_t ahead[T::DEPTH - 1];  // bad pages of the blocks under way
+#pragma unroll
+  for (int d = 0; d < T::DEPTH - 1; ++d) {
+    ahead[d] = next.bad;
+    issue(block_of(d), next, d);
+    next = lookup(block_of(d + 1));
+  }
+
+  // the q operands, zeros past the tree's columns
+  u32x4 q[CT][KC];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int col = mine + 16 * ct + c16;
+    const int node = static_cast<int>((static_cast<uint32_t>(col) * a.group_inverse) >> 16);
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      q[ct][c] = u32x4{0u, 0u, 0u, 0u};
+      if (col < cols)
+        q[ct][c] = *reinterpret_cast<const u32x4 *>(
+            a.q + (token0 + node) * a.q_token +
+            (static_cast<int64_t>(kv) * a.group + col - node * a.group) * a.q_head + 32 * c +
+            8 * g4);
+    }
+  }
+
+  if (tid == 0) s_special = 0;  // (the loop begins with a barrier)
+  TreeColumns<DV> state[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    state[ct].m = -FLT_MAX;
+    state[ct].l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < DV; ++e) state[ct].o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const int krow = 8 * (c16 >> 2) + (c16 & 3);
+  const int kkey = D == 128 ? c16 : 2 * (c16 >> 2) + ((c16 >> 1) & 1);
+
+  auto step = [&](int blk, uint32_t bad, int slot) __attribute__((always_inline)) {
+    // a block with positions of the tree or past the end, or with a bad page
+    const bool tail = bad || (blk + 1) * kPagedBlock > past;
+    const unsigned char *at = s_mem + ring + slot * T::SLOT;
+    const int r0 = blk * kPagedBlock;
+    f32x4 score[CT][2];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+      score[ct][0] = score[ct][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const unsigned char *kp = at + krow * ROW + (((4 * c + g4) ^ kkey) << 4);
+      const u32x4 k0 = *reinterpret_cast<const u32x4 *>(kp);
+      const u32x4 k1 = *reinterpret_cast<const u32x4 *>(kp + 4 * ROW);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        score[ct][0] = mfma_16x16x32_bf16(k0, q[ct][c], score[ct][0]);
+        score[ct][1] = mfma_16x16x32_bf16(k1, q[ct][c], score[ct][1]);
+      }
+    }
+    const bool mine_bad = (bad >> g4) & 1;
+    u32x4 vop[DV];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // (two rows at a time: all of them would not fit beside the columns)
+      __builtin_amdgcn_sched_barrier(0);
+      uint32_t v[2][DV / 2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const unsigned char *vp = at + T::TILE + (8 * g4 + 2 * i + j) * ROW + c16 * (DV * 2);
+        if constexpr (DV == 8) {
+          const u32x4 w = *reinterpret_cast<const u32x4 *>(vp);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) v[j][n] = w[n];
+        } else {
+          const u32x2 w = *reinterpret_cast<const u32x2 *>(vp);
+          v[j][0] = w[0];
+          v[j][1] = w[1];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < DV; ++e)
+        vop[e][i] = __builtin_amdgcn_perm(v[1][e >> 1], v[0][e >> 1],
+                                          (e & 1) ? 0x07060302u : 0x05040100u);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (tail) {
+      // Rows past the end, or of a page outside the pool, take no part
+      // whatever they hold.  An infinity or a NaN of a row that a column does not see must not
+      // reach it, and 0 times one is a NaN: they are left out here, and
+      // added where the columns are joined, to those that see them.
+      uint32_t any = 0;
+#pragma unroll
+      for (int e = 0; e < DV; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at_row = r0 + 8 * g4 + 2 * i;
+          const uint32_t in = mine_bad ? 0u : (at_row < len ? 0xffffu : 0u) |
+                                                  (at_row + 1 < len ? 0xffff0000u : 0u);
+          const uint32_t pair = vop[e][i] & in, bits = special_of(pair);
+          any |= bits;
+          vop[e][i] = pair & ~bits;
+        }
+      if (any != 0) s_special = 1;
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const f32x4 s0 = score[ct][0], s1 = score[ct][1];
+      float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] *= a.scale_log2;
+      if (tail) {
+        // bit j: the column sees position r0 + 8 g4 + j
+        const int col = mine + 16 * ct + c16;
+        const int node =
+            static_cast<int>((static_cast<uint32_t>(col) * a.group_inverse) >> 16);
+        uint64_t mask = col < cols ? static_cast<uint64_t>(a.masks[token0 + node]) : 0;
+        if (nodes < kTreeNodes) mask &= (uint64_t{1} << nodes) - 1;
+        const int rel = r0 + 8 * g4 - past;  // of the lane's first position
+        uint64_t bits = 0xffu;
+        if (rel >= kTreeNodes)
+          bits = 0;
+        else if (rel >= 0)
+          bits = mask >> rel;
+        else if (rel > -8)
+          bits = (mask << -rel) | ((1u << -rel) - 1);
+        const uint32_t sees = mine_bad ? 0u : static_cast<uint32_t>(bits);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = (sees >> j) & 1 ? s[j] : -INFINITY;
+      }
+      float bmax = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bmax = fmaxf(bmax, s[j]);
+      TreeColumns<DV> &x = state[ct];
+      bmax = xor32_max(xor16_max(bmax));
+      const float mnew = fmaxf(x.m, bmax);
+      const float alpha = paged_exp2(x.m - mnew);
+      x.m = mnew;
+      float p[8], psum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = paged_exp2(s[j] - mnew);
+        psum += p[j];
+      }
+      x.l = fmaf(x.l, alpha, psum);
+      u32x4 pop, low;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const SplitWeights w = split_weights(p[2 * i], p[2 * i + 1]);
+        pop[i] = w.upper;
+        low[i] = w.lower;
+      }
+      if (alpha != 1.0f) {
+#pragma unroll
+        for (int e = 0; e < DV; ++e) x.o[e] *= alpha;
+      }
+#pragma unroll
+      for (int e = 0; e < DV; ++e) {
+        x.o[e] = mfma_16x16x32_bf16(vop[e], low, x.o[e]);
+        x.o[e] = mfma_16x16x32_bf16(vop[e], pop, x.o[e]);
+      }
+    }
+  };
+
+  // (the q rows are here: no wait for them inside the loop)
+  __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+  uint32_t all_bad = 0;
+  int slot = 0;
+  for (int i = 0; i < groups_of; ++i) {
+    // the block's own loads are here, then everyone's, and the slot that is
+    // filled next has been read (no fence: it would wait for all loads)
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm((T::DEPTH - 2) * T::LOADS, 15));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t bad = ahead[0];
+#pragma unroll
+    for (int d = 0; d + 1 < T::DEPTH - 1; ++d) ahead[d] = ahead[d + 1];
+    ahead[T::DEPTH - 2] = next.bad;
+    issue(block_of(i + T::DEPTH - 1), next, slot == 0 ? T::DEPTH - 1 : slot - 1);
+    next = lookup(block_of(i + T::DEPTH));
+    __builtin_amdgcn_sched_barrier(0);
+    const int blk = first + i * WP + wp;
+    if (blk < end && mine < cols) {
+      all_bad |= bad;
+      step(blk, bad, slot);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    slot = slot == T::DEPTH - 1 ? 0 : slot + 1;
+  }
+  __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+  __syncthreads();
+  if (all_bad && lane == 0) flag_range(a.error);
+
+  // the groups' columns join, one tile of them after the other
+  float *s_acc = reinterpret_cast<float *>(s_mem);  // [wave][column][dim]
+  float *s_ml = s_acc + T::WAVES * 16 * D;          // [wave][tile][column][2]
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const float l = xor32_sum(xor16_sum(state[ct].l));
+    if (g4 == 0) {
+      s_ml[((wave * CT + ct) * 16 + c16) * 2] = state[ct].m;
+      s_ml[((wave * CT + ct) * 16 + c16) * 2 + 1] = l;
+    }
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    a.out[token * a.out_token + h * a.out_head + E * lane + e] =
-        f32_to_bf16(l == 0.0f ? 0.0f : acc[e] / l);
+  for (int ct = 0; ct < CT; ++ct) {
+    if (ct) __syncthreads();
+    // o[e][r] = O[dim DV (4 g4 + r) + e][column c16]
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < DV; ++e)
+        s_acc[(wave * 16 + c16) * D + DV * (4 * g4 + r) + e] = state[ct].o[e][r];
+    __syncthreads();
+    for (int i = tid; i < WC * 16 * D; i += T::WAVES * kWave) {
+      const int w = i / (16 * D), c = i / D % 16, d = i % D;
+      const int col = col0 + 16 * (CT * w + ct) + c;
+      if (col >= cols) continue;
+      float mm = -FLT_MAX;
+#pragma unroll
+      for (int k = 0; k < WP; ++k)
+        mm = fmaxf(mm, s_ml[(((k * WC + w) * CT + ct) * 16 + c) * 2]);
+      float den = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < WP; ++k) {
+        const float *ml = s_ml + (((k * WC + w) * CT + ct) * 16 + c) * 2;
+        const float wt = paged_exp2(ml[0] - mm);
+        den = fmaf(wt, ml[1], den);
+        sum = fmaf(wt, s_acc[((k * WC + w) * 16 + c) * D + d], sum);
+      }
+      const int node = static_cast<int>((static_cast<uint32_t>(col) * a.group_inverse) >> 16);
+      const int head = kv * a.group + col - node * a.group;
+      if (s_special) {
+        const uint64_t mask = static_cast<uint64_t>(a.masks[token0 + node]);
+        const int to = min(end * kPagedBlock, len);
+        for (int p = max(first, past / kPagedBlock) * kPagedBlock; p < to; ++p) {
+          const int page = table[p >> a.page_shift];
+          if (page < 0 || page >= a.num_pages) continue;
+          if (p >= past && !((mask >> (p - past)) & 1)) continue;
+          const float value =
+              bf16_to_f32(a.v_pages[page * a.page_stride + kv * a.head_stride +
+                                    static_cast<int64_t>(p & page_mask) * D + d]);
+          if (!(fabsf(value) < INFINITY)) sum += value;
+        }
+      }
+      if (!SPLIT || count == 1) {
+        a.out[(token0 + node) * a.out_token + head * a.out_head + d] =
+            f32_to_bf16(den == 0.0f ? 0.0f : sum / den);
+      } else {
+        const int64_t at =
+            (static_cast<int64_t>(run) * a.max_tree + node) * (a.kv_heads * a.group) + head;
+        a.part_acc[at * D + d] = sum;
+        if (d == 0) {
+          a.part_ml[2 * at] = mm;
+          a.part_ml[2 * at + 1] = den;
+        }
+      }
+    }
+  }
+}
+
+// Joins the runs of a node: out = sum_r 2^(m_r - M) acc_r / sum_r 2^(m_r - M) l_r.
+// D / 4 threads (four dims each) are a slice, SLICES slices a head, and each
+// takes every SLICES-th run with a running maximum of its own.
+constexpr int kTreeMergeThreads = 256;
+
+template <int D, int SLICES>
+__global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs a) {
+  constexpr int kHeads = kTreeMergeThreads / (SLICES * D / 4);
+  __shared__ f32x4 s_acc[kHeads][SLICES][D / 4];
+  __shared__ float s_ml[kHeads][SLICES][2];
+  const int heads = a.kv_heads * a.group;
+  const int parts = (heads + kHeads - 1) / kHeads;
+  const int64_t id = blockIdx.x;
+  const int part = static_cast<int>(id % parts);
+  const int node = static_cast<int>(id / parts % a.max_tree);
+  const int b = static_cast<int>(id / parts / a.max_tree);
+  const int index = a.plan[2 * b], count = a.plan[2 * b + 1];
+  // left out, or written already (or, past the workspace, a plan that another
+  // call has overwritten)
+  if (count <= 1 || index < 0 || count > a.runs - index) return;
+  const int token0 = a.starts[b];
+  if (node >= a.starts[b + 1] - token0) return;
+  const int d = threadIdx.x % (D / 4);
+  const int slice = threadIdx.x / (D / 4) % SLICES;
+  const int h = threadIdx.x / (D / 4) / SLICES;
+  const int head = part * kHeads + h;
+  float m = -FLT_MAX, den = 0.0f;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (head < heads) {
+    const int64_t step = static_cast<int64_t>(a.max_tree) * heads;
+    const int64_t base = (static_cast<int64_t>(index) * a.max_tree + node) * heads + head;
+#pragma unroll 4
+    for (int r = slice; r < count; r += SLICES) {
+      const int64_t at = base + r * step;
+      const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * at);
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(a.part_acc + at * D + 4 * d);
+      const float mnew = fmaxf(m, ml.x);
+      const float keep = paged_exp2(m - mnew), w = paged_exp2(ml.x - mnew);
+      m = mnew;
+      den = fmaf(w, ml.y, den * keep);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(w, v[i], acc[i] * keep);
+    }
+  }
+  s_acc[h][slice][d] = acc;
+  if (d == 0) {
+    s_ml[h][slice][0] = m;
+    s_ml[h][slice][1] = den;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kHeads * D; i += kTreeMergeThreads) {
+    const int hh = i / D, dim = i % D;
+    if (part * kHeads + hh >= heads) return;
+    float mm = -FLT_MAX;
+#pragma unroll
+    for (int k = 0; k < SLICES; ++k) mm = fmaxf(mm, s_ml[hh][k][0]);
+    float sum = 0.0f, r = 0.0f;
+#pragma unroll
+    for (int k = 0; k < SLICES; ++k) {
+      const float w = paged_exp2(s_ml[hh][k][0] - mm);
+      sum = fmaf(w, s_ml[hh][k][1], sum);
+      r = fmaf(w, s_acc[hh][k][dim / 4][dim % 4], r);
+    }
+    a.out[(token0 + node) * a.out_token + (part * kHeads + hh) * a.out_head + dim] =
+        f32_to_bf16(sum == 0.0f ? 0.0f : r / sum);
+  }
+}
+
+// Which shape a call takes, whether it splits, and its sizes.
+struct TreePlan {
+  int shape;  // tiles of 16 columns a workgroup: 1, 2, 4, 8, 16
+  int col_groups;
+  bool split;
+  int64_t round, two;  // runs wanted, in one round and in two
+  int64_t runs;        // at most
+  size_t plan_bytes, ml_bytes, acc_bytes;
+};
+
+constexpr int64_t kTreeSlots = 256;      // workgroups that the device holds: one a CU
+constexpr int64_t kTreeMaxBatch = 256;   // of a split launch
+
+static TreePlan tree_plan(int64_t trees, int64_t max_tree, int64_t q_heads, int64_t kv_heads,
+                          int64_t dim, int64_t max_length) {
+  TreePlan p{};
+  const int64_t cols = max_tree * (q_heads / kv_heads);
+  p.shape = cols <= 16 ? 1 : cols <= 32 ? 2 : cols <= 64 ? 4 : cols <= 128 ? 8 : 16;
+  p.col_groups = static_cast<int>((cols + 16 * p.shape - 1) / (16 * p.shape));
+  const int64_t blocks = (max_length + kPagedBlock - 1) / kPagedBlock;
+  p.split = blocks > kWholeBlocks && trees <= kTreeMaxBatch;
+  if (!p.split) return p;
+  const int64_t each = kv_heads * p.col_groups;
+  const int64_t slots = (kTreeSlots + each - 1) / each;
+  auto wanted = [trees](int64_t runs) {
+    return runs - trees / 2 > runs / 2 ? runs - trees / 2 : (runs + 1) / 2;
+  };
+  p.two = wanted(2 * slots);
+  p.round = wanted(slots);
+  if (3 * trees > p.round) p.round = p.two;
+  p.runs = p.two + trees;
+  const int64_t most = trees * ((blocks + kPagedMinRun - 1) / kPagedMinRun);
+  if (p.runs > most) p.runs = most;
+  auto rounded = [](int64_t bytes) {
+    return (static_cast<size_t>(bytes) + kPagedAlign - 1) / kPagedAlign * kPagedAlign;
+  };
+  p.plan_bytes = rounded(trees * 8);
+  p.ml_bytes = rounded(p.runs * max_tree * q_heads * 8);
+  p.acc_bytes = rounded(p.runs * max_tree * q_heads * dim * 4);
+  return p;
+}
+
+template <int D, bool SPLIT>
+static hipError_t launch_tree(const TreeArgs &a, int shape, int64_t blocks, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(blocks));
+#define CASCADE_TREE(CT, WC, WP)                                                     \
+  {                                                                                  \
+    using T = TreeShape<D, CT, WC, WP>;                                              \
+    return launch_kernel(tree_attention_kernel<T, SPLIT>, grid, dim3(T::WAVES * kWave), 0, s, a); \
+  }
+  switch (shape) {
+    case 1: CASCADE_TREE(1, 1, 4)
+    case 2: CASCADE_TREE(2, 1, 4)
+    case 4: CASCADE_TREE(2, 2, 4)
+    case 8: CASCADE_TREE(2, 4, 2)
+    default: CASCADE_TREE(2, 8, 1)
+  }
+#undef CASCADE_TREE
+}
+
+template <int D>
+static hipError_t launch_tree_merge(const TreeArgs &a, int64_t runs_a_tree, hipStream_t s) {
+  const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
+  auto grid = [&](int64_t per) {
+    return dim3(static_cast<unsigned>(a.batch * static_cast<int64_t>(a.max_tree) *
+                                      ((heads + per - 1) / per)));
+  };
+  const dim3 block(kTreeMergeThreads);
+  if (runs_a_tree > 8)
+    return launch_kernel(tree_merge_kernel<D, 8>, grid(128 / D), block, 0, s, a);
+  return launch_kernel(tree_merge_kernel<D, 2>, grid(512 / D), block, 0, s, a);
 }
 
 // ------------------------------------------------------------ acceptance
@@ -215,7 +730,17 @@ extern "C" size_t cascade_paged_tree_attention_workspace_bytes(
       n_q_heads / n_kv_heads > kPagedGroup || n_q_heads > 0xffff ||
       (head_dim != 64 && head_dim != 128) || max_length <= 0 || max_length > 0x7fffffff - 64)
     return 0;
-  return kPagedAlign;
+  // enough for fewer trees, nodes and positions too: a launch of more than
+  // kTreeMaxBatch trees needs none
+  size_t most = 0;
+  const int64_t n = trees < kTreeMaxBatch ? trees : kTreeMaxBatch;
+  for (int64_t nodes = max_tree;; nodes /= 2) {
+    const TreePlan p = tree_plan(n, nodes, n_q_heads, n_kv_heads, head_dim, max_length);
+    const size_t need = p.plan_bytes + p.ml_bytes + p.acc_bytes;
+    most = need > most ? need : most;
+    if (nodes <= 1) break;
+  }
+  return kPagedAlign + most;
 }
 
 extern "C" int cascade_paged_tree_attention_bf16(
@@ -279,12 +804,33 @@ extern "C" int cascade_paged_tree_attention_bf16(
   a.masks = masks;
   a.tokens = tokens;
   a.max_tree = static_cast<int32_t>(max_tree);
+  const TreePlan p = tree_plan(trees, max_tree, n_q_heads, n_kv_heads, head_dim, max_length);
+  a.col_groups = p.col_groups;
+  a.group_inverse = (65536u + a.group - 1) / a.group;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(max_tree), static_cast<unsigned>(n_q_heads),
-                  static_cast<unsigned>(trees));
-  return head_dim == 128
-             ? launch_kernel(tree_attention_kernel<128>, grid, dim3(kWave), 0, s, a)
-             : launch_kernel(tree_attention_kernel<64>, grid, dim3(kWave), 0, s, a);
+  const int64_t each = n_kv_heads * p.col_groups;
+  if (!p.split) {
+    if (trees * each > kMaxThreads / 512) return CASCADE_ESHAPE;
+    return head_dim == 128 ? launch_tree<128, false>(a, p.shape, trees * each, s)
+                           : launch_tree<64, false>(a, p.shape, trees * each, s);
+  }
+  if (p.runs * each > kMaxThreads / 512 ||
+      trees * max_tree > kMaxThreads / kTreeMergeThreads / n_q_heads)
+    return CASCADE_ESHAPE;
+  unsigned char *ws = static_cast<unsigned char *>(workspace);
+  a.runs = static_cast<int32_t>(p.runs);
+  a.per_round = 1.0 / static_cast<double>(p.round);
+  a.per_two = 1.0 / static_cast<double>(p.two);
+  a.plan = reinterpret_cast<int32_t *>(ws);
+  a.part_ml = reinterpret_cast<float *>(ws + p.plan_bytes);
+  a.part_acc = reinterpret_cast<float *>(ws + p.plan_bytes + p.ml_bytes);
+  const int64_t runs_a_tree = p.runs / trees;
+  if (head_dim == 128) {
+    const hipError_t e = launch_tree<128, true>(a, p.shape, p.runs * each, s);
+    return e != hipSuccess ? e : launch_tree_merge<128>(a, runs_a_tree, s);
+  }
+  const hipError_t e = launch_tree<64, true>(a, p.shape, p.runs * each, s);
+  return e != hipSuccess ? e : launch_tree_merge<64>(a, runs_a_tree, s);
 }
 
 extern "C" int cascade_paged_tree_accept(
