@@ -6,7 +6,7 @@
 // last n of the lengths[row] positions of its sequence: "past" below is what
 // lies before it.  As everywhere over pages, device-held indices are checked
 // before they form an address.
-#include <type_traits>
+#include <cmath>
 
 #include "paged_device.h"
 
@@ -20,6 +20,8 @@ struct TreeArgs : PagedAttnArgs {
   int64_t tokens;
   int32_t max_tree;
   int32_t col_groups;      // workgroups that share a run of a KV head
+  uint32_t sign;           // flips the signs of q: scale_log2 is not negative
+  float slack;             // in raw scores, see the running maximum
   uint32_t group_inverse;  // column / group = column * group_inverse >> 16
 };
 
@@ -67,13 +69,19 @@ __device__ __forceinline__ PagedRow tree_row(const TreeArgs &a, int b, bool flag
 
 // Lane l's 16 bytes at base + voff land at LDS byte lds + 16 l (dma_lds16 for
 // a base of 64 bits).
-__device__ __forceinline__ void dma_lds16_from(uint64_t base, uint32_t voff, uint32_t lds) {
+__device__ __forceinline__ void dma_lds16_from(uint64_t base, uint32_t voff, uint32_t lds,
+                                               bool once) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base));
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base >> 32));
   const uint64_t at = (static_cast<uint64_t>(hi) << 32) | lo;
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(at)
-               : "memory", "m0");
+  if (once)
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(at)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(at)
+                 : "memory", "m0");
 }
 
 template <int DIM, int CT_, int WC_, int WP_>
@@ -81,15 +89,19 @@ struct TreeShape {
   static constexpr int D = DIM, CT = CT_, WC = WC_, WP = WP_;
   static constexpr int WAVES = WC * WP;
   static constexpr int COLS = 16 * CT * WC;  // of a workgroup
+  // rows that no other workgroup reads need no place in a cache
+  static constexpr bool ONCE = CT * WC < 16;
   static constexpr int KC = D / 32;          // 32-dim chunks
   static constexpr int DV = D / 16;          // dims a lane holds of a V row
   static constexpr int ROW = 2 * D;          // bytes
   static constexpr int TILE = kPagedBlock * ROW;
   static constexpr int SLOT = 2 * TILE;      // K and V of a block
   static constexpr int LOADS = SLOT / 1024 / WC;  // of a wave
-  static constexpr int FIT = 160 * 1024 / (WP * SLOT);
-  static constexpr int DEPTH = FIT < 4 ? FIT : 4;  // slots
-  static constexpr int SUMS = WAVES * 16 * (D * 4 + CT * 8);
+  static constexpr int FIT = (160 * 1024 - 16) / (WP * SLOT);
+  static constexpr int COUNT = 63 / LOADS + 2, FEW = FIT < COUNT ? FIT : COUNT;
+  static constexpr int DEPTH = FEW < 5 ? FEW : 5;  // slots
+  static constexpr int PITCH = D + 4;  // floats of a column where the groups join
+  static constexpr int SUMS = WAVES * 16 * (PITCH * 4 + 8);
   static constexpr int LDS = DEPTH * WP * SLOT > SUMS ? DEPTH * WP * SLOT : SUMS;
   static_assert(DEPTH >= 2 && LDS <= 160 * 1024 && LOADS >= 1, "shape");
 };
@@ -161,9 +173,6 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   if (col0 >= cols) return;
   const int mine = col0 + 16 * CT * wc;  // the wave's first column
   const int past = len - nodes, last = len - 1;
-  typedef const __attribute__((address_space(4))) int32_t *ConstTable;
-  const ConstTable table = (ConstTable)(reinterpret_cast<uintptr_t>(a.table) +
-                                        4 * static_cast<uint64_t>(row * a.table_stride));
   const uint64_t kb = reinterpret_cast<uint64_t>(a.k_pages + kv * a.head_stride);
   const uint64_t vb = reinterpret_cast<uint64_t>(a.v_pages + kv * a.head_stride);
   const int page_mask = (1 << a.page_shift) - 1;
@@ -176,51 +185,78 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   // share the banks).
   constexpr int CH = D / 8;
   const int lrow = lane / CH, lch = lane % CH;
-  const uint32_t v_off = lane * 16;
-  struct Pages {
-    int of[4];  // of the block's groups of eight positions
-    uint32_t bad;
-  };
-  auto lookup = [&](int blk) {
-    Pages p;
-    p.bad = 0;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int page = table[min(blk * kPagedBlock + 8 * g, last) >> a.page_shift];
-      const bool good = page >= 0 && page < a.num_pages;
-      p.of[g] = good ? page : 0;
-      p.bad |= good ? 0u : 1u << g;
-    }
-    return p;
-  };
-  auto issue = [&](int blk, const Pages &p, int slot) __attribute__((always_inline)) {
-    const uint32_t to = lds + ring + slot * T::SLOT;
-#pragma unroll
-    for (int i = 0; i < T::LOADS; ++i) {
-      const int idx = wc + WC * i;  // K's loads, then V's
-      const bool is_v = idx >= T::SLOT / 2048;
-      const int part = idx % (T::SLOT / 2048);
-      const int grp = D == 128 ? part >> 1 : part;
-      const int half = D == 128 ? part & 1 : 0;
-      const int64_t at = static_cast<int64_t>(grp == 0 ? p.of[0] : grp == 1 ? p.of[1] : grp == 2 ? p.of[2] : p.of[3]) * a.page_stride +
-                         ((blk * kPagedBlock + 8 * grp) & page_mask) * D;
-      const uint32_t key = D == 128 ? 4 * grp + lrow : 2 * grp + ((lrow >> 1) & 1);
-      const uint32_t off = is_v ? v_off : lrow * ROW + ((lch ^ key) << 4);
-      dma_lds16_from((is_v ? vb : kb) + 2 * static_cast<uint64_t>(at) + half * 1024, off,
-                     to + idx * 1024);
-    }
-  };
-  const int groups_of = (end - first + WP - 1) / WP;  // steps of the workgroup
+  // The pages of sixteen of the wave's blocks, a lane a group of eight positions:
+  // what the group's rows lie behind the pools' start, and a bit a bad page.
+  const int steps = (end - first + WP - 1) / WP;  // of the workgroup
   // (past the run's end its last block again, which takes no part)
   auto block_of = [&](int step) { return min(first + step * WP + wp, end - 1); };
-  Pages next = lookup(block_of(0));
-  uint32_t ahead[T::DEPTH - 1];  // bad pages of the blocks under way
+  const int32_t *table = a.table + row * a.table_stride;
+  auto entry_of = [&](int step) {  // of the lane, in the sixteen steps from `step` on
+    return table[min(block_of(step + (lane >> 2)) * kPagedBlock + 8 * (lane & 3), last) >>
+                 a.page_shift];
+  };
+  struct Pages {
+    uint32_t lo, hi;
+    uint64_t bad;
+  };
+  auto pages_of = [&](int step, int page) {
+    Pages p;
+    const bool good = page >= 0 && page < a.num_pages;
+    const int slot = (block_of(step + (lane >> 2)) * kPagedBlock + 8 * (lane & 3)) & page_mask;
+    const uint64_t at = static_cast<uint64_t>(good ? page : 0) *
+                            static_cast<uint64_t>(2 * a.page_stride) +
+                        static_cast<uint64_t>(slot * ROW);
+    p.lo = static_cast<uint32_t>(at);
+    p.hi = static_cast<uint32_t>(at >> 32);
+    p.bad = __ballot(!good);
+    return p;
+  };
+  // A wave's loads: K's and V's of all groups, or one of them, or that of some.
+  constexpr int kGroups = WC <= 2 ? 4 : 8 / WC;  // that a wave loads
+  constexpr int kHalves = D / 64;                // loads of a group
+  const int group0 = (wc >> 1) * kGroups;
+  uint32_t k_off[kGroups][kHalves];
 #pragma unroll
-  for (int d = 0; d < T::DEPTH - 1; ++d) {
-    ahead[d] = next.bad;
-    issue(block_of(d), next, d);
-    next = lookup(block_of(d + 1));
-  }
+  for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      const int grp = group0 + g;
+      const uint32_t key = D == 128 ? 4 * grp + lrow : 2 * grp + ((lrow >> 1) & 1);
+      k_off[g][h] = h * 1024 + lrow * ROW + ((lch ^ key) << 4);
+      if (WC > 1 && (wc & 1)) k_off[g][h] = h * 1024 + lane * 16;  // this wave loads V
+    }
+  Pages pages = pages_of(0, entry_of(0));
+  int entry = entry_of(16);
+  uint32_t all_bad = 0;
+  // Starts the loads of step `step` (they are asked for in order) into a slot.
+  auto issue = [&](int step, int slot) __attribute__((always_inline)) {
+    const int at = (step & 15) * 4;
+    if (at == 0 && step != 0) {
+      pages = pages_of(step, entry);
+      entry = entry_of(step + 16);
+    }
+    const uint32_t to = lds + ring + slot * T::SLOT;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int grp = group0 + g;
+      const uint64_t behind =
+          (static_cast<uint64_t>(__builtin_amdgcn_readlane(pages.hi, at + grp)) << 32) |
+          static_cast<uint32_t>(__builtin_amdgcn_readlane(pages.lo, at + grp));
+#pragma unroll
+      for (int kvs = 0; kvs < (WC == 1 ? 2 : 1); ++kvs) {
+        const bool is_v = WC == 1 ? kvs : wc & 1;
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+          dma_lds16_from((is_v ? vb : kb) + behind,
+                         WC == 1 && kvs ? static_cast<uint32_t>(h * 1024 + lane * 16)
+                                        : k_off[g][h],
+                         to + (is_v ? T::TILE : 0) + (grp * kHalves + h) * 1024, T::ONCE);
+      }
+    }
+    return static_cast<uint32_t>(pages.bad >> at) & 0xfu;
+  };
+  uint32_t bads = 0;  // bad pages of the blocks under way, four bits a step
+  for (int d = 0; d < T::DEPTH; ++d) bads |= issue(d, d) << (4 * d);
 
   // the q operands, zeros past the tree's columns
   u32x4 q[CT][KC];
@@ -230,16 +266,16 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
     const int node = static_cast<int>((static_cast<uint32_t>(col) * a.group_inverse) >> 16);
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      q[ct][c] = u32x4{0u, 0u, 0u, 0u};
-      if (col < cols)
-        q[ct][c] = *reinterpret_cast<const u32x4 *>(
-            a.q + (token0 + node) * a.q_token +
-            (static_cast<int64_t>(kv) * a.group + col - node * a.group) * a.q_head + 32 * c +
-            8 * g4);
+      const int64_t at = (token0 + min(node, nodes - 1)) * a.q_token +
+                         (static_cast<int64_t>(kv) * a.group +
+                          (col < cols ? col - node * a.group : 0)) * a.q_head;
+      u32x4 x = *reinterpret_cast<const u32x4 *>(a.q + at + 32 * c + 8 * g4);
+      x ^= a.sign;
+      q[ct][c] = col < cols ? x : u32x4{0u, 0u, 0u, 0u};
     }
   }
 
-  if (tid == 0) s_special = 0;  // (the loop begins with a barrier)
+  if (tid == 0) s_special = 0;
   TreeColumns<DV> state[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -251,52 +287,81 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   const int krow = 8 * (c16 >> 2) + (c16 & 3);
   const int kkey = D == 128 ? c16 : 2 * (c16 >> 2) + ((c16 >> 1) & 1);
 
-  auto step = [&](int blk, uint32_t bad, int slot) __attribute__((always_inline)) {
+  u32x4 k0[KC], k1[KC];  // the next block's K operands
+  auto read_k = [&](int slot) __attribute__((always_inline)) {
+    const unsigned char *at = s_mem + ring + slot * T::SLOT;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const unsigned char *kp = at + krow * ROW + (((4 * c + g4) ^ kkey) << 4);
+      k0[c] = *reinterpret_cast<const u32x4 *>(kp);
+      k1[c] = *reinterpret_cast<const u32x4 *>(kp + 4 * ROW);
+    }
+  };
+  // The next step's loads are here, and everyone has read this step's slot, which
+  // takes the loads of the step that is DEPTH behind it (no fence: it would
+  // wait for all loads).
+  auto turn = [&](int i, int slot) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm((T::DEPTH - 2) * T::LOADS, 15));
+    if constexpr (WC > 1) __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    bads = (bads >> 4) | (issue(i + T::DEPTH, slot) << (4 * (T::DEPTH - 1)));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto step = [&](int i, int slot) __attribute__((always_inline)) {
+    const int blk = first + i * WP + wp;
+    const bool gone = blk >= end;  // (a group's last turn, where others have one)
+    const uint32_t bad = gone ? 0xfu : bads & 0xfu;
+    all_bad |= gone ? 0u : bad;
     // a block with positions of the tree or past the end, or with a bad page
     const bool tail = bad || (blk + 1) * kPagedBlock > past;
     const unsigned char *at = s_mem + ring + slot * T::SLOT;
     const int r0 = blk * kPagedBlock;
+    uint32_t v[8][DV / 2];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const unsigned char *vp = at + T::TILE + (8 * g4 + j) * ROW + c16 * (DV * 2);
+      if constexpr (DV == 8) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(vp);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) v[j][n] = w[n];
+      } else {
+        const u32x2 w = *reinterpret_cast<const u32x2 *>(vp);
+        v[j][0] = w[0];
+        v[j][1] = w[1];
+      }
+    }
     f32x4 score[CT][2];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
       score[ct][0] = score[ct][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      const unsigned char *kp = at + krow * ROW + (((4 * c + g4) ^ kkey) << 4);
-      const u32x4 k0 = *reinterpret_cast<const u32x4 *>(kp);
-      const u32x4 k1 = *reinterpret_cast<const u32x4 *>(kp + 4 * ROW);
+    for (int c = 0; c < KC; ++c)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        score[ct][0] = mfma_16x16x32_bf16(k0, q[ct][c], score[ct][0]);
-        score[ct][1] = mfma_16x16x32_bf16(k1, q[ct][c], score[ct][1]);
+        score[ct][0] = mfma_16x16x32_bf16(k0[c], q[ct][c], score[ct][0]);
+        score[ct][1] = mfma_16x16x32_bf16(k1[c], q[ct][c], score[ct][1]);
       }
-    }
     const bool mine_bad = (bad >> g4) & 1;
     u32x4 vop[DV];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // (two rows at a time: all of them would not fit beside the columns)
-      __builtin_amdgcn_sched_barrier(0);
-      uint32_t v[2][DV / 2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const unsigned char *vp = at + T::TILE + (8 * g4 + 2 * i + j) * ROW + c16 * (DV * 2);
-        if constexpr (DV == 8) {
-          const u32x4 w = *reinterpret_cast<const u32x4 *>(vp);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) v[j][n] = w[n];
-        } else {
-          const u32x2 w = *reinterpret_cast<const u32x2 *>(vp);
-          v[j][0] = w[0];
-          v[j][1] = w[1];
-        }
-      }
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < DV; ++e)
-        vop[e][i] = __builtin_amdgcn_perm(v[1][e >> 1], v[0][e >> 1],
+        vop[e][i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1],
                                           (e & 1) ? 0x07060302u : 0x05040100u);
+    // V's reads first, then the products, with V's transposition as it comes
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+    for (int n = 0; n < 2 * KC * CT; ++n) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x2, (4 * DV + 2 * KC * CT - 1) / (2 * KC * CT), 0);
     }
-    __builtin_amdgcn_sched_barrier(0);
+    float s[CT][8];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[ct][j] = score[ct][j >> 2][j & 3];
     if (tail) {
       // Rows past the end, or of a page outside the pool, take no part
       // whatever they hold.  An infinity or a NaN of a row that a column does not see must not
@@ -316,20 +381,16 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
         }
       if (any != 0) s_special = 1;
     }
+    if (tail) {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const f32x4 s0 = score[ct][0], s1 = score[ct][1];
-      float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] *= a.scale_log2;
-      if (tail) {
-        // bit j: the column sees position r0 + 8 g4 + j
+      for (int ct = 0; ct < CT; ++ct) {
         const int col = mine + 16 * ct + c16;
         const int node =
             static_cast<int>((static_cast<uint32_t>(col) * a.group_inverse) >> 16);
         uint64_t mask = col < cols ? static_cast<uint64_t>(a.masks[token0 + node]) : 0;
         if (nodes < kTreeNodes) mask &= (uint64_t{1} << nodes) - 1;
-        const int rel = r0 + 8 * g4 - past;  // of the lane's first position
+        // bit j: the column sees position r0 + 8 g4 + j
+        const int rel = r0 + 8 * g4 - past;
         uint64_t bits = 0xffu;
         if (rel >= kTreeNodes)
           bits = 0;
@@ -339,136 +400,187 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
           bits = (mask << -rel) | ((1u << -rel) - 1);
         const uint32_t sees = mine_bad ? 0u : static_cast<uint32_t>(bits);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = (sees >> j) & 1 ? s[j] : -INFINITY;
+        for (int j = 0; j < 8; ++j) s[ct][j] = (sees >> j) & 1 ? s[ct][j] : -INFINITY;
       }
-      float bmax = -INFINITY;
+      // (nothing is left under way that a wait behind this would be for)
+      __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 15));
+    }
+    // The reference of the exponents follows the maximum where it is passed by
+    // more than 2^8: until then weights stay in fp32's range, and the columns
+    // keep their scale.
+    float bmax[CT];
+    bool passed = false;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) bmax = fmaxf(bmax, s[j]);
-      TreeColumns<DV> &x = state[ct];
-      bmax = xor32_max(xor16_max(bmax));
-      const float mnew = fmaxf(x.m, bmax);
-      const float alpha = paged_exp2(x.m - mnew);
-      x.m = mnew;
-      float p[8], psum = 0.0f;
+    for (int ct = 0; ct < CT; ++ct) {
+      bmax[ct] = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = paged_exp2(s[j] - mnew);
-        psum += p[j];
-      }
-      x.l = fmaf(x.l, alpha, psum);
-      u32x4 pop, low;
+      for (int j = 0; j < 8; ++j) bmax[ct] = fmaxf(bmax[ct], s[ct][j]);
+      bmax[ct] = xor32_max(xor16_max(bmax[ct]));
+      passed |= bmax[ct] > state[ct].m + a.slack;
+    }
+    if (__any(passed)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const SplitWeights w = split_weights(p[2 * i], p[2 * i + 1]);
-        pop[i] = w.upper;
-        low[i] = w.lower;
-      }
-      if (alpha != 1.0f) {
+      for (int ct = 0; ct < CT; ++ct) {
+        TreeColumns<DV> &x = state[ct];
+        const float m = bmax[ct] > x.m ? bmax[ct] : x.m;
+        const float alpha = paged_exp2((x.m - m) * a.scale_log2);
+        x.m = m;
+        x.l *= alpha;
 #pragma unroll
         for (int e = 0; e < DV; ++e) x.o[e] *= alpha;
       }
+    }
+    u32x4 pop[CT], low[CT];
+    auto weights = [&](int ct) __attribute__((always_inline)) {
+      TreeColumns<DV> &x = state[ct];
+      // (a masked score's -inf stays so)
+      const float base = fminf(-x.m * a.scale_log2, FLT_MAX);
+      float p[8], psum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = paged_exp2(fmaf(s[ct][j], a.scale_log2, base));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) psum += p[j];
+      x.l += psum;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const SplitWeights w = split_weights(p[2 * n], p[2 * n + 1]);
+        pop[ct][n] = w.upper;
+        low[ct][n] = w.lower;
+      }
+    };
+    weights(0);
+    turn(i, slot);
+    read_k(slot == T::DEPTH - 1 ? 0 : slot + 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      TreeColumns<DV> &x = state[ct];
 #pragma unroll
       for (int e = 0; e < DV; ++e) {
-        x.o[e] = mfma_16x16x32_bf16(vop[e], low, x.o[e]);
-        x.o[e] = mfma_16x16x32_bf16(vop[e], pop, x.o[e]);
+        x.o[e] = mfma_16x16x32_bf16(vop[e], low[ct], x.o[e]);
+        x.o[e] = mfma_16x16x32_bf16(vop[e], pop[ct], x.o[e]);
       }
+      if (ct + 1 < CT) weights(ct + 1);
+    }
+    if constexpr (CT > 1) {
+      // a tile's product with V beside the next one's weights
+#pragma unroll
+      for (int n = 0; n < 2 * DV * (CT - 1); ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, 2 * DV, 0);
     }
   };
 
   // (the q rows are here: no wait for them inside the loop)
   __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
-  uint32_t all_bad = 0;
-  int slot = 0;
-  for (int i = 0; i < groups_of; ++i) {
-    // the block's own loads are here, then everyone's, and the slot that is
-    // filled next has been read (no fence: it would wait for all loads)
-    __builtin_amdgcn_s_waitcnt(waitcnt_imm((T::DEPTH - 2) * T::LOADS, 15));
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    const uint32_t bad = ahead[0];
-#pragma unroll
-    for (int d = 0; d + 1 < T::DEPTH - 1; ++d) ahead[d] = ahead[d + 1];
-    ahead[T::DEPTH - 2] = next.bad;
-    issue(block_of(i + T::DEPTH - 1), next, slot == 0 ? T::DEPTH - 1 : slot - 1);
-    next = lookup(block_of(i + T::DEPTH));
-    __builtin_amdgcn_sched_barrier(0);
-    const int blk = first + i * WP + wp;
-    if (blk < end && mine < cols) {
-      all_bad |= bad;
-      step(blk, bad, slot);
+  __builtin_amdgcn_s_barrier();
+  auto next_slot = [](int slot) { return slot == T::DEPTH - 1 ? 0 : slot + 1; };
+  if (mine < cols) {
+    read_k(0);
+    for (int i = 0, slot = 0; i < steps; ++i, slot = next_slot(slot)) step(i, slot);
+  } else {
+    // (columns that this tree has not: the wave's loads alone)
+    for (int i = 0, slot = 0; i < steps; ++i, slot = next_slot(slot)) {
+      all_bad |= first + i * WP + wp < end ? bads & 0xfu : 0u;
+      turn(i, slot);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    slot = slot == T::DEPTH - 1 ? 0 : slot + 1;
   }
   __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
   __syncthreads();
   if (all_bad && lane == 0) flag_range(a.error);
 
-  // the groups' columns join, one tile of them after the other
-  float *s_acc = reinterpret_cast<float *>(s_mem);  // [wave][column][dim]
-  float *s_ml = s_acc + T::WAVES * 16 * D;          // [wave][tile][column][2]
+  // Writes eight dims of a column from their sums and the weights' sum, or,
+  // where the tree has more runs, what these are joined from.
+  auto put = [&](int col, int d, float m, float den, f32x4 (&sum)[2]) __attribute__((always_inline)) {
+    const int node = static_cast<int>((static_cast<uint32_t>(col) * a.group_inverse) >> 16);
+    const int head = kv * a.group + col - node * a.group;
+    if (s_special) {
+      // the infinities and NaN that the blocks with the tree left out
+      const uint64_t mask = static_cast<uint64_t>(a.masks[token0 + node]);
+      const int to = min(end * kPagedBlock, len);
+      for (int p = max(first, past / kPagedBlock) * kPagedBlock; p < to; ++p) {
+        const int page = table[p >> a.page_shift];
+        if (page < 0 || page >= a.num_pages) continue;
+        if (p >= past && !((mask >> (p - past)) & 1)) continue;
+        const uint16_t *v = a.v_pages + page * a.page_stride + kv * a.head_stride +
+                            static_cast<int64_t>(p & page_mask) * D + d;
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const float l = xor32_sum(xor16_sum(state[ct].l));
-    if (g4 == 0) {
-      s_ml[((wave * CT + ct) * 16 + c16) * 2] = state[ct].m;
-      s_ml[((wave * CT + ct) * 16 + c16) * 2 + 1] = l;
+        for (int i = 0; i < 8; ++i) {
+          const float value = bf16_to_f32(v[i]);
+          if (!(fabsf(value) < INFINITY)) sum[i / 4][i % 4] += value;
+        }
+      }
     }
-  }
+    if (!SPLIT || count == 1) {
+      const float by = den == 0.0f ? 0.0f : 1.0f / den;
+      u32x4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        x[i] = den == 0.0f ? 0u
+                           : pack_bf16x2(sum[i / 2][2 * i % 4] * by, sum[i / 2][2 * i % 4 + 1] * by);
+      *reinterpret_cast<u32x4 *>(a.out + (token0 + node) * a.out_token + head * a.out_head + d) = x;
+    } else {
+      const int64_t at =
+          (static_cast<int64_t>(run) * a.max_tree + node) * (a.kv_heads * a.group) + head;
+      f32x4 *to = reinterpret_cast<f32x4 *>(a.part_acc + at * D + d);
+      to[0] = sum[0];
+      to[1] = sum[1];
+      if (d == 0) {
+        a.part_ml[2 * at] = m;
+        a.part_ml[2 * at + 1] = den;
+      }
+    }
+  };
+  float sums[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) sums[ct] = xor32_sum(xor16_sum(state[ct].l));
+  // The groups' columns join in LDS, one tile of them after the other.  o[e][r]
+  // is O[dim DV (4 g4 + r) + e][column c16]; columns are 16 bytes further apart
+  // than their dims are long, so that a lane's column has banks of its own.
+  constexpr int kPitch = T::PITCH;
+  float *s_acc = reinterpret_cast<float *>(s_mem);  // [wave][column][dim]
+  float *s_ml = s_acc + T::WAVES * 16 * kPitch;     // [wave][column][2]
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     if (ct) __syncthreads();
-    // o[e][r] = O[dim DV (4 g4 + r) + e][column c16]
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int e = 0; e < DV; ++e)
-        s_acc[(wave * 16 + c16) * D + DV * (4 * g4 + r) + e] = state[ct].o[e][r];
+      for (int e = 0; e < DV; e += 4) {
+        const TreeColumns<DV> &x = state[ct];
+        const f32x4 v = {x.o[e][r], x.o[e + 1][r], x.o[e + 2][r], x.o[e + 3][r]};
+        *reinterpret_cast<f32x4 *>(s_acc + (wave * 16 + c16) * kPitch + DV * (4 * g4 + r) + e) = v;
+      }
+    if (g4 == 0) {
+      s_ml[(wave * 16 + c16) * 2] = state[ct].m;
+      s_ml[(wave * 16 + c16) * 2 + 1] = sums[ct];
+    }
     __syncthreads();
-    for (int i = tid; i < WC * 16 * D; i += T::WAVES * kWave) {
-      const int w = i / (16 * D), c = i / D % 16, d = i % D;
+    for (int i = tid; i < WC * 2 * D; i += T::WAVES * kWave) {
+      const int w = i / (2 * D), c = i / (D / 8) % 16, d = 8 * (i % (D / 8));
       const int col = col0 + 16 * (CT * w + ct) + c;
       if (col >= cols) continue;
       float mm = -FLT_MAX;
 #pragma unroll
-      for (int k = 0; k < WP; ++k)
-        mm = fmaxf(mm, s_ml[(((k * WC + w) * CT + ct) * 16 + c) * 2]);
-      float den = 0.0f, sum = 0.0f;
+      for (int k = 0; k < WP; ++k) mm = fmaxf(mm, s_ml[((k * WC + w) * 16 + c) * 2]);
+      float den = 0.0f;
+      f32x4 sum[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
       for (int k = 0; k < WP; ++k) {
-        const float *ml = s_ml + (((k * WC + w) * CT + ct) * 16 + c) * 2;
-        const float wt = paged_exp2(ml[0] - mm);
-        den = fmaf(wt, ml[1], den);
-        sum = fmaf(wt, s_acc[((k * WC + w) * 16 + c) * D + d], sum);
-      }
-      const int node = static_cast<int>((static_cast<uint32_t>(col) * a.group_inverse) >> 16);
-      const int head = kv * a.group + col - node * a.group;
-      if (s_special) {
-        const uint64_t mask = static_cast<uint64_t>(a.masks[token0 + node]);
-        const int to = min(end * kPagedBlock, len);
-        for (int p = max(first, past / kPagedBlock) * kPagedBlock; p < to; ++p) {
-          const int page = table[p >> a.page_shift];
-          if (page < 0 || page >= a.num_pages) continue;
-          if (p >= past && !((mask >> (p - past)) & 1)) continue;
-          const float value =
-              bf16_to_f32(a.v_pages[page * a.page_stride + kv * a.head_stride +
-                                    static_cast<int64_t>(p & page_mask) * D + d]);
-          if (!(fabsf(value) < INFINITY)) sum += value;
+        const int from = (k * WC + w) * 16 + c;
+        const float wt = paged_exp2((s_ml[from * 2] - mm) * a.scale_log2);
+        den = fmaf(wt, s_ml[from * 2 + 1], den);
+        const f32x4 *x = reinterpret_cast<const f32x4 *>(s_acc + from * kPitch + d);
+        const f32x4 x0 = x[0], x1 = x[1];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          sum[0][n] = fmaf(wt, x0[n], sum[0][n]);
+          sum[1][n] = fmaf(wt, x1[n], sum[1][n]);
         }
       }
-      if (!SPLIT || count == 1) {
-        a.out[(token0 + node) * a.out_token + head * a.out_head + d] =
-            f32_to_bf16(den == 0.0f ? 0.0f : sum / den);
-      } else {
-        const int64_t at =
-            (static_cast<int64_t>(run) * a.max_tree + node) * (a.kv_heads * a.group) + head;
-        a.part_acc[at * D + d] = sum;
-        if (d == 0) {
-          a.part_ml[2 * at] = mm;
-          a.part_ml[2 * at + 1] = den;
-        }
-      }
+      put(col, d, mm, den, sum);
     }
   }
 }
@@ -510,7 +622,8 @@ __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs 
       const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * at);
       const f32x4 v = *reinterpret_cast<const f32x4 *>(a.part_acc + at * D + 4 * d);
       const float mnew = fmaxf(m, ml.x);
-      const float keep = paged_exp2(m - mnew), w = paged_exp2(ml.x - mnew);
+      const float keep = paged_exp2((m - mnew) * a.scale_log2);
+      const float w = paged_exp2((ml.x - mnew) * a.scale_log2);
       m = mnew;
       den = fmaf(w, ml.y, den * keep);
 #pragma unroll
@@ -532,7 +645,7 @@ __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs 
     float sum = 0.0f, r = 0.0f;
 #pragma unroll
     for (int k = 0; k < SLICES; ++k) {
-      const float w = paged_exp2(s_ml[hh][k][0] - mm);
+      const float w = paged_exp2((s_ml[hh][k][0] - mm) * a.scale_log2);
       sum = fmaf(w, s_ml[hh][k][1], sum);
       r = fmaf(w, s_acc[hh][k][dim / 4][dim % 4], r);
     }
@@ -568,9 +681,9 @@ static TreePlan tree_plan(int64_t trees, int64_t max_tree, int64_t q_heads, int6
   auto wanted = [trees](int64_t runs) {
     return runs - trees / 2 > runs / 2 ? runs - trees / 2 : (runs + 1) / 2;
   };
-  p.two = wanted(2 * slots);
+  p.two = wanted(4 * slots);
   p.round = wanted(slots);
-  if (3 * trees > p.round) p.round = p.two;
+  if (3 * trees > p.round) p.round = wanted(2 * slots);
   p.runs = p.two + trees;
   const int64_t most = trees * ((blocks + kPagedMinRun - 1) / kPagedMinRun);
   if (p.runs > most) p.runs = most;
@@ -593,8 +706,8 @@ static hipError_t launch_tree(const TreeArgs &a, int shape, int64_t blocks, hipS
   }
   switch (shape) {
     case 1: CASCADE_TREE(1, 1, 4)
-    case 2: CASCADE_TREE(2, 1, 4)
-    case 4: CASCADE_TREE(2, 2, 4)
+    case 2: CASCADE_TREE(1, 2, 2)
+    case 4: CASCADE_TREE(1, 4, 2)
     case 8: CASCADE_TREE(2, 4, 2)
     default: CASCADE_TREE(2, 8, 1)
   }
@@ -793,7 +906,12 @@ extern "C" int cascade_paged_tree_attention_bf16(
   a.rows = rows;
   a.max_length = static_cast<int32_t>(max_length);
   a.group = static_cast<int32_t>(n_q_heads / n_kv_heads);
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
+  a.sign = scale < 0.0f ? 0x80008000u : 0u;
+  // (a scale of zero would make a masked score's infinity a NaN: finite scores do
+  // not show one as small as this)
+  if (a.scale_log2 < 1e-37f) a.scale_log2 = 1e-37f;
+  a.slack = 8.0f / a.scale_log2;
   a.out = static_cast<uint16_t *>(out);
   a.out_token = out_token_stride;
   a.out_head = out_head_stride;
