@@ -1525,28 +1525,10 @@ def paged_tree_attention(q, starts, masks, k_pages, v_pages, page_table, lengths
     return out
 
 
-def paged_tree_accept(starts, ids, parents, targets, path, counts, next_ids,
-                      pages=None, page_table=None, lengths=None, rows=None,
-                      error_flag=None, stream=None):
-    """Follow the drawn tokens through drafted trees, and keep the K and V rows
-    of the nodes on their paths.
-
-    Tree b has the rows ``starts[b]`` .. ``starts[b + 1]`` - 1 (int32 [trees +
-    1]); of each row ``ids`` (int64 [tokens]) is the node's own token,
-    ``parents`` (int32 [tokens]) its parent's place in the tree, before its
-    own, and ``targets`` (int64 [tokens]) the token drawn there.  From node 0 on, the
-    path goes to the first child whose own token is the one drawn.  ``path``
-    (int32 [trees, max_tree], max_tree <= 64) lists its nodes, -1 behind them;
-    ``counts`` (int32 [trees]) their number, ``next_ids`` (int64 [trees]) the
-    token drawn at the last.  No nodes, a negative ``rows[b]`` and a tree out
-    of range: 0 and -1.
-
-    ``pages``: a contiguous pool [layers, 2, pages, kv_heads, page_size, dim]
-    whose rows of the path move to the front of the tree, the j-th node's to
-    position lengths[r] - n + j of page table row r = ``rows[b]`` (b without
-    ``rows``; no row twice) with n nodes.  Rows, lengths and pages out of range
-    are left out and flagged (PAGED_ERANGE in ``error_flag``).  Returns
-    ``path``."""
+def _check_accept(starts, ids, parents, targets, path, counts, next_ids, pages,
+                  page_table, lengths, rows, error_flag):
+    """The checks of paged_tree_accept; returns trees, tokens, the path's width
+    and the sizes of pool and table."""
 
     device = _gpu_of("starts", starts)
     _placed(device, "starts", starts, _I32, 1)
@@ -1585,6 +1567,82 @@ def paged_tree_accept(starts, ids, parents, targets, path, counts, next_ids,
             raise ValueError("more trees than page table rows (give rows)")
     elif page_table is not None or lengths is not None:
         raise ValueError("page_table and lengths without pages")
+    return trees, tokens, max_tree, (planes, plane_bytes, count, kv_heads, page_size,
+                                     row_bytes, table_stride, sequences, width)
+
+
+def paged_tree_accept(starts, ids, parents, targets, path, counts, next_ids,
+                      pages=None, page_table=None, lengths=None, rows=None,
+                      error_flag=None, stream=None):
+    """Follow the drawn tokens through drafted trees, and keep the K and V rows
+    of the nodes on their paths.
+
+    Tree b has the rows ``starts[b]`` .. ``starts[b + 1]`` - 1 (int32 [trees +
+    1]); of each row ``ids`` (int64 [tokens]) is the node's own token,
+    ``parents`` (int32 [tokens]) its parent's place in the tree, before its
+    own, and ``targets`` (int64 [tokens]) the token drawn there.  From node 0 on, the
+    path goes to the first child whose own token is the one drawn.  ``path``
+    (int32 [trees, max_tree], max_tree <= 64) lists its nodes, -1 behind them;
+    ``counts`` (int32 [trees]) their number, ``next_ids`` (int64 [trees]) the
+    token drawn at the last.  No nodes, a negative ``rows[b]`` and a tree out
+    of range: 0 and -1.
+
+    ``pages``: a contiguous pool [layers, 2, pages, kv_heads, page_size, dim]
+    whose rows of the path move to the front of the tree, the j-th node's to
+    position lengths[r] - n + j of page table row r = ``rows[b]`` (b without
+    ``rows``; no row twice) with n nodes.  Rows, lengths and pages out of range
+    are left out and flagged (PAGED_ERANGE in ``error_flag``).  Returns
+    ``path``."""
+
+    try:
+        index = starts.get_device()
+        trees, max_tree = path.shape
+        tokens, = shape = ids.shape
+        each = (trees,)
+        ordinary = (
+            index >= 0 and tokens > 0 and trees > 0 and 0 < max_tree <= 64
+            and starts.dtype is _I32 and ids.dtype is _LONG and parents.dtype is _I32
+            and targets.dtype is _LONG and path.dtype is _I32 and counts.dtype is _I32
+            and next_ids.dtype is _LONG
+            and index == ids.get_device() == parents.get_device() == targets.get_device()
+            == path.get_device() == counts.get_device() == next_ids.get_device()
+            and starts.shape == (trees + 1,) and parents.shape == shape
+            and targets.shape == shape and counts.shape == each and next_ids.shape == each
+            and starts.is_contiguous() and ids.is_contiguous() and parents.is_contiguous()
+            and targets.is_contiguous() and path.is_contiguous() and counts.is_contiguous()
+            and next_ids.is_contiguous()
+            and (rows is None or (
+                rows.dtype is _I32 and rows.get_device() == index and rows.shape == each
+                and rows.is_contiguous()))
+            and (error_flag is None or (
+                error_flag.dtype is _I32 and error_flag.get_device() == index
+                and error_flag.numel() > 0)))
+        planes = plane_bytes = count = kv_heads = page_size = row_bytes = 0
+        table_stride = sequences = width = 0
+        if pages is not None:
+            layers, pair, count, kv_heads, page_size, dim = pages.shape
+            sequences, width = page_table.shape
+            table_stride, table_last = page_table.stride()
+            planes, row_bytes = 2 * layers, 2 * dim
+            plane_bytes = count * kv_heads * page_size * row_bytes
+            ordinary = (
+                ordinary and pair == 2 and pages.dtype is _BF16 and pages.is_contiguous()
+                and page_table.dtype is _I32 and lengths.dtype is _I32
+                and index == pages.get_device() == page_table.get_device()
+                == lengths.get_device()
+                and table_last == 1 and table_stride >= width
+                and lengths.shape == (sequences,) and lengths.is_contiguous()
+                and (rows is not None or trees <= sequences))
+        elif page_table is not None or lengths is not None:
+            ordinary = False
+    except (AttributeError, IndexError, TypeError, ValueError, RuntimeError):
+        ordinary = False
+    if not ordinary:
+        trees, tokens, max_tree, (planes, plane_bytes, count, kv_heads, page_size,
+                                  row_bytes, table_stride, sequences, width) = (
+            _check_accept(starts, ids, parents, targets, path, counts, next_ids, pages,
+                          page_table, lengths, rows, error_flag))
+        index = starts.get_device()
     if trees == 0:
         return path
     if tokens == 0:
@@ -1593,7 +1651,7 @@ def paged_tree_accept(starts, ids, parents, targets, path, counts, next_ids,
         next_ids.fill_(-1)
         return path
     _call_on(
-        device.index, stream, "cascade_paged_tree_accept", starts.data_ptr(),
+        index, stream, "cascade_paged_tree_accept", starts.data_ptr(),
         ids.data_ptr(), parents.data_ptr(), targets.data_ptr(), tokens, trees, max_tree,
         path.data_ptr(), counts.data_ptr(), next_ids.data_ptr(),
         0 if pages is None else pages.data_ptr(), planes, plane_bytes, count, kv_heads,
@@ -1689,75 +1747,90 @@ def _row_stride(device, name, tensor, dtype, shape):
     stride, last = tensor.stride()
     if columns > 1 and last != 1:
         raise ValueError("the rows of {} must be contiguous".format(name))
-    if rows == 1:
-        return columns
-    return stride
+    return columns if rows == 1 else stride
 
 
-def _w4_matrix(name, matrix):
-    if not isinstance(matrix, W4Matrix):
-        raise TypeError("{} must be a W4Matrix".format(name))
-
-
-def _w4_pointers(device, name, matrix, k):
-    if matrix.packed.device != device:
-        raise ValueError("{} must live on {}, got {}".format(
-            name, device, matrix.packed.device))
-    if matrix.k != k:
-        raise ValueError("{} has {} columns, x {}".format(name, matrix.k, k))
-    return (matrix.packed.data_ptr(), matrix.scales.data_ptr(),
-            0 if matrix.zeros is None else matrix.zeros.data_ptr())
-
-
-def _w4_rows(x, out, dtype, n):
-    """Checks x and out of a 4-bit product; returns (device, m, k, strides)."""
+def _check_w4(x, out, dtype, residual, workspace, **matrices):
+    """The checks of the products with 4-bit weights; returns (rows, the row
+    strides of x, out and residual)."""
 
     device = _gpu_of("x", x)
     x_stride = _row_stride(device, "x", x, _BF16, None)
     m, k = x.shape
+    for name, matrix in matrices.items():
+        if not isinstance(matrix, W4Matrix):
+            raise TypeError("{} must be a W4Matrix".format(name))
+        if matrix.device != device:
+            raise ValueError("{} must live on {}, got {}".format(
+                name, device, matrix.device))
+        if matrix.k != k:
+            raise ValueError("{} has {} columns, x {}".format(name, matrix.k, k))
+    n = matrix.n
     y_stride = _row_stride(device, "out", out, dtype, (m, n))
     if m > 1 and y_stride < n:
         raise ValueError("the rows of out overlap")
     if m and x.data_ptr() == out.data_ptr():
         raise ValueError("out may not be x")
-    if m == 1:
-        x_stride = (k + 7) // 8 * 8
-    return device, m, k, x_stride, y_stride
+    residual_stride = 0
+    if residual is not None:
+        residual_stride = _row_stride(device, "residual", residual, _BF16, (m, n))
+    if workspace is not None:
+        _check_bytes(device, workspace)
+    return m, x_stride, y_stride, residual_stride
 
 
 def linear_w4(x, matrix, out, residual=None, workspace=None, stream=None):
     """out = x W^T (+ residual) for a W4Matrix [n, k].
 
     ``x`` bf16 [rows, k] (row stride a multiple of 8), ``out`` [rows, n] bf16,
-    or fp32 for rows that are not rounded (logits; without residual), ``residual`` bf16
-    [rows, n], which may be ``out``.  Sums are fp32, with one rounding at the
-    end.  ``workspace``: linear_w4_workspace_bytes(rows, n, k) uint8, one each for
-    calls that may overlap; None where that is 0."""
+    or fp32 for rows that are not rounded (logits; without residual), ``residual``
+    bf16 [rows, n], which may be ``out``.  Sums are fp32, with one rounding at
+    the end.  ``workspace``: linear_w4_workspace_bytes(rows, n, k) uint8, one
+    each for calls that may overlap; None where that is 0."""
 
-    _w4_matrix("matrix", matrix)
-    logits = isinstance(out, torch.Tensor) and out.dtype is _F32
-    device, m, k, x_stride, y_stride = _w4_rows(x, out, _F32 if logits else _BF16,
-                                                matrix.n)
-    packed, scales, zeros = _w4_pointers(device, "matrix", matrix, k)
-    residual_stride = 0
-    if residual is not None:
-        if logits:
+    try:
+        index, packed, scales, zeros, n, k, group = matrix.launch
+        m, x_columns = x.shape
+        x_stride, x_last = x.stride()
+        y_type = out.dtype
+        x_ptr, y_ptr = x.data_ptr(), out.data_ptr()
+        y_stride = n
+        residual_stride = residual_ptr = 0
+        ordinary = (
+            x_columns == k and x_last == 1 and m > 0 and x.dtype is _BF16
+            and out.shape == (m, n) and out.is_contiguous()
+            and (y_type is _BF16 or (y_type is _F32 and residual is None))
+            and index == x.get_device() == out.get_device() and x_ptr != y_ptr)
+        if residual is not None:
+            residual_stride, residual_ptr = n, residual.data_ptr()
+            ordinary = (
+                ordinary and residual.shape == (m, n) and residual.is_contiguous()
+                and residual.dtype is _BF16 and residual.get_device() == index)
+        space = (0, 0)
+        if workspace is not None:
+            space = workspace.data_ptr(), workspace.numel()
+            ordinary = (
+                ordinary and workspace.dtype is _U8 and workspace.is_contiguous()
+                and workspace.dim() == 1 and workspace.get_device() == index)
+        if m == 1:
+            x_stride = k
+    except (AttributeError, IndexError, TypeError, ValueError, RuntimeError):
+        ordinary = False
+    if not ordinary:
+        y_type = _F32 if isinstance(out, torch.Tensor) and out.dtype is _F32 else _BF16
+        m, x_stride, y_stride, residual_stride = _check_w4(
+            x, out, y_type, residual, workspace, matrix=matrix)
+        if y_type is _F32 and residual is not None:
             raise ValueError("fp32 rows take no residual")
-        residual_stride = _row_stride(device, "residual", residual, _BF16, out.shape)
-    if workspace is not None:
-        _check_bytes(device, workspace)
-    if m == 0:
-        return out
-    space = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
-    if logits:
-        _call_on(device.index, stream, "cascade_linear_w4_f32out_bf16", x.data_ptr(),
-                 x_stride, packed, scales, zeros, m, matrix.n, k, matrix.group,
-                 out.data_ptr(), y_stride, *space)
+        if m == 0:
+            return out
+    if y_type is _F32:
+        _call_on(index, stream, "cascade_linear_w4_f32out_bf16", x_ptr, x_stride, packed,
+                 scales, zeros, m, n, k, group, y_ptr, y_stride, *space)
     else:
-        _call_on(device.index, stream, "cascade_linear_w4_bf16", x.data_ptr(),
-                 x_stride, packed, scales, zeros, m, matrix.n, k, matrix.group,
-                 0 if residual is None else residual.data_ptr(), residual_stride,
-                 out.data_ptr(), y_stride, *space)
+        _call_on(index, stream, "cascade_linear_w4_bf16", x_ptr, x_stride, packed, scales,
+                 zeros, m, n, k, group, residual_ptr, residual_stride, y_ptr, y_stride,
+                 *space)
     return out
 
 
@@ -1766,18 +1839,31 @@ def gate_up_swiglu_w4(x, gate, up, out, stream=None):
     both with zero points or neither; ``x`` bf16 [rows, k], ``out`` bf16
     [rows, n].  Sums are fp32, with one rounding at the end."""
 
-    _w4_matrix("gate", gate)
-    _w4_matrix("up", up)
-    device, m, k, x_stride, y_stride = _w4_rows(x, out, _BF16, gate.n)
-    gate_pointers = _w4_pointers(device, "gate", gate, k)
-    up_pointers = _w4_pointers(device, "up", up, k)
-    if (up.n, up.group, up.zeros is None) != (gate.n, gate.group, gate.zeros is None):
-        raise ValueError("gate and up differ in rows, group size or zero points")
-    if m == 0:
-        return out
-    _call_on(device.index, stream, "cascade_gate_up_swiglu_w4_bf16", x.data_ptr(),
-             x_stride, *gate_pointers, *up_pointers, m, gate.n, k, gate.group,
-             out.data_ptr(), y_stride)
+    try:
+        index, *gate_parts, n, k, group = gate.launch
+        up_index, *up_parts, up_n, up_k, up_group = up.launch
+        m, x_columns = x.shape
+        x_stride, x_last = x.stride()
+        x_ptr, y_ptr = x.data_ptr(), out.data_ptr()
+        y_stride = n
+        ordinary = (
+            x_columns == k == up_k and n == up_n and group == up_group and x_last == 1
+            and m > 0 and (gate_parts[2] == 0) == (up_parts[2] == 0)
+            and x.dtype is _BF16 and out.dtype is _BF16
+            and out.shape == (m, n) and out.is_contiguous()
+            and index == up_index == x.get_device() == out.get_device() and x_ptr != y_ptr)
+        if m == 1:
+            x_stride = k
+    except (AttributeError, IndexError, TypeError, ValueError, RuntimeError):
+        ordinary = False
+    if not ordinary:
+        m, x_stride, y_stride, _ = _check_w4(x, out, _BF16, None, None, gate=gate, up=up)
+        if (up.n, up.group, up.zeros is None) != (gate.n, gate.group, gate.zeros is None):
+            raise ValueError("gate and up differ in rows, group size or zero points")
+        if m == 0:
+            return out
+    _call_on(index, stream, "cascade_gate_up_swiglu_w4_bf16", x_ptr, x_stride, *gate_parts,
+             *up_parts, m, n, k, group, y_ptr, y_stride)
     return out
 
 

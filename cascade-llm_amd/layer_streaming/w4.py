@@ -43,6 +43,9 @@ class W4Matrix:
                 raise ValueError("{} must be contiguous and 16-byte aligned".format(name))
         self._parts = packed, scales, zeros
         self._sizes = n, k, group
+        # what a launch takes of it: device index, addresses, sizes
+        self._launch = (packed.get_device(), packed.data_ptr(), scales.data_ptr(),
+                        0 if zeros is None else zeros.data_ptr(), n, k, group)
 
     packed = property(lambda self: self._parts[0])
     scales = property(lambda self: self._parts[1])
@@ -50,6 +53,7 @@ class W4Matrix:
     n = property(lambda self: self._sizes[0])
     k = property(lambda self: self._sizes[1])
     group = property(lambda self: self._sizes[2])
+    launch = property(lambda self: self._launch)
 
     @classmethod
     def pack(cls, values, scales, zeros=None, group=128):
