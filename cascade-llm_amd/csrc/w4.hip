@@ -28,13 +28,15 @@ struct W4Args {
   void *y;
   int64_t y_stride;
   int32_t f32;  // y's type
+  int32_t once;  // the matrix is read past the caches
+  int32_t wide;  // four columns of y and residual are one access
+  int32_t splits;  // of K over workgroups
+  float *partial;  // [splits][m][16 ceil(n / 16)] of these
 };
 
 enum W4Out { kW4Bf16, kW4F32, kW4Swiglu };
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
-constexpr uint32_t kW4Ones = 0x3f803f80u;  // 1.0 twice
 
 // Eight 4-bit values of a packed word as 16 + q in bf16, an MFMA operand: the
 // value lands in the upper mantissa bits of 16.0, so one rotation and one
@@ -73,185 +75,48 @@ __device__ __forceinline__ Rsrc w4_rsrc(const void *base, int64_t bytes) {
 }
 
 constexpr int kNontemporal = 2;
-constexpr int64_t kW4FewBytes = 64 * 1024;  // of x in LDS
+// Matrices of which the memory-side cache (256 MB) holds little at the next
+// pass go past it: 5 rows by 128256 x 4096 (263 MB) 51.9 -> 49.3 us.  Smaller
+// ones lose: gate and up 14336 x 4096 (59 MB), one row, 12.4 -> 13.4.
+constexpr int64_t kW4OnceBytes = 128 << 20;
 constexpr int kOutside = 0x7f000000;  // past every descriptor's end, with room for 2^24 more
 
-// The output of four matrix rows for one row of x.  (One loop after the other:
-// the residual's loads wait for nothing.)
+// The output of four matrix rows for one row of x.
 __device__ __forceinline__ void w4_store(const W4Args &a, f32x4 v, int row, int col) {
   const int64_t y = row * a.y_stride + col;
-  const int count = min(4, a.n - col);
-  if (a.residual != nullptr) {
-    const uint16_t *from = a.residual + row * a.residual_stride + col;
-    uint16_t add[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (r < count) add[r] = from[r];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] += bf16_to_f32(add[r]);
+  if (a.wide && col + 4 <= a.n) {
+    if (a.f32) {
+      *reinterpret_cast<f32x4 *>(static_cast<float *>(a.y) + y) = v;
+      return;
+    }
+    if (a.residual != nullptr) {
+      const u32x2 add =
+          *reinterpret_cast<const u32x2 *>(a.residual + row * a.residual_stride + col);
+      v[0] += lo_bf16(add[0]);
+      v[1] += hi_bf16(add[0]);
+      v[2] += lo_bf16(add[1]);
+      v[3] += hi_bf16(add[1]);
+    }
+    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.y) + y) =
+        u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    return;
   }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    if (r >= count) break;
-    if (a.f32)
-      static_cast<float *>(a.y)[y + r] = v[r];
-    else
-      static_cast<uint16_t *>(a.y)[y + r] = f32_to_bf16(v[r]);
+  for (int r = 0; r < 4 && col + r < a.n; ++r) {
+    float out = v[0];
+    if (a.f32) {
+      static_cast<float *>(a.y)[y + r] = out;
+    } else {
+      if (a.residual != nullptr)
+        out += bf16_to_f32(a.residual[row * a.residual_stride + col + r]);
+      static_cast<uint16_t *>(a.y)[y + r] = f32_to_bf16(out);
+    }
+    v = f32x4{v[1], v[2], v[3], 0.0f};  // (no indexing of registers)
   }
 }
 
-// Few rows of x, all of them in LDS: M rows as MFMA operands, tile by tile.
-template <bool SWIGLU, bool ZEROS, int NT, int WAVES, int D, int GP>
-__global__ __launch_bounds__(WAVES * kWave) void w4_few_kernel(W4Args a) {
-  constexpr int RT = SWIGLU ? NT / 2 : NT;  // tiles of output columns
-  constexpr int J = 4 / GP;                 // operands a group
-  extern __shared__ u32x4 s_mem[];
-  const int tid = threadIdx.x;
-  const int lane = tid & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int c16 = lane & 15, g4 = lane >> 4;
-  const int t0 = static_cast<int>(blockIdx.x) * RT;
-  const int last_tile = (a.n + 15) / 16 - 1;
-
-  Rsrc wr[NT], sr[NT], zr[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const W4Matrix &w = a.w[SWIGLU ? i / RT : 0];
-    const int64_t row = min(t0 + i % RT, last_tile);
-    wr[i] = w4_rsrc(w.packed + row * a.tiles * kWave, static_cast<int64_t>(a.tiles) * 1024);
-    sr[i] = w4_rsrc(w.scales + row * a.groups * 16, static_cast<int64_t>(a.groups) * 32);
-    if constexpr (ZEROS)
-      zr[i] = w4_rsrc(w.zeros + row * a.groups * 16, static_cast<int64_t>(a.groups) * 16);
-  }
-  const int woff = lane * 16, soff = g4 * 8, zoff = g4 * 4;
-  struct Tile {
-    u32x4 w[NT];
-    u32x2 scale[NT][GP];
-    uint32_t zero[NT][GP];
-  };
-  auto load = [&](int t, Tile &f) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      f.w[i] = __builtin_amdgcn_raw_buffer_load_b128(wr[i], woff + t * 1024, 0, kNontemporal);
-#pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        f.scale[i][g] = __builtin_amdgcn_raw_buffer_load_b64(sr[i], soff + (t * GP + g) * 32, 0, 0);
-        if constexpr (ZEROS)
-          f.zero[i][g] =
-              __builtin_amdgcn_raw_buffer_load_b32(zr[i], zoff + (t * GP + g) * 16, 0, 0);
-      }
-    }
-  };
-  Tile ring[D];
-#pragma unroll
-  for (int p = 0; p < D - 1; ++p) load(wave + p * WAVES, ring[p]);
-  __builtin_amdgcn_sched_barrier(0);
-  // unit (tile and quarter, row, eighth of the quarter)
-  const int units = a.tiles * 16 * a.m;
-  const Rsrc xr = w4_rsrc(a.x, (static_cast<int64_t>(a.m - 1) * a.x_stride + a.k) * 2);
-  for (int u = tid; u < units; u += WAVES * kWave) {
-    const int part = u / (4 * a.m), rest = u - part * (4 * a.m);
-    const int k = 32 * part + 8 * (rest & 3);
-    s_mem[u] = __builtin_amdgcn_raw_buffer_load_b128(
-        xr, k < a.k ? ((rest >> 2) * static_cast<int>(a.x_stride) + k) * 2 : kOutside, 0, 0);
-  }
-  __syncthreads();
-  const int xrow = min(c16, a.m - 1) * 4 + g4;  // columns past the last repeat it
-  f32x4 acc[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr uint32_t kFirst = ZEROS ? kW4Ones : 0xc1c0c1c0u;
-  const u32x4 ones = {kFirst, kFirst, kFirst, kFirst};
-  auto step = [&](int t, const Tile &f) __attribute__((always_inline)) {
-    u32x4 x[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = s_mem[(4 * t + j) * (4 * a.m) + xrow];
-#pragma unroll
-    for (int g = 0; g < GP; ++g) {
-      f32x4 xs = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int j = 0; j < J; ++j) xs = mfma_16x16x32_bf16(ones, x[J * g + j], xs);
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const uint32_t s01 = f.scale[i][g][0], s23 = f.scale[i][g][1];
-        const float scale[4] = {lo_bf16(s01), hi_bf16(s01), lo_bf16(s23), hi_bf16(s23)};
-        f32x4 part = xs;
-        if constexpr (ZEROS) {
-          const uint32_t z = f.zero[i][g];
-          const float x16 = -16.0f * xs[0];  // (a column's sums are all alike)
-          part[0] = fmaf(static_cast<float>(z & 255u), -xs[0], x16);
-          part[1] = fmaf(static_cast<float>((z >> 8) & 255u), -xs[0], x16);
-          part[2] = fmaf(static_cast<float>((z >> 16) & 255u), -xs[0], x16);
-          part[3] = fmaf(static_cast<float>(z >> 24), -xs[0], x16);
-        }
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const uint32_t word = f.w[i][J * g + j];
-          part = mfma_16x16x32_bf16(w4_operand(word), x[J * g + j], part);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(scale[r], part[r], acc[i][r]);
-      }
-    }
-  };
-  for (int t = wave; t < a.tiles;) {
-#pragma unroll
-    for (int p = 0; p < D; ++p) {
-      load(t + (D - 1) * WAVES, ring[(p + D - 1) % D]);
-      __builtin_amdgcn_sched_barrier(0);
-      if (t < a.tiles) step(t, ring[p]);
-      __builtin_amdgcn_sched_barrier(0);
-      t += WAVES;
-    }
-  }
-  __syncthreads();
-  f32x4 *s_sum = reinterpret_cast<f32x4 *>(s_mem);
-#pragma unroll
-  for (int i = 0; i < NT; ++i) s_sum[(wave * NT + i) * kWave + lane] = acc[i];
-  __syncthreads();
-  for (int item = tid; item < RT * kWave; item += WAVES * kWave) {
-    auto joined = [&](int at) {
-      f32x4 v = s_sum[at];
-#pragma unroll
-      for (int w = 1; w < WAVES; ++w) {
-        const f32x4 u = s_sum[w * NT * kWave + at];
-        v += u;
-      }
-      return v;
-    };
-    f32x4 v = joined(item);
-    if constexpr (SWIGLU) {
-      const f32x4 u = joined(item + RT * kWave);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = v[r] / (1.0f + __expf(-v[r])) * u[r];
-    }
-    const int at = item % kWave, row = at & 15;
-    if (row < a.m) w4_store(a, v, row, 16 * (t0 + item / kWave) + 4 * (at >> 4));
-  }
-}
-
-template <bool SWIGLU, int NT, int WAVES, int D>
-static int launch_w4_few(const W4Args &a, hipStream_t s) {
-  constexpr int RT = SWIGLU ? NT / 2 : NT;
-  const int64_t tiles = (a.n + 15) / 16;
-  const int64_t x = (tiles + RT - 1) / RT;
-  if (x > 0xffffffffll / (WAVES * kWave)) return CASCADE_ESHAPE;
-  size_t lds = static_cast<size_t>(a.tiles) * 256 * a.m;
-  if (lds < size_t{WAVES} * NT * 1024) lds = size_t{WAVES} * NT * 1024;
-  const dim3 grid(static_cast<unsigned>(x));
-  const dim3 block(WAVES * kWave);
-  const int which = (a.group_shift - 5) + (a.w[0].zeros != nullptr ? 3 : 0);
-  switch (which) {
-    case 0: return launch_kernel(w4_few_kernel<SWIGLU, false, NT, WAVES, D, 4>, grid, block, lds, s, a);
-    case 1: return launch_kernel(w4_few_kernel<SWIGLU, false, NT, WAVES, D, 2>, grid, block, lds, s, a);
-    case 2: return launch_kernel(w4_few_kernel<SWIGLU, false, NT, WAVES, D, 1>, grid, block, lds, s, a);
-    case 3: return launch_kernel(w4_few_kernel<SWIGLU, true, NT, WAVES, D, 4>, grid, block, lds, s, a);
-    case 4: return launch_kernel(w4_few_kernel<SWIGLU, true, NT, WAVES, D, 2>, grid, block, lds, s, a);
-    default: return launch_kernel(w4_few_kernel<SWIGLU, true, NT, WAVES, D, 1>, grid, block, lds, s, a);
-  }
-}
-
-// Rows of x through LDS: see "Rings".
+// Loads to LDS that the compiler does not see (dma_lds16): 4 bytes a lane, and
+// with a scalar part of the offset, which the bounds do not see: for what is
+// known to lie inside.
 __device__ __forceinline__ void dma_lds4(const u32x4 &rsrc, int voff, uint32_t lds) {
   u32x4 r;
   r.x = __builtin_amdgcn_readfirstlane(rsrc.x);
@@ -263,32 +128,78 @@ __device__ __forceinline__ void dma_lds4(const u32x4 &rsrc, int voff, uint32_t l
                : "memory", "m0");
 }
 
-template <bool SWIGLU, bool ZEROS, int GP, int NT, int MT, int WN, int WK, int D>
-struct W4Ring {
+__device__ __forceinline__ void dma_lds16_inside(const u32x4 &rsrc, int voff, int soff,
+                                                 uint32_t lds) {
+  u32x4 r;
+  r.x = __builtin_amdgcn_readfirstlane(rsrc.x);
+  r.y = __builtin_amdgcn_readfirstlane(rsrc.y);
+  r.z = __builtin_amdgcn_readfirstlane(rsrc.z);
+  r.w = __builtin_amdgcn_readfirstlane(rsrc.w);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r),
+                  "s"(__builtin_amdgcn_readfirstlane(soff))
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma_lds4_inside(const u32x4 &rsrc, int voff, int soff,
+                                                uint32_t lds) {
+  u32x4 r;
+  r.x = __builtin_amdgcn_readfirstlane(rsrc.x);
+  r.y = __builtin_amdgcn_readfirstlane(rsrc.y);
+  r.z = __builtin_amdgcn_readfirstlane(rsrc.z);
+  r.w = __builtin_amdgcn_readfirstlane(rsrc.w);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r),
+                  "s"(__builtin_amdgcn_readfirstlane(soff))
+               : "memory", "m0");
+}
+
+// y[r, i] = sum over K of x[r, k] scale[i, k/group] (q[i, k] - zero[i, k/group]).
+//
+// A wave holds NT tiles of 16 matrix rows (A) by MT of 16 rows of x (B) and goes
+// through K in steps of 128 columns; WN waves share a step's x, WK waves take
+// turns at the steps and are joined at the end, and a long K is split over
+// a.splits workgroups, joined by a second launch.
+//
+// The weights become MFMA operands without a float conversion: 4 bits in the
+// mantissa of 16 (or 32 .. 63) are 16 + q, and the product's sum begins with
+// -24 (or, with zero points in the operand, -48) times the sum of x, which is
+// an MFMA of its own for all NT tiles.  Both are exact in bf16, and sums are
+// fp32; the sum over a group is scaled in fp32, so that no weight is rounded.
+// The start costs what cancels: a group's sum of 16 x instead of q x, 2^-24 of
+// it, far below the rounding of a bf16 result.
+//
+// x, scales and zero points go to LDS without passing registers, the weights,
+// which one wave needs once, to registers, both a step ahead: what a step waits
+// for at its start was sent for a whole step before.
+//
+// What bounds it: vector instructions, of which a SIMD starts one in 4 cycles
+// (2.5 for shifts and masks of other waves), and not one a wave in less than 7,
+// whatever stands between.  Four waves a SIMD (128 registers) go before larger
+// tiles: gate and up of 61 rows by 14336 x 4096, group 64 with zeros, 33 us at
+// 4 waves of 2 x 4 tiles and 45 us at 2 of 4 x 4; a step's 48 MFMAs, their 200
+// vector instructions (64 of them the scaling, 96 the operands) and x's 16 reads
+// from LDS take 1.7 us, the MFMAs alone 0.5.  One row by 14336 x 4096 twice,
+// group 128: 12.5 us, 4.7 TB/s; 5 rows by 128256 x 4096: 50 us, 5.3 TB/s.
+template <bool SWIGLU, bool ZEROS, int GP, int NT, int MT, int WN, int WK>
+struct W4Tile {
   static constexpr int WAVES = WN * WK;
   static constexpr int PARTS = SWIGLU ? 2 : 1;
-  static constexpr int RT = NT / PARTS;        // tiles of one matrix a wave
-  static constexpr int X = MT * 4096;          // bytes of a group's slot
-  static constexpr int META = PARTS * 256 * (ZEROS ? 2 : 1);
-  static constexpr int OWN = NT * 1024 + META;  // bytes of a wave's slot
-  static constexpr int GROUP = X + WN * OWN;
-  static constexpr int SLOT = WK * GROUP;
+  static constexpr int RT = NT / PARTS;                  // tiles of one matrix a wave
+  static constexpr int SCALES = (RT * GP * 8 + 63) / 64;  // loads of 64 dwords
+  static constexpr int META = PARTS * 256 * (SCALES + (ZEROS ? 1 : 0));
+  static constexpr int X = MT * 4096;                    // bytes of a K group's slot
+  static constexpr int SLOT = WK * X + WAVES * META;
   static constexpr int SUM = WAVES * NT * MT * 1024;
   static constexpr int XLOADS = MT * 4 / WN;
-  static constexpr int LOADS = XLOADS + NT + PARTS * (ZEROS ? 2 : 1);
-  static constexpr int FIT = 160 * 1024 / SLOT, COUNT = 63 / LOADS + 1;
-  static constexpr int FEW = FIT < COUNT ? FIT : COUNT;
-  static constexpr int DEPTH = D < FEW ? D : FEW;  // slots
-  static constexpr int LDS = DEPTH * SLOT > SUM ? DEPTH * SLOT : SUM;
-  static_assert(RT * GP * 8 <= 64 && MT * 4 % WN == 0 && LDS <= 160 * 1024, "shape");
-  static_assert(DEPTH >= 2, "a slot in use, a slot to come");
+  static constexpr int LDS = 2 * SLOT > SUM ? 2 * SLOT : SUM;
+  static_assert(RT * GP * 4 <= 64 && MT * 4 % WN == 0 && LDS <= 160 * 1024, "shape");
 };
 
-template <bool SWIGLU, bool ZEROS, int GP, int NT, int MT, int WN, int WK, int D>
-__global__ __launch_bounds__(WN * WK * kWave) void w4_ring_kernel(W4Args a) {
-  using R = W4Ring<SWIGLU, ZEROS, GP, NT, MT, WN, WK, D>;
-  constexpr int RT = R::RT, J = 4 / GP, DEPTH = R::DEPTH;
-  __shared__ __attribute__((aligned(16))) unsigned char s_ring[R::LDS];
+template <bool SWIGLU, bool ZEROS, int GP, int NT, int MT, int WN, int WK>
+__global__ __launch_bounds__(WN * WK * kWave) void w4_tile_kernel(W4Args a) {
+  using R = W4Tile<SWIGLU, ZEROS, GP, NT, MT, WN, WK>;
+  constexpr int RT = R::RT, J = 4 / GP;
+  __shared__ __attribute__((aligned(16))) unsigned char s_tile[R::LDS];
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -302,12 +213,13 @@ __global__ __launch_bounds__(WN * WK * kWave) void w4_ring_kernel(W4Args a) {
   // one: the last one again)
   auto behind = [&](int i) { return static_cast<int>(min(first + i, last_tile) - base_tile); };
 
-  u32x4 wr[R::PARTS], sr[R::PARTS], zr[R::PARTS];
+  Rsrc wr[R::PARTS];
+  u32x4 sr[R::PARTS], zr[R::PARTS];
 #pragma unroll
   for (int p = 0; p < R::PARTS; ++p) {
     const W4Matrix &w = a.w[p];
-    wr[p] = buffer_rsrc_words(w.packed + base_tile * a.tiles * kWave,
-                              static_cast<int64_t>(a.tiles) * 1024 * RT);
+    wr[p] = w4_rsrc(w.packed + base_tile * a.tiles * kWave,
+                    static_cast<int64_t>(a.tiles) * 1024 * RT);
     sr[p] = buffer_rsrc_words(w.scales + base_tile * a.groups * 16,
                               static_cast<int64_t>(a.groups) * 32 * RT);
     if constexpr (ZEROS)
@@ -324,38 +236,61 @@ __global__ __launch_bounds__(WN * WK * kWave) void w4_ring_kernel(W4Args a) {
     const int block = wn + WN * i, row = 16 * (block / 4) + c16;
     xoff[i] = row < rows ? row * pitch + 64 * (block % 4) + 16 * g4 : kOutside;
   }
-  // a lane's dword of the scales (of the zero points) of tile lane / (8 GP)
-  const int stile = lane / (8 * GP), sword = lane % (8 * GP);
-  const int soff = stile < RT ? behind(stile) * a.groups * 32 + sword * 4 : kOutside;
+  // a lane's dword of the scales (of the zero points): tile and dword in it
+  int soff[R::SCALES], sgroup[R::SCALES];
+#pragma unroll
+  for (int i = 0; i < R::SCALES; ++i) {
+    const int at = i * kWave + lane, tile = at / (8 * GP), word = at % (8 * GP);
+    sgroup[i] = word / 8;
+    soff[i] = tile < RT ? behind(tile) * a.groups * 32 + word * 4 : kOutside;
+  }
   const int ztile = lane / (4 * GP), zword = lane % (4 * GP);
   const int zoff = ztile < RT ? behind(ztile) * a.groups * 16 + zword * 4 : kOutside;
-  const uint32_t lds = lds_address(s_ring);
-  const uint32_t x_at = kg * R::GROUP, own_at = x_at + R::X + wn * R::OWN;
+  const uint32_t lds = lds_address(s_tile);
+  const uint32_t x_at = kg * R::X, meta_at = WK * R::X + wave * R::META;
 
-  const int steps = (a.tiles + WK - 1) / WK;
-  auto issue = [&](int s, int slot) __attribute__((always_inline)) {
-    const int t = s * WK + kg;
-    const uint32_t at = lds + slot * R::SLOT;
+  const int steps = (a.tiles + WK * a.splits - 1) / (WK * a.splits);
+  const int t0 = static_cast<int>(blockIdx.z) * steps * WK + kg;
+  const int tend = min(a.tiles, (static_cast<int>(blockIdx.z) + 1) * steps * WK);
+  auto issue = [&](int t, uint32_t at, u32x4 (&w)[NT]) __attribute__((always_inline)) {
+    if (t >= tend) return;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int tile = behind(i % RT) * a.tiles;
-      // (past the end of K: past the end of the last tile)
-      const int off = t >= a.tiles ? kOutside : lane * 16 + (tile + t) * 1024;
-      dma_lds16(wr[i / RT], off, at + own_at + i * 1024);
+      const int from = (behind(i % RT) * a.tiles + t) * 1024;
+      w[i] = a.once ? __builtin_amdgcn_raw_buffer_load_b128(wr[i / RT], lane * 16, from,
+                                                            kNontemporal)
+                    : __builtin_amdgcn_raw_buffer_load_b128(wr[i / RT], lane * 16, from, 0);
     }
+    const uint32_t meta = at + meta_at;
+    constexpr int PITCH = 256 * (R::SCALES + (ZEROS ? 1 : 0));
+    if (128 * (t + 1) <= a.k) {
 #pragma unroll
-    for (int p = 0; p < R::PARTS; ++p) {
-      const uint32_t meta = at + own_at + NT * 1024 + p * 256 * (ZEROS ? 2 : 1);
-      dma_lds4(sr[p], t * GP + sword / 8 < a.groups ? soff + t * GP * 32 : kOutside, meta);
-      if constexpr (ZEROS)
-        dma_lds4(zr[p], t * GP + zword / 4 < a.groups ? zoff + t * GP * 16 : kOutside, meta + 256);
-    }
-    const bool whole = 128 * (t + 1) <= a.k;
+      for (int p = 0; p < R::PARTS; ++p) {
 #pragma unroll
-    for (int i = 0; i < R::XLOADS; ++i) {
-      const int block = wn + WN * i;
-      const bool in = whole || 128 * t + 32 * (block % 4) + 8 * g4 < a.k;
-      dma_lds16(xr, in ? xoff[i] + t * 256 : kOutside, at + x_at + block * 1024);
+        for (int i = 0; i < R::SCALES; ++i)
+          dma_lds4_inside(sr[p], soff[i], t * GP * 32, meta + p * PITCH + i * 256);
+        if constexpr (ZEROS)
+          dma_lds4_inside(zr[p], zoff, t * GP * 16, meta + p * PITCH + R::SCALES * 256);
+      }
+#pragma unroll
+      for (int i = 0; i < R::XLOADS; ++i)
+        dma_lds16_inside(xr, xoff[i], t * 256, at + x_at + (wn + WN * i) * 1024);
+    } else {
+#pragma unroll
+      for (int p = 0; p < R::PARTS; ++p) {
+#pragma unroll
+        for (int i = 0; i < R::SCALES; ++i)
+          dma_lds4(sr[p], t * GP + sgroup[i] < a.groups ? soff[i] + t * GP * 32 : kOutside,
+                   meta + p * PITCH + i * 256);
+        if constexpr (ZEROS)
+          dma_lds4(zr[p], t * GP + zword / 4 < a.groups ? zoff + t * GP * 16 : kOutside,
+                   meta + p * PITCH + R::SCALES * 256);
+      }
+#pragma unroll
+      for (int i = 0; i < R::XLOADS; ++i) {
+        const bool in = 128 * t + 32 * ((wn + WN * i) % 4) + 8 * g4 < a.k;
+        dma_lds16(xr, in ? xoff[i] + t * 256 : kOutside, at + x_at + (wn + WN * i) * 1024);
+      }
     }
   };
   f32x4 acc[NT][MT];
@@ -366,125 +301,209 @@ __global__ __launch_bounds__(WN * WK * kWave) void w4_ring_kernel(W4Args a) {
   // the sum's start: -24 x = -(16 + 8) x, or -48 x
   constexpr uint32_t kFirst = ZEROS ? 0xc240c240u : 0xc1c0c1c0u;
   const u32x4 first_op = {kFirst, kFirst, kFirst, kFirst};
-  auto step = [&](int slot) __attribute__((always_inline)) {
-    const unsigned char *at = s_ring + slot * R::SLOT;
+  auto step = [&](uint32_t slot, const u32x4 (&w)[NT]) __attribute__((always_inline)) {
+    const unsigned char *at = s_tile + slot;
     const u32x4 *xs_at = reinterpret_cast<const u32x4 *>(at + x_at) + lane;
-    const unsigned char *own = at + own_at;
-    u32x4 w[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-      w[i] = reinterpret_cast<const u32x4 *>(own + i * 1024)[lane];
 #pragma unroll
     for (int g = 0; g < GP; ++g) {
-      u32x4 x[MT][J];
-      f32x4 start[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        start[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          x[m][j] = xs_at[(4 * m + J * g + j) * kWave];
-          start[m] = mfma_16x16x32_bf16(first_op, x[m][j], start[m]);
-        }
-      }
+      u32x4 op[NT][J];
+      float scale[NT][4];
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const unsigned char *meta = own + NT * 1024 + (i / RT) * 256 * (ZEROS ? 2 : 1);
-        const u32x2 sc = *reinterpret_cast<const u32x2 *>(
-            meta + ((i % RT) * GP + g) * 32 + 8 * g4);
-        const uint32_t s01 = sc[0], s23 = sc[1];
-        const float scale[4] = {lo_bf16(s01), hi_bf16(s01), lo_bf16(s23), hi_bf16(s23)};
+        const unsigned char *meta =
+            at + meta_at + (i / RT) * 256 * (R::SCALES + (ZEROS ? 1 : 0));
+        const u32x2 two =
+            *reinterpret_cast<const u32x2 *>(meta + ((i % RT) * GP + g) * 32 + 8 * g4);
+        scale[i][0] = lo_bf16(two[0]);
+        scale[i][1] = hi_bf16(two[0]);
+        scale[i][2] = lo_bf16(two[1]);
+        scale[i][3] = hi_bf16(two[1]);
         uint32_t zero = 0;
         if constexpr (ZEROS)
           zero = 0x42404240u -
-                 __umul24(meta[256 + ((i % RT) * GP + g) * 16 + c16], 0x00040004u);
-        u32x4 op[J];
+                 __umul24(meta[R::SCALES * 256 + ((i % RT) * GP + g) * 16 + c16], 0x00040004u);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const uint32_t word = w[i][J * g + j];
-          op[j] = ZEROS ? w4_operand_from(word, zero) : w4_operand(word);
+          op[i][j] = ZEROS ? w4_operand_from(word, zero) : w4_operand(word);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        u32x4 x[J];
+        f32x4 start = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          x[j] = xs_at[(4 * m + J * g + j) * kWave];
+          start = mfma_16x16x32_bf16(first_op, x[j], start);
         }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          f32x4 part = start[m];
+        for (int i = 0; i < NT; ++i) {
+          f32x4 part = start;
 #pragma unroll
-          for (int j = 0; j < J; ++j) part = mfma_16x16x32_bf16(op[j], x[m][j], part);
+          for (int j = 0; j < J; ++j) part = mfma_16x16x32_bf16(op[i][j], x[j], part);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][m][r] = fmaf(scale[r], part[r], acc[i][m][r]);
+          for (int r = 0; r < 4; ++r) acc[i][m][r] = fmaf(scale[i][r], part[r], acc[i][m][r]);
         }
       }
     }
   };
-#pragma unroll
-  for (int d = 0; d < DEPTH - 1; ++d) issue(d, d);
-  int slot = 0;
-  for (int s = 0; s < steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(waitcnt_imm((DEPTH - 2) * R::LOADS, 15));
+  auto turn = [&](int t, uint32_t slot, u32x4 (&w)[NT], u32x4 (&next)[NT])
+      __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
     if constexpr (WN > 1) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    issue(s + DEPTH - 1, slot == 0 ? DEPTH - 1 : slot - 1);
+    issue(t + WK, lds + (R::SLOT - slot), next);
     __builtin_amdgcn_sched_barrier(0);
-    step(slot);
+    if (t < tend) step(slot, w);
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    slot = slot == DEPTH - 1 ? 0 : slot + 1;
+  };
+  u32x4 even[NT], odd[NT];
+  issue(t0, lds, even);
+  for (int s = 0, t = t0; s < steps; s += 2, t += 2 * WK) {
+    turn(t, 0, even, odd);
+    if (s + 1 < steps) turn(t + WK, R::SLOT, odd, even);
   }
   __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
   __syncthreads();
-  f32x4 *s_sum = reinterpret_cast<f32x4 *>(s_ring);
+  // The waves' sums, four matrix rows of one row of x a place.  Places are
+  // turned so that both a wave's tile and a row's neighbours (which leave
+  // together) lie in different banks.
+  constexpr int T = WN * RT, Q = 4 * T, ROUND = T < 4 ? 4 / T : 1;
+  f32x4 *s_sum = reinterpret_cast<f32x4 *>(s_tile);
+  auto place = [&](int tile, int m, int row, int quad) {
+    return (tile * MT + m) * kWave + 16 * (quad & 3) + ((row + ROUND * quad) & 15);
+  };
+  constexpr int kAll = R::PARTS * T * MT * kWave;  // places of a K group
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) s_sum[((wave * NT + i) * MT + m) * kWave + lane] = acc[i][m];
+    for (int m = 0; m < MT; ++m)
+      s_sum[kg * kAll + place((i / RT) * T + wn * RT + i % RT, m, c16,
+                              4 * (wn * RT + i % RT) + g4)] = acc[i][m];
   __syncthreads();
-  // an item: four matrix rows of one row of x
-  for (int item = tid; item < WN * RT * MT * kWave; item += R::WAVES * kWave) {
-    const int at = item % kWave, part = item / kWave;
-    const int m = part % MT, i = part / MT % RT, n = part / MT / RT;
-    auto joined = [&](int tile) {
-      const int from = ((n * NT + tile) * MT + m) * kWave + at;
+  for (int item = tid; item < Q * MT * 16; item += R::WAVES * kWave) {
+    const int quad = item % Q, r16 = item / Q % 16, m = item / (Q * 16);
+    auto joined = [&](int part) {
+      const int from = place(part * T + quad / 4, m, r16, quad);
       f32x4 v = s_sum[from];
 #pragma unroll
       for (int k = 1; k < WK; ++k) {
-        const f32x4 u = s_sum[k * WN * NT * MT * kWave + from];
+        const f32x4 u = s_sum[k * kAll + from];
         v += u;
       }
       return v;
     };
-    f32x4 v = joined(i);
+    f32x4 v = joined(0);
     if constexpr (SWIGLU) {
-      const f32x4 u = joined(i + RT);
+      const f32x4 u = joined(1);
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = v[r] / (1.0f + __expf(-v[r])) * u[r];
     }
-    const int row = m0 + 16 * m + (at & 15);
-    const int tile = (static_cast<int>(blockIdx.x) * WN + n) * RT + i;
-    if (row < a.m && tile <= last_tile) w4_store(a, v, row, 16 * tile + 4 * (at >> 4));
+    const int row = m0 + 16 * m + r16;
+    const int col = 16 * T * static_cast<int>(blockIdx.x) + 4 * quad;
+    if (row >= a.m || col > 16 * last_tile + 15) continue;
+    if (a.splits > 1)
+      *reinterpret_cast<f32x4 *>(
+          a.partial + (static_cast<int64_t>(blockIdx.z) * a.m + row) * 16 * (last_tile + 1) +
+          col) = v;
+    else
+      w4_store(a, v, row, col);
   }
 }
 
-template <bool SWIGLU, int NT, int MT, int WN, int WK, int D>
-static int launch_w4_ring(const W4Args &a, hipStream_t s) {
+// Sums over K that several workgroups took parts of.
+__global__ __launch_bounds__(256) void w4_join_kernel(W4Args a) {
+  const int quads = (a.n + 15) / 16 * 4;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = item / quads;
+  const int col = 4 * static_cast<int>(item - row * quads);
+  if (row >= a.m || col >= a.n) return;
+  const f32x4 *from = reinterpret_cast<const f32x4 *>(a.partial) + item;
+  f32x4 v = *from;
+  for (int z = 1; z < a.splits; ++z) {
+    const f32x4 u = from[static_cast<int64_t>(z) * a.m * quads];
+    v += u;
+  }
+  w4_store(a, v, static_cast<int>(row), col);
+}
+
+template <bool SWIGLU, int NT, int MT, int WN, int WK>
+static int launch_w4_tile(const W4Args &a, hipStream_t s) {
   constexpr int RT = SWIGLU ? NT / 2 : NT;
   const int64_t tiles = (a.n + 15) / 16;
   const int64_t x = (tiles + RT * WN - 1) / (RT * WN), y = (a.m + 16 * MT - 1) / (16 * MT);
   if (y > 0xffff || x > 0xffffffffll / (WN * WK * kWave)) return CASCADE_ESHAPE;
-  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(y));
+  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(y),
+                  static_cast<unsigned>(a.splits));
   const dim3 block(WN * WK * kWave);
   const int which = (a.group_shift - 5) + (a.w[0].zeros != nullptr ? 3 : 0);
+  hipError_t status;
   switch (which) {
-    case 0: return launch_kernel(w4_ring_kernel<SWIGLU, false, 4, NT, MT, WN, WK, D>, grid, block, 0, s, a);
-    case 1: return launch_kernel(w4_ring_kernel<SWIGLU, false, 2, NT, MT, WN, WK, D>, grid, block, 0, s, a);
-    case 2: return launch_kernel(w4_ring_kernel<SWIGLU, false, 1, NT, MT, WN, WK, D>, grid, block, 0, s, a);
-    case 3: return launch_kernel(w4_ring_kernel<SWIGLU, true, 4, NT, MT, WN, WK, D>, grid, block, 0, s, a);
-    case 4: return launch_kernel(w4_ring_kernel<SWIGLU, true, 2, NT, MT, WN, WK, D>, grid, block, 0, s, a);
-    default: return launch_kernel(w4_ring_kernel<SWIGLU, true, 1, NT, MT, WN, WK, D>, grid, block, 0, s, a);
+    case 0: status = launch_kernel(w4_tile_kernel<SWIGLU, false, 4, NT, MT, WN, WK>, grid, block, 0, s, a); break;
+    case 1: status = launch_kernel(w4_tile_kernel<SWIGLU, false, 2, NT, MT, WN, WK>, grid, block, 0, s, a); break;
+    case 2: status = launch_kernel(w4_tile_kernel<SWIGLU, false, 1, NT, MT, WN, WK>, grid, block, 0, s, a); break;
+    case 3: status = launch_kernel(w4_tile_kernel<SWIGLU, true, 4, NT, MT, WN, WK>, grid, block, 0, s, a); break;
+    case 4: status = launch_kernel(w4_tile_kernel<SWIGLU, true, 2, NT, MT, WN, WK>, grid, block, 0, s, a); break;
+    default: status = launch_kernel(w4_tile_kernel<SWIGLU, true, 1, NT, MT, WN, WK>, grid, block, 0, s, a);
   }
+  if (status != hipSuccess || a.splits == 1) return status;
+  const int64_t blocks = (tiles * 4 * a.m + 255) / 256;
+  return launch_kernel(w4_join_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
+}
+
+// The shape of a product's workgroups and the parts that K is split into, from
+// sizes alone; times in us, group 64 with zeros unless said.
+// - Up to 16 rows: 4 tiles a wave, 4 waves share K (x is read from LDS once for
+//   four tiles), where that leaves every CU a workgroup; otherwise 2 tiles, 8
+//   waves.  gate and up 14336 x 4096, 16 rows: 16.6 / 21.6; 4096 x 4096, 16
+//   rows: 9.4 / 7.2.
+// - More rows: 32 of x a workgroup; 64 where two of these a CU are left: 157
+//   rows, gate and up 14336 x 4096: 74 with 64, 80 with 32; 613 rows, 4096 x
+//   4096: 47 / 44.
+// - Parts of K up to a workgroup a CU (two for more than 16 rows): 16 rows 4096
+//   x 14336: 25.5, in 4 parts 12.7; 61 rows 4096 x 14336: 61, 4 parts 22.4, 8
+//   22.3, 10 26.9; 61 rows 4096 x 4096: 19.6, 4 parts 11.7, 8 12.7; 613 rows:
+//   one part 45, four 52.  Gate and up have no workspace and are not split.
+enum W4Shape { kW4Rows16Wide, kW4Rows16, kW4Rows32, kW4Rows64 };
+
+struct W4Plan {
+  W4Shape shape;
+  int32_t splits;
+};
+
+static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, bool swiglu) {
+  const int64_t row_tiles = (n + 15) / 16 * (swiglu ? 2 : 1), tiles = (k + 127) / 128;
+  // parts of 4 steps or more, so many that there are `wanted` workgroups
+  auto splits = [&](int64_t groups, int64_t wanted, int wk) {
+    if (swiglu) return int64_t{1};
+    int64_t parts = wanted / groups;
+    if (parts > tiles / (4 * wk)) parts = tiles / (4 * wk);
+    return parts < 1 ? int64_t{1} : parts;
+  };
+  auto plan = [](W4Shape shape, int64_t parts) {
+    return W4Plan{shape, static_cast<int32_t>(parts)};
+  };
+  if (m <= 16) {
+    const int64_t groups = (row_tiles + 3) / 4, parts = splits(groups, 256, 4);
+    if (groups * parts >= 256) return plan(kW4Rows16Wide, parts);
+    return plan(kW4Rows16, splits((row_tiles + 1) / 2, 256, 8));
+  }
+  const int64_t groups = (row_tiles + 7) / 8;
+  if (groups * ((m + 63) / 64) >= 512) return plan(kW4Rows64, 1);
+  return plan(kW4Rows32, splits(groups * ((m + 31) / 32), 512, 2));
+}
+
+static int64_t w4_workspace_bytes(const W4Plan &plan, int64_t m, int64_t n) {
+  return plan.splits == 1 ? 0 : plan.splits * m * ((n + 15) / 16 * 16) * 4;
 }
 
 template <int OUT>
 static int launch_w4(W4Args a, int64_t x_stride, int64_t m, int64_t n, int64_t k,
-                     int64_t group, void *stream) {
+                     int64_t group, void *workspace, size_t workspace_bytes,
+                     void *stream) {
   if (m <= 0 || n <= 0 || k <= 0) return CASCADE_EINVAL;
   if (k & 7) return CASCADE_EALIGN;
   if ((group != 32 && group != 64 && group != 128) || m > 0x7fffff || n > 0x7fffff ||
@@ -513,34 +532,37 @@ static int launch_w4(W4Args a, int64_t x_stride, int64_t m, int64_t n, int64_t k
   a.group_shift = group == 128 ? 7 : group == 64 ? 6 : 5;
   a.groups = static_cast<int32_t>((k + group - 1) / group);
   a.f32 = OUT == kW4F32;
+  a.wide = (a.y_stride & 3) == 0 && (a.residual_stride & 3) == 0 &&
+           (reinterpret_cast<uintptr_t>(a.y) & (OUT == kW4F32 ? 15 : 7)) == 0 &&
+           (reinterpret_cast<uintptr_t>(a.residual) & 7) == 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   constexpr bool kSwiglu = OUT == kW4Swiglu;
-  const int64_t row_tiles = (n + 15) / 16 * (kSwiglu ? 2 : 1);
-  constexpr int kOne = kSwiglu ? 2 : 1;
-  if (m <= 16 && a.tiles * 256 * m <= kW4FewBytes) {
-    // workgroups of more row tiles where these still fill the device
-    if (row_tiles >= 1536) return launch_w4_few<kSwiglu, 4, 4, 2>(a, s);
-    if (kSwiglu || row_tiles >= 512) return launch_w4_few<kSwiglu, 2, 8, 2>(a, s);
-    return launch_w4_few<kSwiglu, kOne, 8, 2>(a, s);
+  const W4Plan plan = w4_plan(m, n, k, kSwiglu);
+  if (plan.splits > 1) {
+    if (workspace == nullptr || static_cast<int64_t>(workspace_bytes) <
+                                    w4_workspace_bytes(plan, m, n))
+      return CASCADE_EWORKSPACE;
+    if (!aligned16(workspace)) return CASCADE_EALIGN;
   }
-  // the most row tiles a workgroup that leave every CU one
-  const int64_t blocks = (m + 63) / 64;
-  if (m <= 16)
-    return row_tiles >= 1280 ? launch_w4_ring<kSwiglu, 2, 1, 4, 2, 4>(a, s)
-                             : launch_w4_ring<kSwiglu, kOne, 1, 1, 8, 2>(a, s);
-  if (m <= 32)
-    return row_tiles >= 1280 ? launch_w4_ring<kSwiglu, 2, 2, 4, 2, 3>(a, s)
-                             : launch_w4_ring<kSwiglu, 2, 2, 1, 4, 3>(a, s);
-  if (row_tiles * blocks >= 8 * 160) return launch_w4_ring<kSwiglu, 2, 4, 4, 2, 2>(a, s);
-  if (row_tiles * blocks >= 4 * 160) return launch_w4_ring<kSwiglu, 2, 4, 2, 2, 3>(a, s);
-  return launch_w4_ring<kSwiglu, kOne, 4, 1, 4, 2>(a, s);
+  a.splits = plan.splits;
+  a.partial = static_cast<float *>(workspace);
+  a.once = m <= 32 && (n + 15) / 16 * a.tiles * 1024 * (kSwiglu ? 2 : 1) >= kW4OnceBytes;
+  switch (plan.shape) {
+    case kW4Rows16Wide: return launch_w4_tile<kSwiglu, 4, 1, 1, 4>(a, s);
+    case kW4Rows16: return launch_w4_tile<kSwiglu, 2, 1, 1, 8>(a, s);
+    case kW4Rows32: return launch_w4_tile<kSwiglu, 2, 2, 4, 2>(a, s);
+    default: return launch_w4_tile<kSwiglu, 2, 4, 4, 2>(a, s);
+  }
 }
 
 }  // namespace cascade
 
 using namespace cascade;
 
-extern "C" size_t cascade_linear_w4_workspace_bytes(int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t cascade_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || k <= 0 || m > 0x7fffff || n > 0x7fffff || k > 0x7fffff) return 0;
+  return static_cast<size_t>(w4_workspace_bytes(w4_plan(m, n, k, false), m, n));
+}
 
 extern "C" int cascade_linear_w4_bf16(const void *x, int64_t x_stride, const void *packed,
                                       const void *scales, const void *zeros, int64_t m,
@@ -556,7 +578,7 @@ extern "C" int cascade_linear_w4_bf16(const void *x, int64_t x_stride, const voi
   a.residual_stride = residual_stride;
   a.y = y;
   a.y_stride = y_stride;
-  return launch_w4<kW4Bf16>(a, x_stride, m, n, k, group, stream);
+  return launch_w4<kW4Bf16>(a, x_stride, m, n, k, group, workspace, workspace_bytes, stream);
 }
 
 extern "C" int cascade_linear_w4_f32out_bf16(const void *x, int64_t x_stride,
@@ -571,7 +593,7 @@ extern "C" int cascade_linear_w4_f32out_bf16(const void *x, int64_t x_stride,
             static_cast<const uint8_t *>(zeros)};
   a.y = y;
   a.y_stride = y_stride;
-  return launch_w4<kW4F32>(a, x_stride, m, n, k, group, stream);
+  return launch_w4<kW4F32>(a, x_stride, m, n, k, group, workspace, workspace_bytes, stream);
 }
 
 extern "C" int cascade_gate_up_swiglu_w4_bf16(
@@ -588,5 +610,5 @@ extern "C" int cascade_gate_up_swiglu_w4_bf16(
             static_cast<const uint8_t *>(up_zeros)};
   a.y = y;
   a.y_stride = y_stride;
-  return launch_w4<kW4Swiglu>(a, x_stride, m, n_half, k, group, stream);
+  return launch_w4<kW4Swiglu>(a, x_stride, m, n_half, k, group, nullptr, 0, stream);
 }
