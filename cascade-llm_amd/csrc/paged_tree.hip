@@ -92,7 +92,7 @@ struct TreeShape {
   // rows that no other workgroup reads need no place in a cache
   static constexpr bool ONCE = CT * WC < 16;
   static constexpr int KC = D / 32;          // 32-dim chunks
-  static constexpr int DV = D / 16;          // dims a lane holds of a V row
+  static constexpr int DV = D / 16;          // tiles of 16 dims
   static constexpr int ROW = 2 * D;          // bytes
   static constexpr int TILE = kPagedBlock * ROW;
   static constexpr int SLOT = 2 * TILE;      // K and V of a block
@@ -117,6 +117,24 @@ struct TreeColumns {
 __device__ __forceinline__ uint32_t special_of(uint32_t pair) {
   return ((pair & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) |
          ((pair & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+
+// Sixteen lanes read 4 rows of 16 values, eight bytes each, and get a column
+// each, four values.
+__device__ __forceinline__ u32x2 read_turned(const unsigned char *from) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                 (__attribute__((address_space(3))) s16x4 *)(from)));
+}
+
+// split_weights with one instruction a weight less: the upper part is cut off,
+// and the lower one, what remains and 2^-23 of the weight, is positive.
+__device__ __forceinline__ SplitWeights tree_weights(float a, float b) {
+  constexpr float kAbove = 1.0f + 0x1p-23f;
+  const uint32_t upper =
+      __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  return {upper, pack_bf16x2(fmaf(a, kAbove, -lo_bf16(upper)), fmaf(b, kAbove, -hi_bf16(upper)))};
 }
 
 // One workgroup takes the columns (node, query head of the KV head) of a tree
@@ -215,6 +233,10 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   constexpr int kGroups = WC <= 2 ? 4 : 8 / WC;  // that a wave loads
   constexpr int kHalves = D / 64;                // loads of a group
   const int group0 = (wc >> 1) * kGroups;
+  auto v_off = [&](int grp, int h) {
+    const uint32_t key = D == 128 ? 2 * lrow + 8 * (grp & 1) : (lrow & 2) + 4 * (grp & 1);
+    return h * 1024 + lrow * ROW + ((lch ^ key) << 4);
+  };
   uint32_t k_off[kGroups][kHalves];
 #pragma unroll
   for (int g = 0; g < kGroups; ++g)
@@ -223,7 +245,7 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
       const int grp = group0 + g;
       const uint32_t key = D == 128 ? 4 * grp + lrow : 2 * grp + ((lrow >> 1) & 1);
       k_off[g][h] = h * 1024 + lrow * ROW + ((lch ^ key) << 4);
-      if (WC > 1 && (wc & 1)) k_off[g][h] = h * 1024 + lane * 16;  // this wave loads V
+      if (WC > 1 && (wc & 1)) k_off[g][h] = v_off(grp, h);  // this wave loads V
     }
   Pages pages = pages_of(0, entry_of(0));
   int entry = entry_of(16);
@@ -248,8 +270,7 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
 #pragma unroll
         for (int h = 0; h < kHalves; ++h)
           dma_lds16_from((is_v ? vb : kb) + behind,
-                         WC == 1 && kvs ? static_cast<uint32_t>(h * 1024 + lane * 16)
-                                        : k_off[g][h],
+                         WC == 1 && kvs ? v_off(grp, h) : k_off[g][h],
                          to + (is_v ? T::TILE : 0) + (grp * kHalves + h) * 1024, T::ONCE);
       }
     }
@@ -286,6 +307,10 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   }
   const int krow = 8 * (c16 >> 2) + (c16 & 3);
   const int kkey = D == 128 ? c16 : 2 * (c16 >> 2) + ((c16 >> 1) & 1);
+  // of the 16 lanes of a turned read of 4 rows and 16 dims: row 8 g4 + c16 / 4,
+  // four dims from 4 (c16 % 4) on
+  const int vkey = D == 128 ? 2 * (c16 >> 2) + 8 * (g4 & 1) : ((c16 >> 2) & 2) + 4 * (g4 & 1);
+  const int v_at = (8 * g4 + (c16 >> 2)) * ROW + ((((c16 >> 1) & 1) ^ vkey) << 4) + 8 * (c16 & 1);
 
   u32x4 k0[KC], k1[KC];  // the next block's K operands
   auto read_k = [&](int slot) __attribute__((always_inline)) {
@@ -317,19 +342,13 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
     const bool tail = bad || (blk + 1) * kPagedBlock > past;
     const unsigned char *at = s_mem + ring + slot * T::SLOT;
     const int r0 = blk * kPagedBlock;
-    uint32_t v[8][DV / 2];
+    // V's operands, dim 16 e + c16 of eight positions, as the reads turn them
+    u32x4 vop[DV];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const unsigned char *vp = at + T::TILE + (8 * g4 + j) * ROW + c16 * (DV * 2);
-      if constexpr (DV == 8) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(vp);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) v[j][n] = w[n];
-      } else {
-        const u32x2 w = *reinterpret_cast<const u32x2 *>(vp);
-        v[j][0] = w[0];
-        v[j][1] = w[1];
-      }
+    for (int e = 0; e < DV; ++e) {
+      const unsigned char *vp = at + T::TILE + (v_at ^ (32 * e));
+      const u32x2 lo = read_turned(vp), hi = read_turned(vp + 4 * ROW);
+      vop[e] = u32x4{lo[0], lo[1], hi[0], hi[1]};
     }
     f32x4 score[CT][2];
 #pragma unroll
@@ -343,20 +362,6 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
         score[ct][1] = mfma_16x16x32_bf16(k1[c], q[ct][c], score[ct][1]);
       }
     const bool mine_bad = (bad >> g4) & 1;
-    u32x4 vop[DV];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < DV; ++e)
-        vop[e][i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1],
-                                          (e & 1) ? 0x07060302u : 0x05040100u);
-    // V's reads first, then the products, with V's transposition as it comes
-    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-#pragma unroll
-    for (int n = 0; n < 2 * KC * CT; ++n) {
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x2, (4 * DV + 2 * KC * CT - 1) / (2 * KC * CT), 0);
-    }
     float s[CT][8];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
@@ -443,7 +448,7 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
       x.l += psum;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const SplitWeights w = split_weights(p[2 * n], p[2 * n + 1]);
+        const SplitWeights w = tree_weights(p[2 * n], p[2 * n + 1]);
         pop[ct][n] = w.upper;
         low[ct][n] = w.lower;
       }
@@ -537,7 +542,7 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) sums[ct] = xor32_sum(xor16_sum(state[ct].l));
   // The groups' columns join in LDS, one tile of them after the other.  o[e][r]
-  // is O[dim DV (4 g4 + r) + e][column c16]; columns are 16 bytes further apart
+  // is O[dim 16 e + 4 g4 + r][column c16]; columns are 16 bytes further apart
   // than their dims are long, so that a lane's column has banks of its own.
   constexpr int kPitch = T::PITCH;
   float *s_acc = reinterpret_cast<float *>(s_mem);  // [wave][column][dim]
@@ -546,13 +551,9 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   for (int ct = 0; ct < CT; ++ct) {
     if (ct) __syncthreads();
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int e = 0; e < DV; e += 4) {
-        const TreeColumns<DV> &x = state[ct];
-        const f32x4 v = {x.o[e][r], x.o[e + 1][r], x.o[e + 2][r], x.o[e + 3][r]};
-        *reinterpret_cast<f32x4 *>(s_acc + (wave * 16 + c16) * kPitch + DV * (4 * g4 + r) + e) = v;
-      }
+    for (int e = 0; e < DV; ++e)
+      *reinterpret_cast<f32x4 *>(s_acc + (wave * 16 + c16) * kPitch + 16 * e + 4 * g4) =
+          state[ct].o[e];
     if (g4 == 0) {
       s_ml[(wave * 16 + c16) * 2] = state[ct].m;
       s_ml[(wave * 16 + c16) * 2 + 1] = sums[ct];
