@@ -322,11 +322,12 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
       k1[c] = *reinterpret_cast<const u32x4 *>(kp + 4 * ROW);
     }
   };
-  // The next step's loads are here, and everyone has read this step's slot, which
+  // The next step's loads are here, and everyone has read this step's slot (its
+  // reads have ended, not only begun: lgkmcnt), which
   // takes the loads of the step that is DEPTH behind it (no fence: it would
   // wait for all loads).
   auto turn = [&](int i, int slot) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(waitcnt_imm((T::DEPTH - 2) * T::LOADS, 15));
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm((T::DEPTH - 2) * T::LOADS, 0));
     if constexpr (WC > 1) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
