@@ -89,7 +89,9 @@ struct TreeShape {
   static constexpr int D = DIM, CT = CT_, WC = WC_, WP = WP_;
   static constexpr int WAVES = WC * WP;
   static constexpr int COLS = 16 * CT * WC;  // of a workgroup
-  // rows that no other workgroup reads need no place in a cache
+  // Rows that no other workgroup reads need no place in a cache: one tree of 16
+  // nodes over 32768 positions 47.5 -> 44 us, 64 of 8 over up to 4096 148 -> 141
+  // (as the kernel then was).  Of 16 tiles the workgroups may share rows.
   static constexpr bool ONCE = CT * WC < 16;
   static constexpr int KC = D / 32;          // 32-dim chunks
   static constexpr int DV = D / 16;          // tiles of 16 dims
@@ -97,7 +99,13 @@ struct TreeShape {
   static constexpr int TILE = kPagedBlock * ROW;
   static constexpr int SLOT = 2 * TILE;      // K and V of a block
   static constexpr int LOADS = SLOT / 1024 / WC;  // of a wave
-  static constexpr int FIT = (160 * 1024 - 16) / (WP * SLOT);
+  // Workgroups a CU, in whose share of the LDS the slots have to fit: two that
+  // wait at barriers of their own are worth more than one with twice the waves
+  // and slots (19 sequences of up to 2048 positions, 14 heads of 64, 9 nodes:
+  // 26.1 -> 19.4 us; 64 of up to 4096, 8 nodes: 124 -> 117).  Sixteen tiles take
+  // all registers.
+  static constexpr int PAIR = CT * WC <= 8 ? 2 : 1;
+  static constexpr int FIT = (160 * 1024 / PAIR - 16) / (WP * SLOT);
   static constexpr int COUNT = 63 / LOADS + 2, FEW = FIT < COUNT ? FIT : COUNT;
   static constexpr int DEPTH = FEW < 5 ? FEW : 5;  // slots
   static constexpr int PITCH = D + 4;  // floats of a column where the groups join
@@ -138,11 +146,26 @@ __device__ __forceinline__ SplitWeights tree_weights(float a, float b) {
 }
 
 // One workgroup takes the columns (node, query head of the KV head) of a tree
-// and a run of its sequence's blocks of 32 positions.  WP groups of waves take
-// turns at the blocks; a group's K and V rows come into LDS once (loads that
-// go there directly, K rows swizzled as the operands read them), and its
-// WC waves multiply them with 16 CT columns each: scores, online softmax
-// and the product with V on the matrix cores as in paged_attention_kernel.
+// and a run of its sequence's blocks of 32 positions, which find_run cuts out of
+// all trees' blocks.  WP groups of waves take turns at the blocks; a group's K
+// and V rows come into LDS once, by loads that go there directly into a ring of
+// slots, and its WC waves multiply them with 16 CT columns each:
+//   S^T = K q^T, running maximum m and sum l a column, O^T += V^T P^T,
+// all on the matrix cores, S, m, l and O in fp32, and P as two bf16 parts (as
+// in the attention of one token: one rounding of P would show in the result).
+// K and V rows lie swizzled in LDS, K for plain reads of its operands, V for
+// reads that turn 4 x 16 values.  The reference of the exponents follows the
+// maximum only where it is passed by 2^8, so O is rarely scaled, and the next
+// block's K operands are read beside this block's product with V.
+//
+// What bounds it: to 64 columns or so the loads, 64 trees of 8 nodes over up to
+// 4096 positions (606 MB) 117 us, 5.2 TB/s, one of 16 over 32768 (135 MB) 41 us
+// with the join of its runs (the start, page lookups and the join are 14 of it);
+// above, vector and matrix instructions, 2 us a block of 252 columns, of which
+// the 384 MFMAs are 0.7: 24 trees of up to 63 nodes over up to 16384 positions
+// (885 MB) 326 us.  Lookups of sixteen blocks' pages at a time, lane by lane,
+// and operands read ahead took the last from 570 us to 355, V's turned reads in
+// place of 32 permutations a block to 326.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeArgs a) {
   constexpr int D = T::D, CT = T::CT, WC = T::WC, WP = T::WP;
@@ -589,7 +612,11 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
 
 // Joins the runs of a node: out = sum_r 2^(m_r - M) acc_r / sum_r 2^(m_r - M) l_r.
 // D / 4 threads (four dims each) are a slice, SLICES slices a head, and each
-// takes every SLICES-th run with a running maximum of its own.
+// takes every SLICES-th run with a running maximum of its own: eight where a
+// tree has more than eight runs, whose loads would follow each other, two
+// otherwise.  Bound by its three dependent loads (4.6 us for one tree of 32
+// runs), for large batches by the partial results (24 trees of 63 nodes: 19 us
+// for 79 MB).
 constexpr int kTreeMergeThreads = 256;
 
 template <int D, int SLICES>
@@ -657,6 +684,15 @@ __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs 
 }
 
 // Which shape a call takes, whether it splits, and its sizes.
+// - Tiles of 16 columns: the least power of two that takes a tree of max_tree
+//   nodes, to 16; more columns take workgroups of their own.
+// - Split over runs from 17 blocks on (below, one workgroup is a whole tree and
+//   no second launch is needed) and up to 256 trees, which fill the device.
+// - Runs: one workgroup a CU for few trees (one of 16 nodes over 32768
+//   positions: 41.8 us, two a CU 43.4; heads of 64, 4 nodes: 20.9 / 22.6), two
+//   where there are more trees than a third of that (16 trees of 8 nodes, heads
+//   of 64, over up to 4096: 23.6, four a CU 24.9; 24 of 63 nodes: 350 / 381 with
+//   one and two rounds), and two rounds where a run would pass 100 blocks.
 struct TreePlan {
   int shape;  // tiles of 16 columns a workgroup: 1, 2, 4, 8, 16
   int col_groups;
@@ -701,16 +737,20 @@ static TreePlan tree_plan(int64_t trees, int64_t max_tree, int64_t q_heads, int6
 template <int D, bool SPLIT>
 static hipError_t launch_tree(const TreeArgs &a, int shape, int64_t blocks, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(blocks));
+  // Groups of waves: as many as leave each two slots.  (64 dims, 64 columns: two
+  // groups and one 25.7 / 30.7 us for one tree over 32768 positions; 128 dims,
+  // 8 nodes of 4 heads: two groups and one 116.7 / 119.8 for 64 trees.)
+  constexpr int kNarrow = D == 64 ? 4 : 2;
 #define CASCADE_TREE(CT, WC, WP)                                                     \
   {                                                                                  \
     using T = TreeShape<D, CT, WC, WP>;                                              \
     return launch_kernel(tree_attention_kernel<T, SPLIT>, grid, dim3(T::WAVES * kWave), 0, s, a); \
   }
   switch (shape) {
-    case 1: CASCADE_TREE(1, 1, 4)
+    case 1: CASCADE_TREE(1, 1, kNarrow)
     case 2: CASCADE_TREE(1, 2, 2)
-    case 4: CASCADE_TREE(1, 4, 2)
-    case 8: CASCADE_TREE(2, 4, 2)
+    case 4: CASCADE_TREE(1, 4, kNarrow / 2)
+    case 8: CASCADE_TREE(2, 4, 1)
     default: CASCADE_TREE(2, 8, 1)
   }
 #undef CASCADE_TREE
