@@ -103,8 +103,8 @@ struct TreeShape {
   // wait at barriers of their own are worth more than one with twice the waves
   // and slots (19 sequences of up to 2048 positions, 14 heads of 64, 9 nodes:
   // 26.1 -> 19.4 us; 64 of up to 4096, 8 nodes: 124 -> 117).  Sixteen tiles take
-  // all registers.
-  static constexpr int PAIR = CT * WC <= 8 ? 2 : 1;
+  // all registers, four groups of 128 dims all of the LDS.
+  static constexpr int PAIR = CT * WC <= 8 && 4 * WP * SLOT <= 160 * 1024 - 32 ? 2 : 1;
   static constexpr int FIT = (160 * 1024 / PAIR - 16) / (WP * SLOT);
   static constexpr int COUNT = 63 / LOADS + 2, FEW = FIT < COUNT ? FIT : COUNT;
   static constexpr int DEPTH = FEW < 5 ? FEW : 5;  // slots
@@ -734,13 +734,16 @@ static TreePlan tree_plan(int64_t trees, int64_t max_tree, int64_t q_heads, int6
   return p;
 }
 
-template <int D, bool SPLIT>
+// WIDE: twice the groups of waves, for launches that leave CUs with one workgroup
+// or none, which are whole trees of up to 512 positions: one tree of 16 nodes
+// 13.2 us, 15.8 with fewer waves; 64 of them 33.6 and 25.6.
+template <int D, bool SPLIT, bool WIDE>
 static hipError_t launch_tree(const TreeArgs &a, int shape, int64_t blocks, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(blocks));
   // Groups of waves: as many as leave each two slots.  (64 dims, 64 columns: two
   // groups and one 25.7 / 30.7 us for one tree over 32768 positions; 128 dims,
   // 8 nodes of 4 heads: two groups and one 116.7 / 119.8 for 64 trees.)
-  constexpr int kNarrow = D == 64 ? 4 : 2;
+  constexpr int kNarrow = WIDE || D == 64 ? 4 : 2;
 #define CASCADE_TREE(CT, WC, WP)                                                     \
   {                                                                                  \
     using T = TreeShape<D, CT, WC, WP>;                                              \
@@ -750,7 +753,7 @@ static hipError_t launch_tree(const TreeArgs &a, int shape, int64_t blocks, hipS
     case 1: CASCADE_TREE(1, 1, kNarrow)
     case 2: CASCADE_TREE(1, 2, 2)
     case 4: CASCADE_TREE(1, 4, kNarrow / 2)
-    case 8: CASCADE_TREE(2, 4, 1)
+    case 8: CASCADE_TREE(2, 4, WIDE ? 2 : 1)
     default: CASCADE_TREE(2, 8, 1)
   }
 #undef CASCADE_TREE
@@ -971,8 +974,12 @@ extern "C" int cascade_paged_tree_attention_bf16(
   const int64_t each = n_kv_heads * p.col_groups;
   if (!p.split) {
     if (trees * each > kMaxThreads / 512) return CASCADE_ESHAPE;
-    return head_dim == 128 ? launch_tree<128, false>(a, p.shape, trees * each, s)
-                           : launch_tree<64, false>(a, p.shape, trees * each, s);
+    const bool wide = trees * each <= kTreeSlots;
+    if (head_dim == 128)
+      return wide ? launch_tree<128, false, true>(a, p.shape, trees * each, s)
+                  : launch_tree<128, false, false>(a, p.shape, trees * each, s);
+    return wide ? launch_tree<64, false, true>(a, p.shape, trees * each, s)
+                : launch_tree<64, false, false>(a, p.shape, trees * each, s);
   }
   if (p.runs * each > kMaxThreads / 512 ||
       trees * max_tree > kMaxThreads / kTreeMergeThreads / n_q_heads)
@@ -986,10 +993,10 @@ extern "C" int cascade_paged_tree_attention_bf16(
   a.part_acc = reinterpret_cast<float *>(ws + p.plan_bytes + p.ml_bytes);
   const int64_t runs_a_tree = p.runs / trees;
   if (head_dim == 128) {
-    const hipError_t e = launch_tree<128, true>(a, p.shape, p.runs * each, s);
+    const hipError_t e = launch_tree<128, true, false>(a, p.shape, p.runs * each, s);
     return e != hipSuccess ? e : launch_tree_merge<128>(a, runs_a_tree, s);
   }
-  const hipError_t e = launch_tree<64, true>(a, p.shape, p.runs * each, s);
+  const hipError_t e = launch_tree<64, true, false>(a, p.shape, p.runs * each, s);
   return e != hipSuccess ? e : launch_tree_merge<64>(a, runs_a_tree, s);
 }
 
