@@ -1731,7 +1731,8 @@ def sample(logits, uniform, ids, workspace, temperature=1.0, top_k=0, top_p=1.0,
 
 def linear_w4_workspace_bytes(rows, n, k):
     """Workspace bytes of linear_w4 for ``rows`` rows of ``k`` values times a
-    matrix of ``n`` rows (may be 0: none is needed)."""
+    matrix of ``n`` rows (0: none is needed).  Fewer rows may need more: a buffer
+    for several sizes takes the largest of theirs."""
 
     return int(load().cascade_linear_w4_workspace_bytes(int(rows), int(n), int(k)))
 

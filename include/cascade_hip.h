@@ -504,9 +504,11 @@ int cascade_paged_tree_accept(
  * and NaN give NaN or infinite rows where finite ones may be meant; other rows
  * stay as they are.  No counterpart in the reference, whose weights are bf16;
  * stands beside cascade_gemv_residual_bf16 and cascade_gemm_residual_ws_bf16.
- * The workspace (cascade_linear_w4_workspace_bytes; 0: none, null is accepted)
- * needs no zero-fill and holds nothing between calls; calls that may overlap
- * need one each.                                                           */
+ * Where few rows of the matrix meet a long K, parts of K are summed in the
+ * workspace (cascade_linear_w4_workspace_bytes of the same m, n and K, which a
+ * smaller m may exceed; 0: none, null is accepted), by a second launch in their
+ * order.  It is 16-byte aligned, needs no zero-fill and holds nothing between
+ * calls; calls that may overlap need one each.                             */
 size_t cascade_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int cascade_linear_w4_bf16(const void *x, int64_t x_stride, const void *packed,
                            const void *scales, const void *zeros, int64_t m,

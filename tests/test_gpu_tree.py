@@ -112,6 +112,22 @@ def test_batches(gpu_device, trees, past, nodes, page_size):
     assert error == 0
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(16, 4, 128), (16, 4, 64)])
+@pytest.mark.parametrize("trees", [2, 70])
+@pytest.mark.parametrize("width", [4, 8, 16, 30, 60])
+def test_short_trees(gpu_device, trees, width, q_heads, kv_heads, dim):
+    # one workgroup a tree and KV head, of two widths: fewer than the device has
+    # CUs, and more
+    print("short", trees, width, dim, flush=True)
+    sizes = [width if i == 0 else 1 + i * 7 % min(width, 12) for i in range(trees)]
+    past = [i * 61 % 440 for i in range(trees)]
+    pool = Pool([p + n for p, n in zip(past, sizes)], kv_heads, dim, 16, seed=width)
+    step = Step(sizes, range(trees), q_heads, dim, seed=trees)
+    out, error = attend(pool, step, gpu_device, max_tree=width)
+    check(pool, step, out)
+    assert error == 0
+
+
 def test_a_mask_of_nothing(gpu_device):
     # no past and an empty mask: zeros; with a past: the past alone
     pool = Pool([4, 40], 2, 128, 8, seed=1)

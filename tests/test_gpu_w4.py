@@ -70,7 +70,53 @@ def test_linear_of_the_models_sizes(gpu_device, rows):
         linear_case(gpu_device, rows, n, k, 128, rows % 2 == 0, residual=True, seed=4)
 
 
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_linear_of_many_rows(gpu_device, group, zeros):
+    # workgroups of 64 rows
+    print("many rows", group, zeros, flush=True)
+    linear_case(gpu_device, 1001, 4100, 264, group, zeros, residual=True, seed=7)
+    linear_case(gpu_device, 1001, 4100, 264, group, zeros, logits=True, seed=8)
+
+
+def test_linear_past_the_caches(gpu_device):
+    # 128 MB and more of packed weights, read past the caches
+    print("past the caches", flush=True)
+    m, group, rows = 65552, 128, 3
+    g = torch.Generator().manual_seed(1)
+    part = random_matrix(1024, 4096, group, False, 1)
+    times = -(-m // 1024)
+    q = part[0].to(gpu_device).repeat(times, 1)[:m]
+    # (no two of the repeated rows alike)
+    scales = (part[1].to(gpu_device).repeat(times, 1)[:m].float()
+              * (1 + torch.arange(m, device=gpu_device)[:, None] / 65536)).to(BF)
+    x = normal((rows, 4096), g).to(gpu_device)
+    matrix4 = W4Matrix.pack(q, scales, group=group)
+    out = torch.full((rows, m), 7.0, device=gpu_device)
+    _hip.linear_w4(x, matrix4, out, workspace=space(rows, m, 4096, gpu_device))
+    y, tol = product(x, q, scales, None, group)
+    off = (out.double() - y).abs()
+    assert bool((off <= tol).all()), (float((off - tol).max()), float(off.max()))
+
+
+def test_a_split_product_needs_its_workspace(gpu_device):
+    rows, n, k = 16, 256, 14336
+    size = _hip.linear_w4_workspace_bytes(rows, n, k)
+    assert size > 0
+    m = W4Matrix.pack(*(p.to(gpu_device) for p in random_matrix(n, k, 64, True, 3)), group=64)
+    x = normal((rows, k), torch.Generator().manual_seed(3)).to(gpu_device)
+    out = torch.full((rows, n), 7.0, dtype=BF, device=gpu_device)
+    for ws in (None, torch.zeros(size - 1, dtype=U8, device=gpu_device)):
+        with pytest.raises(RuntimeError, match="workspace"):
+            _hip.linear_w4(x, m, out, workspace=ws)
+    odd = torch.zeros(size + 8, dtype=U8, device=gpu_device)[8:]
+    with pytest.raises(RuntimeError, match="align"):
+        _hip.linear_w4(x, m, out, workspace=odd)
+    torch.cuda.synchronize(gpu_device)
+    assert bool((out == 7).all())
+
+
 @pytest.mark.parametrize("rows,n,k,group,zeros", [
+    (157, 14336, 264, 32, False), (100, 33000, 136, 128, True),
     (1, 16, 64, 32, True), (1, 14336, 4096, 128, False), (3, 100, 1000, 64, True),
     (16, 257, 264, 32, False), (17, 2000, 520, 128, True), (61, 14336, 4096, 64, True),
     (64, 48, 14336, 128, False), (65, 300, 72, 32, True), (200, 500, 1032, 64, False),

@@ -187,6 +187,16 @@ def test_gate_up_entry_point_refuses(code, changes):
     assert _hip.load().cascade_gate_up_swiglu_w4_bf16(*args) == code
 
 
+@pytest.mark.parametrize("code,changes", [
+    (1004, dict(workspace=None)), (1004, dict(workspace_bytes=4)), (1002, dict(workspace=24))])
+def test_a_split_product_refuses(code, changes):
+    # 4 rows by 100 x 14336 are split over K
+    assert _hip.linear_w4_workspace_bytes(4, 100, 14336) > 4
+    args = linear_args(k=14336, xs=14336, **changes)
+    assert _hip.load().cascade_linear_w4_bf16(*args) == code
+    assert _hip.load().cascade_linear_w4_f32out_bf16(*args[:9], *args[11:]) == code
+
+
 @pytest.fixture
 def launches(monkeypatch):
     calls = []
@@ -278,4 +288,7 @@ def test_workspaces_of_any_shape():
     size = _hip.linear_w4_workspace_bytes
     for rows in (0, 1, 16, 61, 700):
         for n, k in ((1, 8), (4096, 4096), (4096, 14336), (128256, 4096)):
-            assert size(rows, n, k) >= 0
+            assert size(rows, n, k) >= 0 and size(rows, n, k) % 16 == 0
+    # whole parts of rows of 16 columns
+    assert size(16, 4096, 14336) % (16 * 4096 * 4) == 0 < size(16, 4096, 14336)
+    assert size(1, 128256, 4096) == size(700, 4096, 4096) == size(0, 4096, 14336) == 0

@@ -28,13 +28,13 @@ def matrix(q, scales, zeros, group):
 def product(x, q, scales, zeros, group):
     """(x W^T, bound of an fp32 sum's error), in 64 bits.
 
-    The kernels' terms are x (16 + q) and x (16 + zero), products of bf16
-    values that fp32 holds exactly, of magnitude 31 |x| at most.  A group's sum
-    has at most 2 group such additions, each off by at most 2^-23 of the sum of
-    magnitudes so far (a matrix instruction may cut where fp32 rounds), and the
-    groups' products with their scales are summed with as many roundings as
-    there are groups, one for the product, and 16 of partial sums that are
-    joined."""
+    The kernels' terms are x (16 + q) and 24 x, or with zero points x (48 + q -
+    zero) and 48 x: products of bf16 values that fp32 holds exactly, together of
+    magnitude 55 |x| or 111 |x| at most.  A group's sum has at most 2 group such
+    additions, each off by at most 2^-23 of the sum of magnitudes so far (a
+    matrix instruction may cut where fp32 rounds), and the groups' products with
+    their scales are summed with as many roundings as there are groups, one for
+    the product, and 16 of partial sums that are joined."""
 
     x = x.double()
     size = torch.zeros(x.shape[0], q.shape[0], dtype=torch.float64, device=x.device)
@@ -44,7 +44,7 @@ def product(x, q, scales, zeros, group):
         part = slice(i * group, (i + 1) * group)
         total = x[:, part].abs().sum(1)[:, None]
         s = scales[:, i].double().abs()
-        size += 62 * total * s
+        size += (55 if zeros is None else 111) * total * s
         kept += 16 * total * s
     y = x @ matrix(q, scales, zeros, group).t()
     return y, 2.0 ** -23 * (2 * group * size + (groups + 17) * kept)
