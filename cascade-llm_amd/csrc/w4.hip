@@ -172,14 +172,15 @@ __device__ __forceinline__ void dma_lds4_inside(const u32x4 &rsrc, int voff, int
 // which one wave needs once, to registers, both a step ahead: what a step waits
 // for at its start was sent for a whole step before.
 //
-// What bounds it: vector instructions, of which a SIMD starts one in 4 cycles
-// (2.5 for shifts and masks of other waves), and not one a wave in less than 7,
-// whatever stands between.  Four waves a SIMD (128 registers) go before larger
-// tiles: gate and up of 61 rows by 14336 x 4096, group 64 with zeros, 33 us at
-// 4 waves of 2 x 4 tiles and 45 us at 2 of 4 x 4; a step's 48 MFMAs, their 200
-// vector instructions (64 of them the scaling, 96 the operands) and x's 16 reads
-// from LDS take 1.7 us, the MFMAs alone 0.5.  One row by 14336 x 4096 twice,
-// group 128: 12.5 us, 4.7 TB/s; 5 rows by 128256 x 4096: 50 us, 5.3 TB/s.
+// What bounds it: vector instructions, of which a SIMD starts one in 4.5 cycles
+// (shifts and masks of several waves in 2.5), but one wave alone one in 7.4,
+// whatever it is; so tiles are kept small enough for four waves a SIMD (128
+// registers).  Gate and up of 61 rows by 14336 x 4096, group 64 with zeros: 32 us,
+// where tiles of 4 x 4 took 35 to 49; a step of 2 x 4 tiles, 48 MFMAs beside 200
+// vector instructions (64 the scaling, 96 the operands) and 16 reads of x from
+// LDS, takes two waves of a SIMD 1.7 us, 0.7 of it the MFMAs.  Few rows: one by
+// 14336 x 4096 twice, group 128, 12.0 us, 5.1 TB/s; 5 by 128256 x 4096 44.8 us,
+// 6.1 TB/s.
 template <bool SWIGLU, bool ZEROS, int GP, int NT, int MT, int WN, int WK>
 struct W4Tile {
   static constexpr int WAVES = WN * WK;
