@@ -74,6 +74,7 @@ __device__ __forceinline__ Rsrc w4_rsrc(const void *base, int64_t bytes) {
                                            static_cast<int>(bytes), 0x00020000);
 }
 
+constexpr int64_t kW4Rows = 0xffff * 64;  // of x: a grid's second dimension
 constexpr int kNontemporal = 2;
 // Matrices of which the memory-side cache (256 MB) holds little at the next
 // pass go past it: 5 rows by 128256 x 4096 (263 MB) 51.9 -> 49.3 us.  Smaller
@@ -507,7 +508,7 @@ static int launch_w4(W4Args a, int64_t x_stride, int64_t m, int64_t n, int64_t k
                      void *stream) {
   if (m <= 0 || n <= 0 || k <= 0) return CASCADE_EINVAL;
   if (k & 7) return CASCADE_EALIGN;
-  if ((group != 32 && group != 64 && group != 128) || m > 0x7fffff || n > 0x7fffff ||
+  if ((group != 32 && group != 64 && group != 128) || m > kW4Rows || n > 0x7fffff ||
       k > 0x7fffff || x_stride > 0x7fffff)
     return CASCADE_ESHAPE;
   if (x_stride < 0 || (m > 1 && x_stride < k) || a.y_stride < 0 ||
@@ -561,7 +562,7 @@ static int launch_w4(W4Args a, int64_t x_stride, int64_t m, int64_t n, int64_t k
 using namespace cascade;
 
 extern "C" size_t cascade_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k <= 0 || m > 0x7fffff || n > 0x7fffff || k > 0x7fffff) return 0;
+  if (m <= 0 || n <= 0 || k <= 0 || m > kW4Rows || n > 0x7fffff || k > 0x7fffff) return 0;
   return static_cast<size_t>(w4_workspace_bytes(w4_plan(m, n, k, false), m, n));
 }
 

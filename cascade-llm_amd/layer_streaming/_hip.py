@@ -12,6 +12,7 @@ There is no fallback: if the library is missing or fails to load, every
 entry point raises :class:`HipLibraryError`.
 """
 
+import contextlib
 import ctypes
 import operator
 import os
@@ -1646,9 +1647,10 @@ def paged_tree_accept(starts, ids, parents, targets, path, counts, next_ids,
     if trees == 0:
         return path
     if tokens == 0:
-        path.fill_(-1)
-        counts.zero_()
-        next_ids.fill_(-1)
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+            path.fill_(-1)
+            counts.zero_()
+            next_ids.fill_(-1)
         return path
     _call_on(
         index, stream, "cascade_paged_tree_accept", starts.data_ptr(),

@@ -319,7 +319,8 @@ class PagedKVCache:
     def accept(self, starts, ids, parents, targets, path, counts, next_ids, rows=None):
         """``paged_tree_accept`` in every layer's pages.  The sequences keep
         their length: ``truncate`` them to that of their past and
-        ``counts`` once the host knows these."""
+        ``counts`` once the host knows these.  A ``fork`` since the trees'
+        ``extend`` shares their rows, and sees them move."""
 
         return _hip.paged_tree_accept(
             starts, ids, parents, targets, path, counts, next_ids, pages=self.buffer,

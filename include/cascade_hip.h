@@ -486,7 +486,7 @@ int cascade_paged_tree_accept(
     void *stream);
 
 /* ------------------------------------------------------- 4-bit weights
- * Products of up to any number of rows with a matrix of 4-bit values q and a
+ * Products of up to 4194240 rows with a matrix of 4-bit values q and a
  * bf16 scale for each `group` (32, 64 or 128) consecutive columns of a row:
  *   W[i, k] = scale[i, k / group] * (q[i, k] - zero[i, k / group]),
  * zero an integer of 0..15, 8 everywhere where zeros is null.  n rows of K

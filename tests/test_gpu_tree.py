@@ -440,6 +440,26 @@ def test_the_first_of_equal_children(gpu_device):
     assert run_accept(gpu_device, *case, 5) == ([[0, 1, 4, -1, -1]], [3], [3], 0)
 
 
+def test_no_nodes_at_all_on_another_stream(gpu_device):
+    stream, other = torch.cuda.Stream(gpu_device), torch.cuda.Stream(gpu_device)
+    path = torch.full((2, 5), 7, dtype=I32, device=gpu_device)
+    counts = torch.full((2,), 7, dtype=I32, device=gpu_device)
+    next_ids = torch.full((2,), 7, dtype=I64, device=gpu_device)
+    starts = torch.zeros(3, dtype=I32, device=gpu_device)
+    none, parents = (torch.zeros(0, dtype=t, device=gpu_device) for t in (I64, I32))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize(gpu_device)
+    with torch.cuda.graph(graph, stream=stream):
+        with torch.cuda.stream(other):  # not the one that the call names
+            _hip.paged_tree_accept(starts, none, parents, none, path, counts, next_ids,
+                                   stream=stream)
+    torch.cuda.synchronize(gpu_device)
+    assert bool((path == 7).all()), "ran on the current stream"
+    graph.replay()
+    torch.cuda.synchronize(gpu_device)
+    assert bool((path == -1).all() and (counts == 0).all() and (next_ids == -1).all())
+
+
 def test_trees_out_of_range(gpu_device):
     case = accept_case([4, 3, 6], 5)
     for change, skip in ((lambda s: s.__setitem__(3, 99), [2]),
