@@ -36,9 +36,9 @@ __device__ __forceinline__ Tree tree_of(const int32_t *starts, const int32_t *ro
                                         int64_t tokens, int max_tree, int64_t b,
                                         int32_t *error) {
   Tree t{-1, 0, 0};
+  const int64_t first = starts[b], end = starts[b + 1];
   const int64_t row = rows != nullptr ? rows[b] : b;
   if (row < 0) return t;
-  const int64_t first = starts[b], end = starts[b + 1];
   if (first < 0 || end < first || end > tokens || end - first > max_tree) {
     flag_range(error);
     return t;
@@ -50,20 +50,28 @@ __device__ __forceinline__ Tree tree_of(const int32_t *starts, const int32_t *ro
 }
 
 // ------------------------------------------------------------- attention
-// The rows of a tree, if it and its sequence are in range.
-__device__ __forceinline__ PagedRow tree_row(const TreeArgs &a, int b, bool flag) {
-  PagedRow r{-1, 0};
+// A tree and the length of its sequence, if both are in range.
+struct TreeRow {
+  PagedRow place{-1, 0};
+  int32_t first = 0, nodes = 0;
+};
+
+__device__ __forceinline__ TreeRow tree_row(const TreeArgs &a, int b, bool flag) {
+  TreeRow r;
   if (b >= a.batch) return r;
   int32_t *error = flag ? a.error : nullptr;
+  // (the loads side by side: the length's does not wait for the checks)
+  const int64_t row = a.rows != nullptr ? a.rows[b] : b;
+  const int32_t len = row >= 0 && row < a.sequences ? a.lengths[row] : -1;
   const Tree t = tree_of(a.starts, a.rows, a.tokens, a.max_tree, b, error);
   if (t.row < 0 || t.nodes == 0) return r;
-  const int32_t len = t.row < a.sequences ? a.lengths[t.row] : -1;
   if (len < t.nodes || len > a.max_length) {
     flag_range(error);
     return r;
   }
-  r.row = t.row;
-  r.len = len;
+  r.place = {t.row, len};
+  r.first = t.first;
+  r.nodes = t.nodes;
   return r;
 }
 
@@ -180,12 +188,17 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   const int kv = static_cast<int>(blockIdx.x) % a.kv_heads;
   const int rest = static_cast<int>(blockIdx.x) / a.kv_heads;
   const int cg = rest % a.col_groups, run = rest / a.col_groups;
-  int b = run, len, first = 0, end, count = 1;
+  int b = run, len, first = 0, end, count = 1, token0, nodes;
   int64_t row;
   {
     const bool flags = blockIdx.x == 0 && wave == 0;
-    auto row_of = [&](int i, bool flag) { return tree_row(a, i, flag); };
     if constexpr (SPLIT) {
+      TreeRow head;  // of the first 64 trees, a lane each
+      auto row_of = [&](int i, bool flag) {
+        const TreeRow r = tree_row(a, i, flag);
+        if (i == lane) head = r;
+        return r.place;
+      };
       const PagedRun r = find_run(a, run, lane, flags, row_of);
       if (r.b < 0) return;
       b = r.b;
@@ -194,12 +207,21 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
       first = r.first;
       end = r.end;
       count = r.count;
+      if (b < kWave) {
+        token0 = __builtin_amdgcn_readlane(head.first, b);
+        nodes = __builtin_amdgcn_readlane(head.nodes, b);
+      } else {
+        token0 = a.starts[b];
+        nodes = a.starts[b + 1] - token0;
+      }
     } else {
-      const PagedRow r = tree_row(a, b, kv == 0 && cg == 0 && tid == 0);
-      if (r.row < 0) return;
-      row = r.row;
-      len = r.len;
+      const TreeRow r = tree_row(a, b, kv == 0 && cg == 0 && tid == 0);
+      if (r.place.row < 0) return;
+      row = r.place.row;
+      len = r.place.len;
       end = blocks_of(len);
+      token0 = r.first;
+      nodes = r.nodes;
     }
   }
   row = __builtin_amdgcn_readfirstlane(static_cast<int>(row));
@@ -207,8 +229,8 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   b = __builtin_amdgcn_readfirstlane(b);
   first = __builtin_amdgcn_readfirstlane(first);
   end = __builtin_amdgcn_readfirstlane(end);
-  const int token0 = __builtin_amdgcn_readfirstlane(a.starts[b]);
-  const int nodes = __builtin_amdgcn_readfirstlane(a.starts[b + 1]) - token0;
+  token0 = __builtin_amdgcn_readfirstlane(token0);
+  nodes = __builtin_amdgcn_readfirstlane(nodes);
   const int cols = nodes * a.group;
   const int col0 = cg * T::COLS;
   if (col0 >= cols) return;
@@ -631,11 +653,11 @@ __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs 
   const int node = static_cast<int>(id / parts % a.max_tree);
   const int b = static_cast<int>(id / parts / a.max_tree);
   const int index = a.plan[2 * b], count = a.plan[2 * b + 1];
+  const int token0 = a.starts[b], past = a.starts[b + 1];
   // left out, or written already (or, past the workspace, a plan that another
   // call has overwritten)
   if (count <= 1 || index < 0 || count > a.runs - index) return;
-  const int token0 = a.starts[b];
-  if (node >= a.starts[b + 1] - token0) return;
+  if (node >= past - token0) return;
   const int d = threadIdx.x % (D / 4);
   const int slice = threadIdx.x / (D / 4) % SLICES;
   const int h = threadIdx.x / (D / 4) / SLICES;

@@ -1,4 +1,4 @@
-// Products of a few rows with matrices of 4-bit weights (gfx950).
+// Products of rows with matrices of 4-bit weights (gfx950).
 //
 // The layout (include/cascade_hip.h) is that of a wave's load: a tile of 16
 // matrix rows and 128 columns is 1 KiB, of which lane l takes the 16 bytes at
