@@ -64,7 +64,7 @@ def check(pool, step, out, left_out=()):
     assert bool((out[~live] == 7).all()), "a row of no tree was written"
 
 
-SHAPES = [(32, 8, 128), (5, 5, 64), (16, 1, 128), (12, 4, 64), (6, 2, 128), (48, 3, 64),
+SHAPES = [(32, 8, 128), (5, 5, 64), (16, 1, 128), (12, 4, 64), (6, 2, 128), (32, 2, 64),
           (9, 1, 64)]
 # (past, nodes)
 MIXED = [(0, 1), (0, 64), (1, 2), (31, 1), (7, 16), (30, 5), (32, 17), (200, 33), (0, 0),
