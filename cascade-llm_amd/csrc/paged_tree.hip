@@ -708,8 +708,14 @@ __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs 
 // Which shape a call takes, whether it splits, and its sizes.
 // - Tiles of 16 columns: the least power of two that takes a tree of max_tree
 //   nodes, to 16; more columns take workgroups of their own.
-// - Split over runs from 17 blocks on (below, one workgroup is a whole tree and
-//   no second launch is needed) and up to 256 trees, which fill the device.
+// - Split over runs up to 256 trees, which fill the device, and from so many
+//   blocks on that whole trees would leave it unbalanced: 17, where the launch has
+//   128 workgroups or less, to 65 at 512, in proportion (below, one workgroup is a
+//   whole tree and no second launch is needed).  64 trees of 8 nodes, 8 KV heads,
+//   over up to 1000 positions: 33.1 us whole, 37.4 split, up to 2000 58.6 and
+//   63.2; 40 trees of 4 up to 1000 27.3 and 26.8, of 60 70.5 and 84.8, of 4 up to
+//   2000 51.2 and 44.1.  No tree of more than 2048 positions waits for one
+//   workgroup.
 // - Runs: one workgroup a CU for few trees (one of 16 nodes over 32768
 //   positions: 41.8 us, two a CU 43.4; heads of 64, 4 nodes: 20.9 / 22.6), two
 //   where there are more trees than a third of that (16 trees of 8 nodes, heads
@@ -734,9 +740,12 @@ static TreePlan tree_plan(int64_t trees, int64_t max_tree, int64_t q_heads, int6
   p.shape = cols <= 16 ? 1 : cols <= 32 ? 2 : cols <= 64 ? 4 : cols <= 128 ? 8 : 16;
   p.col_groups = static_cast<int>((cols + 16 * p.shape - 1) / (16 * p.shape));
   const int64_t blocks = (max_length + kPagedBlock - 1) / kPagedBlock;
-  p.split = blocks > kWholeBlocks && trees <= kTreeMaxBatch;
-  if (!p.split) return p;
   const int64_t each = kv_heads * p.col_groups;
+  int64_t whole = kWholeBlocks * trees * each / (kTreeSlots / 2);
+  whole = whole < kWholeBlocks ? kWholeBlocks : whole > 4 * kWholeBlocks ? 4 * kWholeBlocks : whole;
+  p.split = blocks > whole && trees <= kTreeMaxBatch;
+  if (blocks <= kWholeBlocks || trees > kTreeMaxBatch) return p;
+  // (sizes for fewer trees, which are split, too)
   const int64_t slots = (kTreeSlots + each - 1) / each;
   auto wanted = [trees](int64_t runs) {
     return runs - trees / 2 > runs / 2 ? runs - trees / 2 : (runs + 1) / 2;

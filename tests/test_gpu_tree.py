@@ -128,6 +128,20 @@ def test_short_trees(gpu_device, trees, width, q_heads, kv_heads, dim):
     assert error == 0
 
 
+@pytest.mark.parametrize("trees", [64, 30, 12])
+@pytest.mark.parametrize("dim,width", [(128, 3), (64, 9), (128, 20)])
+def test_long_trees_whole_and_split(gpu_device, trees, dim, width):
+    # 512 workgroups take sequences of up to 2048 positions whole, 240 split them
+    print("whole", trees, dim, width, flush=True)
+    sizes = [width if i < 2 else 1 + i % 2 for i in range(trees)]
+    past = [2047 - width, 1000] + [i * 331 % 900 for i in range(2, trees)]
+    pool = Pool([p + n for p, n in zip(past, sizes)], 8, dim, 16, seed=width)
+    step = Step(sizes, range(trees), 16, dim, seed=trees)
+    out, error = attend(pool, step, gpu_device, max_tree=width)
+    check(pool, step, out)
+    assert error == 0
+
+
 def test_a_mask_of_nothing(gpu_device):
     # no past and an empty mask: zeros; with a past: the past alone
     pool = Pool([4, 40], 2, 128, 8, seed=1)
