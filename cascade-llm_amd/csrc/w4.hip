@@ -80,6 +80,7 @@ constexpr int kNontemporal = 2;
 // pass go past it: 5 rows by 128256 x 4096 (263 MB) 51.9 -> 49.3 us.  Smaller
 // ones lose: gate and up 14336 x 4096 (59 MB), one row, 12.4 -> 13.4.
 constexpr int64_t kW4OnceBytes = 128 << 20;
+constexpr int64_t kW4AgainBytes = 60 << 20;  // see w4_plan
 constexpr int kOutside = 0x7f000000;  // past every descriptor's end, with room for 2^24 more
 
 // The output of four matrix rows for one row of x.
@@ -457,18 +458,24 @@ static int launch_w4_tile(const W4Args &a, hipStream_t s) {
 }
 
 // The shape of a product's workgroups and the parts that K is split into, from
-// sizes alone; times in us, group 64 with zeros unless said.
-// - Up to 16 rows: 4 tiles a wave, 4 waves share K (x is read from LDS once for
-//   four tiles), where that leaves every CU a workgroup; otherwise 2 tiles, 8
-//   waves.  gate and up 14336 x 4096, 16 rows: 16.6 / 21.6; 4096 x 4096, 16
-//   rows: 9.4 / 7.2.
+// sizes alone; times in us, group 64 with zeros.
+// - 16 rows of x a workgroup, up to 16 rows and where reading the matrix again
+//   for each 16 costs little, up to 60 MB in all: 2048 x 2048, 64 rows, 5.1 / 9.3;
+//   1024 x 4096, 128 rows, 7.5 / 11.0; 4096 x 4096, 32 rows, 7.5 / 11.4, 65 rows
+//   (42 MB) 14.0 / 14.6; 14336 x 4096, 24 rows (59 MB), 15.0 / 16.7, 64 rows (117
+//   MB) 25.3 / 21.4.  Of these, 4 tiles a wave, of which 4 share K (x is read from
+//   LDS once for four tiles), where the other form, 2 tiles and 8 waves, would
+//   give a CU more than one workgroup: gate and up 14336 x 4096, 16 rows, 16.6 /
+//   21.6, 4096 x 4096, 16 rows, 9.4 / 7.2; up to 4 rows, whose x is short, more
+//   than two: 14336 x 4096, one row, 10.7 / 9.4, 16 rows 11.1 / 12.4.
 // - More rows: 32 of x a workgroup; 64 where two of these a CU are left: 157
 //   rows, gate and up 14336 x 4096: 74 with 64, 80 with 32; 613 rows, 4096 x
 //   4096: 47 / 44.
-// - Parts of K up to a workgroup a CU (two for more than 16 rows): 16 rows 4096
-//   x 14336: 25.5, in 4 parts 12.7; 61 rows 4096 x 14336: 61, 4 parts 22.4, 8
-//   22.3, 10 26.9; 61 rows 4096 x 4096: 19.6, 4 parts 11.7, 8 12.7; 613 rows:
-//   one part 45, four 52.  Gate and up have no workspace and are not split.
+// - Parts of K up to a workgroup a CU (two for more rows), none of them short: 16
+//   rows 4096 x 14336: 25.5, in 4 parts 12.7, while 32 rows 4096 x 4096 take 8.9
+//   in two and 7.4 whole; 61 rows 4096 x 14336: 61, 4 parts 22.4, 8 22.3, 10 26.9;
+//   613 rows 4096 x 4096: one part 45, four 52.  Gate and up have no workspace
+//   and are not split.
 enum W4Shape { kW4Rows16Wide, kW4Rows16, kW4Rows32, kW4Rows64 };
 
 struct W4Plan {
@@ -478,24 +485,25 @@ struct W4Plan {
 
 static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, bool swiglu) {
   const int64_t row_tiles = (n + 15) / 16 * (swiglu ? 2 : 1), tiles = (k + 127) / 128;
-  // parts of 4 steps or more, so many that there are `wanted` workgroups
-  auto splits = [&](int64_t groups, int64_t wanted, int wk) {
+  // parts of `least` tiles or more, so many that there are `wanted` workgroups
+  auto splits = [&](int64_t groups, int64_t wanted, int64_t least) {
     if (swiglu) return int64_t{1};
     int64_t parts = wanted / groups;
-    if (parts > tiles / (4 * wk)) parts = tiles / (4 * wk);
+    if (parts > tiles / least) parts = tiles / least;
     return parts < 1 ? int64_t{1} : parts;
   };
   auto plan = [](W4Shape shape, int64_t parts) {
     return W4Plan{shape, static_cast<int32_t>(parts)};
   };
-  if (m <= 16) {
-    const int64_t groups = (row_tiles + 3) / 4, parts = splits(groups, 256, 4);
-    if (groups * parts >= 256) return plan(kW4Rows16Wide, parts);
-    return plan(kW4Rows16, splits((row_tiles + 1) / 2, 256, 8));
+  const int64_t blocks16 = (m + 15) / 16;
+  if (m <= 16 || row_tiles * tiles * 1024 * blocks16 <= kW4AgainBytes) {
+    const int64_t groups = (row_tiles + 3) / 4 * blocks16, parts = splits(groups, 256, 28);
+    if (groups * parts > (m <= 4 ? 256 : 128)) return plan(kW4Rows16Wide, parts);
+    return plan(kW4Rows16, splits((row_tiles + 1) / 2 * blocks16, 256, 32));
   }
   const int64_t groups = (row_tiles + 7) / 8;
   if (groups * ((m + 63) / 64) >= 512) return plan(kW4Rows64, 1);
-  return plan(kW4Rows32, splits(groups * ((m + 31) / 32), 512, 2));
+  return plan(kW4Rows32, splits(groups * ((m + 31) / 32), 512, 8));
 }
 
 static int64_t w4_workspace_bytes(const W4Plan &plan, int64_t m, int64_t n) {
@@ -548,7 +556,7 @@ static int launch_w4(W4Args a, int64_t x_stride, int64_t m, int64_t n, int64_t k
   }
   a.splits = plan.splits;
   a.partial = static_cast<float *>(workspace);
-  a.once = m <= 32 && (n + 15) / 16 * a.tiles * 1024 * (kSwiglu ? 2 : 1) >= kW4OnceBytes;
+  a.once = m <= 16 && (n + 15) / 16 * a.tiles * 1024 * (kSwiglu ? 2 : 1) >= kW4OnceBytes;
   switch (plan.shape) {
     case kW4Rows16Wide: return launch_w4_tile<kSwiglu, 4, 1, 1, 4>(a, s);
     case kW4Rows16: return launch_w4_tile<kSwiglu, 2, 1, 1, 8>(a, s);

@@ -72,10 +72,11 @@ def test_linear_of_the_models_sizes(gpu_device, rows):
 
 @pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
 def test_linear_of_many_rows(gpu_device, group, zeros):
-    # workgroups of 64 rows
+    # workgroups of 16 rows over a short K, of 64 over a longer one
     print("many rows", group, zeros, flush=True)
-    linear_case(gpu_device, 1001, 4100, 264, group, zeros, residual=True, seed=7)
-    linear_case(gpu_device, 1001, 4100, 264, group, zeros, logits=True, seed=8)
+    for k in (264, 520):
+        linear_case(gpu_device, 1001, 4100, k, group, zeros, residual=True, seed=7)
+        linear_case(gpu_device, 1001, 4100, k, group, zeros, logits=True, seed=8)
 
 
 def test_linear_past_the_caches(gpu_device):
@@ -117,6 +118,7 @@ def test_a_split_product_needs_its_workspace(gpu_device):
 
 @pytest.mark.parametrize("rows,n,k,group,zeros", [
     (157, 14336, 264, 32, False), (100, 33000, 136, 128, True),
+    (157, 14336, 520, 64, True), (130, 14336, 520, 32, False), (100, 33000, 392, 128, True),
     (1, 16, 64, 32, True), (1, 14336, 4096, 128, False), (3, 100, 1000, 64, True),
     (16, 257, 264, 32, False), (17, 2000, 520, 128, True), (61, 14336, 4096, 64, True),
     (64, 48, 14336, 128, False), (65, 300, 72, 32, True), (200, 500, 1032, 64, False),
