@@ -167,13 +167,15 @@ __device__ __forceinline__ SplitWeights tree_weights(float a, float b) {
 // block's K operands are read beside this block's product with V.
 //
 // What bounds it: to 64 columns or so the loads, 64 trees of 8 nodes over up to
-// 4096 positions (606 MB) 117 us, 5.2 TB/s, one of 16 over 32768 (135 MB) 41 us
-// with the join of its runs (the start, page lookups and the join are 14 of it);
-// above, vector and matrix instructions, 2 us a block of 252 columns, of which
-// the 384 MFMAs are 0.7: 24 trees of up to 63 nodes over up to 16384 positions
-// (885 MB) 326 us.  Lookups of sixteen blocks' pages at a time, lane by lane,
-// and operands read ahead took the last from 570 us to 355, V's turned reads in
-// place of 32 permutations a block to 326.
+// 4096 positions (606 MB) 117 us, 5.2 TB/s, one of 16 over 32768 (135 MB) 36 us
+// with the join of its runs (the start, page lookups and the join are 13 of it);
+// above, vector and matrix instructions, which two waves of a SIMD hardly overlap:
+// a wave's block of 32 columns is 48 MFMAs (768 cycles) and 160 vector
+// instructions (720, a sixth of them exponentials), a block of 256 columns 1.7 us;
+// 24 trees of up to 63 nodes over up to 16384 positions (885 MB) 325 us.  Lookups
+// of sixteen blocks' pages at a time, lane by lane, and operands read ahead took
+// that from 570 us to 355, V's turned reads in place of 32 permutations a block to
+// 326.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeArgs a) {
   constexpr int D = T::D, CT = T::CT, WC = T::WC, WP = T::WP;
