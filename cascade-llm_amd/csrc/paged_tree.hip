@@ -144,13 +144,25 @@ __device__ __forceinline__ u32x2 read_turned(const unsigned char *from) {
                  (__attribute__((address_space(3))) s16x4 *)(from)));
 }
 
-// split_weights with one instruction a weight less: the upper part is cut off,
-// and the lower one, what remains and 2^-23 of the weight, is positive.
-__device__ __forceinline__ SplitWeights tree_weights(float a, float b) {
-  constexpr float kAbove = 1.0f + 0x1p-23f;
-  const uint32_t upper =
-      __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-  return {upper, pack_bf16x2(fmaf(a, kAbove, -lo_bf16(upper)), fmaf(b, kAbove, -hi_bf16(upper)))};
+// Two weights as sums of three bf16 values each, cut off one after the other:
+// 8 bits each of the 24 that fp32 has, so nothing is rounded.
+struct WeightParts {
+  uint32_t upper, middle, lower;
+};
+
+__device__ __forceinline__ WeightParts tree_weights(float a, float b) {
+  auto cut = [&] {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  };
+  WeightParts w;
+  w.upper = cut();
+  a -= lo_bf16(w.upper);
+  b -= hi_bf16(w.upper);
+  w.middle = cut();
+  a -= lo_bf16(w.middle);
+  b -= hi_bf16(w.middle);
+  w.lower = cut();
+  return w;
 }
 
 // One workgroup takes the columns (node, query head of the KV head) of a tree
@@ -159,21 +171,24 @@ __device__ __forceinline__ SplitWeights tree_weights(float a, float b) {
 // and V rows come into LDS once, by loads that go there directly into a ring of
 // slots, and its WC waves multiply them with 16 CT columns each:
 //   S^T = K q^T, running maximum m and sum l a column, O^T += V^T P^T,
-// all on the matrix cores, S, m, l and O in fp32, and P as two bf16 parts (as
-// in the attention of one token: one rounding of P would show in the result).
+// all on the matrix cores, S, m, l and O in fp32, and P as three bf16 parts, which
+// are all of its bits.  Two parts are 2^-16 off: enough to turn the rounding of
+// one result in 500 (rows 1.3e-4 from those of exact weights in the mean, 0.5e-4
+// with three, which is what the order of fp32 sums does), for 15% of the time
+// of wide trees (24 of up to 63 nodes 332 us and 390) and 2 to 8% of others'.
 // K and V rows lie swizzled in LDS, K for plain reads of its operands, V for
 // reads that turn 4 x 16 values.  The reference of the exponents follows the
 // maximum only where it is passed by 2^8, so O is rarely scaled, and the next
 // block's K operands are read beside this block's product with V.
 //
 // What bounds it: to 64 columns or so the loads, 64 trees of 8 nodes over up to
-// 4096 positions (606 MB) 117 us, 5.2 TB/s, one of 16 over 32768 (135 MB) 36 us
+// 4096 positions (606 MB) 117 us, 5.2 TB/s, one of 16 over 32768 (135 MB) 39 us
 // with the join of its runs (the start, page lookups and the join are 13 of it);
 // above, vector and matrix instructions, which two waves of a SIMD hardly overlap:
-// a wave's block of 32 columns is 48 MFMAs (768 cycles) and 160 vector
-// instructions (720, a sixth of them exponentials), a block of 256 columns 1.7 us;
-// 24 trees of up to 63 nodes over up to 16384 positions (885 MB) 325 us.  Lookups
-// of sixteen blocks' pages at a time, lane by lane, and operands read ahead took
+// a wave's block of 32 columns is 64 MFMAs (1024 cycles) and 200 vector
+// instructions (900, a sixth of them exponentials); 24 trees of up to 63 nodes
+// over up to 16384 positions (885 MB) 390 us.  With two parts of P, lookups of
+// sixteen blocks' pages at a time, lane by lane, and operands read ahead took
 // that from 570 us to 355, V's turned reads in place of 32 permutations a block to
 // 326.
 template <typename T, bool SPLIT>
@@ -483,7 +498,7 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
         for (int e = 0; e < DV; ++e) x.o[e] *= alpha;
       }
     }
-    u32x4 pop[CT], low[CT];
+    u32x4 upper[CT], middle[CT], lower[CT];
     auto weights = [&](int ct) __attribute__((always_inline)) {
       TreeColumns<DV> &x = state[ct];
       // (a masked score's -inf stays so)
@@ -496,9 +511,10 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
       x.l += psum;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const SplitWeights w = tree_weights(p[2 * n], p[2 * n + 1]);
-        pop[ct][n] = w.upper;
-        low[ct][n] = w.lower;
+        const WeightParts w = tree_weights(p[2 * n], p[2 * n + 1]);
+        upper[ct][n] = w.upper;
+        middle[ct][n] = w.middle;
+        lower[ct][n] = w.lower;
       }
     };
     weights(0);
@@ -510,19 +526,20 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
       TreeColumns<DV> &x = state[ct];
 #pragma unroll
       for (int e = 0; e < DV; ++e) {
-        x.o[e] = mfma_16x16x32_bf16(vop[e], low[ct], x.o[e]);
-        x.o[e] = mfma_16x16x32_bf16(vop[e], pop[ct], x.o[e]);
+        x.o[e] = mfma_16x16x32_bf16(vop[e], lower[ct], x.o[e]);
+        x.o[e] = mfma_16x16x32_bf16(vop[e], middle[ct], x.o[e]);
+        x.o[e] = mfma_16x16x32_bf16(vop[e], upper[ct], x.o[e]);
       }
       if (ct + 1 < CT) weights(ct + 1);
     }
     if constexpr (CT > 1) {
       // a tile's product with V beside the next one's weights
 #pragma unroll
-      for (int n = 0; n < 2 * DV * (CT - 1); ++n) {
+      for (int n = 0; n < 3 * DV * (CT - 1); ++n) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x8, 2 * DV, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, 3 * DV, 0);
     }
   };
 
@@ -549,11 +566,18 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   auto put = [&](int col, int d, float m, float den, f32x4 (&sum)[2]) __attribute__((always_inline)) {
     const int node = static_cast<int>((static_cast<uint32_t>(col) * a.group_inverse) >> 16);
     const int head = kv * a.group + col - node * a.group;
-    if (s_special) {
-      // the infinities and NaN that the blocks with the tree left out
+    // Infinities and NaN of V: the blocks with the tree left theirs out, and in
+    // the others a part of a weight that is zero may have made an infinity a NaN.
+    int from = s_special ? max(first, past / kPagedBlock) : end;
+    if (den < INFINITY)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!(fabsf(sum[i / 4][i % 4]) < INFINITY)) from = first;
+    if (from < end) {
       const uint64_t mask = static_cast<uint64_t>(a.masks[token0 + node]);
       const int to = min(end * kPagedBlock, len);
-      for (int p = max(first, past / kPagedBlock) * kPagedBlock; p < to; ++p) {
+      f32x4 special[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+      for (int p = from * kPagedBlock; p < to; ++p) {
         const int page = table[p >> a.page_shift];
         if (page < 0 || page >= a.num_pages) continue;
         if (p >= past && !((mask >> (p - past)) & 1)) continue;
@@ -562,8 +586,13 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float value = bf16_to_f32(v[i]);
-          if (!(fabsf(value) < INFINITY)) sum[i / 4][i % 4] += value;
+          if (!(fabsf(value) < INFINITY)) special[i / 4][i % 4] += value;
         }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float value = special[i / 4][i % 4];
+        if (!(fabsf(value) < INFINITY)) sum[i / 4][i % 4] = value;
       }
     }
     if (!SPLIT || count == 1) {
@@ -643,6 +672,9 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
 // for 79 MB).
 constexpr int kTreeMergeThreads = 256;
 
+// A run's factor, never zero: that would turn an infinite sum into a NaN.
+__device__ __forceinline__ float run_weight(float x) { return fmaxf(paged_exp2(x), FLT_MIN); }
+
 template <int D, int SLICES>
 __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs a) {
   constexpr int kHeads = kTreeMergeThreads / (SLICES * D / 4);
@@ -675,8 +707,8 @@ __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs 
       const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * at);
       const f32x4 v = *reinterpret_cast<const f32x4 *>(a.part_acc + at * D + 4 * d);
       const float mnew = fmaxf(m, ml.x);
-      const float keep = paged_exp2((m - mnew) * a.scale_log2);
-      const float w = paged_exp2((ml.x - mnew) * a.scale_log2);
+      const float keep = run_weight((m - mnew) * a.scale_log2);
+      const float w = run_weight((ml.x - mnew) * a.scale_log2);
       m = mnew;
       den = fmaf(w, ml.y, den * keep);
 #pragma unroll
@@ -698,7 +730,7 @@ __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs 
     float sum = 0.0f, r = 0.0f;
 #pragma unroll
     for (int k = 0; k < SLICES; ++k) {
-      const float w = paged_exp2((s_ml[hh][k][0] - mm) * a.scale_log2);
+      const float w = run_weight((s_ml[hh][k][0] - mm) * a.scale_log2);
       sum = fmaf(w, s_ml[hh][k][1], sum);
       r = fmaf(w, s_acc[hh][k][dim / 4][dim % 4], r);
     }
