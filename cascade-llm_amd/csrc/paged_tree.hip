@@ -762,10 +762,13 @@ struct TreePlan {
   int64_t round, two;  // runs wanted, in one round and in two
   int64_t runs;        // at most
   size_t plan_bytes, ml_bytes, acc_bytes;
+
+  size_t bytes() const { return kPagedAlign + plan_bytes + ml_bytes + acc_bytes; }
 };
 
 constexpr int64_t kTreeSlots = 256;      // workgroups that the device holds: one a CU
 constexpr int64_t kTreeMaxBatch = 256;   // of a split launch
+constexpr int64_t kTreeColumns = 256;    // that a workgroup takes at most
 
 static TreePlan tree_plan(int64_t trees, int64_t max_tree, int64_t q_heads, int64_t kv_heads,
                           int64_t dim, int64_t max_length) {
@@ -938,6 +941,15 @@ __global__ __launch_bounds__(kAcceptThreads) void tree_accept_kernel(AcceptArgs 
   }
 }
 
+static bool tree_shape_ok(int64_t trees, int64_t max_tree, int64_t n_q_heads,
+                          int64_t n_kv_heads, int64_t head_dim, int64_t max_length) {
+  return trees > 0 && trees <= 0xffff && max_tree > 0 && max_tree <= kTreeNodes &&
+         n_kv_heads > 0 && n_q_heads > 0 && n_q_heads % n_kv_heads == 0 &&
+         n_q_heads / n_kv_heads <= kPagedGroup && n_q_heads <= 0xffff &&
+         (head_dim == 64 || head_dim == 128) && max_length > 0 &&
+         max_length <= 0x7fffffff - 64;
+}
+
 static bool int32_ok(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 static bool int64_ok(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
 
@@ -948,22 +960,20 @@ using namespace cascade;
 extern "C" size_t cascade_paged_tree_attention_workspace_bytes(
     int64_t trees, int64_t max_tree, int64_t n_q_heads, int64_t n_kv_heads,
     int64_t head_dim, int64_t max_length) {
-  if (trees <= 0 || trees > 0xffff || max_tree <= 0 || max_tree > kTreeNodes ||
-      n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads ||
-      n_q_heads / n_kv_heads > kPagedGroup || n_q_heads > 0xffff ||
-      (head_dim != 64 && head_dim != 128) || max_length <= 0 || max_length > 0x7fffffff - 64)
-    return 0;
-  // enough for fewer trees, nodes and positions too: a launch of more than
-  // kTreeMaxBatch trees needs none
-  size_t most = 0;
+  if (!tree_shape_ok(trees, max_tree, n_q_heads, n_kv_heads, head_dim, max_length)) return 0;
+  // Enough for fewer trees, nodes and positions too: a launch of more than
+  // kTreeMaxBatch trees needs none, and more trees or positions have as many
+  // runs or more.  Fewer nodes may take fewer workgroups a run, and so more runs:
+  // the largest trees of each number of workgroups are looked at.
+  const int64_t group = n_q_heads / n_kv_heads;
   const int64_t n = trees < kTreeMaxBatch ? trees : kTreeMaxBatch;
-  for (int64_t nodes = max_tree;; nodes /= 2) {
+  size_t most = 0;
+  for (int64_t nodes = max_tree; nodes > 0;) {
     const TreePlan p = tree_plan(n, nodes, n_q_heads, n_kv_heads, head_dim, max_length);
-    const size_t need = p.plan_bytes + p.ml_bytes + p.acc_bytes;
-    most = need > most ? need : most;
-    if (nodes <= 1) break;
+    most = p.bytes() > most ? p.bytes() : most;
+    nodes = p.col_groups > 1 ? kTreeColumns * (p.col_groups - 1) / group : 0;
   }
-  return kPagedAlign + most;
+  return most;
 }
 
 extern "C" int cascade_paged_tree_attention_bf16(
@@ -984,9 +994,9 @@ extern "C" int cascade_paged_tree_attention_bf16(
       sequences <= 0 || num_pages <= 0 || num_pages > 0x7fffffff || max_length <= 0)
     return CASCADE_EINVAL;
   TreeArgs a{};
-  const size_t need = cascade_paged_tree_attention_workspace_bytes(
-      trees, max_tree, n_q_heads, n_kv_heads, head_dim, max_length);
-  if (need == 0 || !page_shift_of(page_size, &a.page_shift)) return CASCADE_ESHAPE;
+  if (!tree_shape_ok(trees, max_tree, n_q_heads, n_kv_heads, head_dim, max_length) ||
+      !page_shift_of(page_size, &a.page_shift))
+    return CASCADE_ESHAPE;
   if (table_stride < (max_length + page_size - 1) / page_size ||
       page_head_stride < page_size * head_dim ||
       page_stride < (n_kv_heads - 1) * page_head_stride + page_size * head_dim)
@@ -1000,7 +1010,8 @@ extern "C" int cascade_paged_tree_attention_bf16(
                              page_head_stride, out_token_stride, out_head_stride};
   for (int64_t s : strides)
     if (!stride_ok(s)) return CASCADE_EALIGN;
-  if (workspace_bytes < need) return CASCADE_EWORKSPACE;
+  const TreePlan p = tree_plan(trees, max_tree, n_q_heads, n_kv_heads, head_dim, max_length);
+  if (workspace_bytes < (p.split ? p.bytes() : kPagedAlign)) return CASCADE_EWORKSPACE;
   a.q = static_cast<const uint16_t *>(q);
   a.q_token = q_token_stride;
   a.q_head = q_head_stride;
@@ -1032,7 +1043,6 @@ extern "C" int cascade_paged_tree_attention_bf16(
   a.masks = masks;
   a.tokens = tokens;
   a.max_tree = static_cast<int32_t>(max_tree);
-  const TreePlan p = tree_plan(trees, max_tree, n_q_heads, n_kv_heads, head_dim, max_length);
   a.col_groups = p.col_groups;
   a.group_inverse = (65536u + a.group - 1) / a.group;
   const hipStream_t s = static_cast<hipStream_t>(stream);
