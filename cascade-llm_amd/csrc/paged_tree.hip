@@ -196,7 +196,7 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   constexpr int D = T::D, CT = T::CT, WC = T::WC, WP = T::WP;
   constexpr int KC = T::KC, DV = T::DV, ROW = T::ROW;
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[T::LDS];
-  __shared__ int s_special;
+  __shared__ int s_special;  // the first block whose infinities and NaN were left out
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
     }
   }
 
-  if (tid == 0) s_special = 0;
+  if (tid == 0) s_special = end;
   TreeColumns<DV> state[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
           any |= bits;
           vop[e][i] = pair & ~bits;
         }
-      if (any != 0) s_special = 1;
+      if (any != 0) atomicMin(&s_special, blk);
     }
     if (tail) {
 #pragma unroll
@@ -566,9 +566,10 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
   auto put = [&](int col, int d, float m, float den, f32x4 (&sum)[2]) __attribute__((always_inline)) {
     const int node = static_cast<int>((static_cast<uint32_t>(col) * a.group_inverse) >> 16);
     const int head = kv * a.group + col - node * a.group;
-    // Infinities and NaN of V: the blocks with the tree left theirs out, and in
-    // the others a part of a weight that is zero may have made an infinity a NaN.
-    int from = s_special ? max(first, past / kPagedBlock) : end;
+    // Infinities and NaN of V: the blocks with the tree or a bad page left theirs
+    // out, and in the others a part of a weight that is zero may have made an
+    // infinity a NaN.
+    int from = s_special;
     if (den < INFINITY)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
