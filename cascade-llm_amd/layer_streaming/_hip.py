@@ -1763,6 +1763,7 @@ def _check_w4(x, out, dtype, residual, workspace, **matrices):
     for name, matrix in matrices.items():
         if not isinstance(matrix, W4Matrix):
             raise TypeError("{} must be a W4Matrix".format(name))
+        matrix.launch  # raises where its memory is gone
         if matrix.device != device:
             raise ValueError("{} must live on {}, got {}".format(
                 name, device, matrix.device))

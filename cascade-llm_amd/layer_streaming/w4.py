@@ -24,7 +24,10 @@ class W4Matrix:
 
     ``packed`` (uint8), ``scales`` (bf16) and ``zeros`` (uint8, or None for a
     zero point of 8 everywhere) are in the kernels' tiles (cascade_hip.h, "4-bit
-    weights"); ``values`` gives the matrix back."""
+    weights"); ``values`` gives the matrix back.  The three are views of the
+    matrix's memory: writing to them changes it, giving them other memory
+    (``set_``, ``.data =``) does not.  Where that memory's storage is resized to
+    nothing, the products refuse the matrix until it is back."""
 
     def __init__(self, packed, scales, zeros, n, k, group):
         n, k = operator.index(n), operator.index(k)
@@ -41,19 +44,44 @@ class W4Matrix:
             _like(packed, part, name, dtype, shape)
             if not part.is_contiguous() or part.data_ptr() % 16:
                 raise ValueError("{} must be contiguous and 16-byte aligned".format(name))
-        self._parts = packed, scales, zeros
+        # views that nobody else can give other memory
+        self._parts = tuple(None if part is None else part.detach()
+                            for part in (packed, scales, zeros))
         self._sizes = n, k, group
-        # what a launch takes of it: device index, addresses, sizes
-        self._launch = (packed.get_device(), packed.data_ptr(), scales.data_ptr(),
-                        0 if zeros is None else zeros.data_ptr(), n, k, group)
+        self._index = packed.get_device()
+        # their storages; the place of each in its own, and what that has to hold
+        self._storages = [None if part is None else part.untyped_storage()
+                          for part in self._parts]
+        self._places = []
+        for part in self._parts:
+            place = 0 if part is None else part.storage_offset() * part.element_size()
+            end = 0 if part is None else place + part.numel() * part.element_size()
+            self._places += [place, end]
 
-    packed = property(lambda self: self._parts[0])
-    scales = property(lambda self: self._parts[1])
-    zeros = property(lambda self: self._parts[2])
+    def __reduce__(self):  # a copy's addresses are its own
+        return W4Matrix, (*self._parts, *self._sizes)
+
+    def _view(self, i):
+        return None if self._parts[i] is None else self._parts[i].detach()
+
+    packed = property(lambda self: self._view(0))
+    scales = property(lambda self: self._view(1))
+    zeros = property(lambda self: self._view(2))
     n = property(lambda self: self._sizes[0])
     k = property(lambda self: self._sizes[1])
     group = property(lambda self: self._sizes[2])
-    launch = property(lambda self: self._launch)
+
+    @property
+    def launch(self):
+        """What a launch takes of it: device index, addresses, sizes."""
+
+        p, s, z = self._storages
+        p_at, p_end, s_at, s_end, z_at, z_end = self._places
+        if (p.nbytes() < p_end or s.nbytes() < s_end
+                or (z is not None and z.nbytes() < z_end)):
+            raise ValueError("the memory of the matrix was released")
+        return (self._index, p.data_ptr() + p_at, s.data_ptr() + s_at,
+                0 if z is None else z.data_ptr() + z_at, *self._sizes)
 
     @classmethod
     def pack(cls, values, scales, zeros=None, group=128):
