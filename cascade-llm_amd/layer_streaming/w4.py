@@ -125,6 +125,8 @@ class W4Matrix:
             if zeros:
                 low, high = low.clamp(max=0), high.clamp(min=0)
                 scale = (high - low) / 15
+                # (two halves of a range that fp32 does not hold)
+                scale = torch.where(scale.isfinite(), scale, high / 15 - low / 15)
             else:
                 scale = torch.maximum(high, -low) / 7
             scale = scale.to(torch.bfloat16).float()
