@@ -84,6 +84,7 @@ class W4Matrix:
                 0 if z is None else z.data_ptr() + z_at, *self._sizes)
 
     @classmethod
+    @torch.no_grad()
     def pack(cls, values, scales, zeros=None, group=128):
         """Lay out ``values`` (uint8 [n, k], 0..15) with ``scales`` (bf16 [n,
         ceil(k / group)]) and ``zeros`` (uint8, alike, 0..15); k a multiple of
@@ -99,6 +100,7 @@ class W4Matrix:
                    None if zeros is None else _by_tile(zeros, n, groups), n, k, group)
 
     @classmethod
+    @torch.no_grad()
     def quantize(cls, weight, group=128, zeros=False):
         """4-bit weights of a bf16 matrix [n, k]: of each group's values w,
 

@@ -1,8 +1,10 @@
-"""Quantization to 4 bits at the ends of bf16's range, on the CPU."""
+"""Quantization to 4 bits at the ends of bf16's range and of parameters, on the
+CPU."""
 
+import pytest
 import torch
 
-from layer_streaming import W4Matrix
+from layer_streaming import W4Matrix, w4
 from paged_cases import normal
 
 BF = torch.bfloat16
@@ -26,3 +28,18 @@ def test_a_range_past_fp32_has_a_scale():
     # other groups as ever
     assert torch.equal(m.values()[1][1], W4Matrix.quantize(w[1:], group=32, zeros=True)
                        .values()[1][0])
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_a_parameter_leaves_no_graph(monkeypatch, zeros):
+    w = normal((40, 64), torch.Generator().manual_seed(2))
+    seen = []
+    kept = w4._by_tile
+    monkeypatch.setattr(w4, "_by_tile", lambda x, *sizes: (
+        seen.append(x.requires_grad), kept(x, *sizes))[1])
+    m = W4Matrix.quantize(torch.nn.Parameter(w), group=32, zeros=zeros)
+    assert seen and not any(seen) and not m.scales.requires_grad
+    for a, b in zip(m.values(), W4Matrix.quantize(w, group=32, zeros=zeros).values()):
+        assert (a is None and b is None) or torch.equal(a, b)
+    scales = torch.nn.Parameter(torch.ones(40, 2, dtype=BF))
+    assert not W4Matrix.pack(m.values()[0], scales, group=32).scales.requires_grad
