@@ -131,6 +131,48 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs
 }
 
 // ------------------------------------------------------------- attention
+constexpr int kWholeWaves = 8;   // of one that takes a whole row
+constexpr int kPagedMaxBatch = 1024;  // of a split launch
+// Workgroups that the device holds at a time (256 CUs with four and with six).
+constexpr int64_t kPagedSlots128 = 1024, kPagedSlots64 = 1536;
+
+// Two weights as sums of two bf16 values each, for the product with V: one
+// value alone, 2^-8 off, shows next to the rounding of the result where V's
+// rows cancel.  The upper parts are cut off just below the weights (a factor
+// of 1 - 2^-24 leaves no normal fp32 number as it is), so that the lower ones,
+// which fp32 holds exactly, are positive: a zero or a negative one would turn
+// an infinite value of V into a NaN.  Of a weight in [2^e, 2^(e+1)) the lower
+// part is at most 2^(e-7), and its rounding, half a step, 2^(e-16).  The second
+// product hides behind the loads (64 ragged sequences of up to 16384 positions
+// 318 us, 317 with one; 32769 positions 28.8 and 28.6).
+struct SplitWeights {
+  uint32_t upper, lower;
+};
+
+__device__ __forceinline__ SplitWeights split_weights(float a, float b) {
+  constexpr float kBelow = 1.0f - 0x1p-24f;
+  const uint32_t upper = __builtin_amdgcn_perm(__float_as_uint(b * kBelow),
+                                               __float_as_uint(a * kBelow), 0x07060302u);
+  return {upper, pack_bf16x2(a - lo_bf16(upper), b - hi_bf16(upper))};
+}
+
+__device__ __forceinline__ PagedRow paged_row(const PagedAttnArgs &a, int b, bool flag) {
+  PagedRow r{-1, 0};
+  if (b >= a.batch) return r;
+  r.row = a.rows != nullptr ? a.rows[b] : b;
+  if (r.row >= a.sequences) {
+    if (flag) flag_range(a.error);
+    r.row = -1;
+  }
+  if (r.row < 0) return r;
+  r.len = a.lengths[r.row];
+  if (r.len < 0 || r.len > a.max_length) {
+    if (flag) flag_range(a.error);
+    r.len = min(max(r.len, 0), a.max_length);
+  }
+  return r;
+}
+
 // Workgroup (run, KV head), or (batch row, KV head) without SPLIT; each wave
 // runs an online softmax over every WAVES-th block of 32 positions and the
 // waves merge in LDS.  The products are v_mfma_f32_16x16x32_bf16 with the

@@ -1,6 +1,5 @@
 // What the kernels over a paged KV cache share (paged.hip, paged_tree.hip):
-// checks of device-held indices, the runs that a ragged batch is cut into,
-// and softmax weights as pairs of bf16 values.
+// checks of device-held indices and the runs that a ragged batch is cut into.
 #pragma once
 
 #include <cfloat>
@@ -39,7 +38,9 @@ struct PagedAttnArgs {
   // split runs (SPLIT kernels): see "Runs"
   double per_round, per_two;  // 1 / runs wanted, in one round and in two
   int32_t *plan;    // [batch][2]: first run of a batch row, and how many
-  float *part_ml;   // [run][q_heads][2]: maximum (log2 units), sum
+  // [run][q_heads][2]: maximum (of scores as they are summed for trees, in powers
+  // of two for single tokens), sum; of trees [run][node][q_heads], part_acc too
+  float *part_ml;
   float *part_acc;  // [run][q_heads][D]
   int32_t runs;     // that the workspace holds
 };
@@ -47,14 +48,10 @@ struct PagedAttnArgs {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kPagedWaves = 4;   // of a workgroup that takes a run
-constexpr int kWholeWaves = 8;   // of one that takes a whole row
 constexpr int kWholeBlocks = 16;  // rows of at most this many blocks are not split
 constexpr int kPagedBlock = 32;  // positions a wave step
 constexpr int kPagedGroup = 16;  // MFMA columns
 constexpr int kPagedMinRun = 4;  // blocks
-constexpr int kPagedMaxBatch = 1024;  // of a split launch
-// Workgroups that the device holds at a time (256 CUs with four and with six).
-constexpr int64_t kPagedSlots128 = 1024, kPagedSlots64 = 1536;
 constexpr double kPagedLongRun = 100.0;  // blocks
 constexpr size_t kPagedAlign = 256;
 
@@ -62,48 +59,11 @@ __device__ __forceinline__ float paged_exp2(float x) {
   return __builtin_amdgcn_exp2f(x);
 }
 
-// Two weights as sums of two bf16 values each, for the product with V: one
-// value alone, 2^-8 off, shows next to the rounding of the result where V's
-// rows cancel.  The upper parts are cut off just below the weights (a factor
-// of 1 - 2^-24 leaves no normal fp32 number as it is), so that the lower ones,
-// which fp32 holds exactly, are positive: a zero or a negative one would turn
-// an infinite value of V into a NaN.  Of a weight in [2^e, 2^(e+1)) the lower
-// part is at most 2^(e-7), and its rounding, half a step, 2^(e-16).  The second
-// product hides behind the loads (64 ragged sequences of up to 16384 positions
-// 318 us, 317 with one; 32769 positions 28.8 and 28.6).
-struct SplitWeights {
-  uint32_t upper, lower;
-};
-
-__device__ __forceinline__ SplitWeights split_weights(float a, float b) {
-  constexpr float kBelow = 1.0f - 0x1p-24f;
-  const uint32_t upper = __builtin_amdgcn_perm(__float_as_uint(b * kBelow),
-                                               __float_as_uint(a * kBelow), 0x07060302u);
-  return {upper, pack_bf16x2(a - lo_bf16(upper), b - hi_bf16(upper))};
-}
-
 // Table row and length of batch row b.  row < 0: nothing to do.
 struct PagedRow {
   int64_t row;
   int32_t len;
 };
-
-__device__ __forceinline__ PagedRow paged_row(const PagedAttnArgs &a, int b, bool flag) {
-  PagedRow r{-1, 0};
-  if (b >= a.batch) return r;
-  r.row = a.rows != nullptr ? a.rows[b] : b;
-  if (r.row >= a.sequences) {
-    if (flag) flag_range(a.error);
-    r.row = -1;
-  }
-  if (r.row < 0) return r;
-  r.len = a.lengths[r.row];
-  if (r.len < 0 || r.len > a.max_length) {
-    if (flag) flag_range(a.error);
-    r.len = min(max(r.len, 0), a.max_length);
-  }
-  return r;
-}
 
 // Runs.  The lengths are on the device, so the launch is sized for any of
 // them and each workgroup finds its own piece of work: the blocks of 32
