@@ -97,9 +97,9 @@ struct TreeShape {
   static constexpr int D = DIM, CT = CT_, WC = WC_, WP = WP_;
   static constexpr int WAVES = WC * WP;
   static constexpr int COLS = 16 * CT * WC;  // of a workgroup
-  // Rows that no other workgroup reads need no place in a cache: one tree of 16
-  // nodes over 32768 positions 47.5 -> 44 us, 64 of 8 over up to 4096 148 -> 141
-  // (as the kernel then was).  Of 16 tiles the workgroups may share rows.
+  // Rows that no other workgroup reads need no place in a cache: 64 trees of 8
+  // nodes over up to 4096 positions 131 -> 118 us, one of 16 over 32768 45.9 ->
+  // 45.2 (heads of 64 27.3 -> 28.6).  Of 16 tiles the workgroups may share rows.
   static constexpr bool ONCE = CT * WC < 16;
   static constexpr int KC = D / 32;          // 32-dim chunks
   static constexpr int DV = D / 16;          // tiles of 16 dims
@@ -110,7 +110,7 @@ struct TreeShape {
   // Workgroups a CU, in whose share of the LDS the slots have to fit: two that
   // wait at barriers of their own are worth more than one with twice the waves
   // and slots (19 sequences of up to 2048 positions, 14 heads of 64, 9 nodes:
-  // 26.1 -> 19.4 us; 64 of up to 4096, 8 nodes: 124 -> 117).  Sixteen tiles take
+  // 26.7 -> 19.8 us; 64 of up to 4096, 8 nodes: 128 -> 118).  Sixteen tiles take
   // all registers, four groups of 128 dims all of the LDS.
   static constexpr int PAIR = CT * WC <= 8 && 4 * WP * SLOT <= 160 * 1024 - 32 ? 2 : 1;
   static constexpr int FIT = (160 * 1024 / PAIR - 16) / (WP * SLOT);
@@ -183,11 +183,11 @@ __device__ __forceinline__ WeightParts tree_weights(float a, float b) {
 //
 // What bounds it: to 64 columns or so the loads, 64 trees of 8 nodes over up to
 // 4096 positions (606 MB) 117 us, 5.2 TB/s, one of 16 over 32768 (135 MB) 39 us
-// with the join of its runs (the start, page lookups and the join are 13 of it);
+// with the join of its runs (the start, page lookups and the join are 14 of it);
 // above, vector and matrix instructions, which two waves of a SIMD hardly overlap:
 // a wave's block of 32 columns is 64 MFMAs (1024 cycles) and 200 vector
-// instructions (900, a sixth of them exponentials); 24 trees of up to 63 nodes
-// over up to 16384 positions (885 MB) 390 us.  With two parts of P, lookups of
+// instructions (900, a sixth of them exponentials), a block of 256 columns 2.0 us;
+// 24 trees of up to 63 nodes over up to 16384 positions (885 MB) 390 us.  With two parts of P, lookups of
 // sixteen blocks' pages at a time, lane by lane, and operands read ahead took
 // that from 570 us to 355, V's turned reads in place of 32 permutations a block to
 // 326.
@@ -740,22 +740,24 @@ __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs 
   }
 }
 
-// Which shape a call takes, whether it splits, and its sizes.
+// Which shape a call takes, whether it splits, and its sizes (times in us).
 // - Tiles of 16 columns: the least power of two that takes a tree of max_tree
 //   nodes, to 16; more columns take workgroups of their own.
 // - Split over runs up to 256 trees, which fill the device, and from so many
 //   blocks on that whole trees would leave it unbalanced: 17, where the launch has
 //   128 workgroups or less, to 65 at 512, in proportion (below, one workgroup is a
 //   whole tree and no second launch is needed).  64 trees of 8 nodes, 8 KV heads,
-//   over up to 1000 positions: 33.1 us whole, 37.4 split, up to 2000 58.6 and
-//   63.2; 40 trees of 4 up to 1000 27.3 and 26.8, of 60 70.5 and 84.8, of 4 up to
-//   2000 51.2 and 44.1.  No tree of more than 2048 positions waits for one
-//   workgroup.
-// - Runs: one workgroup a CU for few trees (one of 16 nodes over 32768
-//   positions: 41.8 us, two a CU 43.4; heads of 64, 4 nodes: 20.9 / 22.6), two
-//   where there are more trees than a third of that (16 trees of 8 nodes, heads
-//   of 64, over up to 4096: 23.6, four a CU 24.9; 24 of 63 nodes: 350 / 381 with
-//   one and two rounds), and two rounds where a run would pass 100 blocks.
+//   over up to 1000 positions: 32.5 whole, 36.6 split, up to 2000 56.6 and 61.0;
+//   40 trees of 4 up to 1000 26.0 and 26.3, of 60 80.7 and 94.4, of 4 up to 2000
+//   49.2 and 42.4.  So of up to 256 trees none of more than 2048 positions waits
+//   for one workgroup; of more trees the longest does.
+// - Runs: one workgroup a CU for few trees (one over 32768 positions: of 32 nodes
+//   54.7, two a CU 55.4; of 16 39.3 and 37.6; heads of 64, 4 nodes: 20.9 and
+//   20.6), two where there are more trees than a third of that (16 trees of 8
+//   nodes, heads of 64, over up to 4096: 22.9, one a CU 26.2, four 29.2; 19 of 9
+//   over up to 2048: 19.3, one 25.5), and four where a run would pass 100 blocks
+//   (24 of 63 over up to 16384: 383, two 424, one 529; 64 of 8 368, 402 and 402;
+//   8 of 16 over up to 30000 123, 110 and 130).
 struct TreePlan {
   int shape;  // tiles of 16 columns a workgroup: 1, 2, 4, 8, 16
   int col_groups;
@@ -767,7 +769,8 @@ struct TreePlan {
   size_t bytes() const { return kPagedAlign + plan_bytes + ml_bytes + acc_bytes; }
 };
 
-constexpr int64_t kTreeSlots = 256;      // workgroups that the device holds: one a CU
+// Workgroups of a round, one a CU; up to 128 columns a CU holds two (PAIR).
+constexpr int64_t kTreeSlots = 256;
 constexpr int64_t kTreeMaxBatch = 256;   // of a split launch
 constexpr int64_t kTreeColumns = 256;    // that a workgroup takes at most
 
@@ -805,13 +808,13 @@ static TreePlan tree_plan(int64_t trees, int64_t max_tree, int64_t q_heads, int6
 
 // WIDE: twice the groups of waves, for launches that leave CUs with one workgroup
 // or none, which are whole trees of up to 512 positions: one tree of 16 nodes
-// 13.2 us, 15.8 with fewer waves; 64 of them 33.6 and 25.6.
+// 14.3 us, 18.3 with fewer waves; 64 of them 34.1 and 27.9.
 template <int D, bool SPLIT, bool WIDE>
 static hipError_t launch_tree(const TreeArgs &a, int shape, int64_t blocks, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(blocks));
   // Groups of waves: as many as leave each two slots.  (64 dims, 64 columns: two
-  // groups and one 25.7 / 30.7 us for one tree over 32768 positions; 128 dims,
-  // 8 nodes of 4 heads: two groups and one 116.7 / 119.8 for 64 trees.)
+  // groups and one 28.6 / 33.4 us for one tree over 32768 positions; 128 dims,
+  // 8 nodes of 4 heads: two groups and one 117.9 / 121.9 for 64 trees.)
   constexpr int kNarrow = WIDE || D == 64 ? 4 : 2;
 #define CASCADE_TREE(CT, WC, WP)                                                     \
   {                                                                                  \

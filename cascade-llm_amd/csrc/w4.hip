@@ -167,8 +167,12 @@ __device__ __forceinline__ void dma_lds4_inside(const u32x4 &rsrc, int voff, int
 // -24 (or, with zero points in the operand, -48) times the sum of x, which is
 // an MFMA of its own for all NT tiles.  Both are exact in bf16, and sums are
 // fp32; the sum over a group is scaled in fp32, so that no weight is rounded.
-// The start costs what cancels: a group's sum of 16 x instead of q x, 2^-24 of
-// it, far below the rounding of a bf16 result.
+// The start costs what cancels: a group's fp32 sum has terms of 24 |x| (48 |x|
+// with zero points) and rounds as they do, not as (q - zero) x would.  Of rows
+// whose x has no common sign little is seen (4096 columns 0.9e-7 to 1.6e-7 off,
+// plain fp32 sums 3.4e-7), of x all positive 1.2e-7 to 9.7e-7 (3.1e-7).  A large
+// x under weights of zero leaves that rounding of itself behind, and a matrix row
+// of zeros gives as little, not exactly 0.
 //
 // x, scales and zero points go to LDS without passing registers, the weights,
 // which one wave needs once, to registers, both a step ahead: what a step waits
@@ -471,11 +475,16 @@ static int launch_w4_tile(const W4Args &a, hipStream_t s) {
 // - More rows: 32 of x a workgroup; 64 where two of these a CU are left: 157
 //   rows, gate and up 14336 x 4096: 74 with 64, 80 with 32; 613 rows, 4096 x
 //   4096: 47 / 44.
-// - Parts of K up to a workgroup a CU (two for more rows), none of them short: 16
-//   rows 4096 x 14336: 25.5, in 4 parts 12.7, while 32 rows 4096 x 4096 take 8.9
-//   in two and 7.4 whole; 61 rows 4096 x 14336: 61, 4 parts 22.4, 8 22.3, 10 26.9;
-//   613 rows 4096 x 4096: one part 45, four 52.  Gate and up have no workspace
-//   and are not split.
+// - Parts of K up to a workgroup a CU (two for more rows), which have tiles
+//   enough to be worth the second launch.  The wide form from 28 on: 16 rows, 4096
+//   x 14336 whole 25.5, in 4 parts 12.7; 4096 x 8192 10.1 in two parts, 11.0 in four
+//   of 16 tiles; 6144 x 4096 7.5 whole, 9.4 in two of 16.  The other from 32 on: 16
+//   rows, 2048 x 4096 6.8 whole, 6.9 in two of 16, one row 5.6 and 6.1; one row,
+//   1024 x 14336 12.9 whole, 8.3 in three (where K is that long, seven of 16 take
+//   7.3).  More rows from 8 on, where the limit is mostly the workgroups wanted: 61
+//   rows 4096 x 14336 whole 62, 4 parts 22.3, 8 21.3, 14 26.2; 157 rows 4096 x 4096
+//   20.1 in three, 21.5 in two; 613 rows 45 whole, four parts 52.  Gate and up have
+//   no workspace and are not split.
 enum W4Shape { kW4Rows16Wide, kW4Rows16, kW4Rows32, kW4Rows64 };
 
 struct W4Plan {
