@@ -300,7 +300,8 @@ class PagedKVCache:
                     workspace=None, max_tree=64, max_length=None):
         """``paged_tree_attention`` over one layer's pages (heads of 64 or 128):
         ``extend`` the sequences by their trees' nodes and ``append`` them
-        first.  ``scale`` and ``workspace`` as for ``attend``."""
+        first.  ``scale`` and ``workspace`` as for ``attend``.  ``max_tree`` and
+        ``max_length`` size the launch: near what comes they make it shorter."""
 
         if self.head_dim not in (64, 128):
             raise ValueError("attention takes heads of 64 or 128, these have {}".format(

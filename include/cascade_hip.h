@@ -509,7 +509,7 @@ int cascade_paged_tree_accept(
  * is that of terms of up to 55 |x| (111 |x| with zeros), of which 24 (48) cancel,
  * and rounds as those do: a matrix row of zeros may give as little as that
  * rounding instead of 0.  Up to 64 rows they are quicker than the products with
- * bf16 weights at every size measured, from 128 to 157 on these are (14336 x 4096
+ * bf16 weights at every size measured, from 157 on hardly at any (14336 x 4096
  * twice: 61 rows 27 to 38 us by group and zeros, bf16 41; 157 rows 74 to 88 and
  * 56; 613 rows 212 to 251 and 139).  Strides are
  * in elements, x's a multiple of 8.  Values of x of 2^120 and more, infinities
