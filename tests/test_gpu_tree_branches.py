@@ -94,3 +94,24 @@ def test_scales_of_any_sign(gpu_device, past, nodes, scale):
     step = Step([nodes, 3], [0, 1], 8, 64, seed=nodes)
     out = attend(pool, step, gpu_device, nodes, scale)
     check(pool, step, out, scale)
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,dim,largest,nodes", [
+    (40, 8, 128, 64, 51), (28, 4, 128, 64, 36), (7, 1, 64, 64, 36), (16, 1, 128, 64, 48)])
+def test_a_workspace_sized_for_larger_trees(gpu_device, q_heads, kv_heads, dim, largest, nodes):
+    # fewer nodes take fewer workgroups a run, and so more runs
+    print("workspace", q_heads, kv_heads, largest, nodes, flush=True)
+    limit, page = 32768, 64
+    pool = Pool([2900 + nodes], kv_heads, dim, page, seed=nodes, width=limit // page)
+    step = Step([nodes], [0], q_heads, dim, seed=largest)
+    q, starts, masks, rows = step.tensors(gpu_device)
+    size = _hip.paged_tree_attention_workspace_bytes(1, largest, q_heads, kv_heads, dim, limit)
+    # (what lies behind it stays)
+    space = torch.full((size + 4096,), 0xA5, dtype=torch.uint8, device=gpu_device)
+    out = torch.full_like(q, 7.0)
+    _hip.paged_tree_attention(
+        q, starts, masks, pool.k.to(gpu_device), pool.v.to(gpu_device),
+        pool.table.to(gpu_device), pool.lengths.to(gpu_device), out, space[:size], dim ** -0.5,
+        rows=rows, max_tree=nodes)
+    check(pool, step, out.cpu(), dim ** -0.5)
+    assert bool((space[size:] == 0xA5).all())
