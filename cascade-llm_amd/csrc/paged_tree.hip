@@ -187,10 +187,10 @@ __device__ __forceinline__ WeightParts tree_weights(float a, float b) {
 // above, vector and matrix instructions, which two waves of a SIMD hardly overlap:
 // a wave's block of 32 columns is 64 MFMAs (1024 cycles) and 200 vector
 // instructions (900, a sixth of them exponentials), a block of 256 columns 2.0 us;
-// 24 trees of up to 63 nodes over up to 16384 positions (885 MB) 390 us.  With two parts of P, lookups of
-// sixteen blocks' pages at a time, lane by lane, and operands read ahead took
-// that from 570 us to 355, V's turned reads in place of 32 permutations a block to
-// 326.
+// 24 trees of up to 63 nodes over up to 16384 positions (885 MB) 390 us. With two
+// parts of P, lookups of sixteen blocks' pages at a time, lane by lane, and
+// operands read ahead took that from 570 us to 355, V's turned reads in place of
+// 32 permutations a block to 326.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeArgs a) {
   constexpr int D = T::D, CT = T::CT, WC = T::WC, WP = T::WP;
@@ -673,8 +673,11 @@ __global__ __launch_bounds__(T::WAVES * kWave) void tree_attention_kernel(TreeAr
 // for 79 MB).
 constexpr int kTreeMergeThreads = 256;
 
-// A run's factor, never zero: that would turn an infinite sum into a NaN.
-__device__ __forceinline__ float run_weight(float x) { return fmaxf(paged_exp2(x), FLT_MIN); }
+// A run's factor for one of its sums: an infinite one keeps its value, which a
+// factor of zero would make a NaN.
+__device__ __forceinline__ float run_factor(float w, float sum) {
+  return fabsf(sum) < INFINITY ? w : 1.0f;
+}
 
 template <int D, int SLICES>
 __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs a) {
@@ -708,12 +711,13 @@ __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs 
       const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * at);
       const f32x4 v = *reinterpret_cast<const f32x4 *>(a.part_acc + at * D + 4 * d);
       const float mnew = fmaxf(m, ml.x);
-      const float keep = run_weight((m - mnew) * a.scale_log2);
-      const float w = run_weight((ml.x - mnew) * a.scale_log2);
+      const float keep = paged_exp2((m - mnew) * a.scale_log2);
+      const float w = paged_exp2((ml.x - mnew) * a.scale_log2);
       m = mnew;
       den = fmaf(w, ml.y, den * keep);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(w, v[i], acc[i] * keep);
+      for (int i = 0; i < 4; ++i)
+        acc[i] = fmaf(run_factor(w, v[i]), v[i], acc[i] * run_factor(keep, acc[i]));
     }
   }
   s_acc[h][slice][d] = acc;
@@ -731,9 +735,10 @@ __global__ __launch_bounds__(kTreeMergeThreads) void tree_merge_kernel(TreeArgs 
     float sum = 0.0f, r = 0.0f;
 #pragma unroll
     for (int k = 0; k < SLICES; ++k) {
-      const float w = run_weight((s_ml[hh][k][0] - mm) * a.scale_log2);
+      const float w = paged_exp2((s_ml[hh][k][0] - mm) * a.scale_log2);
+      const float part = s_acc[hh][k][dim / 4][dim % 4];
       sum = fmaf(w, s_ml[hh][k][1], sum);
-      r = fmaf(w, s_acc[hh][k][dim / 4][dim % 4], r);
+      r = fmaf(run_factor(w, part), part, r);
     }
     a.out[(token0 + node) * a.out_token + (part * kHeads + hh) * a.out_head + dim] =
         f32_to_bf16(sum == 0.0f ? 0.0f : r / sum);

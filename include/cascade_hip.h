@@ -443,7 +443,9 @@ int cascade_copy_pages(void *pages, int64_t planes, int64_t plane_bytes,
  * zero-fill and holds nothing between calls; calls that may overlap need one
  * each; sized for `trees`, max_tree and max_length it serves calls of fewer.
  * Scores, weights and sums are fp32, weights in the product with V all of its
- * bits; the result is rounded once.  Of more than 256 trees each is one
+ * bits; the result is rounded once.  Sums are divided at the end and hold up to
+ * 2^8 |V| a position until then: where these pass 3.4e38 together the result may
+ * be infinite or NaN.  Of more than 256 trees each is one
  * workgroup's a KV head, however long: a batch of many short sequences with a
  * very long one is quicker in two calls.  max_tree sizes the launch: 4 nodes
  * over 6 positions take 7.1 us, 11.0 with a max_tree of 64 and a max_length of
@@ -509,9 +511,10 @@ int cascade_paged_tree_accept(
  * is that of terms of up to 55 |x| (111 |x| with zeros), of which 24 (48) cancel,
  * and rounds as those do: a matrix row of zeros may give as little as that
  * rounding instead of 0.  Up to 64 rows they are quicker than the products with
- * bf16 weights at every size measured, from 157 on hardly at any (14336 x 4096
- * twice: 61 rows 27 to 38 us by group and zeros, bf16 41; 157 rows 74 to 88 and
- * 56; 613 rows 212 to 251 and 139).  Strides are
+ * bf16 weights at every size measured (but one row by 4096 x 4096 with groups of
+ * 32, 6.5 us and 6.0), from 157 on hardly at any (14336 x 4096 twice: 61 rows 27
+ * to 38 us by group and zeros, bf16 41; 157 rows 74 to 88 and 56; 613 rows 212 to
+ * 251 and 139).  Strides are
  * in elements, x's a multiple of 8.  Values of x of 2^120 and more, infinities
  * and NaN give NaN or infinite rows where finite ones may be meant; other rows
  * stay as they are.  No counterpart in the reference, whose weights are bf16;

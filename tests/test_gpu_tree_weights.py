@@ -118,3 +118,25 @@ def test_an_infinity_before_the_tree(gpu_device, past, nodes, under, value):
     keep = [d for d in range(dim) if d not in (3, dim - 2)]
     assert torch.equal(out[:, :, keep], clean[:, :, keep])
     assert bool(clean.isfinite().all())
+
+
+@pytest.mark.parametrize("value", [3e35, -6e35])
+@pytest.mark.parametrize("past,nodes", [(100, 5), (2500, 40)])
+def test_large_values_under_no_weight(gpu_device, past, nodes, value):
+    # finite, under a weight that fp32 does not hold, in a run of their own: they
+    # are worth nothing.  Two of 6e35, each times 2^8 at most, are 3.1e38: sums that
+    # are divided at the end stay in fp32's range, as the operator asks.
+    print("large", past, nodes, value, flush=True)
+    dim, length = 128, past + nodes
+    pool = Pool([length], 2, dim, 16, seed=past)
+    step = Step([nodes], [0], 8, dim, seed=nodes, spare=0)
+    scores(pool, step, length)
+    for p in range(past // 2):
+        page, slot = place(pool, p)
+        pool.k[page, :, slot, 0] = -300 * dim ** 0.5
+    clean = attend(pool, step, gpu_device, nodes, dim ** -0.5)
+    for p in (3, 37):
+        page, slot = place(pool, p)
+        pool.v[page, :, slot, 3:9] = value
+    out = attend(pool, step, gpu_device, nodes, dim ** -0.5)
+    assert torch.equal(out, clean) and bool(clean.isfinite().all())
